@@ -59,6 +59,8 @@ enum k3x_glu { K3X_GLU_SWIGLU = 0, K3X_GLU_SITU = 1 };
  * FLOAT:  runtime/src/routing_policy.cpp:146-157 (synthetic/resident path).
  * DOUBLE: runtime/src/official_moe.cpp:235-242 (official path). */
 enum k3x_renorm { K3X_RENORM_FLOAT = 0, K3X_RENORM_DOUBLE = 1 };
+/* k3x_hip_route only: the selected scores as they are. */
+#define K3X_RENORM_NONE 2u
 
 /* Matrices of one expert, as addressed by the debug/read-back entry points. */
 enum k3x_matrix { K3X_MATRIX_GATE = 0, K3X_MATRIX_UP = 1, K3X_MATRIX_DOWN = 2 };
@@ -365,6 +367,162 @@ int k3x_hip_moe_forward_routed(k3x_hip_ctx* ctx, k3x_hip_bank* bank,
 int k3x_hip_expert_major_plan(k3x_hip_ctx* ctx, const uint32_t* ids,
                               uint32_t tokens, uint32_t top_k,
                               uint32_t experts, const k3x_hip_moe_taps* taps);
+
+/* ---- routing from given logits -------------------------------------------- */
+
+/* Element types of the operators that take more than one. */
+enum k3x_dtype { K3X_DTYPE_F32 = 0, K3X_DTYPE_BF16 = 1, K3X_DTYPE_F16 = 2 };
+
+/* Score of expert e from its logit l: SIGMOID 1 / (1 + exp(-l)) with the
+ * roundings of k3x_hip_moe_forward's router; SOFTMAX exp(l - max) / sum over
+ * all experts of the token, formed in double and rounded to fp32 once. */
+enum k3x_score { K3X_SCORE_SIGMOID = 0, K3X_SCORE_SOFTMAX = 1 };
+/* Score of a group of experts: its largest score + bias, or the sum of its
+ * two largest (one, where a group has one expert). */
+enum k3x_group_score { K3X_GROUP_MAX = 0, K3X_GROUP_TOP2 = 1 };
+
+typedef struct k3x_hip_route_params {
+    uint32_t tokens;        /* T, 1 .. 2^20 */
+    uint32_t experts;       /* E, 1 .. 4096 */
+    uint32_t top_k;         /* K, 1 .. 64, at most top_groups * E / groups */
+    uint32_t dtype;         /* of the logits: K3X_DTYPE_F32 or K3X_DTYPE_BF16 */
+    uint32_t scoring;       /* enum k3x_score */
+    uint32_t renorm;        /* enum k3x_renorm or K3X_RENORM_NONE */
+    float routed_scale;     /* multiplies the weights */
+    uint32_t groups;        /* G equal groups of consecutive experts, 1 .. 64, divides E */
+    uint32_t top_groups;    /* groups that experts are taken from, 1 .. G */
+    uint32_t group_score;   /* enum k3x_group_score */
+    uint32_t logits_stride; /* elements from token to token, >= E; 0: E */
+} k3x_hip_route_params;
+
+/* Routes T tokens by their router logits (device [T][E]): s = score, a = s +
+ * bias in fp32 (bias device fp32 [E], or NULL); with G > 1 only the experts
+ * of the top_groups groups of the largest group scores stay; the K largest a
+ * in descending order, every tie to the lower index -> ids device u32 [T][K];
+ * weights device fp32 [T][K] = s / (sum of the selected s) * routed_scale, or
+ * s * routed_scale.  With sigmoid scores and G = 1 the route is that of
+ * k3x_hip_moe_forward for the same logits, bit for bit.  ids and weights are
+ * what k3x_hip_moe_forward_routed and k3x_hip_expert_major_plan take.
+ * A logit of minus infinity has the score 0.  Latched, the token's outputs
+ * left as they were: a score, bias or sum that is not finite, with renormalised
+ * weights a sum of 0 (K3X_ERR_INVALID_STATE; with K3X_RENORM_DOUBLE and sigmoid
+ * scores a logit or bias that is not finite, or the sum, as
+ * K3X_ERR_INVALID_EXTENT).  The reference routes on the host
+ * (runtime/src/routing_policy.cpp:31-160; official_moe.cpp:211-245).
+ * Asynchronous. */
+int k3x_hip_route(k3x_hip_ctx* ctx, const k3x_hip_route_params* params, const void* logits,
+                  const float* bias, uint32_t* ids, float* weights);
+
+/* ---- gated delta rule ------------------------------------------------------ */
+
+/* Decay of the state: none, one a value head, one a key channel. */
+enum k3x_gate { K3X_GATE_NONE = 0, K3X_GATE_HEAD = 1, K3X_GATE_CHANNEL = 2 };
+
+typedef struct k3x_hip_delta_params {
+    uint32_t sequences;   /* N, 1 .. 65535 */
+    uint32_t tokens;      /* T rows of q, k, v, gate, beta and out, 0 .. 2^24 */
+    uint32_t key_heads;   /* Hk, divides Hv */
+    uint32_t value_heads; /* Hv, 1 .. 1024; value head h has key head h / (Hv / Hk) */
+    uint32_t key_dim;     /* K, 1 .. 256 */
+    uint32_t value_dim;   /* V, 1 .. 1024 */
+    uint32_t dtype;       /* enum k3x_dtype, of q, k, v and out */
+    uint32_t gate;        /* enum k3x_gate */
+    float scale;          /* of the queries */
+    float norm_epsilon;   /* > 0: q and k each over sqrt(sum of squares + epsilon); 0: as given */
+    uint32_t longest;     /* tokens of the longest sequence if known, 0: not.  Chooses the
+                             kernels only: results hold whatever it says. */
+    uint32_t slots;       /* states in state_in and state_out */
+    /* Elements from token to token of q, k, v and out (q, k and v may be
+     * parts of one projection's rows); 0: packed. */
+    uint64_t q_stride, k_stride, v_stride, out_stride;
+} k3x_hip_delta_params;
+
+/* The gated delta rule over N sequences, for each value head a state S
+ * [K][V] in fp32 and for each of its tokens in order
+ *   S = exp(gate) S            (row c times exp(gate_c), or all by one)
+ *   u = beta (v - S^T k)
+ *   S = S + k u^T
+ *   out = scale S^T q
+ * q, k device [T][Hk][K], v, out [T][Hv][V]; gate fp32 [T][Hv][K] or [T][Hv],
+ * <= 0 (minus infinity empties the state; NULL with K3X_GATE_NONE); beta fp32
+ * [T][Hv].  Sequence n has the rows offsets[n] .. offsets[n + 1] - 1 (device
+ * u32 [N + 1]; NULL: T / N rows each), of which the first limits[n] only are
+ * taken where limits (device u32 [N]) is given: rows of out past them are left
+ * as they were.  So a window of drafted tokens is run with state_out NULL, and
+ * run again up to the accepted count with it.
+ * state_in: device fp32 [slots][Hv][K][V], 16-byte aligned, or NULL (zeros);
+ * state_out: the same, state_in itself or apart from it, or NULL (not
+ * written).  Sequence n has the state slot_index[n] (device u32 [N]), or n
+ * without slot_index (then slots >= N).  A sequence of no tokens has its state
+ * copied.
+ * One token a sequence and short sequences run token by token; longer ones in
+ * chunks whose writes are solved for at once.  workspace: device, 256-byte
+ * aligned, k3x_hip_delta_workspace(params) bytes (NULL where that is 0), the
+ * call's own until it is done: calls that may overlap, and captured graphs
+ * that may, have one each.
+ * Latched: offsets that fall or pass T, a slot past slots, two sequences of
+ * one state with state_out (K3X_ERR_INVALID_STATE; nothing of those sequences
+ * is read or written); a q, k, v, gate or beta that is not finite or a gate
+ * above 0 (K3X_ERR_INVALID_MXFP4, as for the layer's input; the sequence's
+ * outputs are then not defined).  Replaces the recurrence of
+ * ComputeBackend::official_kda (runtime/cuda/official_kda.cuh:11-37), batched.
+ * Asynchronous. */
+int k3x_hip_delta_rule(k3x_hip_ctx* ctx, const k3x_hip_delta_params* params, const void* q,
+                       const void* k, const void* v, const float* gate, const float* beta,
+                       const uint32_t* offsets, const uint32_t* limits,
+                       const uint32_t* slot_index, const float* state_in, float* state_out,
+                       void* out, void* workspace, size_t workspace_bytes);
+/* Bytes of workspace of such a call; 0 also for parameters that it refuses. */
+size_t k3x_hip_delta_workspace(const k3x_hip_delta_params* params);
+
+/* ---- verification of drafted tokens ---------------------------------------- */
+
+/* What a row holds: logits, or probabilities (>= 0; used as they are). */
+enum k3x_dist { K3X_DIST_LOGITS = 0, K3X_DIST_PROBS = 1 };
+
+/* draft_counts[n] of a sequence that is left out. */
+#define K3X_VERIFY_SKIP 0xffffffffu
+
+typedef struct k3x_hip_verify_params {
+    uint32_t sequences;   /* N, 1 .. 65535 */
+    uint32_t drafts;      /* D, drafted tokens a sequence, 0 .. 64 */
+    uint32_t vocab;       /* V, 1 .. 2^20 */
+    uint32_t dtype;       /* of target and draft: K3X_DTYPE_F32 or K3X_DTYPE_BF16 */
+    uint32_t form;        /* enum k3x_dist, of target and draft */
+    uint32_t greedy;      /* 1: the target's largest entry, ties to the lower token */
+    float temperature;    /* > 0; divides logits */
+    uint32_t row_stride;  /* elements from row to row of target and draft, >= V; 0: V */
+} k3x_hip_verify_params;
+
+/* Verifies N sequences' drafted tokens x (device u32 [N][D]) against the
+ * target model's rows (device [N][D + 1][V]; row i follows i drafted tokens).
+ * With p and q the target's and the draft's probabilities (softmax(logits /
+ * temperature), or the rows themselves), draft i is accepted while
+ *   accept_u[n][i] q_i(x_i) < p_i(x_i)
+ * and the next token is drawn from max(p_i - q_i, 0) at the first draft i that
+ * is not, or from p_D: the first token whose cumulative sum is over
+ * sample_u[n] times the whole.  draft (device [N][D][V]) NULL: q_i is 1 at x_i.
+ * accept_u fp32 [N][D], sample_u fp32 [N], in [0, 1).  greedy: accepted while
+ * x_i is the largest entry of the target's row i, and the next token is the
+ * largest of its row (draft, accept_u and sample_u are not read).
+ * Probabilities and their sums are formed in double.
+ * accepted u32 [N]; out_tokens u32 [N][D + 1]: the accepted tokens, the next
+ * token, then 0xffffffff.  draft_counts (device u32 [N], or NULL) gives
+ * sequences fewer drafts than D (the next row is then the last), or
+ * K3X_VERIFY_SKIP: accepted 0, no tokens, nothing read.
+ * workspace as k3x_hip_delta_rule's, k3x_hip_verify_workspace(params) bytes.
+ * Latched as K3X_ERR_INVALID_STATE, the sequence's outputs left as they were: a
+ * drafted token past V that is reached, a used row that holds NaN, plus
+ * infinity (logits) or a negative or infinite entry (probabilities) or nothing
+ * but minus infinity or zeros, a uniform outside [0, 1), a draft count past D.
+ * The reference verifies on the host (generate_speculative,
+ * runtime/src/model.cpp:1507).  Asynchronous. */
+int k3x_hip_verify_draft(k3x_hip_ctx* ctx, const k3x_hip_verify_params* params,
+                         const void* target, const void* draft, const uint32_t* tokens,
+                         const uint32_t* draft_counts, const float* accept_u,
+                         const float* sample_u, uint32_t* accepted, uint32_t* out_tokens,
+                         void* workspace, size_t workspace_bytes);
+size_t k3x_hip_verify_workspace(const k3x_hip_verify_params* params);
 
 /* ---- official K3 MoE FFN (Stable LatentMoE) ------------------------------ */
 

@@ -24,7 +24,13 @@ ERR_BACKEND_UNAVAILABLE = 17
 GLU_SWIGLU, GLU_SITU = 0, 1
 STAGES = ("route", "group", "gate_up", "shared_gate_up", "down", "shared_down", "combine",
           "decode_front", "decode_select", "decode_gate_up", "decode_down")
-RENORM_FLOAT, RENORM_DOUBLE = 0, 1
+RENORM_FLOAT, RENORM_DOUBLE, RENORM_NONE = 0, 1, 2  # NONE: route() only
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
+GATE_NONE, GATE_HEAD, GATE_CHANNEL = 0, 1, 2
+DIST_LOGITS, DIST_PROBS = 0, 1
+VERIFY_SKIP = 0xffffffff
 MATRIX_GATE, MATRIX_UP, MATRIX_DOWN = 0, 1, 2
 
 STREAM_GATE_CODES = 1
@@ -109,6 +115,27 @@ class SynthDesc(C.Structure):
                 ("shared_sigma", C.c_float), ("gamma_value", C.c_float)]
 
 
+class RouteParams(C.Structure):
+    _fields_ = [("tokens", C.c_uint32), ("experts", C.c_uint32), ("top_k", C.c_uint32),
+                ("dtype", C.c_uint32), ("scoring", C.c_uint32), ("renorm", C.c_uint32),
+                ("routed_scale", C.c_float), ("groups", C.c_uint32), ("top_groups", C.c_uint32),
+                ("group_score", C.c_uint32), ("logits_stride", C.c_uint32)]
+
+
+class DeltaParams(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("sequences", "tokens", "key_heads", "value_heads",
+                                         "key_dim", "value_dim", "dtype", "gate")] + \
+               [("scale", C.c_float), ("norm_epsilon", C.c_float), ("longest", C.c_uint32),
+                ("slots", C.c_uint32)] + \
+               [(n, C.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "out_stride")]
+
+
+class VerifyParams(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("sequences", "drafts", "vocab", "dtype", "form",
+                                         "greedy")] + \
+               [("temperature", C.c_float), ("row_stride", C.c_uint32)]
+
+
 class Stats(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in ("forward_calls", "kernel_launches", "scratch_bytes",
                                          "resident_weight_bytes", "weight_h2d_bytes",
@@ -163,6 +190,11 @@ _SIGS = {
                                              _vp, _vp, C.POINTER(MoeTaps)]),
     "k3x_hip_expert_major_plan": (C.c_int, [_vp, _vp, C.c_uint32, C.c_uint32, C.c_uint32,
                                             C.POINTER(MoeTaps)]),
+    "k3x_hip_route": (C.c_int, [_vp, C.POINTER(RouteParams), _vp, _vp, _vp, _vp]),
+    "k3x_hip_delta_rule": (C.c_int, [_vp, C.POINTER(DeltaParams)] + [_vp] * 12 + [C.c_size_t]),
+    "k3x_hip_delta_workspace": (C.c_size_t, [C.POINTER(DeltaParams)]),
+    "k3x_hip_verify_draft": (C.c_int, [_vp, C.POINTER(VerifyParams)] + [_vp] * 9 + [C.c_size_t]),
+    "k3x_hip_verify_workspace": (C.c_size_t, [C.POINTER(VerifyParams)]),
     "k3x_hip_official_create": (C.c_int, [_vp, _vp, C.POINTER(OfficialDesc), C.POINTER(_vp)]),
     "k3x_hip_official_destroy": (C.c_int, [_vp]),
     "k3x_hip_official_upload_ffn": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
@@ -553,6 +585,143 @@ def expert_major_plan(ctx: Context, ids, tokens, top_k, experts, taps: dict) -> 
     t = make_taps(taps)
     return ctx.lib.k3x_hip_expert_major_plan(ctx.handle, ptr(ids), tokens, top_k, experts,
                                              C.byref(t))
+
+
+def _dtype(t) -> int:
+    import torch
+    codes = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+    if t.dtype not in codes:
+        raise ValueError(f"expected float32, bfloat16 or float16, not {t.dtype}")
+    return codes[t.dtype]
+
+
+def _expect(what: str, t, shape, dtypes) -> None:
+    """A tensor of the shape and of one of the types (None passes)."""
+    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype not in dtypes):
+        raise ValueError(f"{what}: expected {tuple(shape)} of {dtypes}, not {tuple(t.shape)} of "
+                         f"{t.dtype}")
+
+
+def _rows(t):
+    """Device pointer of rows that are contiguous in themselves (any distance between rows)."""
+    if t is None or t.is_contiguous():
+        return ptr(t)
+    if not t.is_cuda:
+        raise ValueError("expected a device tensor")
+    if not _row_contiguous(t):
+        raise ValueError("expected rows that are contiguous in themselves")
+    return t.data_ptr()
+
+
+def _row_contiguous(t) -> bool:
+    return t.stride(0) >= t[0].numel() and t[0].is_contiguous()
+
+
+def _row_stride(t) -> int:
+    """Elements from row to row; 0 where that is the row's length or there is one row."""
+    return 0 if t.shape[0] < 2 or t.is_contiguous() else t.stride(0)
+
+
+def make_route_params(tokens, experts, top_k, scoring=SCORE_SIGMOID, renorm=RENORM_FLOAT,
+                      routed_scale=1.0, groups=1, top_groups=None, group_score=GROUP_TOP2,
+                      dtype=DTYPE_F32, logits_stride=0) -> RouteParams:
+    """top_groups None: every group.  route() sets the logits' type and stride."""
+    return RouteParams(tokens, experts, top_k, dtype, scoring, renorm, routed_scale, groups,
+                       groups if top_groups is None else top_groups, group_score, logits_stride)
+
+
+def route(ctx: Context, params: RouteParams, logits, ids, weights, bias=None) -> int:
+    """ids [T][K] (int32) and weights [T][K] (fp32) from router logits [T][E] (fp32 or bf16)
+    and the fp32 bias [E] (k3x_hip_route)."""
+    import torch
+    T, E, K = params.tokens, params.experts, params.top_k
+    _expect("logits", logits, (T, E), (torch.float32, torch.bfloat16))
+    _expect("bias", bias, (E,), (torch.float32,))
+    _expect("ids", ids, (T, K), (torch.int32, torch.uint32))
+    _expect("weights", weights, (T, K), (torch.float32,))
+    p = RouteParams.from_buffer_copy(params)
+    p.dtype, p.logits_stride = _dtype(logits), _row_stride(logits)
+    return ctx.lib.k3x_hip_route(ctx.handle, C.byref(p), _rows(logits), ptr(bias), ptr(ids),
+                                 ptr(weights))
+
+
+def make_delta_params(q, k, v, sequences, gate=None, scale=1.0, norm_epsilon=0.0, longest=0,
+                      slots=None) -> DeltaParams:
+    """Parameters of delta_rule for q, k [T][Hk][K] and v [T][Hv][V] (rows may lie apart) and a
+    gate [T][Hv][K], [T][Hv] or None; slots None: one state a sequence."""
+    T, Hk, K = q.shape
+    H, V = v.shape[1:]
+    kind = GATE_NONE if gate is None else GATE_HEAD if gate.dim() == 2 else GATE_CHANNEL
+    return DeltaParams(sequences, T, Hk, H, K, V, _dtype(v), kind, scale, norm_epsilon, longest,
+                       sequences if slots is None else slots, _row_stride(q), _row_stride(k),
+                       _row_stride(v), 0)
+
+
+def delta_workspace_bytes(params: DeltaParams) -> int:
+    return load().k3x_hip_delta_workspace(C.byref(params))
+
+
+def delta_rule(ctx: Context, params: DeltaParams, q, k, v, beta, out, gate=None, offsets=None,
+               limits=None, slot_index=None, state_in=None, state_out=None,
+               workspace=None) -> int:
+    """The gated delta rule (k3x_hip_delta_rule): out [T][Hv][V] and states [slots][Hv][K][V]
+    (fp32) from q, k, v of one type, gate and beta [T][Hv] (fp32); offsets [N + 1], limits [N]
+    and slot_index [N] int32."""
+    import torch
+    p = DeltaParams.from_buffer_copy(params)
+    T, N, H, K, V = p.tokens, p.sequences, p.value_heads, p.key_dim, p.value_dim
+    _expect("q", q, (T, p.key_heads, K), (v.dtype,))
+    _expect("k", k, (T, p.key_heads, K), (v.dtype,))
+    _expect("v", v, (T, H, V), (v.dtype,))
+    _expect("out", out, (T, H, V), (v.dtype,))
+    _expect("beta", beta, (T, H), (torch.float32,))
+    _expect("gate", gate, (T, H, K) if p.gate == GATE_CHANNEL else (T, H), (torch.float32,))
+    ints = (torch.int32, torch.uint32)
+    _expect("offsets", offsets, (N + 1,), ints)
+    _expect("limits", limits, (N,), ints)
+    _expect("slot_index", slot_index, (N,), ints)
+    _expect("state_in", state_in, (p.slots, H, K, V), (torch.float32,))
+    _expect("state_out", state_out, (p.slots, H, K, V), (torch.float32,))
+    p.dtype = _dtype(v)
+    p.q_stride, p.k_stride, p.v_stride, p.out_stride = map(_row_stride, (q, k, v, out))
+    return ctx.lib.k3x_hip_delta_rule(
+        ctx.handle, C.byref(p), _rows(q), _rows(k), _rows(v), ptr(gate), ptr(beta), ptr(offsets),
+        ptr(limits), ptr(slot_index), ptr(state_in), ptr(state_out), _rows(out), ptr(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size())
+
+
+def make_verify_params(target, form=DIST_LOGITS, greedy=False, temperature=1.0) -> VerifyParams:
+    """Parameters of verify_draft for target rows [N][D + 1][V]."""
+    N, D1, V = target.shape
+    return VerifyParams(N, D1 - 1, V, _dtype(target), form, int(greedy), temperature, 0)
+
+
+def verify_workspace_bytes(params: VerifyParams) -> int:
+    return load().k3x_hip_verify_workspace(C.byref(params))
+
+
+def verify_draft(ctx: Context, params: VerifyParams, target, tokens, accepted, out_tokens,
+                 draft=None, draft_counts=None, accept_u=None, sample_u=None,
+                 workspace=None) -> int:
+    """Verifies drafted tokens [N][D] against the target's rows [N][D + 1][V]
+    (k3x_hip_verify_draft): accepted [N] and out_tokens [N][D + 1] int32."""
+    import torch
+    N, D, V = params.sequences, params.drafts, params.vocab
+    ints = (torch.int32, torch.uint32)
+    _expect("target", target, (N, D + 1, V), (torch.float32, torch.bfloat16))
+    _expect("draft", draft, (N, D, V), (target.dtype,))
+    _expect("tokens", tokens, (N, D), ints)
+    _expect("draft_counts", draft_counts, (N,), ints)
+    _expect("accept_u", accept_u, (N, D), (torch.float32,))
+    _expect("sample_u", sample_u, (N,), (torch.float32,))
+    _expect("accepted", accepted, (N,), ints)
+    _expect("out_tokens", out_tokens, (N, D + 1), ints)
+    if _dtype(target) != params.dtype:
+        raise ValueError("target: not of the parameters' type")
+    return ctx.lib.k3x_hip_verify_draft(
+        ctx.handle, C.byref(params), ptr(target), ptr(draft), ptr(tokens), ptr(draft_counts),
+        ptr(accept_u), ptr(sample_u), ptr(accepted), ptr(out_tokens), ptr(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size())
 
 
 class Storage:

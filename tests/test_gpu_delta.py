@@ -1,0 +1,449 @@
+"""The gated delta rule (k3x_hip_delta_rule) against its definition in 64
+bits, token by token, at the lengths, shapes, gates and offsets where it can go
+wrong.
+
+Bound.  Take one value column s of a head's state, M the largest 2-norm that it
+and the values take.  A token's exact update s -> (I - beta k k^T) D s + beta v k
+does not lengthen an error (|k| <= 1, 0 <= beta <= 1, 0 <= D <= 1), so errors
+only add up over a sequence's L tokens, and those of one token are, in units of
+2^-24 M: the decay's exponential and product 4, the normalised key 6 in each of
+its two uses, the dot product over K (lane sums of 16 and four levels, or chunk
+sums of 32 over halves of 11 bits each, whose products leave 2^-22 each) 24, the
+update 4, the chunk's inverse another 24: below 96 together.  Hence
+|error| <= 96 L 2^-24 M for the state, times scale |q| for an output, plus half a
+step of the output's type."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+DEV = "cuda:0"
+EPS = 1e-6
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def hip():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import k3x_amd
+    ctx = k3x_amd.Context(0)
+    yield k3x_amd, ctx
+    ctx.close()
+
+
+def gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def inputs(lens, Hk, H, K, V, dtype=F32, gate="channel", seed=0, extra=0, strong=1.0):
+    """Inputs of sequences of these lengths, `extra` rows behind the last."""
+    g = gen(seed + 1000 * sum(lens) + K)
+    T = sum(lens) + extra
+
+    def n(*shape):
+        return torch.randn(shape, device=DEV, generator=g)
+
+    s = dict(lens=list(lens), q=n(T, Hk, K).to(dtype), k=n(T, Hk, K).to(dtype),
+             v=n(T, H, V).to(dtype), beta=torch.sigmoid(n(T, H)), gate=None,
+             state=n(len(lens), H, K, V) * 0.3)
+    if gate != "none":
+        s["gate"] = -strong * torch.nn.functional.softplus(
+            n(T, H, K) * 2 - 3 if gate == "channel" else n(T, H) * 2 - 3)
+    cu = [0]
+    for x in lens:
+        cu.append(cu[-1] + x)
+    s["offsets"] = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    return s
+
+
+def definition(s, scale, norm=True, limits=None, state=True):
+    """out, states and their bounds, in 64 bits."""
+    q, k, v = (s[x].double() for x in "qkv")
+    H, K, V = v.shape[1], q.shape[2], v.shape[2]
+    r = H // q.shape[1]
+    if norm:
+        q = q / (q.square().sum(-1, keepdim=True) + EPS).sqrt()
+        k = k / (k.square().sum(-1, keepdim=True) + EPS).sqrt()
+    q, k = q.repeat_interleave(r, 1), k.repeat_interleave(r, 1)
+    S = s["state"].double().clone() if state else torch.zeros_like(s["state"]).double()
+    out, tol = torch.zeros_like(v), torch.zeros_like(v)
+    stol = torch.zeros_like(S)
+    at = 0
+    for n, length in enumerate(s["lens"]):
+        most = length if limits is None else min(length, limits[n])
+        M = S[n].square().sum(1).sqrt()  # [H][V]
+        for i in range(most):
+            t = at + i
+            if s["gate"] is not None:
+                d = s["gate"][t].double().exp()
+                S[n] *= d[..., None] if d.dim() == 2 else d[:, None, None]
+            u = s["beta"][t].double()[:, None] * (v[t] - (S[n] * k[t][..., None]).sum(1))
+            S[n] += k[t][..., None] * u[:, None]
+            out[t] = scale * (S[n] * q[t][..., None]).sum(1)
+            M = torch.maximum(torch.maximum(M, S[n].square().sum(1).sqrt()), v[t].abs())
+            tol[t] = 96 * (i + 1) * 2.0 ** -24 * M * scale * q[t].square().sum(-1).sqrt()[:, None]
+        stol[n] = (96 * most * 2.0 ** -24 * M)[:, None]
+        at += length
+    return out, S, tol, stol
+
+
+def call(hip, s, scale=None, norm=True, limits=None, slot_index=None, state_in="own",
+         state_out="new", slots=None, out=None, offsets="own", longest=None):
+    k3x, ctx = hip
+    scale = s["q"].shape[-1] ** -0.5 if scale is None else scale
+    state_in = s["state"] if isinstance(state_in, str) else state_in
+    N = len(s["lens"])
+    if isinstance(state_out, str):
+        state_out = torch.full_like(s["state"], -7.0)
+    p = k3x.make_delta_params(s["q"], s["k"], s["v"], N, gate=s["gate"], scale=scale,
+                              norm_epsilon=EPS if norm else 0.0,
+                              longest=max(s["lens"]) if longest is None else longest, slots=slots)
+    out = torch.full(s["v"].shape, -7.0, device=DEV).to(s["v"].dtype) if out is None else out
+    need = k3x.delta_workspace_bytes(p)
+    ws = torch.empty((need,), dtype=torch.uint8, device=DEV) if need else None
+    lim = None if limits is None else torch.tensor(limits, dtype=torch.int32, device=DEV)
+    st = k3x.delta_rule(ctx, p, s["q"], s["k"], s["v"], s["beta"], out, gate=s["gate"],
+                        offsets=s["offsets"] if isinstance(offsets, str) else offsets, limits=lim,
+                        slot_index=slot_index, state_in=state_in, state_out=state_out,
+                        workspace=ws)
+    return st, out, state_out
+
+
+def close(got, want, tol, dtype=F32):
+    step = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+    err = (got.double() - want).abs()
+    worst = float((err / (tol + 2.0 ** -24 * want.abs() + step * want.abs() + 1e-30)).max()) \
+        if err.numel() else 0.0
+    assert worst <= 1.0, worst
+    return worst
+
+
+def check(hip, s, parity_report=None, **kw):
+    k3x, ctx = hip
+    lens = s["lens"]
+    print(f"[gpu-test] delta {lens} q{tuple(s['q'].shape)} v{tuple(s['v'].shape)} {s['v'].dtype}"
+          f" gate {None if s['gate'] is None else s['gate'].dim()} {sorted(kw)}", flush=True)
+    scale = kw.get("scale", s["q"].shape[-1] ** -0.5)
+    st, out, state = call(hip, s, **kw)
+    assert st == 0
+    assert ctx.synchronize() == 0
+    want, S, tol, stol = definition(s, scale, kw.get("norm", True), kw.get("limits"),
+                                    isinstance(kw.get("state_in", "own"), str))
+    live = torch.zeros(len(out), dtype=torch.bool, device=DEV)
+    at = 0
+    for n, length in enumerate(lens):
+        live[at:at + min(length, (kw.get("limits") or {n: length})[n])] = True
+        at += length
+    a = close(out[live], want[live], tol[live], s["v"].dtype)
+    b = close(state, S, stol) if state is not None else 0.0
+    assert (out[~live] == -7).all()
+    if parity_report:
+        parity_report(f"out at {a:.3f} and state at {b:.3f} of the bound")
+    return out, state
+
+
+SHAPES = [(1, 1, 1, 1), (1, 1, 16, 16), (2, 2, 33, 47), (1, 4, 64, 64), (2, 2, 96, 80),
+          (2, 4, 128, 128), (1, 2, 128, 20), (1, 1, 129, 33), (1, 2, 256, 64), (1, 1, 8, 200)]
+
+
+@pytest.mark.parametrize("Hk,H,K,V", SHAPES)
+@pytest.mark.parametrize("gate", ["none", "head", "channel"])
+@pytest.mark.parametrize("lens", [(1,), (1, 1, 1), (0, 3, 17), (70, 0, 1, 33)],
+                         ids=lambda x: "_".join(map(str, x)))
+def test_shapes(hip, Hk, H, K, V, gate, lens):
+    check(hip, inputs(lens, Hk, H, K, V, gate=gate))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("gate", ["none", "head", "channel"])
+@pytest.mark.parametrize("lens", [(1, 1), (5, 16, 2), (40, 31, 32, 64, 65), (300, 129)],
+                         ids=lambda x: "_".join(map(str, x)))
+def test_types(hip, dtype, gate, lens, parity_report):
+    check(hip, inputs(lens, 2, 4, 128, 128, dtype, gate), parity_report)
+
+
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 127, 128,
+                                    129, 200])
+@pytest.mark.parametrize("gate", ["head", "channel"])
+def test_lengths(hip, length, gate):
+    check(hip, inputs((length,), 1, 1, 64, 32, BF16, gate))
+
+
+@pytest.mark.parametrize("strong", [0.0, 1e-4, 30.0, 300.0])
+@pytest.mark.parametrize("gate", ["head", "channel"])
+@pytest.mark.parametrize("lens", [(3,), (150,)], ids=["short", "long"])
+def test_decays(hip, strong, gate, lens):
+    """No decay at all, next to none, and decays past every exponent."""
+    check(hip, inputs(lens, 1, 2, 128, 64, gate=gate, strong=strong))
+
+
+@pytest.mark.parametrize("gate", ["head", "channel"])
+@pytest.mark.parametrize("lens", [(6,), (100,)], ids=["short", "long"])
+def test_minus_infinity_empties_the_state(hip, gate, lens):
+    s = inputs(lens, 1, 2, 64, 32, gate=gate)
+    s["gate"][4] = -math.inf
+    s["gate"][lens[0] // 2, 0] = -math.inf
+    check(hip, s)
+
+
+@pytest.mark.parametrize("lens", [(7,), (90,)], ids=["short", "long"])
+@pytest.mark.parametrize("size", [1e-18, 1e-3, 30.0, 1e15])
+def test_sizes_of_values(hip, lens, size):
+    """The state is linear in the values, whatever their size."""
+    s = inputs(lens, 1, 1, 128, 48)
+    s["v"] *= size
+    s["state"] *= size
+    check(hip, s)
+
+
+@pytest.mark.parametrize("lens", [(7,), (90,)], ids=["short", "long"])
+def test_columns_of_unlike_sizes(hip, lens):
+    """A column's error is bounded by its own size, tokens' sizes growing and falling."""
+    s = inputs(lens, 1, 1, 128, 48)
+    size = 10.0 ** torch.linspace(-9, 9, 48, device=DEV)
+    s["v"] *= size
+    s["state"] *= size
+    check(hip, s)
+
+
+@pytest.mark.parametrize("lens", [(9,), (80,)], ids=["short", "long"])
+def test_without_norm(hip, lens):
+    """Keys as given, of length 1 at most; queries of any length."""
+    s = inputs(lens, 1, 2, 128, 64)
+    s["k"] = s["k"] / s["k"].norm(dim=-1, keepdim=True) * 0.999
+    s["q"] *= 37.0
+    check(hip, s, norm=False, scale=0.25)
+
+
+@pytest.mark.parametrize("lens", [(9,), (80,)], ids=["short", "long"])
+def test_equal_keys_and_zero_rows(hip, lens):
+    s = inputs(lens, 1, 1, 128, 32)
+    s["k"][:] = s["k"][0]
+    s["k"][3] = 0
+    s["q"][5] = 0
+    s["v"][6] = 0
+    s["beta"][7] = 0
+    s["beta"][8] = 1
+    check(hip, s)
+
+
+@pytest.mark.parametrize("most", [1, 16, 70])
+def test_limits(hip, most):
+    """The first limits[n] tokens only; rows past them are left, and what lies there
+    is not looked at."""
+    lens = [most, max(1, most // 2), most, most, most]
+    limits = [0, lens[1], 1, most, most // 2]
+    s = inputs(lens, 2, 2, 128, 64, BF16, extra=5)
+    s["v"][-5:] = math.nan
+    s["k"][-5:] = math.nan
+    s["gate"][-5:] = math.nan
+    at = 0
+    for n, length in enumerate(lens):
+        s["q"][at + limits[n]:at + length] = math.nan
+        at += length
+    check(hip, s, limits=limits)
+    check(hip, s, limits=[x + 1000 if x == lens[n] else x for n, x in enumerate(limits)])
+
+
+@pytest.mark.parametrize("lens", [(1, 1, 1), (5, 0, 9), (64, 33, 40)],
+                         ids=lambda x: "_".join(map(str, x)))
+def test_in_place_and_slots(hip, lens):
+    """States in place in a pool of more, others untouched; same bits as apart."""
+    k3x, ctx = hip
+    s = inputs(lens, 1, 2, 128, 128, BF16)
+    _, apart = check(hip, s)
+    pool = torch.randn((7, 2, 128, 128), device=DEV, generator=gen(4))
+    before = pool.clone()
+    index = torch.tensor([5, 0, 3], dtype=torch.int32, device=DEV)
+    pool[index.long()] = s["state"]
+    st, out, _ = call(hip, s, state_in=pool, state_out=pool, slots=7, slot_index=index)
+    assert st == 0 and ctx.synchronize() == 0
+    assert torch.equal(pool[index.long()], apart)
+    rest = [1, 2, 4, 6]
+    assert torch.equal(pool[rest], before[rest])
+
+
+@pytest.mark.parametrize("lens", [(1, 1), (40, 7)], ids=["short", "long"])
+def test_without_states(hip, lens):
+    """No state before: zeros.  None after: nothing written, one state read by both."""
+    k3x, ctx = hip
+    s = inputs(lens, 1, 2, 64, 64)
+    check(hip, s, state_in=None)
+    check(hip, s, state_out=None)
+    one = s["state"][:1].clone()
+    index = torch.zeros(2, dtype=torch.int32, device=DEV)
+    st, out, _ = call(hip, s, state_in=one, state_out=None, slots=1, slot_index=index)
+    assert st == 0 and ctx.synchronize() == 0
+    s["state"][1] = s["state"][0]
+    st, out2, _ = call(hip, s, state_out=None)
+    assert st == 0 and ctx.synchronize() == 0
+    assert torch.equal(out, out2)
+
+
+def test_uniform_without_offsets(hip):
+    k3x, ctx = hip
+    for L in (1, 50):
+        s = inputs((L,) * 3, 1, 2, 64, 64)
+        st, out, S = call(hip, s)
+        st2, out2, S2 = call(hip, s, offsets=None)
+        assert st == st2 == 0 and ctx.synchronize() == 0
+        assert torch.equal(out, out2) and torch.equal(S, S2)
+
+
+@pytest.mark.parametrize("lens", [(1, 1), (45, 20)], ids=["short", "long"])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+def test_rows_of_a_projection(hip, lens, dtype):
+    """q, k and v as parts of one projection's rows, off 16-byte alignment; out too."""
+    k3x, ctx = hip
+    Hk, H, K, V = 2, 4, 64, 32
+    s = inputs(lens, Hk, H, K, V, dtype)
+    st, want, S = call(hip, s)
+    T = sum(lens)
+    row = torch.randn((T, 3 + 2 * Hk * K + H * V + 5), device=DEV, generator=gen(2)).to(dtype)
+    parts = {}
+    at = 3
+    for x, h, d in (("q", Hk, K), ("k", Hk, K), ("v", H, V)):
+        row[:, at:at + h * d] = s[x].reshape(T, -1)
+        parts[x] = row[:, at:at + h * d].unflatten(1, (h, d))
+        at += h * d
+    wide = torch.full((T, H * V + 9), -7.0, device=DEV).to(dtype)
+    st2, out, S2 = call(hip, dict(s, **parts), out=wide[:, 1:1 + H * V].unflatten(1, (H, V)))
+    assert st == st2 == 0 and ctx.synchronize() == 0
+    assert torch.equal(out, want) and torch.equal(S, S2)
+    assert (wide[:, 0] == -7).all() and (wide[:, 1 + H * V:] == -7).all()
+
+
+@pytest.mark.parametrize("longest", [0, 1, 1 << 20])
+def test_longest_is_only_a_hint(hip, longest):
+    check(hip, inputs((1, 80, 3), 1, 1, 128, 32, BF16), longest=longest)
+
+
+def test_split_of_a_sequence(hip):
+    """A prompt in two chunks, the second from the first's state."""
+    k3x, ctx = hip
+    whole = inputs((150,), 1, 2, 128, 64, BF16)
+    out, S = check(hip, whole)
+    for cut in (1, 32, 77, 149):
+        a = {x: whole[x][:cut] if whole[x] is not None and x in "qkvbetagate" else whole[x]
+             for x in whole}
+        b = {x: whole[x][cut:] if whole[x] is not None and x in "qkvbetagate" else whole[x]
+             for x in whole}
+        a["lens"], b["lens"] = [cut], [150 - cut]
+        for part in (a, b):
+            part["offsets"] = torch.tensor([0, part["lens"][0]], dtype=torch.int32, device=DEV)
+        st, o1, S1 = call(hip, a)
+        b["state"] = S1
+        st2, o2, S2 = call(hip, b)
+        assert st == st2 == 0 and ctx.synchronize() == 0
+        want, Sw, tol, stol = definition(whole, 128 ** -0.5)
+        close(torch.cat([o1, o2]), want, tol, BF16)
+        close(S2, Sw, stol)
+
+
+@pytest.mark.parametrize("lens", [(2, 2), (40, 40)], ids=["short", "long"])
+def test_bad_offsets_and_slots_are_latched(hip, lens):
+    """Nothing of the sequences concerned is written."""
+    k3x, ctx = hip
+    s = inputs(lens, 1, 1, 64, 32)
+    T = sum(lens)
+    for cu in ([0, T + 1, T], [T, 1, T], [0, 1, T + 7]):
+        bad = dict(s, offsets=torch.tensor(cu, dtype=torch.int32, device=DEV))
+        st, out, S = call(hip, bad)
+        assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_STATE
+    for index in ([0, 2], [-1, 0], [1, 1]):
+        st, out, S = call(hip, s, slot_index=torch.tensor(index, dtype=torch.int32, device=DEV))
+        assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_STATE
+        if index == [1, 1]:
+            assert (S == -7).all() and (out == -7).all()
+    check(hip, s)
+
+
+@pytest.mark.parametrize("lens", [(4,), (70,)], ids=["short", "long"])
+@pytest.mark.parametrize("what", ["q", "k", "v", "beta", "gate"])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_values_that_are_not_finite_are_latched(hip, lens, what, value):
+    k3x, ctx = hip
+    s = inputs(lens, 1, 2, 64, 32)
+    s[what].view(lens[0], -1)[lens[0] - 2, 3 % s[what][0].numel()] = value
+    st, _, _ = call(hip, s)
+    assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_MXFP4
+    check(hip, inputs(lens, 1, 2, 64, 32))
+
+
+def test_growing_gate_is_latched(hip):
+    k3x, ctx = hip
+    for lens in ((4,), (70,)):
+        s = inputs(lens, 1, 1, 64, 32)
+        s["gate"][2, 0, 5] = 1e-3
+        st, _, _ = call(hip, s)
+        assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_MXFP4
+
+
+def test_no_tokens(hip):
+    """An empty batch: states are copied."""
+    k3x, ctx = hip
+    s = inputs((0, 0), 1, 1, 32, 16)
+    st, _, S = call(hip, s)
+    assert st == 0 and ctx.synchronize() == 0
+    assert torch.equal(S, s["state"])
+
+
+@pytest.mark.parametrize("lens", [(1,) * 5, (75, 40)], ids=["short", "long"])
+def test_captured(hip, lens):
+    """Captured once; replays on changed inputs equal eager calls, bit for bit."""
+    k3x, _ = hip
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ctx = k3x.Context(0)
+        own = (k3x, ctx)
+        s = inputs(lens, 1, 2, 128, 64, BF16)
+        p = k3x.make_delta_params(s["q"], s["k"], s["v"], len(lens), gate=s["gate"], scale=0.1,
+                                  norm_epsilon=EPS, longest=max(lens))
+        need = k3x.delta_workspace_bytes(p)
+        ws = torch.empty((need,), dtype=torch.uint8, device=DEV) if need else None
+        out, S = torch.zeros_like(s["v"]), torch.zeros_like(s["state"])
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            assert k3x.delta_rule(ctx, p, s["q"], s["k"], s["v"], s["beta"], out, gate=s["gate"],
+                                  offsets=s["offsets"], state_in=s["state"], state_out=S,
+                                  workspace=ws) == 0
+        for i in range(3):
+            s["v"].copy_(torch.randn(s["v"].shape, device=DEV, generator=gen(50 + i)))
+            graph.replay()
+            got = out.clone(), S.clone()
+            st, out2, S2 = call(own, s, scale=0.1)
+            assert st == 0 and ctx.synchronize() == 0
+            assert torch.equal(got[0], out2) and torch.equal(got[1], S2)
+        ctx.close()
+
+
+def test_two_calls_at_once(hip):
+    """Two contexts on two streams, a workspace each."""
+    k3x, _ = hip
+    s = [inputs((130, 60), 1, 2, 128, 128, BF16, seed=i) for i in range(2)]
+    want = [call(hip, x) for x in s]
+    assert hip[1].synchronize() == 0
+    streams = [torch.cuda.Stream() for _ in s]
+    torch.cuda.synchronize()
+    ctxs = []
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            ctxs.append(k3x.Context(0))
+    for _ in range(4):
+        got = []
+        for x, ctx, stream in zip(s, ctxs, streams):
+            with torch.cuda.stream(stream):
+                got.append(call((k3x, ctx), x))
+        for ctx in ctxs:
+            assert ctx.synchronize() == 0
+        for a, b in zip(got, want):
+            assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2])
+    for ctx in ctxs:
+        ctx.close()

@@ -1,0 +1,160 @@
+"""Refusals of the routing, delta rule and verification entry points: checked
+before the context or any device pointer is used, so a zeroed buffer stands in
+for both and no GPU is needed."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import k3x_amd as k3x  # noqa: E402
+
+CTX = C.create_string_buffer(1 << 16)
+P = 1 << 20  # a pointer that is never followed
+BAD = k3x.ERR_INVALID_EXTENT
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return k3x.load()
+
+
+def ctx():
+    return C.cast(CTX, C.c_void_p)
+
+
+ROUTE = dict(tokens=4, experts=64, top_k=8, dtype=0, scoring=0, renorm=0, routed_scale=1.0,
+             groups=8, top_groups=4, group_score=0, logits_stride=0)
+
+
+def route(lib, logits=P, bias=None, ids=P, weights=P, c=None, **kw):
+    p = k3x.RouteParams(**dict(ROUTE, **kw))
+    return lib.k3x_hip_route(ctx() if c is None else c, C.byref(p), logits, bias, ids, weights)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(tokens=0), dict(tokens=(1 << 20) + 1), dict(experts=0), dict(experts=4104), dict(top_k=0),
+    dict(top_k=33), dict(top_k=65, experts=4096), dict(dtype=2), dict(scoring=2), dict(renorm=3),
+    dict(routed_scale=math.nan), dict(routed_scale=math.inf), dict(groups=0), dict(groups=7),
+    dict(groups=128, experts=256), dict(top_groups=0), dict(top_groups=9), dict(group_score=2),
+    dict(logits_stride=63), dict(logits=None), dict(ids=None), dict(weights=None),
+    dict(logits=P + 2), dict(bias=P + 1), dict(ids=P + 2), dict(weights=P + 3),
+    dict(logits=P + 1, dtype=1)], ids=str)
+def test_route_refuses(lib, kw):
+    assert route(lib, **kw) == BAD
+
+
+def test_null_contexts(lib):
+    assert lib.k3x_hip_route(None, None, None, None, None, None) == BAD
+    assert lib.k3x_hip_route(ctx(), None, P, None, P, P) == BAD
+    assert lib.k3x_hip_delta_rule(None, None, *[None] * 12, 0) == BAD
+    assert lib.k3x_hip_verify_draft(None, None, *[None] * 9, 0) == BAD
+    assert lib.k3x_hip_delta_workspace(None) == 0
+    assert lib.k3x_hip_verify_workspace(None) == 0
+
+
+DELTA = dict(sequences=2, tokens=200, key_heads=2, value_heads=4, key_dim=128, value_dim=128,
+             dtype=1, gate=2, scale=1.0, norm_epsilon=1e-6, longest=0, slots=2, q_stride=0,
+             k_stride=0, v_stride=0, out_stride=0)
+DELTA_PTRS = dict(q=P, k=P, v=P, g=P, beta=P, offsets=P, limits=None, slot_index=None,
+                  state_in=1 << 30, state_out=1 << 32, out=P, workspace=1 << 40, bytes=1 << 40)
+
+
+def delta(lib, **kw):
+    p = k3x.DeltaParams(**{**DELTA, **{x: y for x, y in kw.items() if x in DELTA}})
+    a = {**DELTA_PTRS, **{x: y for x, y in kw.items() if x not in DELTA}}
+    return lib.k3x_hip_delta_rule(ctx(), C.byref(p), *a.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(sequences=0), dict(sequences=65536), dict(tokens=(1 << 24) + 1), dict(key_heads=0),
+    dict(key_heads=3), dict(value_heads=0), dict(value_heads=1026), dict(key_dim=0),
+    dict(key_dim=257), dict(value_dim=0), dict(value_dim=1025), dict(dtype=3), dict(gate=3),
+    dict(gate=0), dict(g=None), dict(scale=math.inf), dict(norm_epsilon=-1e-6),
+    dict(norm_epsilon=math.nan), dict(slots=0), dict(slots=1), dict(q_stride=255),
+    dict(k_stride=1), dict(v_stride=511), dict(out_stride=3), dict(q_stride=1 << 32),
+    dict(offsets=None, tokens=201), dict(q=None), dict(k=None), dict(v=None), dict(beta=None),
+    dict(out=None), dict(q=P + 1), dict(out=P + 1), dict(dtype=0, v=P + 2), dict(g=P + 2),
+    dict(beta=P + 1), dict(offsets=P + 2), dict(limits=P + 1), dict(slot_index=P + 3),
+    dict(state_in=P + 8), dict(state_out=P + 4),
+    dict(state_out=(1 << 30) + 16), dict(state_out=(1 << 30) - 2 * 4 * 128 * 128 * 4 + 16)],
+    ids=str)
+def test_delta_refuses(lib, kw):
+    assert delta(lib, **kw) == BAD
+
+
+def test_delta_workspace(lib):
+    """A call that needs a workspace refuses one that is missing, short or off alignment."""
+    p = k3x.DeltaParams(**dict(DELTA, tokens=4096, longest=2048))
+    need = k3x.delta_workspace_bytes(p)
+    assert lib.k3x_hip_delta_workspace(C.byref(k3x.DeltaParams(**dict(DELTA, key_dim=0)))) == 0
+    assert lib.k3x_hip_delta_workspace(C.byref(k3x.DeltaParams(**dict(DELTA, tokens=2)))) == 0
+    if need:
+        big = dict(tokens=4096, longest=2048)
+        assert delta(lib, workspace=None, **big) == BAD
+        assert delta(lib, bytes=need - 1, **big) == BAD
+        assert delta(lib, workspace=(1 << 40) + 128, **big) == BAD
+
+
+VERIFY = dict(sequences=2, drafts=4, vocab=1000, dtype=0, form=0, greedy=0, temperature=1.0,
+              row_stride=0)
+VERIFY_PTRS = dict(target=P, draft=P, tokens=P, draft_counts=None, accept_u=P, sample_u=P,
+                   accepted=P, out_tokens=P, workspace=P, bytes=1 << 40)
+
+
+def verify(lib, **kw):
+    p = k3x.VerifyParams(**{**VERIFY, **{x: y for x, y in kw.items() if x in VERIFY}})
+    a = {**VERIFY_PTRS, **{x: y for x, y in kw.items() if x not in VERIFY}}
+    return lib.k3x_hip_verify_draft(ctx(), C.byref(p), *a.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(sequences=0), dict(sequences=65536), dict(drafts=65), dict(vocab=0),
+    dict(vocab=(1 << 20) + 1), dict(dtype=2), dict(form=2), dict(greedy=2), dict(temperature=0.0),
+    dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf),
+    dict(row_stride=999), dict(target=None), dict(tokens=None), dict(accept_u=None),
+    dict(sample_u=None), dict(accepted=None), dict(out_tokens=None), dict(workspace=None),
+    dict(bytes=255), dict(workspace=P + 128), dict(target=P + 2), dict(draft=P + 1),
+    dict(tokens=P + 2), dict(draft_counts=P + 1), dict(accept_u=P + 2), dict(sample_u=P + 2),
+    dict(accepted=P + 1), dict(out_tokens=P + 2)], ids=str)
+def test_verify_refuses(lib, kw):
+    assert verify(lib, **kw) == BAD
+
+
+def test_binding_checks_tensors():
+    """The binding's own checks come before any pointer is taken."""
+    class Fake:
+        handle, lib = None, None
+
+    p = k3x.make_route_params(2, 8, 2)
+    x = torch.zeros((2, 8))
+    with pytest.raises(ValueError):
+        k3x.route(Fake, p, x.double(), torch.zeros((2, 2), dtype=torch.int32), torch.zeros((2, 2)))
+    with pytest.raises(ValueError):
+        k3x.route(Fake, p, x, torch.zeros((2, 2), dtype=torch.int64), torch.zeros((2, 2)))
+    with pytest.raises(ValueError):
+        k3x.route(Fake, p, x[:1], torch.zeros((2, 2), dtype=torch.int32), torch.zeros((2, 2)))
+    q = torch.zeros((3, 1, 4))
+    d = k3x.make_delta_params(q, q, q, 1)
+    with pytest.raises(ValueError):
+        k3x.delta_rule(Fake, d, q, q.bfloat16(), q, torch.zeros((3, 1)), q)
+    with pytest.raises(ValueError):
+        k3x.delta_rule(Fake, d, q, q, q, torch.zeros((3, 1)), q, offsets=torch.zeros(2))
+    t = torch.zeros((1, 3, 9))
+    v = k3x.make_verify_params(t)
+    ints = torch.zeros((1, 3), dtype=torch.int32)
+    with pytest.raises(ValueError):
+        k3x.verify_draft(Fake, v, t, ints, ints[0, :1], ints)
+
+
+def test_strides_of_rows():
+    """Rows that lie apart keep their distance; packed ones and single rows have none."""
+    wide = torch.zeros((4, 30))
+    assert k3x._row_stride(wide) == 0
+    assert k3x._row_stride(wide[:, 3:9]) == 30
+    assert k3x._row_stride(wide[:1, 3:9]) == 0
+    assert k3x._row_stride(wide[:, 2:26].unflatten(1, (2, 12))) == 30
+    assert not k3x._row_contiguous(wide.t())
+    assert not k3x._row_contiguous(wide.unflatten(1, (2, 15))[:, :, :5])
