@@ -433,7 +433,7 @@ typedef struct k3x_hip_delta_params {
                              kernels only: results hold whatever it says. */
     uint32_t slots;       /* states in state_in and state_out */
     /* Elements from token to token of q, k, v and out (q, k and v may be
-     * parts of one projection's rows); 0: packed. */
+     * parts of one projection's rows), 2^24 at most; 0: packed. */
     uint64_t q_stride, k_stride, v_stride, out_stride;
 } k3x_hip_delta_params;
 
