@@ -273,23 +273,36 @@ __device__ inline f32x4 mfma_pairs(const Pair8& a, const Pair8& b, f32x4 c) {
     return mfma_f16(a.hi, b.hi, c);
 }
 
-// What the scan needs of one chunk of one head.  T and Pq in the order of the
-// matrix operand: lane l, element j of tile r is row 16 r + l % 16, column
-// token_of(l / 16, j); the columns' order is that in which a lane holds the
-// rows of a product's result, so that results feed the next product as they
-// are.
+// What the scan needs of one chunk of one value head.  T and Pq in the order
+// of the matrix operand: lane l, element j of tile r is row 16 r + l % 16,
+// column token_of(l / 16, j); the columns' order is that in which a lane holds
+// the rows of a product's result, so that results feed the next product as
+// they are.
 struct ChunkRecord {
-    f16x8 T[2][2][64];   // [tile][hi, lo]; a row times row_t is c (I + L)^-1 beta
-    f16x8 P[2][2][64];   // Pq times kOperand
-    float key_mul[kChunk], query_mul[kChunk];  // element -> operand / kOperand
-    float row_r[kChunk];                       // of (k S) in V - c (P k) S
-    float row_o[kChunk], row_p[kChunk];        // of (q S) and (Pq U) in O
+    f16x8 T[2][2][64];           // [tile][hi, lo]; a row times row_t is c (I + L)^-1 beta
+    f16x8 P[2][2][64];           // Pq times kOperand
+    float row_r[kChunk];         // of (k S) in V - c (P k) S
+    float row_o[kChunk];         // of (q S) and
+    float row_p[kChunk];         //   (Pq U) in O
     float row_t[kChunk];
-    float row_u[kChunk];                       // head gates: of U in the state's update
-    float unused[kChunk];
-    float total[2][128];  // decay over tokens 0 .. 15 and 16 .. 31, by channel
+    float row_u[kChunk];         // head gates: of U in the state's update
+    float unused[3 * kChunk];
+    float decay[128];            // of the state over the chunk, by channel
+    float unused2[128];
 };
-static_assert(sizeof(ChunkRecord) == 10240, "chunk record");
+static_assert(sizeof(ChunkRecord) == 10240, "ten loads of a wave");
+
+// Its keys and queries as operands, times kOperand: hi and, where they need
+// one, lo.  With a decay a channel they carry it (P k, P q and D_31 k, of a
+// value head); with one a head they are the elements times a power of two (of a
+// key head), 8 or 11 bits, which need no lo.
+template <bool LO, int KB>
+struct ChunkOperands {
+    static constexpr int kParts = LO ? 2 : 1;
+    f16x8 K[kParts][2][KB][64];    // [tile of tokens][channels by 32]
+    f16x8 Q[kParts][2][KB][64];
+    f16x8 Kt[kParts][2 * KB][64];  // [channels by 16][tokens]
+};
 
 __device__ inline uint32_t token_of(uint32_t q, uint32_t j) { return 4 * q + (j & 3) + 4 * (j & 4); }
 
@@ -350,20 +363,6 @@ __device__ inline Vec4<E> load4(const E* row, uint32_t c, uint32_t n, bool vec) 
     return y;
 }
 
-// Eight elements from c on in fp32, 0 past the row's end or where it is not
-// live; z takes a NaN where one is not finite.
-template <uint32_t DT>
-__device__ inline void load8(const typename Elem<DT>::type* row, uint32_t c, uint32_t n, bool live,
-                             bool vec, float (&y)[8], float& z) {
-    const auto a = load4(row, c, n, vec), b = load4(row, c + 4, n, vec);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float x = Elem<DT>::load(j < 4 ? a[j & 3] : b[j & 3]);
-        y[j] = live && c + j < n ? x : 0.0f;
-        z = __builtin_fmaf(y[j], 0.0f, z);
-    }
-}
-
 // Which sequence and chunk of it has record slot x: sequence n's chunks begin at
 // slot offsets[n] / 32 + n, which leaves room for each one's last part.
 __device__ inline uint32_t first_slot(const DeltaArgs& a, uint32_t n) {
@@ -381,127 +380,247 @@ __device__ inline uint32_t sequence_of_slot(const DeltaArgs& a, uint32_t x) {
     return lo;
 }
 
-// LDS written before is seen after, by the whole workgroup; loads from global
-// memory stay in flight across it.
-__device__ inline void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+// A chunk's place: its sequence, first token and slot.
+struct ChunkPlace {
+    Sequence sq;
+    uint32_t first;
+};
+
+__device__ inline bool find_chunk(const DeltaArgs& a, uint32_t slot, ChunkPlace* c) {
+    const uint32_t n = sequence_of_slot(a, slot), slot0 = first_slot(a, n);
+    if (find_sequence(a, n, &c->sq)) return false;  // latched by the scan
+    if (slot < slot0 || slot - slot0 >= (c->sq.len + kChunk - 1) / kChunk) return false;
+    c->first = (slot - slot0) * kChunk;
+    return true;
 }
 
-// (I + L)^-1 and Pq of one chunk of one head, by two waves: wave w has tokens
-// 16 w .. + 15, lane l token l % 16 and the channels 32 b + 8 (l / 16) .. + 7.
-//
-// A decay a channel does not factor over (i, j) without overflow, so a tile's
-// lower triangle is made level by level: pairs (i, j) whose highest differing
-// bit is b have D_ij = pre_b(i) suf_b(j), the decays up to the border between
-// i's and j's blocks of 2^b tokens and from there on, both at most 1.  Each
-// level is one product of the whole tile, of which its own pairs are kept.
-// pre, suf and a block's total come from the level before by one exchange over
-// the lanes of a row.  A decay a head is one factor exp(G_i - G_j) a pair, G
-// summed in double.
-template <uint32_t DT, bool CHANNEL, int KB>
-__global__ __launch_bounds__(128) void delta_prep_kernel(DeltaArgs a, ChunkRecord* records,
-                                                         bool vec) {
-    typedef typename Elem<DT>::type E;
-    constexpr int kLevels = CHANNEL ? 4 : 1;
-    __shared__ float Ls[kChunk][36], Ps[kChunk][36];
-    __shared__ Pair8 cross[KB][64];
-    __shared__ float beta_s[kChunk], c_s[kChunk];
-    __shared__ double G_s[kChunk];  // head gates: log decay from the tile's start
-    const uint32_t h = blockIdx.x % a.H, slot = blockIdx.x / a.H;
-    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
-    const uint32_t n = sequence_of_slot(a, slot);
-    Sequence sq;
-    if (find_sequence(a, n, &sq)) return;  // latched by the scan
-    const uint32_t slot0 = first_slot(a, n);
-    if (slot < slot0 || slot - slot0 >= (sq.len + kChunk - 1) / kChunk) return;
-    const uint32_t first = (slot - slot0) * kChunk;
-    ChunkRecord* rec = records + (size_t)slot * a.H + h;
-    const uint32_t t = 16 * w + m, hk = h / (a.H / a.Hk);
-    const bool live = first + t < sq.len;
-    const size_t row = (size_t)sq.begin + first + (live ? t : 0);
-    float z = 0.0f;  // NaN once an input is not finite
-    bool wrong = false;
-    float q[KB][8], k[KB][8];
+// What a wave sees of another lane's LDS writes, in order.
+__device__ inline void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
+typedef float Tile32[kChunk][36];  // rows of 16-byte alignment that spread over the banks
+
+// T of a chunk from L (strictly lower triangular; overwritten), by one wave in
+// fp32: the inverses of the two diagonal tiles by forward substitution, a
+// column a lane, and -T22 L21 T11 below them.
+__device__ inline void write_inverse(Tile32& L, const float* c, const float* beta,
+                                     ChunkRecord* rec) {
+    const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const uint32_t half = 16 * (g & 1);
+    float x[16];
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-        const uint32_t c = 32 * b + 8 * g;
-        load8<DT>(static_cast<const E*>(a.q) + row * a.qs + (size_t)hk * a.K, c, a.K, live, vec,
-                  q[b], z);
-        load8<DT>(static_cast<const E*>(a.k) + row * a.ks + (size_t)hk * a.K, c, a.K, live, vec,
-                  k[b], z);
+    for (int i = 0; i < 16; ++i) {
+        float s = (uint32_t)i == m ? 1.0f : 0.0f;
+#pragma unroll
+        for (int j = 0; j < i; ++j) s = __builtin_fmaf(-L[half + i][half + j], x[j], s);
+        x[i] = s;
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // not every row of L at once
     }
-    const float beta = live ? a.beta[row * a.H + h] : 0.0f;
-    z = __builtin_fmaf(beta, 0.0f, z);
-    // Operands' scales: the norm, or a power of two.
-    float qd, qu, kd, ku, qn = 1.0f, kn = 1.0f;
-    {
+    wave_sync();
+    if (g < 2) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) L[half + i][half + m] = x[i];
+    }
+    wave_sync();
+    // Rows 4 g + i of a result are rows k = 4 g + s of the next product's right
+    // operand; its left operand takes the columns in the same order.
+    f32x4 y = {}, z = {};
+    const f32x4 l21 = *reinterpret_cast<const f32x4*>(&L[16 + m][4 * g]);
+    const f32x4 t22 = *reinterpret_cast<const f32x4*>(&L[16 + m][16 + 4 * g]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        y = __builtin_amdgcn_mfma_f32_16x16x4f32(l21[i], L[4 * g + i][m], y, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        z = __builtin_amdgcn_mfma_f32_16x16x4f32(t22[i], y[i], z, 0, 0, 0);
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        L[16 + 4 * g + i][m] = -z[i];
+        L[4 * g + i][16 + m] = 0.0f;
+    }
+    wave_sync();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        float e[8], most = 0.0f, down, up;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t t = token_of(g, j);
+            e[j] = L[16 * r + m][t] * c[16 * r + m] * beta[t];
+            most = fmaxf(most, fabsf(e[j]));
+        }
+        unit_scale(max_groups(most), &down, &up);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] *= down * kOperand;
+        const Pair8 p = split8(e);
+        rec->T[r][0][lane] = p.hi;
+        rec->T[r][1][lane] = p.lo;
+        if (g == 0) rec->row_t[16 * r + m] = up / kOperand;
+    }
+}
+
+__device__ inline void write_scores(const Tile32& P, ChunkRecord* rec) {
+    const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = P[16 * r + m][token_of(g, j)];
+        const Pair8 p = split8(e);
+        rec->P[r][0][lane] = p.hi;
+        rec->P[r][1][lane] = p.lo;
+    }
+}
+
+// A wave's tile of 16 tokens (lane: token l % 16) of keys and queries, the
+// channels in the operand's order: element j of part b is channel
+// 32 b + token_of(l / 16, j).
+template <uint32_t DT, int KB>
+struct TokenRows {
+    typedef typename Elem<DT>::type E;
+    Vec4<E> q[KB][2], k[KB][2];
+    float qd, qu, kd, ku;  // 2^-e and 2^e of the largest element
+    float qn, kn;          // 1 / norm
+
+    // q and k: the rows' heads; z takes a NaN where an element is not finite.
+    __device__ inline void load(const DeltaArgs& a, const E* qr, const E* kr, uint32_t g,
+                                bool live, bool vec, float& z) {
         float qm = 0.0f, km = 0.0f, qq = 0.0f, kk = 0.0f;
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                qm = fmaxf(qm, fabsf(q[b][j]));
-                km = fmaxf(km, fabsf(k[b][j]));
-                qq = __builtin_fmaf(q[b][j], q[b][j], qq);
-                kk = __builtin_fmaf(k[b][j], k[b][j], kk);
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t c = 32 * b + 16 * x + 4 * g;
+                q[b][x] = load4(qr, c, a.K, vec);
+                k[b][x] = load4(kr, c, a.K, vec);
             }
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (!live || 32 * b + 16 * x + 4 * g + j >= a.K)
+                        q[b][x][j] = k[b][x][j] = E{};
+                    const float y = Elem<DT>::load(q[b][x][j]), w = Elem<DT>::load(k[b][x][j]);
+                    z = __builtin_fmaf(y, 0.0f, z);
+                    z = __builtin_fmaf(w, 0.0f, z);
+                    qm = fmaxf(qm, fabsf(y));
+                    km = fmaxf(km, fabsf(w));
+                    qq = __builtin_fmaf(y, y, qq);
+                    kk = __builtin_fmaf(w, w, kk);
+                }
         unit_scale(max_groups(qm), &qd, &qu);
         unit_scale(max_groups(km), &kd, &ku);
         qn = 1.0f / sqrtf(sum_groups(qq) + a.eps);
         kn = 1.0f / sqrtf(sum_groups(kk) + a.eps);
     }
+    __device__ inline void part(int b, float qs, float ks, float (&x)[8], float (&y)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[j] = Elem<DT>::load(q[b][j / 4][j % 4]) * qs;
+            y[j] = Elem<DT>::load(k[b][j / 4][j % 4]) * ks;
+        }
+    }
+};
+
+// Keys by channel, for the state's update: a wave's tokens into `tr` (a row a
+// channel), and from there, once all are in, as operands.
+template <int KB>
+using ByChannel = _Float16[32 * KB][kChunk + 8];
+
+template <int KB>
+__device__ inline void put_by_channel(ByChannel<KB>& tr, int b, uint32_t g, uint32_t token,
+                                      const f16x8& x) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) tr[32 * b + token_of(g, j)][token] = x[j];
+}
+
+template <int KB>
+__device__ inline void write_by_channel(const ByChannel<KB>& tr, uint32_t wave, uint32_t waves,
+                                        f16x8 (&out)[2 * KB][64]) {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    for (uint32_t t = wave; t < 2 * KB; t += waves) {
+        const f16x4 lo = *reinterpret_cast<const f16x4*>(&tr[16 * t + m][4 * g]);
+        const f16x4 hi = *reinterpret_cast<const f16x4*>(&tr[16 * t + m][16 + 4 * g]);
+        out[t][lane] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+}
+
+// One chunk of one head under a decay a channel, by two waves of 16 tokens.
+//
+// Such a decay does not factor over (i, j) without overflow, so a tile's lower
+// triangle is made level by level: pairs (i, j) whose highest differing bit is
+// b have D_ij = pre_b(i) suf_b(j), the decays up to the border between i's and
+// j's blocks of 2^b tokens and from there on, both at most 1.  Each level is
+// one product of the whole tile, of which its own pairs are kept.  pre, suf and
+// a block's total come from the level before by one exchange over the lanes of
+// a row; after the last they are those of the tile.
+template <uint32_t DT, int KB>
+__global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
+    DeltaArgs a, ChunkRecord* records, ChunkOperands<true, KB>* operands, bool vec) {
+    typedef typename Elem<DT>::type E;
+    __shared__ Tile32 Ls, Ps;
+    __shared__ Pair8 cross[KB][64];
+    __shared__ float total[2][32 * KB];
+    __shared__ __attribute__((aligned(16))) ByChannel<KB> tr[2];
+    __shared__ float beta_s[kChunk], c_s[kChunk];
+    const uint32_t h = blockIdx.x % a.H, slot = blockIdx.x / a.H;
+    const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
+    ChunkPlace place;
+    if (!find_chunk(a, slot, &place)) return;
+    ChunkRecord* rec = records + (size_t)slot * a.H + h;
+    ChunkOperands<true, KB>* ops = operands + (size_t)slot * a.H + h;
+    const uint32_t t = 16 * w + m, hk = h / (a.H / a.Hk);
+    const bool live = place.first + t < place.sq.len;
+    const size_t row = (size_t)place.sq.begin + place.first + (live ? t : 0);
+    float z = 0.0f;  // NaN once an input is not finite
+    bool wrong = false;
+    TokenRows<DT, KB> rows;
+    rows.load(a, static_cast<const E*>(a.q) + row * a.qs + (size_t)hk * a.K,
+              static_cast<const E*>(a.k) + row * a.ks + (size_t)hk * a.K, g, live, vec, z);
+    const float beta = live ? a.beta[row * a.H + h] : 0.0f;
+    z = __builtin_fmaf(beta, 0.0f, z);
     const bool norm = a.eps > 0.0f;
-    const float kmul = norm ? kn : kd, qmul = norm ? qn : qd;
-    const float c_up = norm ? 1.0f : ku, o_up = a.scale * (norm ? 1.0f : qu);
+    const float kmul = (norm ? rows.kn : rows.kd) * kOperand;
+    const float qmul = (norm ? rows.qn : rows.qd) * kOperand;
+    const float c_up = norm ? 1.0f : rows.ku, o_up = a.scale * (norm ? 1.0f : rows.qu);
     if (lane < 16) {
         beta_s[t] = beta;
         c_s[t] = c_up;
+        rec->row_r[t] = c_up / (kOperand * kOperand);
+        rec->row_o[t] = o_up / (kOperand * kOperand);
+        rec->row_p[t] = o_up / kOperand;
     }
-    if (!CHANNEL) {
-        const float gate = live && a.gate ? a.gate[row * a.H + h] : 0.0f;
-        wrong |= !(gate <= 0.0f);
-        double G = (double)fmaxf(gate, -128.0f);  // exp of less is 0 in fp32
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            const double o = __shfl_up(G, d, 16);
-            if (m >= (uint32_t)d) G += o;
-        }
-        if (lane < 16) G_s[t] = G;
-    }
-    f32x4 accL[kLevels] = {}, accP[kLevels] = {};
-    Pair8 krow[KB], qrow[KB];  // wave 1: rows of the tile below the diagonal
+    f32x4 accL[4] = {}, accP[4] = {}, l21 = {}, p21 = {};
     float diag = 0.0f;
+    const float* gr = a.gate + (row * a.H + h) * a.K;
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-        float kk[8], qq[8], x[8];
+        float kk[8], qq[8], x[8], pre[8], suf[8], tot[8];
+        rows.part(b, qmul, kmul, qq, kk);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            kk[j] = k[b][j] * kmul * kOperand;
-            qq[j] = q[b][j] * qmul * kOperand;
-            diag = __builtin_fmaf(kk[j], qq[j], diag);
-        }
-        if (!CHANNEL) {
-            krow[b] = split8(kk);
-            qrow[b] = split8(qq);
-            accL[0] = mfma_pairs(krow[b], krow[b], accL[0]);
-            accP[0] = mfma_pairs(qrow[b], krow[b], accP[0]);
-            if (w == 0) cross[b][lane] = krow[b];
-            continue;
-        }
-        float pre[8], suf[8], tot[8], gate[8], any = 0.0f;
-        const uint32_t c = 32 * b + 8 * g;
-        load8<K3X_DTYPE_F32>(a.gate + (row * a.H + h) * a.K, c, a.K, live, vec, gate, any);
+        for (int y = 0; y < 2; ++y) {
+            const uint32_t c = 32 * b + 16 * y + 4 * g;
+            const f32x4 gate = load4(gr, c, a.K, vec);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            wrong |= !(gate[j] <= 0.0f);
-            pre[j] = tot[j] = exp_decay(gate[j]);
-            suf[j] = 1.0f;
+            for (int j = 0; j < 4; ++j) {
+                const float e = live && c + j < a.K ? gate[j] : 0.0f;
+                wrong |= !(e <= 0.0f);
+                pre[4 * y + j] = tot[4 * y + j] = exp_decay(e);
+                suf[4 * y + j] = 1.0f;
+            }
         }
 #pragma unroll
-        for (int level = 0; level < kLevels; ++level) {
+        for (int j = 0; j < 8; ++j) diag = __builtin_fmaf(kk[j], qq[j], diag);
+#pragma unroll
+        for (int level = 0; level < 4; ++level) {
             const bool bit = m >> level & 1;
             float f[8];
 #pragma unroll
@@ -528,151 +647,227 @@ __global__ __launch_bounds__(128) void delta_prep_kernel(DeltaArgs a, ChunkRecor
                 tot[j] *= o;
             }
         }
+        // Tile 0's keys up to the border of the tiles, for tile 1.
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = kk[j] * (w ? pre[j] : suf[j]);
-        krow[b] = split8(x);
-        if (w == 0) {
-            cross[b][lane] = krow[b];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = qq[j] * pre[j];
-            qrow[b] = split8(x);
-        }
+        for (int j = 0; j < 8; ++j) suf[j] *= kk[j];
+        if (w == 0) cross[b][lane] = split8(suf);
         if (m == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) rec->total[w][c + j] = tot[j];
+            for (int j = 0; j < 8; ++j) total[w][32 * b + token_of(g, j)] = tot[j];
+        }
+        __syncthreads();
+        float other[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) other[j] = total[1 - w][32 * b + token_of(g, j)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            kk[j] *= pre[j];
+            qq[j] *= pre[j];
+        }
+        Pair8 kp = split8(kk), qp = split8(qq);
+        if (w == 1) {
+            const Pair8 before = cross[b][lane];
+            l21 = mfma_pairs(kp, before, l21);
+            p21 = mfma_pairs(qp, before, p21);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                kk[j] *= other[j];
+                qq[j] *= other[j];
+            }
+            kp = split8(kk);
+            qp = split8(qq);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) suf[j] *= other[j];
+        }
+        ops->K[0][w][b][lane] = kp.hi;
+        ops->K[1][w][b][lane] = kp.lo;
+        ops->Q[0][w][b][lane] = qp.hi;
+        ops->Q[1][w][b][lane] = qp.lo;
+        const Pair8 sp = split8(suf);
+        put_by_channel<KB>(tr[0], b, g, t, sp.hi);
+        put_by_channel<KB>(tr[1], b, g, t, sp.lo);
+        if (w == 0 && m == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rec->decay[32 * b + token_of(g, j)] = tot[j] * other[j];
         }
     }
     diag = sum_groups(diag);
     if (wrong || z != z) latch(a.status, K3X_ERR_INVALID_MXFP4);
+    // Row 4 g + i and column m of the wave's tile on the diagonal.
+    const float un = 1.0f / (kOperand * kOperand);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t r = 4 * g + i, ti = 16 * w + r, differ = r ^ m;
+        float l = accL[0][i], p = accP[0][i];
+#pragma unroll
+        for (int level = 1; level < 4; ++level)
+            if (differ >= 1u << level) {
+                l = accL[level][i];
+                p = accP[level][i];
+            }
+        Ls[ti][t] = r > m ? l * un * beta_s[ti] * c_s[ti] * c_s[t] : 0.0f;
+        Ps[ti][t] = (r > m ? p : r == m ? diag : 0.0f) / kOperand;
+        if (w == 0) {
+            Ps[r][16 + m] = 0.0f;
+        } else {
+            Ls[ti][m] = l21[i] * un * beta_s[ti] * c_s[ti] * c_s[m];
+            Ps[ti][m] = p21[i] / kOperand;
+        }
+    }
+    __syncthreads();
+    write_by_channel<KB>(tr[0], w, 2, ops->Kt[0]);
+    write_by_channel<KB>(tr[1], w, 2, ops->Kt[1]);
+    if (w == 0) write_inverse(Ls, c_s, beta_s, rec);
+    else write_scores(Ps, rec);
+}
+
+// One chunk of one key head under a decay a value head, by two waves of 16
+// tokens: the products of keys and queries once, and for each value head (a
+// wave every other one) its factors exp(G_i - G_j), G the log decays summed in
+// double.
+template <uint32_t DT, int KB>
+__global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
+    DeltaArgs a, ChunkRecord* records, ChunkOperands<DT == K3X_DTYPE_F32, KB>* operands,
+    bool vec) {
+    typedef typename Elem<DT>::type E;
+    constexpr bool LO = DT == K3X_DTYPE_F32;
+    __shared__ Tile32 Gk, Gq, work[2];
+    __shared__ Pair8 cross[KB][64];
+    __shared__ __attribute__((aligned(16))) ByChannel<KB> tr[LO ? 2 : 1];
+    __shared__ float c_s[kChunk], rk_s[kChunk], rq_s[kChunk], o_s[kChunk], beta_s[2][kChunk];
+    __shared__ double G_s[2][kChunk];
+    const uint32_t hk = blockIdx.x % a.Hk, slot = blockIdx.x / a.Hk, per = a.H / a.Hk;
+    const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
+    ChunkPlace place;
+    if (!find_chunk(a, slot, &place)) return;
+    ChunkOperands<LO, KB>* ops = operands + (size_t)slot * a.Hk + hk;
+    const uint32_t t = 16 * w + m;
+    const bool live = place.first + t < place.sq.len;
+    const size_t row0 = (size_t)place.sq.begin + place.first, row = row0 + (live ? t : 0);
+    float z = 0.0f;  // NaN once an input is not finite
+    bool wrong = false;
+    TokenRows<DT, KB> rows;
+    rows.load(a, static_cast<const E*>(a.q) + row * a.qs + (size_t)hk * a.K,
+              static_cast<const E*>(a.k) + row * a.ks + (size_t)hk * a.K, g, live, vec, z);
+    const bool norm = a.eps > 0.0f;
+    if (lane < 16) {
+        c_s[t] = norm ? 1.0f : rows.ku;
+        rk_s[t] = norm ? rows.kn * rows.ku : 1.0f;
+        rq_s[t] = norm ? rows.qn * rows.qu : 1.0f;
+        o_s[t] = a.scale * (norm ? 1.0f : rows.qu);
+    }
+    f32x4 accK = {}, accQ = {};
+    Pair8 kp[KB], qp[KB];
+    float diag = 0.0f;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+        float kk[8], qq[8];
+        rows.part(b, rows.qd * kOperand, rows.kd * kOperand, qq, kk);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) diag = __builtin_fmaf(kk[j], qq[j], diag);
+        kp[b] = split8(kk);
+        qp[b] = split8(qq);
+        accK = mfma_pairs(kp[b], kp[b], accK);
+        accQ = mfma_pairs(qp[b], kp[b], accQ);
+        if (w == 0) cross[b][lane] = kp[b];
+        ops->K[0][w][b][lane] = kp[b].hi;
+        ops->Q[0][w][b][lane] = qp[b].hi;
+        put_by_channel<KB>(tr[0], b, g, t, kp[b].hi);
+        if (LO) {
+            ops->K[LO ? 1 : 0][w][b][lane] = kp[b].lo;
+            ops->Q[LO ? 1 : 0][w][b][lane] = qp[b].lo;
+            put_by_channel<KB>(tr[LO ? 1 : 0], b, g, t, kp[b].lo);
+        }
+    }
+    diag = sum_groups(diag);
     __syncthreads();
     const float un = 1.0f / (kOperand * kOperand);
-    if (lane < 16) {
-        const float rk = CHANNEL || !norm ? 1.0f : kn * ku, rq = CHANNEL || !norm ? 1.0f : qn * qu;
-        float p = 1.0f, s = 1.0f;
-        if (!CHANNEL) {
-            const double G = G_s[t] + (w ? G_s[15] : 0.0), all = G_s[15] + G_s[31];
-            p = (float)exp(G);
-            s = (float)exp(all - G);
-            if (t == 31) rec->total[0][0] = p;
+    f32x4 k21 = {}, q21 = {};
+    if (w == 1) {
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const Pair8 before = cross[b][lane];
+            k21 = mfma_pairs(kp[b], before, k21);
+            q21 = mfma_pairs(qp[b], before, q21);
         }
-        // 0 past the sequence's end, where the scan reads another row.
-        rec->key_mul[t] = !live ? 0.0f : CHANNEL ? kmul : kd;
-        rec->query_mul[t] = !live ? 0.0f : CHANNEL ? qmul : qd;
-        rec->row_r[t] = c_up * un * p * rk;
-        rec->row_o[t] = o_up * un * p * rq;
-        rec->row_p[t] = o_up / kOperand;
-        rec->row_u[t] = s * rk;
     }
-    // Row 4 g + i and column m of the wave's tile on the diagonal.
+    // Products of the normalised rows: row 4 g + i, column m.
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t r = 4 * g + i, ti = 16 * w + r;
-        float l = accL[0][i], p = accP[0][i];
-        if (CHANNEL) {
-            const uint32_t differ = r ^ m;
-#pragma unroll
-            for (int level = 1; level < kLevels; ++level)
-                if (differ >= 1u << level) {
-                    l = accL[level][i];
-                    p = accP[level][i];
-                }
-        } else {
-            const float f = r > m ? (float)exp(G_s[ti] - G_s[t]) : 1.0f;
-            l *= f;
-            p *= f;
-        }
-        Ls[ti][t] = r > m ? l * un * beta_s[ti] * c_s[ti] * c_s[t] : 0.0f;
-        Ps[ti][t] = (r > m ? p : r == m ? diag : 0.0f) / kOperand;
-        if (w == 0) Ps[r][16 + m] = 0.0f;
-    }
-    if (w == 1) {  // rows 16 .. 31, columns 0 .. 15
-        f32x4 l = {}, p = {};
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            const Pair8 kp = cross[b][lane];
-            l = mfma_pairs(krow[b], kp, l);
-            p = mfma_pairs(qrow[b], kp, p);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t ti = 16 + 4 * g + i;
-            const float f = CHANNEL ? 1.0f : (float)exp(G_s[ti] + (G_s[15] - G_s[m]));
-            Ls[ti][m] = l[i] * f * un * beta_s[ti] * c_s[ti] * c_s[m];
-            Ps[ti][m] = p[i] * f / kOperand;
+        Gk[ti][t] = accK[i] * un * rk_s[ti] * rk_s[t];
+        Gq[ti][t] = (r == m ? diag : accQ[i]) * un * rq_s[ti] * rk_s[t];
+        if (w == 1) {
+            Gk[ti][m] = k21[i] * un * rk_s[ti] * rk_s[m];
+            Gq[ti][m] = q21[i] * un * rq_s[ti] * rk_s[m];
         }
     }
     __syncthreads();
-    if (w == 1) {
+    write_by_channel<KB>(tr[0], w, 2, ops->Kt[0]);
+    if (LO) write_by_channel<KB>(tr[LO ? 1 : 0], w, 2, ops->Kt[LO ? 1 : 0]);
+    for (uint32_t v = w; v < per; v += 2) {
+        const uint32_t h = hk * per + v;
+        ChunkRecord* rec = records + (size_t)slot * a.H + h;
+        const uint32_t tok = lane & 31;
+        const bool in = place.first + tok < place.sq.len;
+        const size_t at = (row0 + (in ? tok : 0)) * a.H + h;
+        const float beta = in ? a.beta[at] : 0.0f, gate = in && a.gate ? a.gate[at] : 0.0f;
+        z = __builtin_fmaf(beta, 0.0f, z);
+        wrong |= !(gate <= 0.0f);
+        double G = (double)fmaxf(gate, -128.0f);  // exp of less is 0 in fp32
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = Ps[16 * r + m][token_of(g, j)];
-            const Pair8 s = split8(x);
-            rec->P[r][0][lane] = s.hi;
-            rec->P[r][1][lane] = s.lo;
+        for (int d = 1; d < 32; d <<= 1) {
+            const double o = __shfl_up(G, d, 32);
+            if (tok >= (uint32_t)d) G += o;
         }
-        return;
-    }
-    // Column lane % 32 of (I + L)^-1 by forward substitution, in fp32.
-    const uint32_t col = lane & 31;
-    float x[kChunk];
-#pragma unroll
-    for (int i = 0; i < (int)kChunk; ++i) {
-        float s = (uint32_t)i == col ? 1.0f : 0.0f;
-#pragma unroll
-        for (int j = 0; j < i; ++j) s = __builtin_fmaf(-Ls[i][j], x[j], s);
-        x[i] = s;
-    }
-    if (lane < 32) {
-        const float right = beta_s[col];
-#pragma unroll
-        for (int i = 0; i < (int)kChunk; ++i) Ls[i][col] = x[i] * c_s[i] * right;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        float y[8], most = 0.0f, down, up;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            y[j] = Ls[16 * r + m][token_of(g, j)];
-            most = fmaxf(most, fabsf(y[j]));
+        const double all = __shfl(G, 31, 32);
+        wave_sync();  // the head before is done with its LDS
+        if (lane < 32) {
+            beta_s[w][tok] = beta;
+            G_s[w][tok] = G;
+            const float p = exp_decay((float)G), s = exp_decay((float)(all - G));
+            rec->row_r[tok] = c_s[tok] * un * p * rk_s[tok];
+            rec->row_o[tok] = o_s[tok] * un * p * rq_s[tok];
+            rec->row_p[tok] = o_s[tok] / kOperand;
+            rec->row_u[tok] = s * rk_s[tok];
         }
-        unit_scale(max_groups(most), &down, &up);
+        const float whole = exp_decay((float)all);
+        rec->decay[lane] = whole;
+        rec->decay[64 + lane] = whole;
+        wave_sync();
+        auto factor = [&](uint32_t i, uint32_t j) {
+            return i >= j ? exp_decay((float)(G_s[w][i] - G_s[w][j])) : 0.0f;
+        };
+        // Pq first, through the same tile.
+        Tile32& tile = work[w];
+        float f[3][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] *= down * kOperand;
-        const Pair8 s = split8(y);
-        rec->T[r][0][lane] = s.hi;
-        rec->T[r][1][lane] = s.lo;
-        if (g == 0) rec->row_t[16 * r + m] = up / kOperand;
+        for (int x = 0; x < 3; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t ri = 4 * g + i + (x ? 16 : 0), cj = m + (x == 2 ? 16 : 0);
+                f[x][i] = factor(ri, cj);
+                tile[ri][cj] = Gq[ri][cj] * f[x][i] * kOperand;
+                if (x == 0) tile[ri][16 + m] = 0.0f;
+            }
+        wave_sync();
+        write_scores(tile, rec);
+        wave_sync();
+#pragma unroll
+        for (int x = 0; x < 3; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t ri = 4 * g + i + (x ? 16 : 0), cj = m + (x == 2 ? 16 : 0);
+                tile[ri][cj] = ri > cj ? Gk[ri][cj] * f[x][i] * beta_s[w][ri] * c_s[ri] * c_s[cj]
+                                       : 0.0f;
+            }
+        wave_sync();
+        write_inverse(tile, c_s, beta_s[w], rec);
     }
-}
-
-// One chunk's operands in LDS, in the order of the matrix operand: hi and,
-// where the terms need it, lo.
-template <uint32_t DT, bool CHANNEL, int KB>
-struct ScanTerms {
-    // Keys and queries under a head's decay are the elements themselves times a
-    // power of two: 8 and 11 bits are f16 without rest.
-    static constexpr bool kKeyLo = CHANNEL || DT == K3X_DTYPE_F32;
-    struct Chunk {
-        f16x8 K[kKeyLo ? 2 : 1][2][KB][64];    // [tile of tokens][channels]: decayed keys
-        f16x8 Q[kKeyLo ? 2 : 1][2][KB][64];
-        f16x8 Kt[kKeyLo ? 2 : 1][2 * KB][64];  // [tile of channels][tokens]: keys for the state
-        f16x8 T[2][2][64], P[2][2][64];        // as in the chunk's record
-        float row_r[kChunk], row_o[kChunk], row_p[kChunk], row_t[kChunk], row_u[kChunk];
-        float decay[32 * KB];
-    };
-};
-
-// Product over the lanes of a row up to and with the lane's own.
-__device__ inline float scan_row(float x) {
-    x *= dpp<0x111>(x, 1.0f);  // row_shr
-    x *= dpp<0x112>(x, 1.0f);
-    x *= dpp<0x114>(x, 1.0f);
-    return x * dpp<0x118>(x, 1.0f);
+    if (wrong || z != z) latch(a.status, K3X_ERR_INVALID_MXFP4);
 }
 
 // Rows of a tensor from `base` on as a buffer: 32 at most, of `width` bytes
@@ -699,16 +894,6 @@ __device__ inline E load_one(__amdgpu_buffer_rsrc_t r, uint32_t voffset, uint32_
 }
 
 template <typename E>
-__device__ inline Vec4<E> load_four(__amdgpu_buffer_rsrc_t r, uint32_t voffset, uint32_t soffset) {
-    if constexpr (sizeof(E) == 4)
-        return __builtin_bit_cast(Vec4<E>,
-                                  __builtin_amdgcn_raw_buffer_load_b128(r, voffset, soffset, 0));
-    else
-        return __builtin_bit_cast(Vec4<E>,
-                                  __builtin_amdgcn_raw_buffer_load_b64(r, voffset, soffset, 0));
-}
-
-template <typename E>
 __device__ inline void store_one(E x, __amdgpu_buffer_rsrc_t r, uint32_t voffset,
                                  uint32_t soffset) {
     if constexpr (sizeof(E) == 4)
@@ -719,22 +904,39 @@ __device__ inline void store_one(E x, __amdgpu_buffer_rsrc_t r, uint32_t voffset
                                               0);
 }
 
-// Walks one sequence's chunks for 64 value columns of one head.  Waves 0 .. 3
-// hold 16 columns of the state each, as the results of eight products (rows by
+// Walks one sequence's chunks for 16 W value columns of one head.  Each of the W
+// waves holds 16 columns of the state as the results of 2 KB products (rows by
 // 16): row 16 t + 4 (l / 16) + i and column l % 16 in register i of tile t of
-// lane l, and split it into the next products' operands where it is.  Waves 4
-// .. 7 make the next chunk's key and query operands meanwhile: two of them a
-// tile of 16 tokens each, lane = token, decays by a product along the lanes;
-// two the keys by channel, lane = channel, decays by a walk back over the
-// tokens.
-template <uint32_t DT, bool CHANNEL, int KB, int NT>
-__global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a, const ChunkRecord* records,
-                                                         bool vec) {
+// lane l, and splits it into the next products' operands where it is.  While a
+// chunk is multiplied, the next one's record, operands and values come to LDS
+// as they lie, the loads spread over the products.
+template <bool LO, int KB>
+struct ScanChunk {
+    ChunkRecord r;
+    ChunkOperands<LO, KB> o;
+};
+// A wave's values of a chunk, [32][16]; its outputs go out through them.
+template <uint32_t DT>
+using ScanTile = typename Elem<DT>::type[kChunk][16];
+
+template <uint32_t DT, bool LO, int KB, int W>
+constexpr size_t scan_lds() {
+    return 2 * sizeof(ScanChunk<LO, KB>) + 2 * W * sizeof(ScanTile<DT>);
+}
+
+// vec: bit 0, rows of v by 16 bytes; bit 1, rows of out.
+template <uint32_t DT, bool CHANNEL, int KB, int W>
+__global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
+    DeltaArgs a, const ChunkRecord* records,
+    const ChunkOperands<CHANNEL || DT == K3X_DTYPE_F32, KB>* operands, uint32_t vec) {
     typedef typename Elem<DT>::type E;
-    typedef ScanTerms<DT, CHANNEL, KB> Terms;
-    typedef typename Terms::Chunk Chunk;
-    __shared__ Chunk buf[2];
-    const uint32_t blocks = (a.V + 64 * NT - 1) / (64 * NT);
+    constexpr bool LO = CHANNEL || DT == K3X_DTYPE_F32;
+    typedef ScanChunk<LO, KB> Chunk;
+    // Sized at the launch: were the extent known here, the compiler would count
+    // on one wave a SIMD and move results through the accumulation registers.
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    Chunk* buf = reinterpret_cast<Chunk*>(lds);
+    const uint32_t blocks = (a.V + 16 * W - 1) / (16 * W);
     // Quotients come from the vector unit: kept scalar, as buffers want them.
     const uint32_t cb = __builtin_amdgcn_readfirstlane(blockIdx.x % blocks);
     const uint32_t h = __builtin_amdgcn_readfirstlane(blockIdx.x / blocks % a.H);
@@ -751,261 +953,108 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a, const Chun
     if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
     const uint32_t begin = __builtin_amdgcn_readfirstlane(sq.begin);
     const uint32_t len = __builtin_amdgcn_readfirstlane(sq.len);
-    const uint32_t chunks = (len + kChunk - 1) / kChunk, hk = __builtin_amdgcn_readfirstlane(h / (a.H / a.Hk));
-    // The record of chunk i is i a.H on.
-    const ChunkRecord* rec =
-        records + (size_t)__builtin_amdgcn_readfirstlane(first_slot(a, n)) * a.H + h;
-
+    const uint32_t chunks = (len + kChunk - 1) / kChunk;
+    const uint32_t hk = __builtin_amdgcn_readfirstlane(h / (a.H / a.Hk));
+    const size_t slot0 = __builtin_amdgcn_readfirstlane(first_slot(a, n));
     constexpr uint32_t es = sizeof(E);
-    const uint32_t kst = (uint32_t)a.ks * es, qst = (uint32_t)a.qs * es, gst = a.H * a.K * 4;
-    auto left = [&](uint32_t i) { return i < chunks ? min(len - i * kChunk, kChunk) : 0; };
-    // Chunk i's rows of this head (none past the last chunk).
-    auto key_rows = [&](uint32_t i) {
-        return rows_buffer(static_cast<const E*>(a.k) + (begin + (size_t)i * kChunk) * a.ks +
-                               (size_t)hk * a.K,
-                           left(i), kst, a.K * es);
-    };
-    auto query_rows = [&](uint32_t i) {
-        return rows_buffer(static_cast<const E*>(a.q) + (begin + (size_t)i * kChunk) * a.qs +
-                               (size_t)hk * a.K,
-                           left(i), qst, a.K * es);
-    };
-    auto gate_rows = [&](uint32_t i) {
-        return rows_buffer(a.gate + ((begin + (size_t)i * kChunk) * a.H + h) * a.K, left(i), gst,
-                           a.K * 4);
-    };
-    auto record = [&](uint32_t i) { return rec + (size_t)min(i, chunks - 1) * a.H; };
-    // Each of waves 4 .. 7 also copies two of the eight operands T and P.
-    auto copied = [&](const ChunkRecord* r, uint32_t x) {
-        return (&r->T[0][0][0])[64 * (2 * (wave - 4) + x) + lane];
-    };
-    static_assert(offsetof(ChunkRecord, P) == sizeof(ChunkRecord::T), "T, then P");
-    static_assert(offsetof(Chunk, P) - offsetof(Chunk, T) == sizeof(ChunkRecord::T), "T, then P");
-    auto paste = [&](Chunk& o, const f16x8 (&x)[2]) {
-#pragma unroll
-        for (uint32_t j = 0; j < 2; ++j) (&o.T[0][0][0])[64 * (2 * (wave - 4) + j) + lane] = x[j];
-    };
-    // The makers hold one chunk's elements and, as they use them up, load the
-    // next one's in their place, so that loads have a chunk's time to arrive.
-    if (wave >= 6) {  // keys by channel, and the rows' factors
-        const uint32_t c = 64 * (wave - 6) + lane;
-        const uint32_t koff = c < a.K ? c * es : kOutside, goff = c < a.K ? c * 4 : kOutside;
-        E k[kChunk];
-        float gate[CHANNEL ? kChunk : 1], mul = 0.0f, total = 0.0f, factor[3] = {};
-        f16x8 copy[2] = {};
-        auto scalars = [&](uint32_t i) {
-            const ChunkRecord* r = record(i);
-            copy[0] = copied(r, 0);
-            copy[1] = copied(r, 1);
-            mul = r->key_mul[lane & 31];
-            if (!CHANNEL) total = r->total[0][0];
-            if (wave == 6) {
-                factor[0] = (&r->row_r[0])[lane];
-                factor[1] = (&r->row_r[0])[64 + lane];
-                factor[2] = (&r->row_r[0])[128 + (lane & 31)];
-            }
-        };
-        auto make = [&](uint32_t i, Chunk& o) {
-            const auto kr = key_rows(i + 1), gr = gate_rows(i + 1);
-            const float own = mul;
-            // Row offsets are formed anew: held over the loop they would not fit.
-            uint32_t ks = kst, gs = gst;
-            asm volatile("" : "+s"(ks), "+s"(gs));
-            paste(o, copy);
-            if (wave == 6) {
-                (&o.row_r[0])[lane] = factor[0];
-                (&o.row_r[0])[64 + lane] = factor[1];
-                if (lane < 32) (&o.row_r[0])[128 + lane] = factor[2];
-            }
-            if (!CHANNEL && c < 32 * KB) o.decay[c] = total;
-            scalars(i + 1);
-            float s = kOperand, late[kChunk / 2];
-            auto next = [&](int t) {
-                const float one =
-                    __int_as_float(__builtin_amdgcn_readlane(__float_as_int(own), t));
-                const float x = Elem<DT>::load(k[t]) * one * s;
-                k[t] = load_one<E>(kr, koff, t * ks);
-                if (CHANNEL) {
-                    s *= exp_decay(gate[t]);
-                    gate[t] = load_one<float>(gr, goff, t * gs);
-                }
-                return x;
-            };
-#pragma unroll
-            for (int t = kChunk - 1; t >= (int)kChunk / 2; --t) late[t - kChunk / 2] = next(t);
-#pragma unroll
-            for (int q = 3; q >= 0; --q) {
-                float y[8];
-#pragma unroll
-                for (int j = 3; j >= 0; --j) {
-                    y[j] = next(4 * q + j);
-                    y[4 + j] = late[4 * q + j];
-                }
-                const Pair8 p = split8(y);
-                if (c >= 32 * KB) continue;
-                o.Kt[0][c / 16][q * 16 + c % 16] = p.hi;
-                if (Terms::kKeyLo) o.Kt[Terms::kKeyLo ? 1 : 0][c / 16][q * 16 + c % 16] = p.lo;
-            }
-            if (CHANNEL && c < 32 * KB) o.decay[c] = s * (1.0f / kOperand);
-        };
-        if (chunks) {
-            const auto kr = key_rows(0), gr = gate_rows(0);
-            scalars(0);
-#pragma unroll
-            for (int t = kChunk - 1; t >= 0; --t) {
-                k[t] = load_one<E>(kr, koff, t * kst);
-                if (CHANNEL) gate[t] = load_one<float>(gr, goff, t * gst);
-            }
-            make(0, buf[0]);
-        }
-        lds_barrier();
-        for (uint32_t i = 1; i <= chunks; ++i) {
-            if (i < chunks) make(i, buf[i & 1]);
-            lds_barrier();
-        }
-        return;
-    }
-    if (wave >= 4) {  // keys and queries by token
-        const uint32_t r = wave - 4;
-        Vec4<E> k[KB][2], q[KB][2];
-        f32x4 gate[CHANNEL ? KB : 1][2], before[CHANNEL ? KB : 1][2];
-        float kmul = 0.0f, qmul = 0.0f;
-        f16x8 copy[2] = {};
-        const uint32_t t = 16 * r + m;
-        const bool whole = vec && a.K == 32 * KB;
-        auto scalars = [&](uint32_t i) {
-            const ChunkRecord* rc = record(i);
-            copy[0] = copied(rc, 0);
-            copy[1] = copied(rc, 1);
-            kmul = rc->key_mul[t] * kOperand;
-            qmul = rc->query_mul[t] * kOperand;
-        };
-        auto total_row = [&](uint32_t i) { return rows_buffer(record(i)->total[0], 1, 0, 512); };
-        auto load = [&](int b, __amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t qr,
-                        __amdgpu_buffer_rsrc_t gr, __amdgpu_buffer_rsrc_t tr) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t c = 32 * b + 16 * j + 4 * g;
-                if (whole) {
-                    k[b][j] = load_four<E>(kr, t * kst + c * es, 0);
-                    q[b][j] = load_four<E>(qr, t * qst + c * es, 0);
-                    if (CHANNEL) gate[b][j] = load_four<float>(gr, t * gst + c * 4, 0);
-                } else {
-                    uint32_t row = t, first = c;  // offsets formed anew, as above
-                    asm volatile("" : "+v"(row), "+v"(first));
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const uint32_t at = first + x;
-                        const bool in = at < a.K;
-                        k[b][j][x] = load_one<E>(kr, in ? row * kst + at * es : kOutside, 0);
-                        q[b][j][x] = load_one<E>(qr, in ? row * qst + at * es : kOutside, 0);
-                        if (CHANNEL)
-                            gate[b][j][x] =
-                                load_one<float>(gr, in ? row * gst + at * 4 : kOutside, 0);
-                    }
-                }
-                if (CHANNEL && r) before[b][j] = load_four<float>(tr, c * 4, 0);
-            }
-        };
-        auto make = [&](uint32_t i, Chunk& o) {
-            const auto kr = key_rows(i + 1), qr = query_rows(i + 1), gr = gate_rows(i + 1);
-            const auto tr = total_row(i + 1);
-            const float km = kmul, qm = qmul;
-            paste(o, copy);
-            scalars(i + 1);
-#pragma unroll
-            for (int b = 0; b < KB; ++b) {
-                float kx[8], qx[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    kx[j] = Elem<DT>::load(k[b][j / 4][j % 4]) * km;
-                    qx[j] = Elem<DT>::load(q[b][j / 4][j % 4]) * qm;
-                    if (CHANNEL) {
-                        float p = scan_row(exp_decay(gate[b][j / 4][j % 4]));
-                        if (r) p *= before[b][j / 4][j % 4];
-                        kx[j] *= p;
-                        qx[j] *= p;
-                    }
-                }
-                load(b, kr, qr, gr, tr);
-                const Pair8 kp = split8(kx), qp = split8(qx);
-                o.K[0][r][b][lane] = kp.hi;
-                if (Terms::kKeyLo) o.K[Terms::kKeyLo ? 1 : 0][r][b][lane] = kp.lo;
-                o.Q[0][r][b][lane] = qp.hi;
-                if (Terms::kKeyLo) o.Q[Terms::kKeyLo ? 1 : 0][r][b][lane] = qp.lo;
-            }
-        };
-        if (chunks) {
-            const auto kr = key_rows(0), qr = query_rows(0), gr = gate_rows(0);
-            const auto tr = total_row(0);
-            scalars(0);
-#pragma unroll
-            for (int b = 0; b < KB; ++b) load(b, kr, qr, gr, tr);
-            make(0, buf[0]);
-        }
-        lds_barrier();
-        for (uint32_t i = 1; i <= chunks; ++i) {
-            if (i < chunks) make(i, buf[i & 1]);
-            lds_barrier();
-        }
-        return;
-    }
-
-    const size_t base = ((size_t)sq.slot * a.H + h) * a.K * a.V;
+    constexpr int kTileLoads = sizeof(ScanTile<DT>) / 1024;
+    ScanTile<DT>* tiles = reinterpret_cast<ScanTile<DT>*>(lds + 2 * sizeof(Chunk)) + 2 * wave;
     const uint32_t vst = (uint32_t)a.vs * es, ost = (uint32_t)a.os * es;
-    uint32_t col[NT], voff[NT], ooff[NT];
-    // A column is held times 2^-shift, the state times kOperand besides.
-    f32x4 S[NT][2 * KB];
-    int shift[NT];
+    const uint32_t col0 = (cb * W + wave) * 16, col = col0 + m;
+    const bool in = col < a.V;
+    // Sixteen bytes of a row of the tile: lane's row (of each load's) and column.
+    constexpr uint32_t kRowLanes = 16 * es / 16;
+    const uint32_t trow = lane / kRowLanes, tcol = col0 + lane % kRowLanes * (16 / es);
+    auto left = [&](uint32_t i) { return i < chunks ? min(len - i * kChunk, kChunk) : 0; };
+    auto value_rows = [&](uint32_t i) {
+        return rows_buffer(static_cast<const E*>(a.v) + (begin + (size_t)i * kChunk) * a.vs +
+                               (size_t)h * a.V,
+                           left(i), vst, a.V * es);
+    };
+    E direct[8];  // a chunk's values where rows are not by 16 bytes
+    auto bring_values = [&](uint32_t i) {
+        const auto r = value_rows(i);
+        if (vec & 1) {
+            // What lies past the last row or column is not used, but finite.
+            const uint32_t c = tcol < a.V ? tcol * es : 0, last = left(i) - 1;
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-        col[x] = (cb * 4 + wave) * 16 * NT + 16 * x + m;
-        const bool in = col[x] < a.V;
-        voff[x] = in ? 4 * g * vst + col[x] * es : kOutside;
-        ooff[x] = in ? 4 * g * ost + col[x] * es : kOutside;
+            for (int x = 0; x < kTileLoads; ++x)
+                load_lds16(r, reinterpret_cast<u32x4*>(tiles[i & 1]) + 64 * x,
+                           min(trow + x * (64 / kRowLanes), last) * vst + c, 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                direct[j] = load_one<E>(r, in ? (4 * g + 16 * (j / 4) + j % 4) * vst + col * es
+                                              : kOutside, 0);
+        }
+    };
+    auto put_values = [&](uint32_t i) {
+        if (vec & 1) return;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tiles[i & 1][4 * g + 16 * (j / 4) + j % 4][m] = direct[j];
+    };
+    // The wave's share of chunk i, 1 KiB a load: parts x of `of`.
+    constexpr uint32_t kRecord = sizeof(ChunkRecord) / 1024, kAll = sizeof(Chunk) / 1024;
+    static_assert(sizeof(Chunk) % 1024 == 0, "whole loads");
+    constexpr uint32_t kUnits = (kAll + W - 1) / W;
+    auto bring = [&](uint32_t i, uint32_t x, uint32_t of) {
+        const size_t slot = slot0 + i;
+        const auto rr = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<ChunkRecord*>(records + slot * a.H + h), (short)0, sizeof(ChunkRecord),
+            0x00020000);
+        const auto ro = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<ChunkOperands<LO, KB>*>(
+                operands + (CHANNEL ? slot * a.H + h : slot * a.Hk + hk)),
+            (short)0, sizeof(ChunkOperands<LO, KB>), 0x00020000);
+        u32x4* dst = reinterpret_cast<u32x4*>(&buf[i & 1]);
+#pragma unroll
+        for (uint32_t y = 0; y < kUnits; ++y) {
+            if (y % of != x) continue;
+            const uint32_t unit = W * y + wave;
+            if (unit < kRecord) load_lds16(rr, dst + 64 * unit, lane * 16, unit * 1024);
+            else if (unit < kAll)
+                load_lds16(ro, dst + 64 * unit, lane * 16, (unit - kRecord) * 1024);
+        }
+    };
+    const size_t base = ((size_t)sq.slot * a.H + h) * a.K * a.V;
+    // A column is held times 2^-shift, the state times kOperand besides.
+    f32x4 S[2 * KB];
+    int shift = 0;
+    {
         float most = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t r = 16 * t + 4 * g + i;
-                S[x][t][i] = a.state_in && in && r < a.K
-                                 ? a.state_in[base + (size_t)r * a.V + col[x]]
-                                 : 0.0f;
-                most = fmaxf(most, fabsf(S[x][t][i]));
+                S[t][i] = a.state_in && in && r < a.K ? a.state_in[base + (size_t)r * a.V + col]
+                                                      : 0.0f;
+                most = fmaxf(most, fabsf(S[t][i]));
             }
         most = max_groups(most);
-        shift[x] = most > 0.0f ? __builtin_amdgcn_frexp_expf(most) - 3 : 0;
+        if (most > 0.0f) shift = __builtin_amdgcn_frexp_expf(most) - 3;
 #pragma unroll
         for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                S[x][t][i] = kOperand * __builtin_ldexpf(S[x][t][i], -shift[x]);
+            for (int i = 0; i < 4; ++i) S[t][i] = kOperand * __builtin_ldexpf(S[t][i], -shift);
     }
-    E next[NT][2][4];
-    auto fetch = [&](uint32_t i) {
-        const auto r = rows_buffer(static_cast<const E*>(a.v) +
-                                       (begin + (size_t)i * kChunk) * a.vs + (size_t)h * a.V,
-                                   left(i), vst, a.V * es);
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    next[x][t][j] = load_one<E>(r, voff[x], (16 * t + j) * vst);
-    };
     float z = 0.0f;
-    if (chunks) fetch(0);
-    lds_barrier();
+    if (chunks) {
+        bring_values(0);
+        bring(0, 0, 1);
+        put_values(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
     for (uint32_t ci = 0; ci < chunks; ++ci) {
-        const Chunk& o = buf[ci & 1];
-        f32x4 v[NT][2], aq[NT][2] = {}, ak[NT][2] = {};
+        const ChunkRecord& rc = buf[ci & 1].r;
+        const ChunkOperands<LO, KB>& o = buf[ci & 1].o;
+        const bool more = ci + 1 < chunks;
+        f32x4 v[2], aq[2] = {}, ak[2] = {};
         // Operands of 32 channels, the next ones on their way while these are
         // multiplied.
-        constexpr int kParts = Terms::kKeyLo ? 2 : 1;
+        constexpr int kParts = LO ? 2 : 1;
         f16x8 kf[2][kParts][2], qf[2][kParts][2];
-        auto operands = [&](int b) {
+        auto frags = [&](int b) {
 #pragma unroll
             for (int p = 0; p < kParts; ++p)
 #pragma unroll
@@ -1014,95 +1063,95 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a, const Chun
                     qf[b & 1][p][t] = o.Q[p][t][b][lane];
                 }
         };
-        operands(0);
-        float most[NT];
+        auto factors = [&](const float* f, int t) {
+            return *reinterpret_cast<const f32x4*>(f + 16 * t + 4 * g);
+        };
+        float most = 0.0f;
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
-            most[x] = 0.0f;
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[t][j] = Elem<DT>::load(tiles[ci & 1][16 * t + 4 * g + j][m]);
+        frags(0);
+        if (more) bring_values(ci + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 2 * KB; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(S[t][i]));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                z = __builtin_fmaf(v[t][j], 0.0f, z);
+                v[t][j] = __builtin_ldexpf(v[t][j], -shift);
+                most = fmaxf(most, fabsf(v[t][j]) * kOperand);
+            }
+        // Column sizes near 1 leave both the products' growth and the parts
+        // below hi their room.
+        most = max_groups(most);
+        const bool off = most > 32.0f * kOperand || (most < 0.5f * kOperand && most > 0.0f);
+        if (__any(off)) {
+            const int d = off ? __builtin_amdgcn_frexp_expf(most) - 3 - 6 : 0;
+            shift += d;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float y = Elem<DT>::load(next[x][t][j]);
-                    z = __builtin_fmaf(y, 0.0f, z);
-                    v[x][t][j] = __builtin_ldexpf(y, -shift[x]);
-                    most[x] = fmaxf(most[x], fabsf(v[x][t][j]) * kOperand);
-                }
+                for (int j = 0; j < 4; ++j) v[t][j] = __builtin_ldexpf(v[t][j], -d);
 #pragma unroll
             for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) most[x] = fmaxf(most[x], fabsf(S[x][t][i]));
-        }
-        fetch(ci + 1);
-        // Column sizes near 1 leave both the products' growth and the parts
-        // below hi their room.
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-            const float all = max_groups(most[x]);
-            const bool off = all > 32.0f * kOperand || (all < 0.5f * kOperand && all > 0.0f);
-            if (__any(off)) {
-                const int d = off ? __builtin_amdgcn_frexp_expf(all) - 3 - 6 : 0;
-                shift[x] += d;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[x][t][j] = __builtin_ldexpf(v[x][t][j], -d);
-#pragma unroll
-                for (int t = 0; t < 2 * KB; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) S[x][t][i] = __builtin_ldexpf(S[x][t][i], -d);
-            }
+                for (int i = 0; i < 4; ++i) S[t][i] = __builtin_ldexpf(S[t][i], -d);
         }
         // (P k) S and (P q) S; the products of one sum lie apart.
+        f16x8 tf[2][2];
+        f32x4 rt[2], rr[2];
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-            if (b + 1 < KB) operands(b + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            Pair8 s[NT];
+            if (b + 1 < KB) {
+                frags(b + 1);
+            } else {
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                const f32x4 &l = S[x][2 * b], &u = S[x][2 * b + 1];
-                const float y[8] = {l[0], l[1], l[2], l[3], u[0], u[1], u[2], u[3]};
-                s[x] = split8(y);
+                for (int t = 0; t < 2; ++t) {
+                    tf[0][t] = rc.T[t][0][lane];
+                    tf[1][t] = rc.T[t][1][lane];
+                    rr[t] = factors(rc.row_r, t);
+                    rt[t] = factors(rc.row_t, t);
+                }
             }
+            if (more) bring(ci + 1, b, KB);
+            __builtin_amdgcn_sched_barrier(0);
+            const f32x4 &l = S[2 * b], &u = S[2 * b + 1];
+            const float y[8] = {l[0], l[1], l[2], l[3], u[0], u[1], u[2], u[3]};
+            const Pair8 s = split8(y);
             const auto& kp = kf[b & 1];
             const auto& qp = qf[b & 1];
-            if (Terms::kKeyLo) {
+            if (LO) {
 #pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        ak[x][t] = mfma_f16(kp[kParts - 1][t], s[x].hi, ak[x][t]);
-                        aq[x][t] = mfma_f16(qp[kParts - 1][t], s[x].hi, aq[x][t]);
-                    }
+                for (int t = 0; t < 2; ++t) {
+                    ak[t] = mfma_f16(kp[kParts - 1][t], s.hi, ak[t]);
+                    aq[t] = mfma_f16(qp[kParts - 1][t], s.hi, aq[t]);
+                }
             }
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
+            for (int t = 0; t < 2; ++t) {
+                ak[t] = mfma_f16(kp[0][t], s.lo, ak[t]);
+                aq[t] = mfma_f16(qp[0][t], s.lo, aq[t]);
+            }
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    ak[x][t] = mfma_f16(kp[0][t], s[x].lo, ak[x][t]);
-                    aq[x][t] = mfma_f16(qp[0][t], s[x].lo, aq[x][t]);
-                }
-#pragma unroll
-            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    ak[x][t] = mfma_f16(kp[0][t], s[x].hi, ak[x][t]);
-                    aq[x][t] = mfma_f16(qp[0][t], s[x].hi, aq[x][t]);
-                }
+            for (int t = 0; t < 2; ++t) {
+                ak[t] = mfma_f16(kp[0][t], s.hi, ak[t]);
+                aq[t] = mfma_f16(qp[0][t], s.hi, aq[t]);
+            }
             // The state's decay, for the update.
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                const f32x4 f =
-                    *reinterpret_cast<const f32x4*>(&o.decay[16 * (2 * b + y) + 4 * g]);
+                const f32x4 f = factors(rc.decay, 2 * b + y);
 #pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) S[x][2 * b + y][i] *= f[i];
+                for (int i = 0; i < 4; ++i) S[2 * b + y][i] *= f[i];
             }
         }
         // A column that a product would take past f16 is made smaller.
-        auto fit = [&](f32x4 (&y)[2], int x) {
+        auto fit = [&](f32x4 (&y)[2]) {
             float big = 0.0f;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -1111,97 +1160,39 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a, const Chun
             if (!__any(big > 16384.0f)) return;
             big = max_groups(big);
             const int d = big > 16384.0f ? __builtin_amdgcn_frexp_expf(big) - 5 : 0;
-            shift[x] += d;
+            shift += d;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     y[t][j] = __builtin_ldexpf(y[t][j], -d);
-                    aq[x][t][j] = __builtin_ldexpf(aq[x][t][j], -d);
+                    aq[t][j] = __builtin_ldexpf(aq[t][j], -d);
                 }
 #pragma unroll
             for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) S[x][t][i] = __builtin_ldexpf(S[x][t][i], -d);
+                for (int i = 0; i < 4; ++i) S[t][i] = __builtin_ldexpf(S[t][i], -d);
         };
         auto operand = [&](const f32x4 (&x)[2]) {
             const float y[8] = {x[0][0], x[0][1], x[0][2], x[0][3],
                                 x[1][0], x[1][1], x[1][2], x[1][3]};
             return split8(y);
         };
-        auto factors = [&](const float* f, int t) {
-            return *reinterpret_cast<const f32x4*>(f + 16 * t + 4 * g);
-        };
-        f32x4 u[NT][2];
-        Pair8 up[NT];
-        {
-            f16x8 tf[2][2];
-            f32x4 rt[2], rr[2];
+        f32x4 u[2], ap[2] = {};
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                tf[0][t] = o.T[t][0][lane];
-                tf[1][t] = o.T[t][1][lane];
-                rr[t] = factors(o.row_r, t);
-                rt[t] = factors(o.row_t, t);
-            }
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
+            for (int j = 0; j < 4; ++j) u[t][j] = __builtin_fmaf(-rr[t][j], ak[t][j], v[t][j]);
+        fit(u);
+        Pair8 up = operand(u);
+        u[0] = u[1] = f32x4{};
+        f16x8 pf[2][2], tk[2][kParts][2];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        u[x][t][j] = __builtin_fmaf(-rr[t][j], ak[x][t][j], v[x][t][j]);
-                fit(u[x], x);
-                up[x] = operand(u[x]);
-                u[x][0] = u[x][1] = f32x4{};
-            }
-#pragma unroll
-            for (int y = 0; y < 3; ++y)
-#pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        u[x][t] = mfma_f16(tf[y == 0][t], y == 1 ? up[x].lo : up[x].hi, u[x][t]);
-#pragma unroll
-            for (int x = 0; x < NT; ++x) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) u[x][t][j] *= rt[t][j];
-                fit(u[x], x);
-                up[x] = operand(u[x]);
-            }
+        for (int t = 0; t < 2; ++t) {
+            pf[0][t] = rc.P[t][0][lane];
+            pf[1][t] = rc.P[t][1][lane];
         }
-        f32x4 ap[NT][2] = {};
-        {
-            f16x8 pf[2][2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                pf[0][t] = o.P[t][0][lane];
-                pf[1][t] = o.P[t][1][lane];
-            }
-#pragma unroll
-            for (int y = 0; y < 3; ++y)
-#pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        ap[x][t] = mfma_f16(pf[y == 0][t], y == 1 ? up[x].lo : up[x].hi, ap[x][t]);
-        }
-        if (!CHANNEL) {
-#pragma unroll
-            for (int x = 0; x < NT; ++x) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const f32x4 f = factors(o.row_u, t);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) u[x][t][j] *= f[j];
-                }
-                up[x] = operand(u[x]);
-            }
-        }
-        // The state's update, two tiles of channels at a time.
-        f16x8 tk[2][kParts][2];
+        // Two tiles of channels of the keys for the update.
         auto channels = [&](int y) {
 #pragma unroll
             for (int p = 0; p < kParts; ++p)
@@ -1209,59 +1200,101 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs a, const Chun
                 for (int t = 0; t < 2; ++t) tk[y & 1][p][t] = o.Kt[p][2 * y + t][lane];
         };
         channels(0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < 3; ++y)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                u[t] = mfma_f16(tf[y == 0][t], y == 1 ? up.lo : up.hi, u[t]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[t][j] *= rt[t][j];
+        fit(u);
+        up = operand(u);
+        f32x4 fo[2], fp[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            fo[t] = factors(rc.row_o, t);
+            fp[t] = factors(rc.row_p, t);
+        }
+#pragma unroll
+        for (int y = 0; y < 3; ++y)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                ap[t] = mfma_f16(pf[y == 0][t], y == 1 ? up.lo : up.hi, ap[t]);
+        if (!CHANNEL) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const f32x4 f = factors(rc.row_u, t);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u[t][j] *= f[j];
+            }
+            up = operand(u);
+        }
+        // The state's update.
 #pragma unroll
         for (int y = 0; y < KB; ++y) {
             if (y + 1 < KB) channels(y + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if (Terms::kKeyLo) {
+            if (LO) {
 #pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        S[x][2 * y + t] =
-                            mfma_f16(tk[y & 1][kParts - 1][t], up[x].hi, S[x][2 * y + t]);
+                for (int t = 0; t < 2; ++t)
+                    S[2 * y + t] = mfma_f16(tk[y & 1][kParts - 1][t], up.hi, S[2 * y + t]);
             }
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
+            for (int t = 0; t < 2; ++t)
+                S[2 * y + t] = mfma_f16(tk[y & 1][0][t], up.lo, S[2 * y + t]);
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    S[x][2 * y + t] = mfma_f16(tk[y & 1][0][t], up[x].lo, S[x][2 * y + t]);
-#pragma unroll
-            for (int x = 0; x < NT; ++x)
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    S[x][2 * y + t] = mfma_f16(tk[y & 1][0][t], up[x].hi, S[x][2 * y + t]);
+            for (int t = 0; t < 2; ++t)
+                S[2 * y + t] = mfma_f16(tk[y & 1][0][t], up.hi, S[2 * y + t]);
         }
         const auto outs = rows_buffer(static_cast<E*>(a.out) +
                                           (begin + (size_t)ci * kChunk) * a.os + (size_t)h * a.V,
                                       left(ci), ost, a.V * es);
+        // The next chunk is in LDS (only this one's outputs may still be on
+        // their way) and every wave is done with this one.
+        if (vec & 2) {
+            ScanTile<DT>& tile = tiles[ci & 1];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const f32x4 fo = factors(o.row_o, t), fp = factors(o.row_p, t);
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
+                for (int j = 0; j < 4; ++j)
+                    tile[16 * t + 4 * g + j][m] = Elem<DT>::store(__builtin_ldexpf(
+                        __builtin_fmaf(fp[t][j], ap[t][j], fo[t][j] * aq[t][j]), shift));
+            wave_sync();
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float y = __builtin_fmaf(fp[j], ap[x][t][j], fo[j] * aq[x][t][j]);
-                    store_one<E>(Elem<DT>::store(__builtin_ldexpf(y, shift[x])), outs, ooff[x],
-                                 (16 * t + j) * ost);
-                }
+            for (int x = 0; x < kTileLoads; ++x)
+                __builtin_amdgcn_raw_buffer_store_b128(
+                    reinterpret_cast<const u32x4*>(tile)[64 * x + lane], outs,
+                    tcol < a.V ? (trow + x * (64 / kRowLanes)) * ost + tcol * es : kOutside, 0, 0);
+            if (more) put_values(ci + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kTileLoads)
+                         : "memory");
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int t = j / 4, i = j % 4;
+                const float y = __builtin_fmaf(fp[t][i], ap[t][i], fo[t][i] * aq[t][i]);
+                store_one<E>(Elem<DT>::store(__builtin_ldexpf(y, shift)), outs,
+                             in ? (4 * g + 16 * t + i) * ost + col * es : kOutside, 0);
+            }
+            if (more) put_values(ci + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
-        lds_barrier();
     }
     if (z != z) latch(a.status, K3X_ERR_INVALID_MXFP4);
-    if (!a.state_out || (!chunks && a.state_in == a.state_out)) return;
+    if (!a.state_out || !in || (!chunks && a.state_in == a.state_out)) return;
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+    for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
-        for (int t = 0; t < 2 * KB; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t r = 16 * t + 4 * g + i;
-                if (r < a.K && col[x] < a.V)
-                    a.state_out[base + (size_t)r * a.V + col[x]] =
-                        __builtin_ldexpf(S[x][t][i], shift[x] - 6);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t r = 16 * t + 4 * g + i;
+            if (r < a.K)
+                a.state_out[base + (size_t)r * a.V + col] = __builtin_ldexpf(S[t][i], shift - 6);
+        }
 }
 
 // Chunks for sequences that fill one and heads that the products' tiles take.
@@ -1273,33 +1306,60 @@ bool runs_in_chunks(const k3x_hip_delta_params* p) {
     return p->key_dim <= 128 && longest >= kChunkMinTokens;
 }
 
-uint64_t chunk_slots(const k3x_hip_delta_params* p) { return p->tokens / kChunk + p->sequences; }
+// Where a call's records and operands lie in its workspace.
+struct ChunkSpace {
+    uint64_t slots;
+    size_t operands_at, bytes;
+};
+
+ChunkSpace chunk_space(const k3x_hip_delta_params* p) {
+    const bool channel = p->gate == K3X_GATE_CHANNEL;
+    const uint64_t slots = p->tokens / kChunk + p->sequences;
+    const size_t part = p->key_dim <= 64 ? sizeof(ChunkOperands<false, 2>)
+                                         : sizeof(ChunkOperands<false, 4>);
+    const size_t one = channel || p->dtype == K3X_DTYPE_F32 ? 2 * part : part;
+    const size_t at = slots * p->value_heads * sizeof(ChunkRecord);
+    return {slots, at, at + slots * (channel ? p->value_heads : p->key_heads) * one};
+}
 
 template <uint32_t DT, bool CHANNEL, int KB>
-int launch_chunks(k3x_hip_ctx* ctx, const DeltaArgs& a, ChunkRecord* records, uint32_t slots,
+int launch_chunks(k3x_hip_ctx* ctx, const DeltaArgs& a, void* workspace, const ChunkSpace& space,
                   bool vec) {
-    hipLaunchKernelGGL((delta_prep_kernel<DT, CHANNEL, KB>), dim3(slots * a.H), dim3(128), 0,
-                       ctx->stream, a, records, vec);
-    const uint32_t heads = a.N * a.H;
-    if (a.V > 64 && heads >= ctx->cu_count / 2)
-        hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB, 2>),
-                           dim3(heads * ((a.V + 127) / 128)), dim3(512), 0, ctx->stream, a, records,
-                           vec);
+    typedef ChunkOperands<CHANNEL || DT == K3X_DTYPE_F32, KB> Operands;
+    ChunkRecord* records = static_cast<ChunkRecord*>(workspace);
+    Operands* ops = reinterpret_cast<Operands*>(static_cast<uint8_t*>(workspace) +
+                                                space.operands_at);
+    const uint32_t slots = (uint32_t)space.slots;
+    if constexpr (CHANNEL)
+        hipLaunchKernelGGL((delta_prep_channel_kernel<DT, KB>), dim3(slots * a.H), dim3(128), 0,
+                           ctx->stream, a, records, ops, vec);
     else
-        hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB, 1>),
-                           dim3(heads * ((a.V + 63) / 64)), dim3(512), 0, ctx->stream, a, records,
-                           vec);
+        hipLaunchKernelGGL((delta_prep_head_kernel<DT, KB>), dim3(slots * a.Hk), dim3(128), 0,
+                           ctx->stream, a, records, ops, vec);
+    constexpr bool LO = CHANNEL || DT == K3X_DTYPE_F32;
+    const uint32_t heads = a.N * a.H;
+    const uint32_t es = sizeof(typename Elem<DT>::type);
+    const uint32_t rows = (a.V * es % 16 == 0 && a.vs * es % 16 == 0 && aligned(a.v, 16) ? 1 : 0) |
+                          (a.V * es % 16 == 0 && a.os * es % 16 == 0 && aligned(a.out, 16) ? 2 : 0);
+    if (a.V > 64 && heads >= ctx->cu_count / 2)
+        hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB, 8>),
+                           dim3(heads * ((a.V + 127) / 128)), dim3(512),
+                           (scan_lds<DT, LO, KB, 8>()), ctx->stream, a, records, ops, rows);
+    else
+        hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB, 4>),
+                           dim3(heads * ((a.V + 63) / 64)), dim3(256),
+                           (scan_lds<DT, LO, KB, 4>()), ctx->stream, a, records, ops, rows);
     return launched(ctx, 2);
 }
 
 template <uint32_t DT>
-int launch_chunks_of(k3x_hip_ctx* ctx, const DeltaArgs& a, ChunkRecord* records, uint32_t slots,
-                     bool channel, bool vec) {
+int launch_chunks_of(k3x_hip_ctx* ctx, const DeltaArgs& a, void* workspace,
+                     const ChunkSpace& space, bool channel, bool vec) {
     if (a.K <= 64)
-        return channel ? launch_chunks<DT, true, 2>(ctx, a, records, slots, vec)
-                       : launch_chunks<DT, false, 2>(ctx, a, records, slots, vec);
-    return channel ? launch_chunks<DT, true, 4>(ctx, a, records, slots, vec)
-                   : launch_chunks<DT, false, 4>(ctx, a, records, slots, vec);
+        return channel ? launch_chunks<DT, true, 2>(ctx, a, workspace, space, vec)
+                       : launch_chunks<DT, false, 2>(ctx, a, workspace, space, vec);
+    return channel ? launch_chunks<DT, true, 4>(ctx, a, workspace, space, vec)
+                   : launch_chunks<DT, false, 4>(ctx, a, workspace, space, vec);
 }
 
 bool delta_ok(const k3x_hip_delta_params* p) {
@@ -1326,7 +1386,7 @@ extern "C" {
 
 size_t k3x_hip_delta_workspace(const k3x_hip_delta_params* p) {
     if (!p || !delta_ok(p) || !runs_in_chunks(p)) return 0;
-    return chunk_slots(p) * p->value_heads * sizeof(ChunkRecord);
+    return chunk_space(p).bytes;
 }
 
 int k3x_hip_delta_rule(k3x_hip_ctx* ctx, const k3x_hip_delta_params* p, const void* q,
@@ -1387,14 +1447,13 @@ int k3x_hip_delta_rule(k3x_hip_ctx* ctx, const k3x_hip_delta_params* p, const vo
         // Four elements a load: rows and heads that keep the alignment.
         const bool vec = a.K % 4 == 0 && a.qs % 4 == 0 && a.ks % 4 == 0 && aligned(q, 4 * es) &&
                          aligned(k, 4 * es) && aligned(gate, 16);
-        ChunkRecord* records = static_cast<ChunkRecord*>(workspace);
-        const uint32_t slots = (uint32_t)chunk_slots(p);
+        const ChunkSpace space = chunk_space(p);
         const bool channel = p->gate == K3X_GATE_CHANNEL;
         return p->dtype == K3X_DTYPE_F32
-                   ? launch_chunks_of<K3X_DTYPE_F32>(ctx, a, records, slots, channel, vec)
+                   ? launch_chunks_of<K3X_DTYPE_F32>(ctx, a, workspace, space, channel, vec)
                : p->dtype == K3X_DTYPE_BF16
-                   ? launch_chunks_of<K3X_DTYPE_BF16>(ctx, a, records, slots, channel, vec)
-                   : launch_chunks_of<K3X_DTYPE_F16>(ctx, a, records, slots, channel, vec);
+                   ? launch_chunks_of<K3X_DTYPE_BF16>(ctx, a, workspace, space, channel, vec)
+                   : launch_chunks_of<K3X_DTYPE_F16>(ctx, a, workspace, space, channel, vec);
     }
     const uint32_t grid = a.N * a.H * ((a.V + kStepCols - 1) / kStepCols);
     if (p->dtype == K3X_DTYPE_F32)

@@ -23,7 +23,9 @@ template <>
 struct Elem<K3X_DTYPE_BF16> {
     typedef uint16_t type;
     static __device__ inline float load(type v) { return k3x_dev::bf16_to_f32(v); }
-    static __device__ inline type store(float v) { return k3x_dev::f32_to_bf16(v); }
+    static __device__ inline type store(float v) {
+        return __builtin_bit_cast(uint16_t, (__bf16)v);
+    }
 };
 template <>
 struct Elem<K3X_DTYPE_F16> {
