@@ -64,41 +64,75 @@ __device__ inline bool slot_taken(const DeltaArgs& a, uint32_t n, uint32_t slot)
     return __syncthreads_or(taken);
 }
 
-// Sum over the lanes that share a lane's column: lanes of equal lane % 4.
-__device__ inline float sum_rows(float v) {
-#pragma unroll
-    for (int d = 4; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
-}
-
-// R values from x (element r0 on; those past n are 0) as fp32.  z takes a NaN
-// where one of them is not finite.
-template <uint32_t DT, int R>
-__device__ inline void load_rows(const typename Elem<DT>::type* x, uint32_t r0, uint32_t n,
-                                 float (&y)[R], float& z) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        y[i] = r0 + i < n ? Elem<DT>::load(x[r0 + i]) : 0.0f;
-        z = __builtin_fmaf(y[i], 0.0f, z);
-    }
-}
-
 __device__ inline float exp_decay(float g) {
     return __builtin_amdgcn_exp2f(g * 1.44269504088896341f);
+}
+
+// Registers exchanged between rows of 16 lanes, or halves of the wave: a gets
+// [x row 0, y row 0, x row 2, y row 2] and b the odd rows (or a the lower
+// halves, b the upper ones).
+__device__ inline void swap_rows(float x, float y, float* a, float* b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false,
+                                                    false);
+    *a = __uint_as_float(r[0]);
+    *b = __uint_as_float(r[1]);
+}
+__device__ inline void swap_halves(float x, float y, float* a, float* b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false,
+                                                    false);
+    *a = __uint_as_float(r[0]);
+    *b = __uint_as_float(r[1]);
+}
+// x summed over both halves in the lower one and y in the upper one; the same
+// with even and odd rows.
+__device__ inline float fold_halves(float x, float y) {
+    float a, b;
+    swap_halves(x, y, &a, &b);
+    return a + b;
+}
+__device__ inline float fold_rows(float x, float y) {
+    float a, b;
+    swap_rows(x, y, &a, &b);
+    return a + b;
+}
+
+template <int Ctrl>
+__device__ inline float dpp(float x, float old = 0.0f) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(x), Ctrl,
+                                                      0xf, 0xf, false));
+}
+
+// Four elements as they lie.
+template <typename E>
+using Vec4 = E __attribute__((ext_vector_type(4)));
+
+// Four elements from c on of a row of n; those past it are some others of the
+// row.  vec (n a multiple of 4, the row aligned to four): one load.  Nothing
+// here branches by lane, so that many loads are in flight at once.
+template <typename E>
+__device__ inline Vec4<E> load4(const E* row, uint32_t c, uint32_t n, bool vec) {
+    if (vec) return *reinterpret_cast<const Vec4<E>*>(row + min(c, n - 4));
+    Vec4<E> y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = row[min(c + j, n - 1)];
+    return y;
 }
 
 // Token by token.  A wave holds 16 columns of one head's state: lane l has
 // columns 4 (l % 4) .. + 3 and the R rows from R (l / 4), all in registers.
 // The two products over the rows, S^T k and S^T q, are taken of the decayed
-// state before its update (S_new^T q = S^T q + (k . q) u), so that a token
-// costs one pass over the registers for both, one for the update, and one
-// round of sums over the 16 row groups.  A workgroup's waves are neighbours
-// in the columns of one head and share nothing else.
+// state before its update (S_new^T q = S^T q + (k . q) u) and of q and k as
+// they are (norms scale the sums), so that a token is one pass over the
+// registers for all of its sums, one for the update, and one round of sums
+// over the 16 row groups, in which each exchange folds two sums into one
+// register.  The next token's rows are loaded meanwhile.  A workgroup's waves
+// are neighbours in the columns of one head and share nothing else.
 constexpr int kStepWaves = 4;
 constexpr uint32_t kStepCols = 16 * kStepWaves;
 
+// vec: bit 0, q, k and gate by four elements; bit 1, v; bit 2, states.
 template <uint32_t DT, int R, uint32_t GATE>
-__global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a, uint32_t vec) {
     typedef typename Elem<DT>::type E;
     const uint32_t blocks = (a.V + kStepCols - 1) / kStepCols;
     const uint32_t cb = blockIdx.x % blocks, h = blockIdx.x / blocks % a.H;
@@ -114,101 +148,162 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
     // From here on the waves of the workgroup do not wait for one another.
     if (*(volatile uint32_t*)a.status) return;
     const uint32_t c0 = cb * kStepCols + wave * 16 + 4 * (lane % 4), r0 = R * (lane / 4);
+    if (cb * kStepCols + wave * 16 >= a.V) return;
     const uint32_t hk = h / (a.H / a.Hk);
     const size_t base = ((size_t)sq.slot * a.H + h) * a.K * a.V;
-    float S[R][4];
+    f32x4 S[R] = {};
+    if (a.state_in) {
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+        for (int i = 0; i < R; ++i)
+            S[i] = load4(a.state_in + base + (size_t)min(r0 + i, a.K - 1) * a.V, c0, a.V, vec & 4);
+    }
+    struct Row {
+        Vec4<E> q[R / 4], k[R / 4], v;
+        f32x4 gate[GATE == K3X_GATE_CHANNEL ? R / 4 : 1];
+        float beta;
+    } next, now;
+    auto fetch = [&](uint32_t t) {
+        const size_t row = (size_t)sq.begin + t;
+        const E* q = static_cast<const E*>(a.q) + row * a.qs + (size_t)hk * a.K;
+        const E* k = static_cast<const E*>(a.k) + row * a.ks + (size_t)hk * a.K;
+        const float* g = a.gate + (row * a.H + h) * (GATE == K3X_GATE_CHANNEL ? a.K : 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            S[i][j] = a.state_in && r0 + i < a.K && c0 + j < a.V
-                          ? a.state_in[base + (size_t)(r0 + i) * a.V + c0 + j]
-                          : 0.0f;
+        for (int i = 0; i < R / 4; ++i) {
+            next.q[i] = load4(q, r0 + 4 * i, a.K, vec & 1);
+            next.k[i] = load4(k, r0 + 4 * i, a.K, vec & 1);
+            if (GATE == K3X_GATE_CHANNEL) next.gate[i] = load4(g, r0 + 4 * i, a.K, vec & 1);
+        }
+        if (GATE == K3X_GATE_HEAD) next.gate[0][0] = g[0];
+        next.v = load4(static_cast<const E*>(a.v) + row * a.vs + (size_t)h * a.V, c0, a.V, vec & 2);
+        next.beta = a.beta[row * a.H + h];
+    };
+    if (sq.len) fetch(0);
+    // Rows past the head's end hold another's: they are 0, and stay so.
+    if (r0 + R > a.K) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (r0 + i >= a.K) S[i] = f32x4{};
+    }
     float z = 0.0f;  // NaN once an input is not finite
     bool wrong = false;
     for (uint32_t t = 0; t < sq.len; ++t) {
-        const size_t row = (size_t)sq.begin + t;
-        float q[R], k[R], v[4];
-        load_rows<DT>(static_cast<const E*>(a.q) + row * a.qs + (size_t)hk * a.K, r0, a.K, q, z);
-        load_rows<DT>(static_cast<const E*>(a.k) + row * a.ks + (size_t)hk * a.K, r0, a.K, k, z);
-        load_rows<DT>(static_cast<const E*>(a.v) + row * a.vs + (size_t)h * a.V, c0, a.V, v, z);
-        const float beta = a.beta[row * a.H + h];
-        z = __builtin_fmaf(beta, 0.0f, z);
-        float rq = a.scale, rk = 1.0f;
-        if (a.eps > 0.0f) {
-            float qq = 0.0f, kk = 0.0f;
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                qq = __builtin_fmaf(q[i], q[i], qq);
-                kk = __builtin_fmaf(k[i], k[i], kk);
-            }
-            rq = a.scale / sqrtf(sum_rows(qq) + a.eps);
-            rk = 1.0f / sqrtf(sum_rows(kk) + a.eps);
-        }
-        if (GATE != K3X_GATE_NONE) {
-            const float* g = a.gate + (row * a.H + h) * (GATE == K3X_GATE_CHANNEL ? a.K : 1);
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const float gi = GATE == K3X_GATE_HEAD ? g[0] : r0 + i < a.K ? g[r0 + i] : 0.0f;
-                wrong |= !(gi <= 0.0f);
-                const float d = exp_decay(gi);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) S[i][j] *= d;
-            }
-        }
-        float p[4] = {}, o[4] = {}, kq = 0.0f;
+        now = next;
+        fetch(min(t + 1, sq.len - 1));
+        float q[R], k[R], v[4], d[R];
+        float qq = 0.0f, kk = 0.0f, kq = 0.0f;
+        f32x4 p = {}, o = {};
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            k[i] *= rk;
+            q[i] = Elem<DT>::load(now.q[i / 4][i % 4]);
+            k[i] = Elem<DT>::load(now.k[i / 4][i % 4]);
+            d[i] = GATE == K3X_GATE_CHANNEL ? now.gate[i / 4][i % 4] : now.gate[0][0];
+        }
+        if (r0 + R > a.K) {
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (r0 + i >= a.K) q[i] = k[i] = 0.0f, d[i] = 0.0f;
+        }
+        z = __builtin_fmaf(now.beta, 0.0f, z);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = Elem<DT>::load(now.v[j]);
+            z = __builtin_fmaf(v[j], 0.0f, z);
+        }
+        if (GATE == K3X_GATE_HEAD) {
+            wrong |= !(now.gate[0][0] <= 0.0f);
+            d[0] = exp_decay(now.gate[0][0]);
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            z = __builtin_fmaf(q[i], 0.0f, z);
+            z = __builtin_fmaf(k[i], 0.0f, z);
+            if (GATE == K3X_GATE_CHANNEL) {
+                wrong |= !(d[i] <= 0.0f);
+                d[i] = exp_decay(d[i]);
+            }
+            qq = __builtin_fmaf(q[i], q[i], qq);
+            kk = __builtin_fmaf(k[i], k[i], kk);
             kq = __builtin_fmaf(k[i], q[i], kq);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                if (GATE != K3X_GATE_NONE) S[i][j] *= d[GATE == K3X_GATE_HEAD ? 0 : i];
                 p[j] = __builtin_fmaf(S[i][j], k[i], p[j]);
                 o[j] = __builtin_fmaf(S[i][j], q[i], o[j]);
             }
         }
-        kq = sum_rows(kq);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float u = beta * (v[j] - sum_rows(p[j]));
-            o[j] = rq * __builtin_fmaf(kq, u, sum_rows(o[j]));
-#pragma unroll
-            for (int i = 0; i < R; ++i) S[i][j] = __builtin_fmaf(k[i], u, S[i][j]);
+        // Rows of 16 lanes then hold: x the sums of p0, p1, o0, o1, y those of
+        // p2, p3, o2, o3, w those of kk, kq, qq, kq.
+        float x = fold_rows(fold_halves(p[0], o[0]), fold_halves(p[1], o[1]));
+        float y = fold_rows(fold_halves(p[2], o[2]), fold_halves(p[3], o[3]));
+        float w = fold_rows(fold_halves(kk, qq), fold_halves(kq, kq));
+        x += dpp<0x124>(x);  // row_ror:4
+        y += dpp<0x124>(y);
+        w += dpp<0x124>(w);
+        x += dpp<0x128>(x);  // row_ror:8
+        y += dpp<0x128>(y);
+        w += dpp<0x128>(w);
+        const float sk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), 0));
+        const float skq = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), 16));
+        const float sq2 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), 32));
+        const float rk = a.eps > 0.0f ? rsqrtf(sk + a.eps) : 1.0f;
+        const float rq = a.eps > 0.0f ? a.scale * rsqrtf(sq2 + a.eps) : a.scale;
+        const bool odd = lane & 16;
+        // u of rows 0 and 1, then of every row.
+        float ux = now.beta * __builtin_fmaf(-rk, x, odd ? v[1] : v[0]);
+        float uy = now.beta * __builtin_fmaf(-rk, y, odd ? v[3] : v[2]);
+        float any, u[4];
+        swap_halves(ux, ux, &ux, &any);
+        swap_halves(uy, uy, &uy, &any);
+        const float kqr = rk * skq;
+        const float ox = rq * __builtin_fmaf(kqr, ux, x), oy = rq * __builtin_fmaf(kqr, uy, y);
+        swap_rows(ux, ux, &u[0], &u[1]);
+        swap_rows(uy, uy, &u[2], &u[3]);
+        if ((lane & 44) == 32) {  // rows 2 and 3, one lane a column group
+            E* out = static_cast<E*>(a.out) + ((size_t)sq.begin + t) * a.os + (size_t)h * a.V;
+            const uint32_t c = c0 + (odd ? 1 : 0);
+            if (c < a.V) out[c] = Elem<DT>::store(ox);
+            if (c + 2 < a.V) out[c + 2] = Elem<DT>::store(oy);
         }
-        if (lane < 4) {
-            E* out = static_cast<E*>(a.out) + row * a.os + (size_t)h * a.V;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (c0 + j < a.V) out[c0 + j] = Elem<DT>::store(o[j]);
-        }
+        for (int j = 0; j < 4; ++j) u[j] *= rk;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) S[i][j] = __builtin_fmaf(k[i], u[j], S[i][j]);
     }
     if (wrong || z != z) latch(a.status, K3X_ERR_INVALID_MXFP4);
     if (!a.state_out || (!sq.len && a.state_in == a.state_out)) return;
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int i = 0; i < R; ++i) {
+        if (r0 + i >= a.K) continue;
+        float* row = a.state_out + base + (size_t)(r0 + i) * a.V;
+        if (vec & 4) {
+            if (c0 < a.V) *reinterpret_cast<f32x4*>(row + c0) = S[i];
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (r0 + i < a.K && c0 + j < a.V)
-                a.state_out[base + (size_t)(r0 + i) * a.V + c0 + j] = S[i][j];
+            for (int j = 0; j < 4; ++j)
+                if (c0 + j < a.V) row[c0 + j] = S[i][j];
+        }
+    }
 }
 
 template <uint32_t DT, int R>
-void launch_step(const DeltaArgs& a, uint32_t gate, uint32_t grid, hipStream_t stream) {
-    const dim3 b(64 * kStepWaves);
+void launch_step(const DeltaArgs& a, uint32_t gate, uint32_t vec, hipStream_t stream) {
+    const dim3 b(64 * kStepWaves), grid(a.N * a.H * ((a.V + kStepCols - 1) / kStepCols));
     if (gate == K3X_GATE_NONE)
-        hipLaunchKernelGGL((delta_step_kernel<DT, R, K3X_GATE_NONE>), dim3(grid), b, 0, stream, a);
+        hipLaunchKernelGGL((delta_step_kernel<DT, R, K3X_GATE_NONE>), grid, b, 0, stream, a, vec);
     else if (gate == K3X_GATE_HEAD)
-        hipLaunchKernelGGL((delta_step_kernel<DT, R, K3X_GATE_HEAD>), dim3(grid), b, 0, stream, a);
+        hipLaunchKernelGGL((delta_step_kernel<DT, R, K3X_GATE_HEAD>), grid, b, 0, stream, a, vec);
     else
-        hipLaunchKernelGGL((delta_step_kernel<DT, R, K3X_GATE_CHANNEL>), dim3(grid), b, 0, stream,
-                           a);
+        hipLaunchKernelGGL((delta_step_kernel<DT, R, K3X_GATE_CHANNEL>), grid, b, 0, stream, a,
+                           vec);
 }
 
 template <uint32_t DT>
-void launch_step_rows(const DeltaArgs& a, uint32_t gate, uint32_t grid, hipStream_t stream) {
-    if (a.K <= 64) launch_step<DT, 4>(a, gate, grid, stream);
-    else if (a.K <= 128) launch_step<DT, 8>(a, gate, grid, stream);
-    else launch_step<DT, 16>(a, gate, grid, stream);
+void launch_step_rows(const DeltaArgs& a, uint32_t gate, uint32_t vec, hipStream_t stream) {
+    if (a.K <= 64) launch_step<DT, 4>(a, gate, vec, stream);
+    else if (a.K <= 128) launch_step<DT, 8>(a, gate, vec, stream);
+    else launch_step<DT, 16>(a, gate, vec, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -306,36 +401,16 @@ struct ChunkOperands {
 
 __device__ inline uint32_t token_of(uint32_t q, uint32_t j) { return 4 * q + (j & 3) + 4 * (j & 4); }
 
-template <int Ctrl>
-__device__ inline float dpp(float x, float old = 0.0f) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(x), Ctrl,
-                                                      0xf, 0xf, false));
-}
-
-// Sum and maximum over the lanes of equal lane % 16: rows of 16 lanes, then
-// halves of the wave, exchanged in registers.
-__device__ inline void swap_rows(float x, float* a, float* b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                    false);
-    *a = __uint_as_float(r[0]);
-    *b = __uint_as_float(r[1]);
-}
-__device__ inline void swap_halves(float x, float* a, float* b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                    false);
-    *a = __uint_as_float(r[0]);
-    *b = __uint_as_float(r[1]);
-}
+// Sum and maximum over the lanes of equal lane % 16.
 __device__ inline float sum_groups(float v) {
-    float a, b;
-    swap_rows(v, &a, &b);
-    swap_halves(a + b, &a, &b);
-    return a + b;
+    v = fold_rows(v, v);
+    return fold_halves(v, v);
 }
 __device__ inline float max_groups(float v) {
     float a, b;
-    swap_rows(v, &a, &b);
-    swap_halves(fmaxf(a, b), &a, &b);
+    swap_rows(v, v, &a, &b);
+    v = fmaxf(a, b);
+    swap_halves(v, v, &a, &b);
     return fmaxf(a, b);
 }
 
@@ -345,22 +420,6 @@ __device__ inline void unit_scale(float x, float* down, float* up) {
     e = e < -100 ? -100 : e > 100 ? 100 : e;
     *down = __builtin_ldexpf(1.0f, -e);
     *up = __builtin_ldexpf(1.0f, e);
-}
-
-// Four elements as they lie.
-template <typename E>
-using Vec4 = E __attribute__((ext_vector_type(4)));
-
-// Four elements from c on of a row of n; those past it are some others of the
-// row.  vec (n a multiple of 4, the row aligned to four): one load.  Nothing
-// here branches by lane, so that many loads are in flight at once.
-template <typename E>
-__device__ inline Vec4<E> load4(const E* row, uint32_t c, uint32_t n, bool vec) {
-    if (vec) return *reinterpret_cast<const Vec4<E>*>(row + min(c, n - 4));
-    Vec4<E> y;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = row[min(c + j, n - 1)];
-    return y;
 }
 
 // Which sequence and chunk of it has record slot x: sequence n's chunks begin at
@@ -1443,10 +1502,10 @@ int k3x_hip_delta_rule(k3x_hip_ctx* ctx, const k3x_hip_delta_params* p, const vo
     a.vs = p->v_stride ? p->v_stride : vw;
     a.os = p->out_stride ? p->out_stride : vw;
     a.status = ctx->status;
+    // Four elements a load: rows and heads that keep the alignment.
+    const bool vec = a.K % 4 == 0 && a.qs % 4 == 0 && a.ks % 4 == 0 && aligned(q, 4 * es) &&
+                     aligned(k, 4 * es) && aligned(gate, 16);
     if (need) {
-        // Four elements a load: rows and heads that keep the alignment.
-        const bool vec = a.K % 4 == 0 && a.qs % 4 == 0 && a.ks % 4 == 0 && aligned(q, 4 * es) &&
-                         aligned(k, 4 * es) && aligned(gate, 16);
         const ChunkSpace space = chunk_space(p);
         const bool channel = p->gate == K3X_GATE_CHANNEL;
         return p->dtype == K3X_DTYPE_F32
@@ -1455,13 +1514,13 @@ int k3x_hip_delta_rule(k3x_hip_ctx* ctx, const k3x_hip_delta_params* p, const vo
                    ? launch_chunks_of<K3X_DTYPE_BF16>(ctx, a, workspace, space, channel, vec)
                    : launch_chunks_of<K3X_DTYPE_F16>(ctx, a, workspace, space, channel, vec);
     }
-    const uint32_t grid = a.N * a.H * ((a.V + kStepCols - 1) / kStepCols);
-    if (p->dtype == K3X_DTYPE_F32)
-        launch_step_rows<K3X_DTYPE_F32>(a, p->gate, grid, ctx->stream);
+    const uint32_t by_four = (vec ? 1 : 0) |
+                             (a.V % 4 == 0 && a.vs % 4 == 0 && aligned(v, 4 * es) ? 2 : 0) |
+                             (a.V % 4 == 0 ? 4 : 0);
+    if (p->dtype == K3X_DTYPE_F32) launch_step_rows<K3X_DTYPE_F32>(a, p->gate, by_four, ctx->stream);
     else if (p->dtype == K3X_DTYPE_BF16)
-        launch_step_rows<K3X_DTYPE_BF16>(a, p->gate, grid, ctx->stream);
-    else
-        launch_step_rows<K3X_DTYPE_F16>(a, p->gate, grid, ctx->stream);
+        launch_step_rows<K3X_DTYPE_BF16>(a, p->gate, by_four, ctx->stream);
+    else launch_step_rows<K3X_DTYPE_F16>(a, p->gate, by_four, ctx->stream);
     return launched(ctx, 1);
 }
 
