@@ -453,13 +453,6 @@ __device__ inline bool find_chunk(const DeltaArgs& a, uint32_t slot, ChunkPlace*
     return true;
 }
 
-// What a wave sees of another lane's LDS writes, in order.
-__device__ inline void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-}
-
 typedef float Tile32[kChunk][36];  // rows of 16-byte alignment that spread over the banks
 
 // T of a chunk from L (strictly lower triangular; overwritten), by one wave in

@@ -80,7 +80,38 @@ __device__ inline uint32_t route_check(const RouteArgs& a, float logit, float s,
                : K3X_ERR_INVALID_STATE;
 }
 
-// Any E: one wave a token, keys and scores in LDS, K passes over the keys.
+// x or, if that is larger, its neighbour's by the DPP control; the same for
+// the smaller one.
+template <int Ctrl>
+__device__ inline uint32_t dpp_max(uint32_t x) {
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, Ctrl, 0xf, 0xf, false));
+}
+template <int Ctrl>
+__device__ inline uint32_t dpp_min(uint32_t x) {
+    return min(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, Ctrl, 0xf, 0xf, false));
+}
+template <bool MAX>
+__device__ inline uint32_t across_rows(uint32_t x, bool halves) {
+    const auto r = halves ? __builtin_amdgcn_permlane32_swap(x, x, false, false)
+                          : __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return MAX ? max(r[0], r[1]) : min(r[0], r[1]);
+}
+
+// A bound that at least K keys reach: the smallest of the largest keys of the
+// 64 / n groups of n neighbouring lanes, n the largest with 64 / n >= K (head:
+// the lane's largest key).  Few others reach it, about 64 / n times its log.
+__device__ inline uint32_t reached_by(uint32_t head, uint32_t K) {
+    uint32_t x = head;
+    const uint32_t steps = K > 32 ? 0 : K > 16 ? 1 : K > 8 ? 2 : K > 4 ? 3 : K > 2 ? 4 : K > 1 ? 5 : 6;
+    x = steps > 0 ? dpp_max<0xb1>(x) : dpp_min<0xb1>(x);    // quad_perm [1,0,3,2]
+    x = steps > 1 ? dpp_max<0x4e>(x) : dpp_min<0x4e>(x);    // quad_perm [2,3,0,1]
+    x = steps > 2 ? dpp_max<0x141>(x) : dpp_min<0x141>(x);  // row_half_mirror
+    x = steps > 3 ? dpp_max<0x140>(x) : dpp_min<0x140>(x);  // row_mirror
+    x = steps > 4 ? across_rows<true>(x, false) : across_rows<false>(x, false);
+    return steps > 5 ? across_rows<true>(x, true) : across_rows<false>(x, true);
+}
+
+// More experts: one wave a token, keys and scores in LDS, K passes over the keys.
 template <uint32_t DT>
 __global__ __launch_bounds__(64) void route_lds_kernel(RouteArgs a) {
     extern __shared__ uint64_t keys[];  // [E], then the scores [E]
@@ -102,14 +133,14 @@ __global__ __launch_bounds__(64) void route_lds_kernel(RouteArgs a) {
         for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
         mx = __any(nan) ? (double)__builtin_nanf("") : (double)m;
         den = 0.0;
-        for (uint32_t e = lane; e < E; e += 64) den += exp((double)Elem<DT>::load(row[e]) - mx);
-        den = wave_sum_f64(den);
+        for (uint32_t e = lane; e < E; e += 64) den += exp_f64((double)Elem<DT>::load(row[e]) - mx);
+        den = 1.0 / wave_sum_f64(den);
     }
     uint32_t bad = 0;
     for (uint32_t e = lane; e < E; e += 64) {
         const float l = Elem<DT>::load(row[e]);
         const float b = a.bias ? a.bias[e] : 0.0f;
-        const float s = a.scoring == K3X_SCORE_SOFTMAX ? (float)(exp((double)l - mx) / den)
+        const float s = a.scoring == K3X_SCORE_SOFTMAX ? (float)(exp_f64((double)l - mx) * den)
                                                        : sigmoid_cr(l);
         const float adj = __fadd_rn(s, b);
         bad = max(bad, route_check(a, l, s, b, adj));
@@ -177,6 +208,160 @@ __global__ __launch_bounds__(64) void route_lds_kernel(RouteArgs a) {
     }
 }
 
+// E <= 64 KPL: a wave a token, lane l with experts l + 64 i in registers.  The
+// keys that reach a bound which K of them reach are written to LDS in the
+// experts' order, and each is ranked by counting those above it: a pass over a
+// few dozen keys in place of K passes over all.
+constexpr int kRouteWaves = 4;
+
+template <uint32_t DT, int KPL>
+__global__ __launch_bounds__(64 * kRouteWaves) void route_wave_kernel(RouteArgs a) {
+    typedef typename Elem<DT>::type T;
+    struct Wave {
+        uint64_t key[64 * KPL];
+        float score[64 * KPL];
+        uint32_t id[64];
+        float sel[64];
+    };
+    __shared__ Wave waves[kRouteWaves];
+    const uint32_t lane = threadIdx.x & 63, E = a.E;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t t = blockIdx.x * kRouteWaves + w;
+    if (t >= a.T) return;
+    Wave& s = waves[w];
+    const T* row = static_cast<const T*>(a.logits) + (size_t)t * a.stride;
+    float l[KPL], b[KPL], sc[KPL];
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        const uint32_t e = min(lane + 64u * i, E - 1);
+        l[i] = Elem<DT>::load(row[e]);
+        b[i] = a.bias ? a.bias[e] : 0.0f;
+    }
+    if (*(volatile uint32_t*)a.status) return;
+    if (a.scoring == K3X_SCORE_SOFTMAX) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+            const uint32_t u = __float_as_uint(l[i]);
+            top = max(top, (u & 0x80000000u) ? ~u : (u | 0x80000000u));
+        }
+        top = wave_max_u32(top);
+        const double mx = (double)__uint_as_float((top & 0x80000000u) ? (top & 0x7fffffffu) : ~top);
+        double e[KPL], den = 0.0;
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+            e[i] = lane + 64u * i < E ? exp_f64((double)l[i] - mx) : 0.0;
+            den += e[i];
+        }
+        const double inv = 1.0 / wave_sum_f64(den);
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) sc[i] = (float)(e[i] * inv);
+    } else {
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) sc[i] = sigmoid_cr(l[i]);
+    }
+    uint32_t bad = 0, ord[KPL];
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        const float adj = __fadd_rn(sc[i], b[i]);
+        const bool in = lane + 64u * i < E;
+        if (in) bad = max(bad, route_check(a, l[i], sc[i], b[i], adj));
+        ord[i] = in ? (uint32_t)(topk_key(adj, 0) >> 32) : 0u;
+    }
+    if (__any(bad)) {
+        bad = wave_max_u32(bad);
+        if (lane == 0) latch(a.status, bad);
+        return;
+    }
+    if (a.G > 1) {
+        // Several lanes a group: each takes every so many-th of its experts'
+        // keys, then they join their two largest.
+        uint32_t* keys = reinterpret_cast<uint32_t*>(s.key);
+#pragma unroll
+        for (int i = 0; i < KPL; ++i)
+            if (lane + 64u * i < E) keys[lane + 64u * i] = ord[i];
+        wave_sync();
+        const uint32_t n = E / a.G, width = 64u >> (32 - __clz(a.G - 1));  // lanes a group
+        const uint32_t g = lane / width;
+        uint32_t k1 = 0, k2 = 0;
+        if (g < a.G)
+            for (uint32_t i = lane % width; i < n; i += width) {
+                const uint32_t k = keys[g * n + i];
+                k2 = max(k2, min(k1, k));
+                k1 = max(k1, k);
+            }
+        for (uint32_t d = 1; d < width; d <<= 1) {
+            const uint32_t o1 = (uint32_t)__shfl_xor((int)k1, d);
+            const uint32_t o2 = (uint32_t)__shfl_xor((int)k2, d);
+            k2 = max(max(k2, o2), min(k1, o1));
+            k1 = max(k1, o1);
+        }
+        float gs = key_score((uint64_t)k1 << 32);
+        if (a.group_score == K3X_GROUP_TOP2 && n > 1)
+            gs = __fadd_rn(gs, key_score((uint64_t)k2 << 32));
+        const uint64_t gk = topk_key(gs, g);
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < a.G; ++i) rank += __shfl(gk, i * width) > gk;
+        const uint64_t kept = __ballot(g < a.G && rank < a.top_groups);
+#pragma unroll
+        for (int i = 0; i < KPL; ++i)
+            if (!(kept >> ((lane + 64u * i) / n * width & 63) & 1)) ord[i] = 0;
+        wave_sync();
+    }
+    uint32_t head = 0;
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) head = max(head, ord[i]);
+    const uint32_t bound = max(reached_by(head, a.K), 1u);
+    uint32_t count = 0;
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        const bool up = ord[i] >= bound;
+        const uint64_t mask = __ballot(up);
+        if (up) {
+            const uint32_t at = count + __builtin_amdgcn_mbcnt_hi(
+                                            (uint32_t)(mask >> 32),
+                                            __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+            s.key[at] = (uint64_t)ord[i] << 32 | (0xffffffffu - (lane + 64u * i));
+            s.score[at] = sc[i];
+        }
+        count += (uint32_t)__popcll(mask);
+    }
+    wave_sync();
+    for (uint32_t c0 = 0; c0 < count; c0 += 64) {
+        const uint32_t c = c0 + lane;
+        const uint64_t key = s.key[min(c, count - 1)];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < count; ++j) rank += s.key[j] > key;
+        if (c < count && rank < a.K) {
+            s.id[rank] = 0xffffffffu - (uint32_t)key;
+            s.sel[rank] = s.score[c];
+        }
+    }
+    wave_sync();
+    const float selsc = lane < a.K ? s.sel[lane] : 0.0f;
+    uint32_t err;
+    const float weight = route_weight(a, selsc, &err);
+    if (err) {
+        if (lane == 0) latch(a.status, err);
+        return;
+    }
+    if (lane < a.K) {
+        a.ids[(size_t)t * a.K + lane] = s.id[lane];
+        a.weights[(size_t)t * a.K + lane] = weight;
+    }
+}
+
+template <uint32_t DT>
+void launch_route(const RouteArgs& a, hipStream_t stream) {
+    const dim3 grid((a.T + kRouteWaves - 1) / kRouteWaves), block(64 * kRouteWaves);
+    if (a.E <= 256) hipLaunchKernelGGL((route_wave_kernel<DT, 4>), grid, block, 0, stream, a);
+    else if (a.E <= 512) hipLaunchKernelGGL((route_wave_kernel<DT, 8>), grid, block, 0, stream, a);
+    else if (a.E <= 1024)
+        hipLaunchKernelGGL((route_wave_kernel<DT, 16>), grid, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL(route_lds_kernel<DT>, dim3(a.T), dim3(64), (size_t)a.E * 12, stream, a);
+}
+
 bool route_ok(const k3x_hip_route_params* p) {
     if (!p->tokens || p->tokens > (1u << 20) || !p->experts || p->experts > 4096 || !p->top_k ||
         p->top_k > 64 || p->dtype > K3X_DTYPE_BF16 || p->scoring > K3X_SCORE_SOFTMAX ||
@@ -216,12 +401,8 @@ int k3x_hip_route(k3x_hip_ctx* ctx, const k3x_hip_route_params* p, const void* l
     a.ids = ids;
     a.weights = weights;
     a.status = ctx->status;
-    if (p->dtype == K3X_DTYPE_F32)
-        hipLaunchKernelGGL(route_lds_kernel<K3X_DTYPE_F32>, dim3(a.T), dim3(64),
-                           (size_t)a.E * 12, ctx->stream, a);
-    else
-        hipLaunchKernelGGL(route_lds_kernel<K3X_DTYPE_BF16>, dim3(a.T), dim3(64),
-                           (size_t)a.E * 12, ctx->stream, a);
+    if (p->dtype == K3X_DTYPE_F32) launch_route<K3X_DTYPE_F32>(a, ctx->stream);
+    else launch_route<K3X_DTYPE_BF16>(a, ctx->stream);
     return launched(ctx, 1);
 }
 

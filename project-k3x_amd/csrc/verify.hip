@@ -1,10 +1,16 @@
 // verify.hip -- verification of drafted tokens against the target's rows.
 //
-// Four launches: each row's parts (largest entry, sum of exponentials), the
-// accepted count of each sequence, the parts' sums of the distribution that
-// its next token is drawn from, and the draw.  Everything that a choice
-// rests on is formed in double: the sums run over a whole vocabulary, and
-// the drawn token sits next to a border of the cumulative sum.
+//   rows     each row by parts of 4096 entries: the largest entry and the sum of
+//            exponentials over it (logits, and greedy choices);
+//   accept   one workgroup a sequence: every row's totals and drafted token's
+//            probabilities at once, then the walk over the drafts;
+//   draw     the row that the next token is drawn from, by the same parts: their
+//            sums, and by the sequence's last workgroup the part and the entry
+//            that the border falls in.
+//
+// Everything that a choice rests on is formed in double: the sums run over a
+// whole vocabulary, and a drawn token lies next to a border of the cumulative
+// sum (at 10^5 entries a sum off by 10^-9 moves one draw in 10^4).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -18,22 +24,22 @@ using namespace k3x_ops;
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMaxParts = 64;  // parts of a row
-constexpr uint32_t kPartEntries = 4096;
+constexpr uint32_t kEntries = 16;  // of a part, a thread
+constexpr uint32_t kPart = kThreads * kEntries;
+constexpr uint32_t kMaxDrafts = 64;
 
-// A row's entries [part * len, ...) by workgroup.  max NaN: the part holds an
-// entry that no row may.
+// One part of a row; max NaN: it holds an entry that no row may.
 struct RowPart {
-    double sum;        // sum of exp((l - max) / temperature)
+    double sum;    // of exp((l - max) / temperature)
     float max;
-    uint32_t arg;      // first entry that is max
+    uint32_t arg;  // first entry that is max
 };
 
-// What the draw needs of sequence n.
+// What the draw needs of a sequence.
 struct Drawn {
-    uint32_t accepted, rows;  // rows: drafts of this sequence
-    uint32_t bad;             // status to latch, 0
-    uint32_t next;            // greedy: the next token
+    uint32_t accepted, rows;  // rows: drafts of this sequence, or K3X_VERIFY_SKIP
+    uint32_t done;            // its result is out (or it is unfit)
+    uint32_t arrived;         // workgroups of the draw that have written their sum
     double pmax, pinv, qmax, qinv;
 };
 
@@ -43,12 +49,13 @@ struct VerifyArgs {
     const float *accept_u, *sample_u;
     uint32_t *accepted, *out_tokens;
     uint32_t N, D, V, stride;
-    uint32_t parts, part_len;
+    uint32_t parts;
     uint32_t form, greedy;
-    double temperature;
-    RowPart* row_parts;   // [N (2 D + 1)][parts]: a sequence's target rows, then its draft's
-    Drawn* drawn;         // [N]
-    double* sums;         // [N][parts]
+    uint32_t vec;       // rows by 16 bytes
+    double inv_temperature;
+    RowPart* row_parts; // [N (2 D + 1)][parts]: a sequence's target rows, then its draft's
+    Drawn* drawn;       // [N]
+    double* sums;       // [N][parts]
     uint32_t* status;
 };
 
@@ -76,6 +83,44 @@ __device__ inline void take_max(float& m, uint32_t& i, float om, uint32_t oi) {
     }
 }
 
+// A thread's sixteen entries of a part, neighbours by 16 bytes where rows are,
+// so that a wave's loads are whole lines; where() rises with j.
+template <uint32_t DT>
+struct Entries {
+    typedef typename Elem<DT>::type E;
+    static constexpr uint32_t kWide = 16 / sizeof(E);
+    static __device__ inline uint32_t where(const VerifyArgs& a, uint32_t lo, int j) {
+        return a.vec ? lo + j / kWide * (kThreads * kWide) + threadIdx.x * kWide + j % kWide
+                     : lo + j * kThreads + threadIdx.x;
+    }
+    // Past hi: `past`.
+    static __device__ inline void load(const VerifyArgs& a, const E* x, uint32_t lo, uint32_t hi,
+                                       float past, float (&l)[kEntries]) {
+        typedef E Vec __attribute__((ext_vector_type(kWide)));
+        if (a.vec && lo + kPart <= hi) {
+#pragma unroll
+            for (int j = 0; j < (int)kEntries; j += kWide) {
+                const Vec v = *reinterpret_cast<const Vec*>(x + where(a, lo, j));
+#pragma unroll
+                for (int y = 0; y < (int)kWide; ++y) l[j + y] = Elem<DT>::load(v[y]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < (int)kEntries; ++j) {
+                const uint32_t i = where(a, lo, j);
+                l[j] = Elem<DT>::load(x[min(i, hi - 1)]);
+                if (i >= hi) l[j] = past;
+            }
+        }
+    }
+};
+
+__device__ inline double wave_sum(double v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
 template <uint32_t DT>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a) {
     __shared__ float sm[kThreads / 64];
@@ -85,18 +130,27 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a) {
     const uint32_t rows = a.draft ? 2 * a.D + 1 : a.D + 1;
     const uint32_t n = rr / rows, r = rr % rows, tid = threadIdx.x, wave = tid >> 6;
     const uint32_t count = drafts_of(a, n);
-    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
     if (count > a.D || (r <= a.D ? r > count : r - a.D - 1 >= count)) return;
-    const auto* x = row_of<DT>(a, n, r);
-    const uint32_t lo = part * a.part_len, hi = min(a.V, lo + a.part_len);
+    const uint32_t lo = part * kPart, hi = min(a.V, lo + kPart);
+    float l[kEntries];
+    Entries<DT>::load(a, row_of<DT>(a, n, r), lo, hi, -__builtin_inff(), l);
+    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
     float m = -__builtin_inff();
     uint32_t arg = 0xffffffffu;
     bool wrong = false;
-    for (uint32_t i = lo + tid; i < hi; i += kThreads) {
-        const float l = Elem<DT>::load(x[i]);
-        wrong |= !(l < __builtin_inff()) || (a.form == K3X_DIST_PROBS && l < 0.0f);
-        take_max(m, arg, l, i);
+#pragma unroll
+    for (int j = 0; j < (int)kEntries; ++j) {
+        // Past the row's end minus infinity: no entry of a row of
+        // probabilities, but not one that is looked at either.
+        const bool past = Entries<DT>::where(a, lo, j) >= hi;
+        wrong |= !(l[j] < __builtin_inff()) ||
+                 (a.form == K3X_DIST_PROBS && l[j] < 0.0f && !past);
+        if (l[j] > m) {
+            m = l[j];
+            arg = Entries<DT>::where(a, lo, j);
+        }
     }
+#pragma unroll
     for (int d = 1; d < 64; d <<= 1)
         take_max(m, arg, __shfl_xor(m, d), (uint32_t)__shfl_xor((int)arg, d));
     if ((tid & 63) == 0) {
@@ -104,90 +158,141 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a) {
         si[wave] = arg;
     }
     wrong = __syncthreads_or(wrong);
+#pragma unroll
     for (uint32_t w = 0; w < kThreads / 64; ++w) take_max(m, arg, sm[w], si[w]);
     double s = 0.0;
-    if (!a.greedy && m > -__builtin_inff())
-        for (uint32_t i = lo + tid; i < hi; i += kThreads)
-            s += exp(((double)Elem<DT>::load(x[i]) - (double)m) / a.temperature);
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    if ((tid & 63) == 0) sd[wave] = s;
-    __syncthreads();
-    if (tid) return;
-    s = 0.0;
-    for (uint32_t w = 0; w < kThreads / 64; ++w) s += sd[w];
-    a.row_parts[part_index(a, n, r) + part] =
-        RowPart{s, wrong ? __builtin_nanf("") : m, arg};
+    if (!a.greedy && m > -__builtin_inff()) {
+#pragma unroll
+        for (int j = 0; j < (int)kEntries; ++j)
+            s += exp_f64(((double)l[j] - (double)m) * a.inv_temperature);
+        s = wave_sum(s);
+        if ((tid & 63) == 0) sd[wave] = s;
+        __syncthreads();
+        s = sd[0] + sd[1] + sd[2] + sd[3];
+    }
+    if (tid == 0)
+        a.row_parts[part_index(a, n, r) + part] = RowPart{s, wrong ? __builtin_nanf("") : m, arg};
 }
 
-// A row's largest entry and 1 / sum from its parts, by a wave (lane = part);
-// false: the row is unfit.
+// A row's largest entry and 1 / sum from its parts, by a wave; false: the row
+// is unfit.
 __device__ inline bool row_total(const VerifyArgs& a, uint32_t n, uint32_t r, double* mx,
                                  double* inv, uint32_t* arg) {
     const uint32_t lane = threadIdx.x & 63;
-    RowPart p{0.0, -__builtin_inff(), 0xffffffffu};
-    if (lane < a.parts) p = a.row_parts[part_index(a, n, r) + lane];
-    if (__any(p.max != p.max)) return false;
-    float m = p.max;
-    uint32_t at = p.arg;
+    const RowPart* parts = a.row_parts + part_index(a, n, r);
+    float m = -__builtin_inff();
+    uint32_t at = 0xffffffffu;
+    bool nan = false;
+    for (uint32_t i = lane; i < a.parts; i += 64) {
+        nan |= parts[i].max != parts[i].max;
+        take_max(m, at, parts[i].max, parts[i].arg);
+    }
+    if (__any(nan)) return false;
+#pragma unroll
     for (int d = 1; d < 64; d <<= 1)
         take_max(m, at, __shfl_xor(m, d), (uint32_t)__shfl_xor((int)at, d));
     if (m == -__builtin_inff() || (a.form == K3X_DIST_PROBS && m == 0.0f)) return false;
-    double s = p.sum > 0.0 ? p.sum * exp(((double)p.max - (double)m) / a.temperature) : 0.0;
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+    double s = 0.0;
+    if (!a.greedy)
+        for (uint32_t i = lane; i < a.parts; i += 64)
+            if (parts[i].sum > 0.0)
+                s += parts[i].sum *
+                     exp_f64(((double)parts[i].max - (double)m) * a.inv_temperature);
     *mx = m;
-    *inv = 1.0 / s;
+    *inv = 1.0 / wave_sum(s);
     *arg = at;
     return true;
 }
 
 __device__ inline double prob(const VerifyArgs& a, float l, double mx, double inv) {
-    return a.form == K3X_DIST_PROBS ? (double)l : exp(((double)l - mx) / a.temperature) * inv;
+    return a.form == K3X_DIST_PROBS ? (double)l
+                                    : exp_f64(((double)l - mx) * a.inv_temperature) * inv;
 }
 
-// One wave a sequence walks its drafts (every lane the same).
+// One workgroup a sequence: a wave a row, the drafts' rows together.
 template <uint32_t DT>
-__global__ __launch_bounds__(64) void verify_accept_kernel(VerifyArgs a) {
-    if (*(volatile uint32_t*)a.status) return;
-    const uint32_t n = blockIdx.x;
+__global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a) {
+    struct Row {
+        double max, inv, prob;  // prob: of the drafted token
+        uint32_t arg, fit;
+    };
+    __shared__ Row rows[2 * kMaxDrafts + 1];
+    __shared__ uint32_t verdict;
+    const uint32_t n = blockIdx.x, tid = threadIdx.x;
+    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
     const uint32_t count = drafts_of(a, n);
-    Drawn d{};
-    d.rows = count;
-    d.pinv = d.qinv = 1.0;
+    uint32_t* out = a.out_tokens + (size_t)n * (a.D + 1);
+    if (count > a.D) {  // left out, or out of range
+        if (count == K3X_VERIFY_SKIP) {
+            for (uint32_t i = tid; i <= a.D; i += blockDim.x) out[i] = 0xffffffffu;
+            if (tid == 0) a.accepted[n] = 0;
+        } else if (tid == 0) {
+            latch(a.status, K3X_ERR_INVALID_STATE);
+        }
+        if (tid == 0) a.drawn[n].done = 1;
+        return;
+    }
     const bool totals = a.form == K3X_DIST_LOGITS || a.greedy;
-    uint32_t arg = 0, i = 0;
-    if (count > a.D && count != K3X_VERIFY_SKIP) d.bad = K3X_ERR_INVALID_STATE;
-    for (; !d.bad && count != K3X_VERIFY_SKIP; ++i) {
-        if (totals && !row_total(a, n, i, &d.pmax, &d.pinv, &arg)) d.bad = K3X_ERR_INVALID_STATE;
-        if (d.bad || i == count) break;
-        const uint32_t x = a.tokens[(size_t)n * a.D + i];
-        if (x >= a.V) {
-            d.bad = K3X_ERR_INVALID_STATE;
-            break;
-        }
-        if (a.greedy) {
-            if (arg != x) break;
-            continue;
-        }
-        const float u = a.accept_u[(size_t)n * a.D + i];
-        const double p = prob(a, Elem<DT>::load(row_of<DT>(a, n, i)[x]), d.pmax, d.pinv);
-        double q = 1.0;
-        if (a.draft) {
-            if (totals && !row_total(a, n, a.D + 1 + i, &d.qmax, &d.qinv, &arg)) {
-                d.bad = K3X_ERR_INVALID_STATE;
+    // Target rows 0 .. count, then the draft's.
+    const uint32_t all = count + 1 + (a.draft ? count : 0);
+    for (uint32_t i = tid >> 6; i < all; i += blockDim.x >> 6) {
+        const bool target = i <= count;
+        const uint32_t d = target ? i : i - count - 1, r = target ? i : a.D + 1 + d;
+        const uint32_t x = d < count ? a.tokens[(size_t)n * a.D + d] : 0;
+        const float l = x < a.V && !a.greedy ? Elem<DT>::load(row_of<DT>(a, n, r)[x]) : 0.0f;
+        Row row{0.0, 1.0, 0.0, 0, 1};
+        if (totals) row.fit = row_total(a, n, r, &row.max, &row.inv, &row.arg);
+        if (row.fit && !a.greedy) row.prob = prob(a, l, row.max, row.inv);
+        if ((tid & 63) == 0) rows[i] = row;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t bad = 0, i = 0;
+        for (;; ++i) {
+            const Row& p = rows[i];
+            if (!p.fit) bad = 1;
+            if (bad || i == count) break;
+            const uint32_t x = a.tokens[(size_t)n * a.D + i];
+            if (x >= a.V) {
+                bad = 1;
                 break;
             }
-            q = prob(a, Elem<DT>::load(row_of<DT>(a, n, a.D + 1 + i)[x]), d.qmax, d.qinv);
+            if (a.greedy) {
+                if (p.arg != x) break;
+                continue;
+            }
+            const float u = a.accept_u[(size_t)n * a.D + i];
+            const Row one{0.0, 1.0, 1.0, 0, 1};
+            const Row& q = a.draft ? rows[count + 1 + i] : one;
+            if (!q.fit || !(u >= 0.0f && u < 1.0f) ||
+                !(p.prob >= 0.0 && p.prob < __builtin_inf()) ||
+                !(q.prob >= 0.0 && q.prob < __builtin_inf())) {
+                bad = 1;
+                break;
+            }
+            if (!((double)u * q.prob < p.prob)) break;
         }
-        if (!(u >= 0.0f && u < 1.0f) || !(p >= 0.0 && p < __builtin_inf()) ||
-            !(q >= 0.0 && q < __builtin_inf())) {
-            d.bad = K3X_ERR_INVALID_STATE;
-            break;
+        if (bad) latch(a.status, K3X_ERR_INVALID_STATE);
+        Drawn d{};
+        d.accepted = i;
+        d.rows = count;
+        d.done = bad || a.greedy;
+        d.pmax = rows[i].max;
+        d.pinv = rows[i].inv;
+        if (a.draft && i < count) {
+            d.qmax = rows[count + 1 + i].max;
+            d.qinv = rows[count + 1 + i].inv;
         }
-        if (!((double)u * q < p)) break;
+        a.drawn[n] = d;
+        if (!bad && a.greedy) a.accepted[n] = i;
+        verdict = bad ? 0xffffffffu : i;
     }
-    d.accepted = count == K3X_VERIFY_SKIP ? 0 : i;
-    d.next = arg;
-    if (threadIdx.x == 0) a.drawn[n] = d;
+    __syncthreads();
+    if (!a.greedy || verdict == 0xffffffffu) return;
+    for (uint32_t i = tid; i <= a.D; i += blockDim.x)
+        out[i] = i < verdict    ? a.tokens[(size_t)n * a.D + i]
+                 : i == verdict ? rows[verdict].arg
+                                : 0xffffffffu;
 }
 
 // The distribution that sequence n's next token is drawn from: entry i is
@@ -209,11 +314,14 @@ struct Rest {
         qmax = d.qmax;
         qinv = d.qinv;
     }
-    __device__ inline double at(const VerifyArgs& a, uint32_t i) const {
-        const double r = prob(a, Elem<DT>::load(p[i]), pmax, pinv);
-        const double o = q ? prob(a, Elem<DT>::load(q[i]), qmax, qinv) : 0.0;
+    __device__ inline double of(const VerifyArgs& a, uint32_t i, float pl, float ql) const {
+        const double r = prob(a, pl, pmax, pinv);
+        const double o = q ? prob(a, ql, qmax, qinv) : 0.0;
         if (!(r >= 0.0 && o >= 0.0 && o < __builtin_inf())) return __builtin_nan("");
         return i == token || r <= o ? 0.0 : r - o;
+    }
+    __device__ inline double at(const VerifyArgs& a, uint32_t i) const {
+        return of(a, i, Elem<DT>::load(p[i]), q ? Elem<DT>::load(q[i]) : 0.0f);
     }
     // Only the target's probabilities.
     __device__ inline void whole() {
@@ -223,47 +331,39 @@ struct Rest {
 };
 
 __device__ inline double block_sum(double s, double* sd) {
-    for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+    s = wave_sum(s);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sd[threadIdx.x >> 6] = s;
     __syncthreads();
-    s = 0.0;
-    for (uint32_t w = 0; w < kThreads / 64; ++w) s += sd[w];
-    return s;
-}
-
-template <uint32_t DT>
-__global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
-    __shared__ double sd[kThreads / 64];
-    const uint32_t part = blockIdx.x % a.parts, n = blockIdx.x / a.parts, tid = threadIdx.x;
-    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
-    const Drawn d = a.drawn[n];
-    if (d.bad || d.rows == K3X_VERIFY_SKIP) return;
-    const Rest<DT> rest(a, d, n);
-    const uint32_t lo = part * a.part_len, hi = min(a.V, lo + a.part_len);
-    double s = 0.0;
-    for (uint32_t i = lo + tid; i < hi; i += kThreads) s += rest.at(a, i);
-    s = block_sum(s, sd);
-    if (tid == 0) a.sums[(size_t)n * a.parts + part] = s;
+    return sd[0] + sd[1] + sd[2] + sd[3];
 }
 
 // The token of [lo, hi) that the border falls in: the last entry over 0 that
-// the cumulative sum (start before lo) has not passed the border before.
-// By the whole workgroup; the range holds an entry over 0 and start <= border.
+// the cumulative sum (start before lo) has not passed the border before.  By the
+// whole workgroup, a run of entries a thread; the range holds an entry over 0
+// and start <= border.
 template <uint32_t DT>
 __device__ inline uint32_t draw_token(const VerifyArgs& a, const Rest<DT>& rest, uint32_t lo,
                                       uint32_t hi, double start, double border, double* sd,
                                       uint32_t* found) {
-    const uint32_t tid = threadIdx.x, per = (hi - lo + kThreads - 1) / kThreads;
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint32_t per = (hi - lo + kThreads - 1) / kThreads;
     const uint32_t b = min(hi, lo + tid * per), e = min(hi, b + per);
     double s = 0.0;
     for (uint32_t i = b; i < e; ++i) s += rest.at(a, i);
+    double c = s;  // of this and the wave's threads before
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double o = __shfl_up(c, d);
+        if (lane >= (uint32_t)d) c += o;
+    }
     __syncthreads();
-    sd[tid] = s;
+    if (lane == 63) sd[tid >> 6] = c;
     if (tid == 0) *found = 0;
     __syncthreads();
-    double c = start;
-    for (uint32_t w = 0; w < tid; ++w) c += sd[w];
+    c = __shfl_up(c, 1);
+    c = start + (lane ? c : 0.0);
+    for (uint32_t w = 0; w < tid >> 6; ++w) c += sd[w];
     uint32_t hit = 0;
     for (uint32_t i = b; i < e && c <= border; ++i) {
         const double r = rest.at(a, i);
@@ -275,101 +375,128 @@ __device__ inline uint32_t draw_token(const VerifyArgs& a, const Rest<DT>& rest,
     return *found - 1;
 }
 
-// One workgroup a sequence: the part that the drawn border falls in, then the
-// entry, then the sequence's outputs.
 template <uint32_t DT>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
-    __shared__ double sd[kThreads];
-    __shared__ uint32_t found;
-    const uint32_t n = blockIdx.x, tid = threadIdx.x;
+    __shared__ double sd[kThreads / 64];
+    __shared__ uint32_t found, last;
+    const uint32_t part = blockIdx.x % a.parts, n = blockIdx.x / a.parts, tid = threadIdx.x;
     if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
     const Drawn d = a.drawn[n];
-    uint32_t* out = a.out_tokens + (size_t)n * (a.D + 1);
-    if (d.rows == K3X_VERIFY_SKIP) {
-        if (tid == 0) a.accepted[n] = 0;
-        if (tid <= a.D) out[tid] = 0xffffffffu;
-        return;
-    }
-    uint32_t bad = d.bad, next = d.next;
-    if (!bad && !a.greedy) {
-        const float u = a.sample_u[n];
-        double total = 0.0;
-        for (uint32_t i = 0; i < a.parts; ++i) total += a.sums[(size_t)n * a.parts + i];
-        if (!(u >= 0.0f && u < 1.0f) || !(total >= 0.0 && total < __builtin_inf())) {
-            bad = K3X_ERR_INVALID_STATE;
-        } else {
-            Rest<DT> rest(a, d, n);
-            uint32_t lo = 0, hi = a.V;
-            double start = 0.0, border = (double)u * total;
-            if (total > 0.0) {
-                double before = 0.0;
-                uint32_t part = 0;
-                for (uint32_t i = 0; i < a.parts; ++i) {
-                    const double s = a.sums[(size_t)n * a.parts + i];
-                    if (s > 0.0 && before <= border) {
-                        part = i;
-                        start = before;
-                    }
-                    before += s;
-                }
-                lo = part * a.part_len;
-                hi = min(a.V, lo + a.part_len);
-            } else {
-                // Nothing is left over q (or of a row without its drafted
-                // token): the target's own probabilities.
-                rest.whole();
-                double s = 0.0;
-                for (uint32_t i = tid; i < a.V; i += kThreads) s += rest.at(a, i);
-                total = block_sum(s, sd);
-                border = (double)u * total;
-                if (!(total > 0.0 && total < __builtin_inf())) bad = K3X_ERR_INVALID_STATE;
-            }
-            if (!bad) next = draw_token<DT>(a, rest, lo, hi, start, border, sd, &found);
+    if (d.done) return;
+    Rest<DT> rest(a, d, n);
+    const uint32_t lo = part * kPart, hi = min(a.V, lo + kPart);
+    {
+        float pl[kEntries], ql[kEntries] = {};
+        const float past = a.form == K3X_DIST_PROBS ? 0.0f : -__builtin_inff();
+        Entries<DT>::load(a, rest.p, lo, hi, past, pl);
+        if (rest.q) Entries<DT>::load(a, rest.q, lo, hi, past, ql);
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < (int)kEntries; ++j)
+            s += rest.of(a, Entries<DT>::where(a, lo, j), pl[j], ql[j]);
+        s = block_sum(s, sd);
+        // The sum, then the arrival: the last workgroup sees every sum.
+        if (tid == 0) {
+            __hip_atomic_store(a.sums + (size_t)n * a.parts + part, s, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+            last = __hip_atomic_fetch_add(&a.drawn[n].arrived, 1u, __ATOMIC_ACQ_REL,
+                                          __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
         }
+        __syncthreads();
+        if (!last) return;
+    }
+    // Parts by lane, in order: their sums and what lies before each.
+    const uint32_t lane = tid & 63;
+    double total = 0.0, start = 0.0;
+    uint32_t bad = 0, next = 0;
+    const float u = a.sample_u[n];
+    uint32_t* out = a.out_tokens + (size_t)n * (a.D + 1);
+    double run[4], own[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const uint32_t i = 64 * x + lane;
+        own[x] = i < a.parts ? __hip_atomic_load(a.sums + (size_t)n * a.parts + i,
+                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                             : 0.0;
+        double c = own[x];
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) {
+            const double o = __shfl_up(c, k);
+            if (lane >= (uint32_t)k) c += o;
+        }
+        run[x] = total + (c - own[x]);
+        total += __shfl(c, 63);
+    }
+    if (!(u >= 0.0f && u < 1.0f) || !(total >= 0.0 && total < __builtin_inf())) bad = 1;
+    if (!bad) {
+        uint32_t from = 0, to = a.V;
+        double border = (double)u * total;
+        if (total > 0.0) {
+            // The last part over 0 that starts at the border or before.
+            uint32_t in = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint64_t mask = __ballot(own[x] > 0.0 && run[x] <= border);
+                if (!mask) continue;
+                const int l = 63 - __clzll((unsigned long long)mask);
+                in = 64 * x + l;
+                start = __shfl(run[x], l);
+            }
+            from = in * kPart;
+            to = min(a.V, from + kPart);
+        } else {
+            // Nothing is left over q (or of a row without its drafted token):
+            // the target's own probabilities.
+            rest.whole();
+            double s = 0.0;
+            for (uint32_t i = tid; i < a.V; i += kThreads) s += rest.at(a, i);
+            total = block_sum(s, sd);
+            border = (double)u * total;
+            if (!(total > 0.0 && total < __builtin_inf())) bad = 1;
+        }
+        if (!bad) next = draw_token<DT>(a, rest, from, to, start, border, sd, &found);
     }
     if (bad) {
-        if (tid == 0) latch(a.status, bad);
+        if (tid == 0) latch(a.status, K3X_ERR_INVALID_STATE);
         return;
     }
     if (tid == 0) a.accepted[n] = d.accepted;
-    if (tid <= a.D)
-        out[tid] = tid < d.accepted    ? a.tokens[(size_t)n * a.D + tid]
-                   : tid == d.accepted ? next
-                                       : 0xffffffffu;
+    for (uint32_t i = tid; i <= a.D; i += kThreads)
+        out[i] = i < d.accepted    ? a.tokens[(size_t)n * a.D + i]
+                 : i == d.accepted ? next
+                                   : 0xffffffffu;
 }
 
 template <uint32_t DT>
 int launch_verify(k3x_hip_ctx* ctx, const VerifyArgs& a) {
-    unsigned launches = 2;
+    unsigned launches = 1;
+    const uint32_t rows = a.draft ? 2 * a.D + 1 : a.D + 1;
     if (a.form == K3X_DIST_LOGITS || a.greedy) {
-        const uint32_t rows = a.draft ? 2 * a.D + 1 : a.D + 1;
         hipLaunchKernelGGL(verify_rows_kernel<DT>, dim3(a.N * rows * a.parts), dim3(kThreads), 0,
                            ctx->stream, a);
         ++launches;
     }
-    hipLaunchKernelGGL(verify_accept_kernel<DT>, dim3(a.N), dim3(64), 0, ctx->stream, a);
+    hipLaunchKernelGGL(verify_accept_kernel<DT>, dim3(a.N), dim3(64 * std::min(rows, 16u)), 0,
+                       ctx->stream, a);
     if (!a.greedy) {
-        hipLaunchKernelGGL(verify_sums_kernel<DT>, dim3(a.N * a.parts), dim3(kThreads), 0,
+        hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3(a.N * a.parts), dim3(kThreads), 0,
                            ctx->stream, a);
         ++launches;
     }
-    hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3(a.N), dim3(kThreads), 0, ctx->stream, a);
     return launched(ctx, launches);
 }
 
+uint32_t parts_of(const k3x_hip_verify_params* p) { return (p->vocab + kPart - 1) / kPart; }
+
 bool verify_ok(const k3x_hip_verify_params* p) {
-    return p->sequences && p->sequences <= 65535 && p->drafts <= 64 && p->vocab &&
+    return p->sequences && p->sequences <= 65535 && p->drafts <= kMaxDrafts && p->vocab &&
            p->vocab <= (1u << 20) && p->dtype <= K3X_DTYPE_BF16 && p->form <= K3X_DIST_PROBS &&
            p->greedy <= 1 && std::isfinite(p->temperature) && p->temperature > 0.0f &&
            (!p->row_stride || p->row_stride >= p->vocab) &&
-           (uint64_t)p->sequences * (2 * p->drafts + 1) * kMaxParts < (1ull << 31);
+           (uint64_t)p->sequences * (2 * p->drafts + 1) * parts_of(p) < (1ull << 31);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-
-uint32_t parts_of(const k3x_hip_verify_params* p) {
-    return std::min((p->vocab + kPartEntries - 1) / kPartEntries, kMaxParts);
-}
 
 }  // namespace
 
@@ -413,10 +540,10 @@ int k3x_hip_verify_draft(k3x_hip_ctx* ctx, const k3x_hip_verify_params* p, const
     a.V = p->vocab;
     a.stride = p->row_stride ? p->row_stride : p->vocab;
     a.parts = parts_of(p);
-    a.part_len = (a.V + a.parts - 1) / a.parts;
+    a.vec = a.stride * es % 16 == 0 && aligned(target, 16) && aligned(draft, 16);
     a.form = p->form;
     a.greedy = p->greedy;
-    a.temperature = p->temperature;
+    a.inv_temperature = 1.0 / p->temperature;
     uint8_t* w = static_cast<uint8_t*>(workspace);
     a.row_parts = reinterpret_cast<RowPart*>(w);
     w += up256((size_t)a.N * (2 * a.D + 1) * a.parts * sizeof(RowPart));

@@ -587,39 +587,50 @@ def expert_major_plan(ctx: Context, ids, tokens, top_k, experts, taps: dict) -> 
                                              C.byref(t))
 
 
+_TYPES: dict = {}  # torch's types, once it is imported
+
+
+def _types() -> dict:
+    if not _TYPES:
+        import torch
+        _TYPES.update(
+            codes={torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16},
+            ints=(torch.int32, torch.uint32), f32=(torch.float32,),
+            logits=(torch.float32, torch.bfloat16))
+    return _TYPES
+
+
 def _dtype(t) -> int:
-    import torch
-    codes = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
-    if t.dtype not in codes:
+    code = _types()["codes"].get(t.dtype)
+    if code is None:
         raise ValueError(f"expected float32, bfloat16 or float16, not {t.dtype}")
-    return codes[t.dtype]
+    return code
 
 
 def _expect(what: str, t, shape, dtypes) -> None:
-    """A tensor of the shape and of one of the types (None passes)."""
-    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype not in dtypes):
-        raise ValueError(f"{what}: expected {tuple(shape)} of {dtypes}, not {tuple(t.shape)} of "
+    """A tensor of the shape and of one of the types."""
+    if t.shape != shape or t.dtype not in dtypes:
+        raise ValueError(f"{what}: expected {shape} of {dtypes}, not {tuple(t.shape)} of "
                          f"{t.dtype}")
 
 
 def _rows(t):
-    """Device pointer of rows that are contiguous in themselves (any distance between rows)."""
-    if t is None or t.is_contiguous():
-        return ptr(t)
+    """(device pointer, elements from row to row) of rows that are contiguous in themselves; the
+    distance is 0 where it is the row's length or there is one row."""
     if not t.is_cuda:
         raise ValueError("expected a device tensor")
-    if not _row_contiguous(t):
-        raise ValueError("expected rows that are contiguous in themselves")
-    return t.data_ptr()
-
-
-def _row_contiguous(t) -> bool:
-    return t.stride(0) >= t[0].numel() and t[0].is_contiguous()
+    if t.is_contiguous():
+        return t.data_ptr(), 0
+    return t.data_ptr(), _row_stride(t)
 
 
 def _row_stride(t) -> int:
-    """Elements from row to row; 0 where that is the row's length or there is one row."""
-    return 0 if t.shape[0] < 2 or t.is_contiguous() else t.stride(0)
+    if t.is_contiguous():
+        return 0
+    row = t[0]
+    if not row.is_contiguous() or (t.shape[0] > 1 and t.stride(0) < row.numel()):
+        raise ValueError("expected rows that are contiguous in themselves")
+    return t.stride(0) if t.shape[0] > 1 else 0
 
 
 def make_route_params(tokens, experts, top_k, scoring=SCORE_SIGMOID, renorm=RENORM_FLOAT,
@@ -633,28 +644,28 @@ def make_route_params(tokens, experts, top_k, scoring=SCORE_SIGMOID, renorm=RENO
 def route(ctx: Context, params: RouteParams, logits, ids, weights, bias=None) -> int:
     """ids [T][K] (int32) and weights [T][K] (fp32) from router logits [T][E] (fp32 or bf16)
     and the fp32 bias [E] (k3x_hip_route)."""
-    import torch
-    T, E, K = params.tokens, params.experts, params.top_k
-    _expect("logits", logits, (T, E), (torch.float32, torch.bfloat16))
-    _expect("bias", bias, (E,), (torch.float32,))
-    _expect("ids", ids, (T, K), (torch.int32, torch.uint32))
-    _expect("weights", weights, (T, K), (torch.float32,))
+    T, E, K, types = params.tokens, params.experts, params.top_k, _types()
+    _expect("logits", logits, (T, E), types["logits"])
+    if bias is not None:
+        _expect("bias", bias, (E,), types["f32"])
+    _expect("ids", ids, (T, K), types["ints"])
+    _expect("weights", weights, (T, K), types["f32"])
     p = RouteParams.from_buffer_copy(params)
-    p.dtype, p.logits_stride = _dtype(logits), _row_stride(logits)
-    return ctx.lib.k3x_hip_route(ctx.handle, C.byref(p), _rows(logits), ptr(bias), ptr(ids),
-                                 ptr(weights))
+    at, p.logits_stride = _rows(logits)
+    p.dtype = _dtype(logits)
+    return ctx.lib.k3x_hip_route(ctx.handle, C.byref(p), at, ptr(bias), ptr(ids), ptr(weights))
 
 
 def make_delta_params(q, k, v, sequences, gate=None, scale=1.0, norm_epsilon=0.0, longest=0,
                       slots=None) -> DeltaParams:
-    """Parameters of delta_rule for q, k [T][Hk][K] and v [T][Hv][V] (rows may lie apart) and a
-    gate [T][Hv][K], [T][Hv] or None; slots None: one state a sequence."""
+    """Parameters of delta_rule for q, k [T][Hk][K] and v [T][Hv][V] (rows may lie apart:
+    delta_rule takes their distances from the tensors) and a gate [T][Hv][K], [T][Hv] or None;
+    slots None: one state a sequence."""
     T, Hk, K = q.shape
-    H, V = v.shape[1:]
+    _, H, V = v.shape
     kind = GATE_NONE if gate is None else GATE_HEAD if gate.dim() == 2 else GATE_CHANNEL
     return DeltaParams(sequences, T, Hk, H, K, V, _dtype(v), kind, scale, norm_epsilon, longest,
-                       sequences if slots is None else slots, _row_stride(q), _row_stride(k),
-                       _row_stride(v), 0)
+                       sequences if slots is None else slots, 0, 0, 0, 0)
 
 
 def delta_workspace_bytes(params: DeltaParams) -> int:
@@ -667,26 +678,31 @@ def delta_rule(ctx: Context, params: DeltaParams, q, k, v, beta, out, gate=None,
     """The gated delta rule (k3x_hip_delta_rule): out [T][Hv][V] and states [slots][Hv][K][V]
     (fp32) from q, k, v of one type, gate and beta [T][Hv] (fp32); offsets [N + 1], limits [N]
     and slot_index [N] int32."""
-    import torch
     p = DeltaParams.from_buffer_copy(params)
     T, N, H, K, V = p.tokens, p.sequences, p.value_heads, p.key_dim, p.value_dim
-    _expect("q", q, (T, p.key_heads, K), (v.dtype,))
-    _expect("k", k, (T, p.key_heads, K), (v.dtype,))
-    _expect("v", v, (T, H, V), (v.dtype,))
-    _expect("out", out, (T, H, V), (v.dtype,))
-    _expect("beta", beta, (T, H), (torch.float32,))
-    _expect("gate", gate, (T, H, K) if p.gate == GATE_CHANNEL else (T, H), (torch.float32,))
-    ints = (torch.int32, torch.uint32)
-    _expect("offsets", offsets, (N + 1,), ints)
-    _expect("limits", limits, (N,), ints)
-    _expect("slot_index", slot_index, (N,), ints)
-    _expect("state_in", state_in, (p.slots, H, K, V), (torch.float32,))
-    _expect("state_out", state_out, (p.slots, H, K, V), (torch.float32,))
+    types, same = _types(), (v.dtype,)
+    _expect("q", q, (T, p.key_heads, K), same)
+    _expect("k", k, (T, p.key_heads, K), same)
+    _expect("v", v, (T, H, V), same)
+    _expect("out", out, (T, H, V), same)
+    _expect("beta", beta, (T, H), types["f32"])
+    if gate is not None:
+        _expect("gate", gate, (T, H, K) if p.gate == GATE_CHANNEL else (T, H), types["f32"])
+    for what, t, n in (("offsets", offsets, N + 1), ("limits", limits, N),
+                       ("slot_index", slot_index, N)):
+        if t is not None:
+            _expect(what, t, (n,), types["ints"])
+    for what, t in (("state_in", state_in), ("state_out", state_out)):
+        if t is not None:
+            _expect(what, t, (p.slots, H, K, V), types["f32"])
     p.dtype = _dtype(v)
-    p.q_stride, p.k_stride, p.v_stride, p.out_stride = map(_row_stride, (q, k, v, out))
+    qp, p.q_stride = _rows(q)
+    kp, p.k_stride = _rows(k)
+    vp, p.v_stride = _rows(v)
+    op, p.out_stride = _rows(out)
     return ctx.lib.k3x_hip_delta_rule(
-        ctx.handle, C.byref(p), _rows(q), _rows(k), _rows(v), ptr(gate), ptr(beta), ptr(offsets),
-        ptr(limits), ptr(slot_index), ptr(state_in), ptr(state_out), _rows(out), ptr(workspace),
+        ctx.handle, C.byref(p), qp, kp, vp, ptr(gate), ptr(beta), ptr(offsets), ptr(limits),
+        ptr(slot_index), ptr(state_in), ptr(state_out), op, ptr(workspace),
         0 if workspace is None else workspace.numel() * workspace.element_size())
 
 
@@ -705,17 +721,19 @@ def verify_draft(ctx: Context, params: VerifyParams, target, tokens, accepted, o
                  workspace=None) -> int:
     """Verifies drafted tokens [N][D] against the target's rows [N][D + 1][V]
     (k3x_hip_verify_draft): accepted [N] and out_tokens [N][D + 1] int32."""
-    import torch
-    N, D, V = params.sequences, params.drafts, params.vocab
-    ints = (torch.int32, torch.uint32)
-    _expect("target", target, (N, D + 1, V), (torch.float32, torch.bfloat16))
-    _expect("draft", draft, (N, D, V), (target.dtype,))
-    _expect("tokens", tokens, (N, D), ints)
-    _expect("draft_counts", draft_counts, (N,), ints)
-    _expect("accept_u", accept_u, (N, D), (torch.float32,))
-    _expect("sample_u", sample_u, (N,), (torch.float32,))
-    _expect("accepted", accepted, (N,), ints)
-    _expect("out_tokens", out_tokens, (N, D + 1), ints)
+    N, D, V, types = params.sequences, params.drafts, params.vocab, _types()
+    _expect("target", target, (N, D + 1, V), types["logits"])
+    if draft is not None:
+        _expect("draft", draft, (N, D, V), (target.dtype,))
+    _expect("tokens", tokens, (N, D), types["ints"])
+    if draft_counts is not None:
+        _expect("draft_counts", draft_counts, (N,), types["ints"])
+    if accept_u is not None:
+        _expect("accept_u", accept_u, (N, D), types["f32"])
+    if sample_u is not None:
+        _expect("sample_u", sample_u, (N,), types["f32"])
+    _expect("accepted", accepted, (N,), types["ints"])
+    _expect("out_tokens", out_tokens, (N, D + 1), types["ints"])
     if _dtype(target) != params.dtype:
         raise ValueError("target: not of the parameters' type")
     return ctx.lib.k3x_hip_verify_draft(

@@ -156,5 +156,6 @@ def test_strides_of_rows():
     assert k3x._row_stride(wide[:, 3:9]) == 30
     assert k3x._row_stride(wide[:1, 3:9]) == 0
     assert k3x._row_stride(wide[:, 2:26].unflatten(1, (2, 12))) == 30
-    assert not k3x._row_contiguous(wide.t())
-    assert not k3x._row_contiguous(wide.unflatten(1, (2, 15))[:, :, :5])
+    for bad in (wide.t(), wide.unflatten(1, (2, 15))[:, :, :5]):
+        with pytest.raises(ValueError):
+            k3x._row_stride(bad)
