@@ -28,12 +28,6 @@ struct RouteArgs {
     uint32_t* status;
 };
 
-__device__ inline double wave_sum_f64(double v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
-}
-
 __device__ inline uint64_t wave_max_u64(uint64_t v) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -44,9 +38,16 @@ __device__ inline uint64_t wave_max_u64(uint64_t v) {
 }
 
 // The adjusted score of a sort key (topk_key).
-__device__ inline float key_score(uint64_t key) {
-    const uint32_t ord = (uint32_t)(key >> 32);
-    return __uint_as_float((ord & 0x80000000u) ? (ord & 0x7fffffffu) : ~ord);
+__device__ inline float key_score(uint64_t key) { return unordered((uint32_t)(key >> 32)); }
+
+// sigmoid_cr without its branches: past +-200 the exponential is infinite or 0
+// in fp32 already, so the argument may stop there.
+__device__ inline float sigmoid_flat(float v) {
+    const float x = fminf(fmaxf(-v, -200.0f), 200.0f);
+    const double xd = (double)x;
+    const double k = __builtin_rint(xd * 1.4426950408889634);
+    const float t = __fadd_rn(1.0f, (float)__builtin_ldexp(exp_series(xd, k), (int)k));
+    return v == v ? __fdiv_rn(1.0f, t) : v;
 }
 
 // Renormalised weight of slot `lane` of K whose scores the lanes hold;
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(64) void route_lds_kernel(RouteArgs a) {
         mx = __any(nan) ? (double)__builtin_nanf("") : (double)m;
         den = 0.0;
         for (uint32_t e = lane; e < E; e += 64) den += exp_f64((double)Elem<DT>::load(row[e]) - mx);
-        den = 1.0 / wave_sum_f64(den);
+        den = 1.0 / wave_sum(den);
     }
     uint32_t bad = 0;
     for (uint32_t e = lane; e < E; e += 64) {
@@ -218,7 +219,7 @@ template <uint32_t DT, int KPL>
 __global__ __launch_bounds__(64 * kRouteWaves) void route_wave_kernel(RouteArgs a) {
     typedef typename Elem<DT>::type T;
     struct Wave {
-        uint64_t key[64 * KPL];
+        __attribute__((aligned(16))) uint64_t key[64 * KPL + 8];
         float score[64 * KPL];
         uint32_t id[64];
         float sel[64];
@@ -241,24 +242,20 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_wave_kernel(RouteArgs 
     if (a.scoring == K3X_SCORE_SOFTMAX) {
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < KPL; ++i) {
-            const uint32_t u = __float_as_uint(l[i]);
-            top = max(top, (u & 0x80000000u) ? ~u : (u | 0x80000000u));
-        }
-        top = wave_max_u32(top);
-        const double mx = (double)__uint_as_float((top & 0x80000000u) ? (top & 0x7fffffffu) : ~top);
+        for (int i = 0; i < KPL; ++i) top = max(top, ordered(l[i]));
+        const double mx = (double)unordered(wave_max_u32(top));
         double e[KPL], den = 0.0;
 #pragma unroll
         for (int i = 0; i < KPL; ++i) {
             e[i] = lane + 64u * i < E ? exp_f64((double)l[i] - mx) : 0.0;
             den += e[i];
         }
-        const double inv = 1.0 / wave_sum_f64(den);
+        const double inv = 1.0 / wave_sum(den);
 #pragma unroll
         for (int i = 0; i < KPL; ++i) sc[i] = (float)(e[i] * inv);
     } else {
 #pragma unroll
-        for (int i = 0; i < KPL; ++i) sc[i] = sigmoid_cr(l[i]);
+        for (int i = 0; i < KPL; ++i) sc[i] = sigmoid_flat(l[i]);
     }
     uint32_t bad = 0, ord[KPL];
 #pragma unroll
@@ -301,7 +298,13 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_wave_kernel(RouteArgs 
             gs = __fadd_rn(gs, key_score((uint64_t)k2 << 32));
         const uint64_t gk = topk_key(gs, g);
         uint32_t rank = 0;
-        for (uint32_t i = 0; i < a.G; ++i) rank += __shfl(gk, i * width) > gk;
+        for (uint32_t i = 0; i < a.G; ++i) {
+            const uint64_t o =
+                (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(gk >> 32), i * width)
+                    << 32 |
+                (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)gk, i * width);
+            rank += o > gk;
+        }
         const uint64_t kept = __ballot(g < a.G && rank < a.top_groups);
 #pragma unroll
         for (int i = 0; i < KPL; ++i)
@@ -326,12 +329,20 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_wave_kernel(RouteArgs 
         }
         count += (uint32_t)__popcll(mask);
     }
+    // Eight keys at a time are counted; 0 is below every key.
+    if (lane < 8) s.key[count + lane] = 0;
     wave_sync();
     for (uint32_t c0 = 0; c0 < count; c0 += 64) {
         const uint32_t c = c0 + lane;
         const uint64_t key = s.key[min(c, count - 1)];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < count; ++j) rank += s.key[j] > key;
+        for (uint32_t j = 0; j < count; j += 8) {
+            typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+            const u64x2* p = reinterpret_cast<const u64x2*>(&s.key[j]);
+            const u64x2 o[4] = {p[0], p[1], p[2], p[3]};
+#pragma unroll
+            for (int x = 0; x < 8; ++x) rank += o[x / 2][x % 2] > key;
+        }
         if (c < count && rank < a.K) {
             s.id[rank] = 0xffffffffu - (uint32_t)key;
             s.sel[rank] = s.score[c];

@@ -1,10 +1,10 @@
 // verify.hip -- verification of drafted tokens against the target's rows.
 //
-//   rows     each row by parts of 4096 entries: the largest entry and the sum of
-//            exponentials over it (logits, and greedy choices);
+//   rows     each row by parts of 1024 entries, a wave each: the largest entry and
+//            the sum of exponentials over it (logits, and greedy choices);
 //   accept   one workgroup a sequence: every row's totals and drafted token's
 //            probabilities at once, then the walk over the drafts;
-//   draw     the row that the next token is drawn from, by the same parts: their
+//   draw     the row that the next token is drawn from, by parts of 4096: their
 //            sums, and by the sequence's last workgroup the part and the entry
 //            that the border falls in.
 //
@@ -49,11 +49,12 @@ struct VerifyArgs {
     const float *accept_u, *sample_u;
     uint32_t *accepted, *out_tokens;
     uint32_t N, D, V, stride;
-    uint32_t parts;
+    uint32_t row_parts_of;  // a row, in waves' parts
+    uint32_t parts;         // of the draw, in workgroups' parts
     uint32_t form, greedy;
     uint32_t vec;       // rows by 16 bytes
-    double inv_temperature;
-    RowPart* row_parts; // [N (2 D + 1)][parts]: a sequence's target rows, then its draft's
+    double rate;        // log2(e) / temperature
+    RowPart* row_parts; // [N (2 D + 1)][row_parts_of]: a sequence's target rows, then its draft's
     Drawn* drawn;       // [N]
     double* sums;       // [N][parts]
     uint32_t* status;
@@ -72,7 +73,7 @@ __device__ inline const typename Elem<DT>::type* row_of(const VerifyArgs& a, uin
 }
 
 __device__ inline size_t part_index(const VerifyArgs& a, uint32_t n, uint32_t r) {
-    return ((size_t)n * (2 * a.D + 1) + r) * a.parts;
+    return ((size_t)n * (2 * a.D + 1) + r) * a.row_parts_of;
 }
 
 // The larger of two (entry, index) pairs, the lower index on a tie.
@@ -83,31 +84,52 @@ __device__ inline void take_max(float& m, uint32_t& i, float om, uint32_t oi) {
     }
 }
 
-// A thread's sixteen entries of a part, neighbours by 16 bytes where rows are,
-// so that a wave's loads are whole lines; where() rises with j.
-template <uint32_t DT>
+// 2^y in double, y <= 0 (a NaN gives 0: a row that holds one is unfit): the series
+// (ln2 f)^n / n! to n = 11 on |f| <= 1 / 2, 7e-15 of it at most.
+__device__ inline double exp2_f64(double y) {
+    y = __builtin_fmax(y, -1080.0);  // 2^y is 0 from there on
+    const double k = __builtin_rint(y), f = y - k;
+    double p = 4.4455382718708116e-10;
+    p = __builtin_fma(p, f, 7.054911620801123e-09);
+    p = __builtin_fma(p, f, 1.01780860092397e-07);
+    p = __builtin_fma(p, f, 1.321548679014431e-06);
+    p = __builtin_fma(p, f, 1.5252733804059841e-05);
+    p = __builtin_fma(p, f, 0.0001540353039338161);
+    p = __builtin_fma(p, f, 0.0013333558146428443);
+    p = __builtin_fma(p, f, 0.009618129107628477);
+    p = __builtin_fma(p, f, 0.05550410866482158);
+    p = __builtin_fma(p, f, 0.24022650695910072);
+    p = __builtin_fma(p, f, 0.6931471805599453);
+    p = __builtin_fma(p, f, 1.0);
+    return __builtin_ldexp(p, (int)k);
+}
+
+// A thread's sixteen entries of a part of TH threads, neighbours by 16 bytes
+// where rows are, so that a wave's loads are whole lines; where() rises with j.
+template <uint32_t DT, uint32_t TH>
 struct Entries {
     typedef typename Elem<DT>::type E;
-    static constexpr uint32_t kWide = 16 / sizeof(E);
-    static __device__ inline uint32_t where(const VerifyArgs& a, uint32_t lo, int j) {
-        return a.vec ? lo + j / kWide * (kThreads * kWide) + threadIdx.x * kWide + j % kWide
-                     : lo + j * kThreads + threadIdx.x;
+    static constexpr uint32_t kWide = 16 / sizeof(E), kAll = TH * kEntries;
+    static __device__ inline uint32_t where(const VerifyArgs& a, uint32_t lo, uint32_t thread,
+                                            int j) {
+        return a.vec ? lo + j / kWide * (TH * kWide) + thread * kWide + j % kWide
+                     : lo + j * TH + thread;
     }
     // Past hi: `past`.
     static __device__ inline void load(const VerifyArgs& a, const E* x, uint32_t lo, uint32_t hi,
-                                       float past, float (&l)[kEntries]) {
+                                       uint32_t thread, float past, float (&l)[kEntries]) {
         typedef E Vec __attribute__((ext_vector_type(kWide)));
-        if (a.vec && lo + kPart <= hi) {
+        if (a.vec && lo + kAll <= hi) {
 #pragma unroll
             for (int j = 0; j < (int)kEntries; j += kWide) {
-                const Vec v = *reinterpret_cast<const Vec*>(x + where(a, lo, j));
+                const Vec v = *reinterpret_cast<const Vec*>(x + where(a, lo, thread, j));
 #pragma unroll
                 for (int y = 0; y < (int)kWide; ++y) l[j + y] = Elem<DT>::load(v[y]);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < (int)kEntries; ++j) {
-                const uint32_t i = where(a, lo, j);
+                const uint32_t i = where(a, lo, thread, j);
                 l[j] = Elem<DT>::load(x[min(i, hi - 1)]);
                 if (i >= hi) l[j] = past;
             }
@@ -115,26 +137,22 @@ struct Entries {
     }
 };
 
-__device__ inline double wave_sum(double v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
-}
-
+// Parts of a row by waves, which do not wait for one another.
 template <uint32_t DT>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a) {
-    __shared__ float sm[kThreads / 64];
-    __shared__ uint32_t si[kThreads / 64];
-    __shared__ double sd[kThreads / 64];
-    const uint32_t part = blockIdx.x % a.parts, rr = blockIdx.x / a.parts;
     const uint32_t rows = a.draft ? 2 * a.D + 1 : a.D + 1;
-    const uint32_t n = rr / rows, r = rr % rows, tid = threadIdx.x, wave = tid >> 6;
+    const uint32_t blocks = (a.row_parts_of + kThreads / 64 - 1) / (kThreads / 64);
+    const uint32_t rr = blockIdx.x / blocks, n = rr / rows, r = rr % rows, lane = threadIdx.x & 63;
+    const uint32_t part = blockIdx.x % blocks * (kThreads / 64) +
+                          __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t count = drafts_of(a, n);
-    if (count > a.D || (r <= a.D ? r > count : r - a.D - 1 >= count)) return;
-    const uint32_t lo = part * kPart, hi = min(a.V, lo + kPart);
+    if (part >= a.row_parts_of || count > a.D || (r <= a.D ? r > count : r - a.D - 1 >= count))
+        return;
+    typedef Entries<DT, 64> Mine;
+    const uint32_t lo = part * Mine::kAll, hi = min(a.V, lo + Mine::kAll);
     float l[kEntries];
-    Entries<DT>::load(a, row_of<DT>(a, n, r), lo, hi, -__builtin_inff(), l);
-    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
+    Mine::load(a, row_of<DT>(a, n, r), lo, hi, lane, -__builtin_inff(), l);
+    if (*(volatile uint32_t*)a.status) return;
     float m = -__builtin_inff();
     uint32_t arg = 0xffffffffu;
     bool wrong = false;
@@ -142,36 +160,28 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a) {
     for (int j = 0; j < (int)kEntries; ++j) {
         // Past the row's end minus infinity: no entry of a row of
         // probabilities, but not one that is looked at either.
-        const bool past = Entries<DT>::where(a, lo, j) >= hi;
+        const uint32_t i = Mine::where(a, lo, lane, j);
         wrong |= !(l[j] < __builtin_inff()) ||
-                 (a.form == K3X_DIST_PROBS && l[j] < 0.0f && !past);
-        if (l[j] > m) {
+                 (a.form == K3X_DIST_PROBS && l[j] < 0.0f && i < hi);
+        if (!a.greedy) {
+            m = fmaxf(m, l[j]);
+        } else if (l[j] > m) {
             m = l[j];
-            arg = Entries<DT>::where(a, lo, j);
+            arg = i;
         }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1)
-        take_max(m, arg, __shfl_xor(m, d), (uint32_t)__shfl_xor((int)arg, d));
-    if ((tid & 63) == 0) {
-        sm[wave] = m;
-        si[wave] = arg;
-    }
-    wrong = __syncthreads_or(wrong);
-#pragma unroll
-    for (uint32_t w = 0; w < kThreads / 64; ++w) take_max(m, arg, sm[w], si[w]);
+    const float top = unordered(wave_max_u32(ordered(m)));
+    if (a.greedy) arg = ~wave_max_u32(m == top ? ~arg : 0u);
     double s = 0.0;
-    if (!a.greedy && m > -__builtin_inff()) {
+    if (!a.greedy && top > -__builtin_inff()) {
 #pragma unroll
         for (int j = 0; j < (int)kEntries; ++j)
-            s += exp_f64(((double)l[j] - (double)m) * a.inv_temperature);
+            s += exp2_f64(((double)l[j] - (double)top) * a.rate);
         s = wave_sum(s);
-        if ((tid & 63) == 0) sd[wave] = s;
-        __syncthreads();
-        s = sd[0] + sd[1] + sd[2] + sd[3];
     }
-    if (tid == 0)
-        a.row_parts[part_index(a, n, r) + part] = RowPart{s, wrong ? __builtin_nanf("") : m, arg};
+    wrong = __any(wrong);
+    if (lane == 0)
+        a.row_parts[part_index(a, n, r) + part] = RowPart{s, wrong ? __builtin_nanf("") : top, arg};
 }
 
 // A row's largest entry and 1 / sum from its parts, by a wave; false: the row
@@ -183,7 +193,7 @@ __device__ inline bool row_total(const VerifyArgs& a, uint32_t n, uint32_t r, do
     float m = -__builtin_inff();
     uint32_t at = 0xffffffffu;
     bool nan = false;
-    for (uint32_t i = lane; i < a.parts; i += 64) {
+    for (uint32_t i = lane; i < a.row_parts_of; i += 64) {
         nan |= parts[i].max != parts[i].max;
         take_max(m, at, parts[i].max, parts[i].arg);
     }
@@ -194,10 +204,10 @@ __device__ inline bool row_total(const VerifyArgs& a, uint32_t n, uint32_t r, do
     if (m == -__builtin_inff() || (a.form == K3X_DIST_PROBS && m == 0.0f)) return false;
     double s = 0.0;
     if (!a.greedy)
-        for (uint32_t i = lane; i < a.parts; i += 64)
+        for (uint32_t i = lane; i < a.row_parts_of; i += 64)
             if (parts[i].sum > 0.0)
                 s += parts[i].sum *
-                     exp_f64(((double)parts[i].max - (double)m) * a.inv_temperature);
+                     exp2_f64(((double)parts[i].max - (double)m) * a.rate);
     *mx = m;
     *inv = 1.0 / wave_sum(s);
     *arg = at;
@@ -206,7 +216,7 @@ __device__ inline bool row_total(const VerifyArgs& a, uint32_t n, uint32_t r, do
 
 __device__ inline double prob(const VerifyArgs& a, float l, double mx, double inv) {
     return a.form == K3X_DIST_PROBS ? (double)l
-                                    : exp_f64(((double)l - mx) * a.inv_temperature) * inv;
+                                    : exp2_f64(((double)l - mx) * a.rate) * inv;
 }
 
 // One workgroup a sequence: a wave a row, the drafts' rows together.
@@ -215,6 +225,8 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a) {
     struct Row {
         double max, inv, prob;  // prob: of the drafted token
         uint32_t arg, fit;
+        uint32_t token;  // drafted after it
+        float u;
     };
     __shared__ Row rows[2 * kMaxDrafts + 1];
     __shared__ uint32_t verdict;
@@ -240,7 +252,8 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a) {
         const uint32_t d = target ? i : i - count - 1, r = target ? i : a.D + 1 + d;
         const uint32_t x = d < count ? a.tokens[(size_t)n * a.D + d] : 0;
         const float l = x < a.V && !a.greedy ? Elem<DT>::load(row_of<DT>(a, n, r)[x]) : 0.0f;
-        Row row{0.0, 1.0, 0.0, 0, 1};
+        Row row{0.0, 1.0, 0.0, 0, 1, x, 0.0f};
+        if (target && d < count && !a.greedy) row.u = a.accept_u[(size_t)n * a.D + d];
         if (totals) row.fit = row_total(a, n, r, &row.max, &row.inv, &row.arg);
         if (row.fit && !a.greedy) row.prob = prob(a, l, row.max, row.inv);
         if ((tid & 63) == 0) rows[i] = row;
@@ -252,17 +265,16 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a) {
             const Row& p = rows[i];
             if (!p.fit) bad = 1;
             if (bad || i == count) break;
-            const uint32_t x = a.tokens[(size_t)n * a.D + i];
-            if (x >= a.V) {
+            if (p.token >= a.V) {
                 bad = 1;
                 break;
             }
             if (a.greedy) {
-                if (p.arg != x) break;
+                if (p.arg != p.token) break;
                 continue;
             }
-            const float u = a.accept_u[(size_t)n * a.D + i];
-            const Row one{0.0, 1.0, 1.0, 0, 1};
+            const float u = p.u;
+            const Row one{0.0, 1.0, 1.0, 0, 1, 0, 0.0f};
             const Row& q = a.draft ? rows[count + 1 + i] : one;
             if (!q.fit || !(u >= 0.0f && u < 1.0f) ||
                 !(p.prob >= 0.0 && p.prob < __builtin_inf()) ||
@@ -290,7 +302,7 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a) {
     __syncthreads();
     if (!a.greedy || verdict == 0xffffffffu) return;
     for (uint32_t i = tid; i <= a.D; i += blockDim.x)
-        out[i] = i < verdict    ? a.tokens[(size_t)n * a.D + i]
+        out[i] = i < verdict    ? rows[i].token
                  : i == verdict ? rows[verdict].arg
                                 : 0xffffffffu;
 }
@@ -338,19 +350,11 @@ __device__ inline double block_sum(double s, double* sd) {
     return sd[0] + sd[1] + sd[2] + sd[3];
 }
 
-// The token of [lo, hi) that the border falls in: the last entry over 0 that
-// the cumulative sum (start before lo) has not passed the border before.  By the
-// whole workgroup, a run of entries a thread; the range holds an entry over 0
-// and start <= border.
-template <uint32_t DT>
-__device__ inline uint32_t draw_token(const VerifyArgs& a, const Rest<DT>& rest, uint32_t lo,
-                                      uint32_t hi, double start, double border, double* sd,
-                                      uint32_t* found) {
+// Where a cumulative sum over [lo, ...), a run of `per` entries a thread, passes
+// the border: start lies before lo, s is the thread's sum; returns what lies
+// before the thread's run.  By the whole workgroup.
+__device__ inline double run_start(double s, double start, double* sd) {
     const uint32_t tid = threadIdx.x, lane = tid & 63;
-    const uint32_t per = (hi - lo + kThreads - 1) / kThreads;
-    const uint32_t b = min(hi, lo + tid * per), e = min(hi, b + per);
-    double s = 0.0;
-    for (uint32_t i = b; i < e; ++i) s += rest.at(a, i);
     double c = s;  // of this and the wave's threads before
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -359,11 +363,55 @@ __device__ inline uint32_t draw_token(const VerifyArgs& a, const Rest<DT>& rest,
     }
     __syncthreads();
     if (lane == 63) sd[tid >> 6] = c;
-    if (tid == 0) *found = 0;
     __syncthreads();
     c = __shfl_up(c, 1);
     c = start + (lane ? c : 0.0);
     for (uint32_t w = 0; w < tid >> 6; ++w) c += sd[w];
+    return c;
+}
+
+// The token of a part that the border falls in: the last entry over 0 that the
+// cumulative sum (start before the part) has not passed the border before.  By
+// the whole workgroup, sixteen neighbours a thread; the part holds an entry
+// over 0 and start <= border.  found: 0 before.
+template <uint32_t DT>
+__device__ inline uint32_t draw_token(const VerifyArgs& a, const Rest<DT>& rest, uint32_t lo,
+                                      double start, double border, double* sd, uint32_t* found) {
+    const uint32_t b = lo + threadIdx.x * kEntries;
+    float pl[kEntries], ql[kEntries];
+#pragma unroll
+    for (int j = 0; j < (int)kEntries; ++j) {
+        const uint32_t i = min(b + j, a.V - 1);
+        pl[j] = Elem<DT>::load(rest.p[i]);
+        ql[j] = rest.q ? Elem<DT>::load(rest.q[i]) : 0.0f;
+    }
+    double r[kEntries], s = 0.0;
+#pragma unroll
+    for (int j = 0; j < (int)kEntries; ++j) {
+        r[j] = b + j < a.V ? rest.of(a, b + j, pl[j], ql[j]) : 0.0;
+        s += r[j];
+    }
+    double c = run_start(s, start, sd);
+    uint32_t hit = 0;
+#pragma unroll
+    for (int j = 0; j < (int)kEntries; ++j) {
+        if (r[j] > 0.0 && c <= border) hit = b + j + 1;
+        c += r[j];
+    }
+    if (hit) atomicMax(found, hit);
+    __syncthreads();
+    return *found - 1;
+}
+
+// The same over the whole row.
+template <uint32_t DT>
+__device__ inline uint32_t draw_whole(const VerifyArgs& a, const Rest<DT>& rest, double border,
+                                      double* sd, uint32_t* found) {
+    const uint32_t per = (a.V + kThreads - 1) / kThreads;
+    const uint32_t b = min(a.V, threadIdx.x * per), e = min(a.V, b + per);
+    double s = 0.0;
+    for (uint32_t i = b; i < e; ++i) s += rest.at(a, i);
+    double c = run_start(s, 0.0, sd);
     uint32_t hit = 0;
     for (uint32_t i = b; i < e && c <= border; ++i) {
         const double r = rest.at(a, i);
@@ -388,18 +436,24 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
     {
         float pl[kEntries], ql[kEntries] = {};
         const float past = a.form == K3X_DIST_PROBS ? 0.0f : -__builtin_inff();
-        Entries<DT>::load(a, rest.p, lo, hi, past, pl);
-        if (rest.q) Entries<DT>::load(a, rest.q, lo, hi, past, ql);
+        typedef Entries<DT, kThreads> Mine;
+        Mine::load(a, rest.p, lo, hi, tid, past, pl);
+        if (rest.q) Mine::load(a, rest.q, lo, hi, tid, past, ql);
         double s = 0.0;
 #pragma unroll
         for (int j = 0; j < (int)kEntries; ++j)
-            s += rest.of(a, Entries<DT>::where(a, lo, j), pl[j], ql[j]);
+            s += rest.of(a, Mine::where(a, lo, tid, j), pl[j], ql[j]);
         s = block_sum(s, sd);
-        // The sum, then the arrival: the last workgroup sees every sum.
+        // The sum, then the arrival, both past the caches of one die: the last
+        // workgroup sees every sum.  (A releasing add would write back the
+        // die's whole cache for each workgroup: 91 us in place of 17 for 64
+        // sequences of 131072 probabilities.)
         if (tid == 0) {
+            found = 0;
             __hip_atomic_store(a.sums + (size_t)n * a.parts + part, s, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
-            last = __hip_atomic_fetch_add(&a.drawn[n].arrived, 1u, __ATOMIC_ACQ_REL,
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            last = __hip_atomic_fetch_add(&a.drawn[n].arrived, 1u, __ATOMIC_RELAXED,
                                           __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
         }
         __syncthreads();
@@ -429,7 +483,6 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
     }
     if (!(u >= 0.0f && u < 1.0f) || !(total >= 0.0 && total < __builtin_inf())) bad = 1;
     if (!bad) {
-        uint32_t from = 0, to = a.V;
         double border = (double)u * total;
         if (total > 0.0) {
             // The last part over 0 that starts at the border or before.
@@ -442,8 +495,7 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
                 in = 64 * x + l;
                 start = __shfl(run[x], l);
             }
-            from = in * kPart;
-            to = min(a.V, from + kPart);
+            next = draw_token<DT>(a, rest, in * kPart, start, border, sd, &found);
         } else {
             // Nothing is left over q (or of a row without its drafted token):
             // the target's own probabilities.
@@ -453,8 +505,8 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
             total = block_sum(s, sd);
             border = (double)u * total;
             if (!(total > 0.0 && total < __builtin_inf())) bad = 1;
+            if (!bad) next = draw_whole<DT>(a, rest, border, sd, &found);
         }
-        if (!bad) next = draw_token<DT>(a, rest, from, to, start, border, sd, &found);
     }
     if (bad) {
         if (tid == 0) latch(a.status, K3X_ERR_INVALID_STATE);
@@ -472,8 +524,9 @@ int launch_verify(k3x_hip_ctx* ctx, const VerifyArgs& a) {
     unsigned launches = 1;
     const uint32_t rows = a.draft ? 2 * a.D + 1 : a.D + 1;
     if (a.form == K3X_DIST_LOGITS || a.greedy) {
-        hipLaunchKernelGGL(verify_rows_kernel<DT>, dim3(a.N * rows * a.parts), dim3(kThreads), 0,
-                           ctx->stream, a);
+        hipLaunchKernelGGL(verify_rows_kernel<DT>,
+                           dim3(a.N * rows * ((a.row_parts_of + kThreads / 64 - 1) / (kThreads / 64))),
+                           dim3(kThreads), 0, ctx->stream, a);
         ++launches;
     }
     hipLaunchKernelGGL(verify_accept_kernel<DT>, dim3(a.N), dim3(64 * std::min(rows, 16u)), 0,
@@ -487,6 +540,9 @@ int launch_verify(k3x_hip_ctx* ctx, const VerifyArgs& a) {
 }
 
 uint32_t parts_of(const k3x_hip_verify_params* p) { return (p->vocab + kPart - 1) / kPart; }
+uint32_t row_parts_of(const k3x_hip_verify_params* p) {
+    return (p->vocab + 64 * kEntries - 1) / (64 * kEntries);
+}
 
 bool verify_ok(const k3x_hip_verify_params* p) {
     return p->sequences && p->sequences <= 65535 && p->drafts <= kMaxDrafts && p->vocab &&
@@ -505,7 +561,7 @@ extern "C" {
 size_t k3x_hip_verify_workspace(const k3x_hip_verify_params* p) {
     if (!p || !verify_ok(p)) return 0;
     const size_t n = p->sequences, parts = parts_of(p);
-    return up256(n * (2 * p->drafts + 1) * parts * sizeof(RowPart)) + up256(n * sizeof(Drawn)) +
+    return up256(n * (2 * p->drafts + 1) * row_parts_of(p) * sizeof(RowPart)) + up256(n * sizeof(Drawn)) +
            up256(n * parts * sizeof(double));
 }
 
@@ -540,13 +596,14 @@ int k3x_hip_verify_draft(k3x_hip_ctx* ctx, const k3x_hip_verify_params* p, const
     a.V = p->vocab;
     a.stride = p->row_stride ? p->row_stride : p->vocab;
     a.parts = parts_of(p);
+    a.row_parts_of = row_parts_of(p);
     a.vec = a.stride * es % 16 == 0 && aligned(target, 16) && aligned(draft, 16);
     a.form = p->form;
     a.greedy = p->greedy;
-    a.inv_temperature = 1.0 / p->temperature;
+    a.rate = 1.4426950408889634 / p->temperature;
     uint8_t* w = static_cast<uint8_t*>(workspace);
     a.row_parts = reinterpret_cast<RowPart*>(w);
-    w += up256((size_t)a.N * (2 * a.D + 1) * a.parts * sizeof(RowPart));
+    w += up256((size_t)a.N * (2 * a.D + 1) * a.row_parts_of * sizeof(RowPart));
     a.drawn = reinterpret_cast<Drawn*>(w);
     w += up256((size_t)a.N * sizeof(Drawn));
     a.sums = reinterpret_cast<double*>(w);
