@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstddef>
+#include <type_traits>
 
 #include "k3x_ops.hpp"
 
@@ -330,6 +331,9 @@ void launch_step_rows(const DeltaArgs& a, uint32_t gate, uint32_t vec, hipStream
 constexpr uint32_t kChunk = 32;
 constexpr float kOperand = 64.0f;  // keys, queries and Pq are held times this
 
+// Eight values of a lane as a vector and not an array: what the loops over them
+// index stays in registers whatever is unrolled when.
+typedef __attribute__((ext_vector_type(8))) float f32x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
@@ -338,8 +342,8 @@ struct Pair8 {
 };
 
 // hi = f16(x), lo = f16(x - hi).  The factor -1 is kept from the compiler so
-// that the difference is one fused instruction on the packed halves.
-__device__ inline Pair8 split8(const float (&x)[8]) {
+// that difference and rounding are one fused instruction on the packed halves.
+__device__ __forceinline__ Pair8 split8(f32x8 x) {
     typedef __attribute__((ext_vector_type(2))) float f32x2;
     float minus = -1.0f;
     asm("" : "+s"(minus));
@@ -350,10 +354,10 @@ __device__ inline Pair8 split8(const float (&x)[8]) {
         uint32_t u = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
         asm("" : "+v"(u));
         const f16x2 h = __builtin_bit_cast(f16x2, u);
-        const f32x2 r = {__builtin_fmaf((float)h[0], minus, v[0]),
-                         __builtin_fmaf((float)h[1], minus, v[1])};
+        const f16x2 r = {(_Float16)__builtin_fmaf((float)h[0], minus, v[0]),
+                         (_Float16)__builtin_fmaf((float)h[1], minus, v[1])};
         hi[j] = u;
-        lo[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, f16x2));
+        lo[j] = __builtin_bit_cast(uint32_t, r);
     }
     return Pair8{__builtin_bit_cast(f16x8, hi), __builtin_bit_cast(f16x8, lo)};
 }
@@ -453,12 +457,20 @@ __device__ inline bool find_chunk(const DeltaArgs& a, uint32_t slot, ChunkPlace*
     return true;
 }
 
+// LDS written before is seen after, by the whole workgroup; loads from and
+// stores to global memory stay in flight across it.
+__device__ inline void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 typedef float Tile32[kChunk][36];  // rows of 16-byte alignment that spread over the banks
 
 // T of a chunk from L (strictly lower triangular; overwritten), by one wave in
 // fp32: the inverses of the two diagonal tiles by forward substitution, a
 // column a lane, and -T22 L21 T11 below them.
-__device__ inline void write_inverse(Tile32& L, const float* c, const float* beta,
+__device__ __forceinline__ void write_inverse(Tile32& L, const float* c, const float* beta,
                                      ChunkRecord* rec) {
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const uint32_t half = 16 * (g & 1);
@@ -497,7 +509,8 @@ __device__ inline void write_inverse(Tile32& L, const float* c, const float* bet
     wave_sync();
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        float e[8], most = 0.0f, down, up;
+        f32x8 e;
+        float most = 0.0f, down, up;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t t = token_of(g, j);
@@ -505,20 +518,18 @@ __device__ inline void write_inverse(Tile32& L, const float* c, const float* bet
             most = fmaxf(most, fabsf(e[j]));
         }
         unit_scale(max_groups(most), &down, &up);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] *= down * kOperand;
-        const Pair8 p = split8(e);
+        const Pair8 p = split8(e * (down * kOperand));
         rec->T[r][0][lane] = p.hi;
         rec->T[r][1][lane] = p.lo;
         if (g == 0) rec->row_t[16 * r + m] = up / kOperand;
     }
 }
 
-__device__ inline void write_scores(const Tile32& P, ChunkRecord* rec) {
+__device__ __forceinline__ void write_scores(const Tile32& P, ChunkRecord* rec) {
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        float e[8];
+        f32x8 e;
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = P[16 * r + m][token_of(g, j)];
         const Pair8 p = split8(e);
@@ -527,55 +538,71 @@ __device__ inline void write_scores(const Tile32& P, ChunkRecord* rec) {
     }
 }
 
-// A wave's tile of 16 tokens (lane: token l % 16) of keys and queries, the
-// channels in the operand's order: element j of part b is channel
-// 32 b + token_of(l / 16, j).
-template <uint32_t DT, int KB>
-struct TokenRows {
+// Eight channels of a lane's token in the operand's order: element j of part b is
+// channel 32 b + token_of(l / 16, j).  WHOLE: the head fills its parts and its
+// rows are loaded by four; else elements past the head's end are 0.
+template <uint32_t DT, bool WHOLE>
+struct TokenPart {
     typedef typename Elem<DT>::type E;
-    Vec4<E> q[KB][2], k[KB][2];
+    Vec4<E> q[2], k[2];
+    __device__ __forceinline__ void load(const DeltaArgs& a, const E* qr, const E* kr, int b,
+                                         uint32_t g) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t c = 32 * b + 16 * x + 4 * g;
+            if constexpr (WHOLE) {
+                q[x] = *reinterpret_cast<const Vec4<E>*>(qr + c);
+                k[x] = *reinterpret_cast<const Vec4<E>*>(kr + c);
+            } else {
+                q[x] = load4(qr, c, a.K, false);
+                k[x] = load4(kr, c, a.K, false);
+            }
+        }
+    }
+    __device__ __forceinline__ void values(const DeltaArgs& a, int b, uint32_t g, f32x8& x,
+                                           f32x8& y) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool in = WHOLE || 32 * b + token_of(g, j) < a.K;
+            x[j] = in ? Elem<DT>::load(q[j / 4][j % 4]) : 0.0f;
+            y[j] = in ? Elem<DT>::load(k[j / 4][j % 4]) : 0.0f;
+        }
+    }
+};
+
+// What a token's key and query are scaled by.
+struct TokenScales {
     float qd, qu, kd, ku;  // 2^-e and 2^e of the largest element
     float qn, kn;          // 1 / norm
-
-    // q and k: the rows' heads; z takes a NaN where an element is not finite.
-    __device__ inline void load(const DeltaArgs& a, const E* qr, const E* kr, uint32_t g,
-                                bool live, bool vec, float& z) {
-        float qm = 0.0f, km = 0.0f, qq = 0.0f, kk = 0.0f;
+    // By the whole wave; latches an element that is not finite (here and now: a
+    // check at the end would hold every element until then).
+    template <uint32_t DT, int KB, bool WHOLE>
+    __device__ __forceinline__ void find(const DeltaArgs& a, const typename Elem<DT>::type* qr,
+                                         const typename Elem<DT>::type* kr, uint32_t g) {
+        TokenPart<DT, WHOLE> part[KB];
 #pragma unroll
-        for (int b = 0; b < KB; ++b)
+        for (int b = 0; b < KB; ++b) part[b].load(a, qr, kr, b, g);
+        float qm = 0.0f, km = 0.0f, qq = 0.0f, kk = 0.0f, z = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const uint32_t c = 32 * b + 16 * x + 4 * g;
-                q[b][x] = load4(qr, c, a.K, vec);
-                k[b][x] = load4(kr, c, a.K, vec);
+        for (int b = 0; b < KB; ++b) {
+            __builtin_amdgcn_sched_barrier(0);  // one part's values at a time
+            f32x8 x, y;
+            part[b].values(a, b, g, x, y);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                z = __builtin_fmaf(x[j], 0.0f, z);
+                z = __builtin_fmaf(y[j], 0.0f, z);
+                qm = fmaxf(qm, fabsf(x[j]));
+                km = fmaxf(km, fabsf(y[j]));
+                qq = __builtin_fmaf(x[j], x[j], qq);
+                kk = __builtin_fmaf(y[j], y[j], kk);
             }
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (!live || 32 * b + 16 * x + 4 * g + j >= a.K)
-                        q[b][x][j] = k[b][x][j] = E{};
-                    const float y = Elem<DT>::load(q[b][x][j]), w = Elem<DT>::load(k[b][x][j]);
-                    z = __builtin_fmaf(y, 0.0f, z);
-                    z = __builtin_fmaf(w, 0.0f, z);
-                    qm = fmaxf(qm, fabsf(y));
-                    km = fmaxf(km, fabsf(w));
-                    qq = __builtin_fmaf(y, y, qq);
-                    kk = __builtin_fmaf(w, w, kk);
-                }
+        }
+        if (z != z) latch(a.status, K3X_ERR_INVALID_MXFP4);
         unit_scale(max_groups(qm), &qd, &qu);
         unit_scale(max_groups(km), &kd, &ku);
         qn = 1.0f / sqrtf(sum_groups(qq) + a.eps);
         kn = 1.0f / sqrtf(sum_groups(kk) + a.eps);
-    }
-    __device__ inline void part(int b, float qs, float ks, float (&x)[8], float (&y)[8]) const {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[j] = Elem<DT>::load(q[b][j / 4][j % 4]) * qs;
-            y[j] = Elem<DT>::load(k[b][j / 4][j % 4]) * ks;
-        }
     }
 };
 
@@ -592,15 +619,12 @@ __device__ inline void put_by_channel(ByChannel<KB>& tr, int b, uint32_t g, uint
 }
 
 template <int KB>
-__device__ inline void write_by_channel(const ByChannel<KB>& tr, uint32_t wave, uint32_t waves,
-                                        f16x8 (&out)[2 * KB][64]) {
+__device__ inline f16x8 by_channel(const ByChannel<KB>& tr, uint32_t tile) {
     typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    for (uint32_t t = wave; t < 2 * KB; t += waves) {
-        const f16x4 lo = *reinterpret_cast<const f16x4*>(&tr[16 * t + m][4 * g]);
-        const f16x4 hi = *reinterpret_cast<const f16x4*>(&tr[16 * t + m][16 + 4 * g]);
-        out[t][lane] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    }
+    const f16x4 lo = *reinterpret_cast<const f16x4*>(&tr[16 * tile + m][4 * g]);
+    const f16x4 hi = *reinterpret_cast<const f16x4*>(&tr[16 * tile + m][16 + 4 * g]);
+    return f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
 // One chunk of one head under a decay a channel, by two waves of 16 tokens.
@@ -612,14 +636,14 @@ __device__ inline void write_by_channel(const ByChannel<KB>& tr, uint32_t wave, 
 // one product of the whole tile, of which its own pairs are kept.  pre, suf and
 // a block's total come from the level before by one exchange over the lanes of
 // a row; after the last they are those of the tile.
-template <uint32_t DT, int KB>
+template <uint32_t DT, int KB, bool WHOLE>
 __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
-    DeltaArgs a, ChunkRecord* records, ChunkOperands<true, KB>* operands, bool vec) {
+    DeltaArgs a, ChunkRecord* records, ChunkOperands<true, KB>* operands) {
     typedef typename Elem<DT>::type E;
     __shared__ Tile32 Ls, Ps;
-    __shared__ Pair8 cross[KB][64];
-    __shared__ float total[2][32 * KB];
-    __shared__ __attribute__((aligned(16))) ByChannel<KB> tr[2];
+    __shared__ Pair8 cross[64];
+    __shared__ float total[2][32];
+    __shared__ __attribute__((aligned(16))) ByChannel<1> tr[2];
     __shared__ float beta_s[kChunk], c_s[kChunk];
     const uint32_t h = blockIdx.x % a.H, slot = blockIdx.x / a.H;
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -634,14 +658,17 @@ __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
     const size_t row = (size_t)place.sq.begin + place.first + (live ? t : 0);
     float z = 0.0f;  // NaN once an input is not finite
     bool wrong = false;
-    TokenRows<DT, KB> rows;
-    rows.load(a, static_cast<const E*>(a.q) + row * a.qs + (size_t)hk * a.K,
-              static_cast<const E*>(a.k) + row * a.ks + (size_t)hk * a.K, g, live, vec, z);
+    const E* qr = static_cast<const E*>(a.q) + row * a.qs + (size_t)hk * a.K;
+    const E* kr = static_cast<const E*>(a.k) + row * a.ks + (size_t)hk * a.K;
+    const float* gr = a.gate + (row * a.H + h) * a.K;
+    TokenScales rows;
+    rows.find<DT, KB, WHOLE>(a, qr, kr, g);
     const float beta = live ? a.beta[row * a.H + h] : 0.0f;
     z = __builtin_fmaf(beta, 0.0f, z);
     const bool norm = a.eps > 0.0f;
-    const float kmul = (norm ? rows.kn : rows.kd) * kOperand;
-    const float qmul = (norm ? rows.qn : rows.qd) * kOperand;
+    // A row past the sequence's end (read as the chunk's first) counts as 0.
+    const float kmul = live ? (norm ? rows.kn : rows.kd) * kOperand : 0.0f;
+    const float qmul = live ? (norm ? rows.qn : rows.qd) * kOperand : 0.0f;
     const float c_up = norm ? 1.0f : rows.ku, o_up = a.scale * (norm ? 1.0f : rows.qu);
     if (lane < 16) {
         beta_s[t] = beta;
@@ -652,97 +679,94 @@ __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
     }
     f32x4 accL[4] = {}, accP[4] = {}, l21 = {}, p21 = {};
     float diag = 0.0f;
-    const float* gr = a.gate + (row * a.H + h) * a.K;
-#pragma unroll
+    // The parts one after another, the next one's loads on their way (the first
+    // pass has them in the cache).
+    TokenPart<DT, WHOLE> next;
+    next.load(a, qr, kr, 0, g);
+    auto gates = [&](uint32_t c) {
+        if constexpr (WHOLE) return *reinterpret_cast<const f32x4*>(gr + c);
+        else return load4(gr, c, a.K, false);
+    };
+    f32x4 gate[2] = {gates(4 * g), gates(16 + 4 * g)};
+#pragma unroll 1
     for (int b = 0; b < KB; ++b) {
-        float kk[8], qq[8], x[8], pre[8], suf[8], tot[8];
-        rows.part(b, qmul, kmul, qq, kk);
+        f32x8 kk, qq, pre, suf, tot;
+        next.values(a, b, g, qq, kk);
+        qq *= qmul;
+        kk *= kmul;
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            const uint32_t c = 32 * b + 16 * y + 4 * g;
-            const f32x4 gate = load4(gr, c, a.K, vec);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float e = live && c + j < a.K ? gate[j] : 0.0f;
-                wrong |= !(e <= 0.0f);
-                pre[4 * y + j] = tot[4 * y + j] = exp_decay(e);
-                suf[4 * y + j] = 1.0f;
-            }
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t c = 32 * b + token_of(g, j);
+            const float e = live && (WHOLE || c < a.K) ? gate[j / 4][j % 4] : 0.0f;
+            wrong |= !(e <= 0.0f);
+            tot[j] = exp_decay(e);
+            suf[j] = 1.0f;
+            diag = __builtin_fmaf(kk[j], qq[j], diag);
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) diag = __builtin_fmaf(kk[j], qq[j], diag);
+        pre = tot;
+        if (b + 1 < KB) {
+            next.load(a, qr, kr, b + 1, g);
+            gate[0] = gates(32 * (b + 1) + 4 * g);
+            gate[1] = gates(32 * (b + 1) + 16 + 4 * g);
+        }
 #pragma unroll
         for (int level = 0; level < 4; ++level) {
             const bool bit = m >> level & 1;
-            float f[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                f[j] = bit ? pre[j] : suf[j];
-                x[j] = kk[j] * f[j];
-            }
-            const Pair8 kp = split8(x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = qq[j] * f[j];
-            const Pair8 qp = split8(x);
+            const f32x8 f = bit ? pre : suf;
+            const Pair8 kp = split8(kk * f), qp = split8(qq * f);
             accL[level] = mfma_pairs(kp, kp, accL[level]);
             accP[level] = mfma_pairs(qp, kp, accP[level]);
+            // The other block's total: from across bit `level` (a total is the
+            // same on every lane of its block, so that mirrors do).
+            f32x8 o;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // The other block's total: from across bit `level` (a total is
-                // the same on every lane of its block, so that mirrors do).
-                const float o = level == 0   ? dpp<0xb1>(tot[j])
-                                : level == 1 ? dpp<0x4e>(tot[j])
-                                : level == 2 ? dpp<0x141>(tot[j])
-                                             : dpp<0x140>(tot[j]);
-                pre[j] *= bit ? o : 1.0f;
-                suf[j] *= bit ? 1.0f : o;
-                tot[j] *= o;
-            }
+            for (int j = 0; j < 8; ++j)
+                o[j] = level == 0   ? dpp<0xb1>(tot[j])
+                       : level == 1 ? dpp<0x4e>(tot[j])
+                       : level == 2 ? dpp<0x141>(tot[j])
+                                    : dpp<0x140>(tot[j]);
+            const f32x8 one = 1.0f;
+            pre *= bit ? o : one;
+            suf *= bit ? one : o;
+            tot *= o;
         }
         // Tile 0's keys up to the border of the tiles, for tile 1.
-#pragma unroll
-        for (int j = 0; j < 8; ++j) suf[j] *= kk[j];
-        if (w == 0) cross[b][lane] = split8(suf);
+        suf *= kk;
+        if (w == 0) cross[lane] = split8(suf);
         if (m == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) total[w][32 * b + token_of(g, j)] = tot[j];
+            for (int j = 0; j < 8; ++j) total[w][token_of(g, j)] = tot[j];
         }
-        __syncthreads();
-        float other[8];
+        lds_barrier();
+        f32x8 other;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) other[j] = total[1 - w][32 * b + token_of(g, j)];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            kk[j] *= pre[j];
-            qq[j] *= pre[j];
-        }
+        for (int j = 0; j < 8; ++j) other[j] = total[1 - w][token_of(g, j)];
+        kk *= pre;
+        qq *= pre;
         Pair8 kp = split8(kk), qp = split8(qq);
         if (w == 1) {
-            const Pair8 before = cross[b][lane];
+            const Pair8 before = cross[lane];
             l21 = mfma_pairs(kp, before, l21);
             p21 = mfma_pairs(qp, before, p21);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                kk[j] *= other[j];
-                qq[j] *= other[j];
-            }
-            kp = split8(kk);
-            qp = split8(qq);
+            kp = split8(kk * other);
+            qp = split8(qq * other);
         } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) suf[j] *= other[j];
+            suf *= other;
         }
         ops->K[0][w][b][lane] = kp.hi;
         ops->K[1][w][b][lane] = kp.lo;
         ops->Q[0][w][b][lane] = qp.hi;
         ops->Q[1][w][b][lane] = qp.lo;
         const Pair8 sp = split8(suf);
-        put_by_channel<KB>(tr[0], b, g, t, sp.hi);
-        put_by_channel<KB>(tr[1], b, g, t, sp.lo);
+        put_by_channel<1>(tr[0], 0, g, t, sp.hi);
+        put_by_channel<1>(tr[1], 0, g, t, sp.lo);
         if (w == 0 && m == 0) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) rec->decay[32 * b + token_of(g, j)] = tot[j] * other[j];
         }
+        lds_barrier();
+        ops->Kt[0][2 * b + w][lane] = by_channel<1>(tr[0], w);
+        ops->Kt[1][2 * b + w][lane] = by_channel<1>(tr[1], w);
     }
     diag = sum_groups(diag);
     if (wrong || z != z) latch(a.status, K3X_ERR_INVALID_MXFP4);
@@ -767,9 +791,7 @@ __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
             Ps[ti][m] = p21[i] / kOperand;
         }
     }
-    __syncthreads();
-    write_by_channel<KB>(tr[0], w, 2, ops->Kt[0]);
-    write_by_channel<KB>(tr[1], w, 2, ops->Kt[1]);
+    lds_barrier();
     if (w == 0) write_inverse(Ls, c_s, beta_s, rec);
     else write_scores(Ps, rec);
 }
@@ -778,15 +800,14 @@ __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
 // tokens: the products of keys and queries once, and for each value head (a
 // wave every other one) its factors exp(G_i - G_j), G the log decays summed in
 // double.
-template <uint32_t DT, int KB>
+template <uint32_t DT, int KB, bool WHOLE>
 __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
-    DeltaArgs a, ChunkRecord* records, ChunkOperands<DT == K3X_DTYPE_F32, KB>* operands,
-    bool vec) {
+    DeltaArgs a, ChunkRecord* records, ChunkOperands<DT == K3X_DTYPE_F32, KB>* operands) {
     typedef typename Elem<DT>::type E;
     constexpr bool LO = DT == K3X_DTYPE_F32;
     __shared__ Tile32 Gk, Gq, work[2];
-    __shared__ Pair8 cross[KB][64];
-    __shared__ __attribute__((aligned(16))) ByChannel<KB> tr[LO ? 2 : 1];
+    __shared__ Pair8 cross[64];
+    __shared__ __attribute__((aligned(16))) ByChannel<1> tr[LO ? 2 : 1];
     __shared__ float c_s[kChunk], rk_s[kChunk], rq_s[kChunk], o_s[kChunk], beta_s[2][kChunk];
     __shared__ double G_s[2][kChunk];
     const uint32_t hk = blockIdx.x % a.Hk, slot = blockIdx.x / a.Hk, per = a.H / a.Hk;
@@ -801,9 +822,10 @@ __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
     const size_t row0 = (size_t)place.sq.begin + place.first, row = row0 + (live ? t : 0);
     float z = 0.0f;  // NaN once an input is not finite
     bool wrong = false;
-    TokenRows<DT, KB> rows;
-    rows.load(a, static_cast<const E*>(a.q) + row * a.qs + (size_t)hk * a.K,
-              static_cast<const E*>(a.k) + row * a.ks + (size_t)hk * a.K, g, live, vec, z);
+    const E* qr = static_cast<const E*>(a.q) + row * a.qs + (size_t)hk * a.K;
+    const E* kr = static_cast<const E*>(a.k) + row * a.ks + (size_t)hk * a.K;
+    TokenScales rows;
+    rows.find<DT, KB, WHOLE>(a, qr, kr, g);
     const bool norm = a.eps > 0.0f;
     if (lane < 16) {
         c_s[t] = norm ? 1.0f : rows.ku;
@@ -811,41 +833,46 @@ __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
         rq_s[t] = norm ? rows.qn * rows.qu : 1.0f;
         o_s[t] = a.scale * (norm ? 1.0f : rows.qu);
     }
-    f32x4 accK = {}, accQ = {};
-    Pair8 kp[KB], qp[KB];
+    const float qmul = live ? rows.qd * kOperand : 0.0f, kmul = live ? rows.kd * kOperand : 0.0f;
+    f32x4 accK = {}, accQ = {}, k21 = {}, q21 = {};
     float diag = 0.0f;
-#pragma unroll
+    // The parts one after another, the next one's loads on their way (the first
+    // pass has them in the cache).
+    TokenPart<DT, WHOLE> next;
+    next.load(a, qr, kr, 0, g);
+#pragma unroll 1
     for (int b = 0; b < KB; ++b) {
-        float kk[8], qq[8];
-        rows.part(b, rows.qd * kOperand, rows.kd * kOperand, qq, kk);
+        f32x8 kk, qq;
+        next.values(a, b, g, qq, kk);
+        if (b + 1 < KB) next.load(a, qr, kr, b + 1, g);
+        qq *= qmul;
+        kk *= kmul;
 #pragma unroll
         for (int j = 0; j < 8; ++j) diag = __builtin_fmaf(kk[j], qq[j], diag);
-        kp[b] = split8(kk);
-        qp[b] = split8(qq);
-        accK = mfma_pairs(kp[b], kp[b], accK);
-        accQ = mfma_pairs(qp[b], kp[b], accQ);
-        if (w == 0) cross[b][lane] = kp[b];
-        ops->K[0][w][b][lane] = kp[b].hi;
-        ops->Q[0][w][b][lane] = qp[b].hi;
-        put_by_channel<KB>(tr[0], b, g, t, kp[b].hi);
+        const Pair8 kp = split8(kk), qp = split8(qq);
+        accK = mfma_pairs(kp, kp, accK);
+        accQ = mfma_pairs(qp, kp, accQ);
+        if (w == 0) cross[lane] = kp;
+        ops->K[0][w][b][lane] = kp.hi;
+        ops->Q[0][w][b][lane] = qp.hi;
+        put_by_channel<1>(tr[0], 0, g, t, kp.hi);
         if (LO) {
-            ops->K[LO ? 1 : 0][w][b][lane] = kp[b].lo;
-            ops->Q[LO ? 1 : 0][w][b][lane] = qp[b].lo;
-            put_by_channel<KB>(tr[LO ? 1 : 0], b, g, t, kp[b].lo);
+            ops->K[LO ? 1 : 0][w][b][lane] = kp.lo;
+            ops->Q[LO ? 1 : 0][w][b][lane] = qp.lo;
+            put_by_channel<1>(tr[LO ? 1 : 0], 0, g, t, kp.lo);
         }
+        lds_barrier();
+        if (w == 1) {
+            const Pair8 before = cross[lane];
+            k21 = mfma_pairs(kp, before, k21);
+            q21 = mfma_pairs(qp, before, q21);
+        }
+#pragma unroll
+        for (int y = 0; y < (LO ? 2 : 1); ++y) ops->Kt[y][2 * b + w][lane] = by_channel<1>(tr[y], w);
+        lds_barrier();
     }
     diag = sum_groups(diag);
-    __syncthreads();
     const float un = 1.0f / (kOperand * kOperand);
-    f32x4 k21 = {}, q21 = {};
-    if (w == 1) {
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            const Pair8 before = cross[b][lane];
-            k21 = mfma_pairs(kp[b], before, k21);
-            q21 = mfma_pairs(qp[b], before, q21);
-        }
-    }
     // Products of the normalised rows: row 4 g + i, column m.
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -857,9 +884,7 @@ __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
             Gq[ti][m] = q21[i] * un * rq_s[ti] * rk_s[m];
         }
     }
-    __syncthreads();
-    write_by_channel<KB>(tr[0], w, 2, ops->Kt[0]);
-    if (LO) write_by_channel<KB>(tr[LO ? 1 : 0], w, 2, ops->Kt[LO ? 1 : 0]);
+    lds_barrier();
     for (uint32_t v = w; v < per; v += 2) {
         const uint32_t h = hk * per + v;
         ChunkRecord* rec = records + (size_t)slot * a.H + h;
@@ -1045,27 +1070,37 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
 #pragma unroll
         for (int j = 0; j < 8; ++j) tiles[i & 1][4 * g + 16 * (j / 4) + j % 4][m] = direct[j];
     };
-    // The wave's share of chunk i, 1 KiB a load: parts x of `of`.
-    constexpr uint32_t kRecord = sizeof(ChunkRecord) / 1024, kAll = sizeof(Chunk) / 1024;
-    static_assert(sizeof(Chunk) % 1024 == 0, "whole loads");
-    constexpr uint32_t kUnits = (kAll + W - 1) / W;
-    auto bring = [&](uint32_t i, uint32_t x, uint32_t of) {
-        const size_t slot = slot0 + i;
-        const auto rr = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<ChunkRecord*>(records + slot * a.H + h), (short)0, sizeof(ChunkRecord),
-            0x00020000);
-        const auto ro = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<ChunkOperands<LO, KB>*>(
-                operands + (CHANNEL ? slot * a.H + h : slot * a.Hk + hk)),
-            (short)0, sizeof(ChunkOperands<LO, KB>), 0x00020000);
+    // The wave's share of a chunk, 1 KiB a load: the parts x of `of`.
+    const ChunkRecord* rec = records + slot0 * a.H + h;
+    const ChunkOperands<LO, KB>* ops = operands + (CHANNEL ? slot0 * a.H + h : slot0 * a.Hk + hk);
+    const uint32_t heads = CHANNEL ? a.H : a.Hk;
+    struct Source {
+        __amdgpu_buffer_rsrc_t rec, ops;
+    };
+    auto source = [&]() {
+        return Source{__builtin_amdgcn_make_buffer_rsrc(const_cast<ChunkRecord*>(rec), (short)0,
+                                                        sizeof(ChunkRecord), 0x00020000),
+                      __builtin_amdgcn_make_buffer_rsrc(
+                          const_cast<ChunkOperands<LO, KB>*>(ops), (short)0,
+                          sizeof(ChunkOperands<LO, KB>), 0x00020000)};
+    };
+    auto bring = [&](const Source& from, uint32_t i, uint32_t x, uint32_t of) {
+        constexpr uint32_t kRec = sizeof(ChunkRecord) / 1024;
+        constexpr uint32_t kOps = sizeof(ChunkOperands<LO, KB>) / 1024;
+        constexpr uint32_t kRecLoads = (kRec + W - 1) / W, kOpsLoads = (kOps + W - 1) / W;
         u32x4* dst = reinterpret_cast<u32x4*>(&buf[i & 1]);
 #pragma unroll
-        for (uint32_t y = 0; y < kUnits; ++y) {
+        for (uint32_t y = 0; y < kRecLoads + kOpsLoads; ++y) {
             if (y % of != x) continue;
-            const uint32_t unit = W * y + wave;
-            if (unit < kRecord) load_lds16(rr, dst + 64 * unit, lane * 16, unit * 1024);
-            else if (unit < kAll)
-                load_lds16(ro, dst + 64 * unit, lane * 16, (unit - kRecord) * 1024);
+            if (y < kRecLoads) {
+                const uint32_t unit = W * y + wave;
+                if (W * (y + 1) <= kRec || unit < kRec)
+                    load_lds16(from.rec, dst + 64 * unit, lane * 16, unit * 1024);
+            } else {
+                const uint32_t unit = W * (y - kRecLoads) + wave;
+                if (W * (y + 1 - kRecLoads) <= kOps || unit < kOps)
+                    load_lds16(from.ops, dst + 64 * (kRec + unit), lane * 16, unit * 1024);
+            }
         }
     };
     const size_t base = ((size_t)sq.slot * a.H + h) * a.K * a.V;
@@ -1090,10 +1125,9 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
 #pragma unroll
             for (int i = 0; i < 4; ++i) S[t][i] = kOperand * __builtin_ldexpf(S[t][i], -shift);
     }
-    float z = 0.0f;
     if (chunks) {
         bring_values(0);
-        bring(0, 0, 1);
+        bring(source(), 0, 0, 1);
         put_values(0);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
@@ -1101,6 +1135,9 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
         const ChunkRecord& rc = buf[ci & 1].r;
         const ChunkOperands<LO, KB>& o = buf[ci & 1].o;
         const bool more = ci + 1 < chunks;
+        rec += a.H;
+        ops += heads;
+        const Source from = source();  // the next chunk
         f32x4 v[2], aq[2] = {}, ak[2] = {};
         // Operands of 32 channels, the next ones on their way while these are
         // multiplied.
@@ -1134,7 +1171,6 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                z = __builtin_fmaf(v[t][j], 0.0f, z);
                 v[t][j] = __builtin_ldexpf(v[t][j], -shift);
                 most = fmaxf(most, fabsf(v[t][j]) * kOperand);
             }
@@ -1170,11 +1206,10 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
                     rt[t] = factors(rc.row_t, t);
                 }
             }
-            if (more) bring(ci + 1, b, KB);
+            if (more) bring(from, ci + 1, b, KB);
             __builtin_amdgcn_sched_barrier(0);
             const f32x4 &l = S[2 * b], &u = S[2 * b + 1];
-            const float y[8] = {l[0], l[1], l[2], l[3], u[0], u[1], u[2], u[3]};
-            const Pair8 s = split8(y);
+            const Pair8 s = split8(f32x8{l[0], l[1], l[2], l[3], u[0], u[1], u[2], u[3]});
             const auto& kp = kf[b & 1];
             const auto& qp = qf[b & 1];
             if (LO) {
@@ -1226,9 +1261,8 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
                 for (int i = 0; i < 4; ++i) S[t][i] = __builtin_ldexpf(S[t][i], -d);
         };
         auto operand = [&](const f32x4 (&x)[2]) {
-            const float y[8] = {x[0][0], x[0][1], x[0][2], x[0][3],
-                                x[1][0], x[1][1], x[1][2], x[1][3]};
-            return split8(y);
+            return split8(f32x8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2],
+                                x[1][3]});
         };
         f32x4 u[2], ap[2] = {};
 #pragma unroll
@@ -1337,7 +1371,9 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
             asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
     }
-    if (z != z) latch(a.status, K3X_ERR_INVALID_MXFP4);
+    // A value that is not finite has made every row of its column NaN (the
+    // products' operands hold no infinity that is not NaN in a sum).
+    if (chunks && !(S[0][0] - S[0][0] == 0.0f)) latch(a.status, K3X_ERR_INVALID_MXFP4);
     if (!a.state_out || !in || (!chunks && a.state_in == a.state_out)) return;
 #pragma unroll
     for (int t = 0; t < 2 * KB; ++t)
@@ -1382,12 +1418,17 @@ int launch_chunks(k3x_hip_ctx* ctx, const DeltaArgs& a, void* workspace, const C
     Operands* ops = reinterpret_cast<Operands*>(static_cast<uint8_t*>(workspace) +
                                                 space.operands_at);
     const uint32_t slots = (uint32_t)space.slots;
-    if constexpr (CHANNEL)
-        hipLaunchKernelGGL((delta_prep_channel_kernel<DT, KB>), dim3(slots * a.H), dim3(128), 0,
-                           ctx->stream, a, records, ops, vec);
-    else
-        hipLaunchKernelGGL((delta_prep_head_kernel<DT, KB>), dim3(slots * a.Hk), dim3(128), 0,
-                           ctx->stream, a, records, ops, vec);
+    auto prepare = [&](auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
+        if constexpr (CHANNEL)
+            hipLaunchKernelGGL((delta_prep_channel_kernel<DT, KB, kWhole>), dim3(slots * a.H),
+                               dim3(128), 0, ctx->stream, a, records, ops);
+        else
+            hipLaunchKernelGGL((delta_prep_head_kernel<DT, KB, kWhole>), dim3(slots * a.Hk),
+                               dim3(128), 0, ctx->stream, a, records, ops);
+    };
+    if (vec && a.K == 32 * KB) prepare(std::true_type{});
+    else prepare(std::false_type{});
     constexpr bool LO = CHANNEL || DT == K3X_DTYPE_F32;
     const uint32_t heads = a.N * a.H;
     const uint32_t es = sizeof(typename Elem<DT>::type);
