@@ -443,12 +443,12 @@ typedef struct k3x_hip_delta_params {
  *   u = beta (v - S^T k)
  *   S = S + k u^T
  *   out = scale S^T q
- * q, k device [T][Hk][K], v, out [T][Hv][V]; gate fp32 [T][Hv][K] or [T][Hv],
- * <= 0 (minus infinity empties the state; NULL with K3X_GATE_NONE); beta fp32
- * [T][Hv].  Sequence n has the rows offsets[n] .. offsets[n + 1] - 1 (device
- * u32 [N + 1]; NULL: T / N rows each), of which the first limits[n] only are
- * taken where limits (device u32 [N]) is given: rows of out past them are left
- * as they were.  So a window of drafted tokens is run with state_out NULL, and
+ * q, k device [T][Hk][K], v, out [T][Hv][V], out apart from the inputs; gate
+ * fp32 [T][Hv][K] or [T][Hv], <= 0 (minus infinity empties the state; NULL with
+ * K3X_GATE_NONE); beta fp32 [T][Hv].  Sequence n has the rows offsets[n] ..
+ * offsets[n + 1] - 1 (device u32 [N + 1]; NULL: T / N rows each), of which the
+ * first limits[n] only are taken where limits (device u32 [N]) is given: rows of
+ * out past them are left as they were.  So a window of drafted tokens is run with state_out NULL, and
  * run again up to the accepted count with it.
  * state_in: device fp32 [slots][Hv][K][V], 16-byte aligned, or NULL (zeros);
  * state_out: the same, state_in itself or apart from it, or NULL (not

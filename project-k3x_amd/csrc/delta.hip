@@ -128,10 +128,15 @@ __device__ inline Vec4<E> load4(const E* row, uint32_t c, uint32_t n, bool vec) 
 // over the 16 row groups, in which each exchange folds two sums into one
 // register.  The next token's rows are loaded meanwhile.  A workgroup's waves
 // are neighbours in the columns of one head and share nothing else.
+//
+// One token a sequence is the state's read and write: 64 sequences of 32 heads
+// of 128 x 128 take 48 us, 5.6 TB/s.  More tokens are bound by the sums' chain:
+// 16 tokens a sequence (8 sequences, limits) 26 us, 1.3 us a token.
 constexpr int kStepWaves = 4;
 constexpr uint32_t kStepCols = 16 * kStepWaves;
 
-// vec: bit 0, q, k and gate by four elements; bit 1, v; bit 2, states.
+// vec: bit 0, q, k and gate by four elements (of the calls above 48 and 26 us;
+// by one 57 and 37); bit 1, v (by one 27 of the second); bit 2, states.
 template <uint32_t DT, int R, uint32_t GATE>
 __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a, uint32_t vec) {
     typedef typename Elem<DT>::type E;
@@ -319,8 +324,11 @@ void launch_step_rows(const DeltaArgs& a, uint32_t gate, uint32_t vec, hipStream
 //   S    = P_31 S + sum_j (D_31,j k_j) U_j^T
 //
 // all of them products of 16 x 16 tiles on the matrix cores.  Two launches:
-// delta_prep_kernel makes (I + L)^-1 and Pq of every chunk, all at once;
-// delta_scan_kernel walks a sequence's chunks with the state in registers.
+// delta_prep_channel_kernel or delta_prep_head_kernel makes (I + L)^-1 and Pq of
+// every chunk and its keys and queries as operands, all chunks at once;
+// delta_scan_kernel walks a sequence's chunks with the state in registers.  The
+// operands are made once and not by each of the scan's workgroups (a head's
+// columns lie in several), whose chain of chunks is what a long prompt waits for.
 //
 // Operands are f16 pairs hi + lo (22 bits: what is left out of a product of two
 // pairs, lo lo, is 2^-22 of it), sums fp32.  f16 ends at 65504 and 2^-24, so
@@ -636,6 +644,12 @@ __device__ inline f16x8 by_channel(const ByChannel<KB>& tr, uint32_t tile) {
 // one product of the whole tile, of which its own pairs are kept.  pre, suf and
 // a block's total come from the level before by one exchange over the lanes of
 // a row; after the last they are those of the tile.
+//
+// 2048 tokens of 32 heads of 128: 50 us for 66 MB read and 119 MB written, 3.7
+// TB/s; one 32-channel part in registers at a time, two workgroups a SIMD pair
+// (three or four do not fit without spills).
+// WHOLE: K = 32 KB and rows by four elements, so that no load is guarded (rows
+// off by one element: 199 us in place of 179 with the scan).
 template <uint32_t DT, int KB, bool WHOLE>
 __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
     DeltaArgs a, ChunkRecord* records, ChunkOperands<true, KB>* operands) {
@@ -799,7 +813,8 @@ __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
 // One chunk of one key head under a decay a value head, by two waves of 16
 // tokens: the products of keys and queries once, and for each value head (a
 // wave every other one) its factors exp(G_i - G_j), G the log decays summed in
-// double.
+// double.  8192 tokens of 16 key and 32 value heads of 128: 72 us for 67 MB read
+// and 185 MB written, 3.5 TB/s.  WHOLE as above (242 in place of 215 us).
 template <uint32_t DT, int KB, bool WHOLE>
 __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
     DeltaArgs a, ChunkRecord* records, ChunkOperands<DT == K3X_DTYPE_F32, KB>* operands) {
@@ -981,12 +996,20 @@ __device__ inline void store_one(E x, __amdgpu_buffer_rsrc_t r, uint32_t voffset
                                               0);
 }
 
-// Walks one sequence's chunks for 16 W value columns of one head.  Each of the W
+// Walks one sequence's chunks for 64 value columns of one head.  Each of the four
 // waves holds 16 columns of the state as the results of 2 KB products (rows by
 // 16): row 16 t + 4 (l / 16) + i and column l % 16 in register i of tile t of
 // lane l, and splits it into the next products' operands where it is.  While a
 // chunk is multiplied, the next one's record, operands and values come to LDS
 // as they lie, the loads spread over the products.
+//
+// A chunk takes 2.1 us: (P k) S, U, its operand, T U and the update follow one
+// another, and one wave a SIMD issues all of them, 645 instructions of which 84
+// are products (1344 of 4900 cycles).  So a sequence of 2048 tokens takes 135 us,
+// and seven of 8192 together (448 workgroups, two a CU) 153 us.  Neither fewer
+// columns a workgroup (two waves: 136 us of the first, one: 156), nor more (eight
+// waves: 170 us of the second), nor two waves to 16 columns, each with half of
+// the channels (155 us), shorten that.
 template <bool LO, int KB>
 struct ScanChunk {
     ChunkRecord r;
@@ -996,14 +1019,18 @@ struct ScanChunk {
 template <uint32_t DT>
 using ScanTile = typename Elem<DT>::type[kChunk][16];
 
-template <uint32_t DT, bool LO, int KB, int W>
+constexpr int kScanWaves = 4;
+constexpr uint32_t kScanCols = 16 * kScanWaves;
+
+template <uint32_t DT, bool LO, int KB>
 constexpr size_t scan_lds() {
-    return 2 * sizeof(ScanChunk<LO, KB>) + 2 * W * sizeof(ScanTile<DT>);
+    return 2 * sizeof(ScanChunk<LO, KB>) + 2 * kScanWaves * sizeof(ScanTile<DT>);
 }
 
-// vec: bit 0, rows of v by 16 bytes; bit 1, rows of out.
-template <uint32_t DT, bool CHANNEL, int KB, int W>
-__global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
+// vec: bit 0, rows of v by 16 bytes (179 us with the operands' kernel, by one
+// element 187, of the first call above); bit 1, rows of out.
+template <uint32_t DT, bool CHANNEL, int KB>
+__global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
     DeltaArgs a, const ChunkRecord* records,
     const ChunkOperands<CHANNEL || DT == K3X_DTYPE_F32, KB>* operands, uint32_t vec) {
     typedef typename Elem<DT>::type E;
@@ -1013,7 +1040,7 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
     // on one wave a SIMD and move results through the accumulation registers.
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     Chunk* buf = reinterpret_cast<Chunk*>(lds);
-    const uint32_t blocks = (a.V + 16 * W - 1) / (16 * W);
+    const uint32_t blocks = (a.V + kScanCols - 1) / kScanCols;
     // Quotients come from the vector unit: kept scalar, as buffers want them.
     const uint32_t cb = __builtin_amdgcn_readfirstlane(blockIdx.x % blocks);
     const uint32_t h = __builtin_amdgcn_readfirstlane(blockIdx.x / blocks % a.H);
@@ -1037,7 +1064,7 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
     constexpr int kTileLoads = sizeof(ScanTile<DT>) / 1024;
     ScanTile<DT>* tiles = reinterpret_cast<ScanTile<DT>*>(lds + 2 * sizeof(Chunk)) + 2 * wave;
     const uint32_t vst = (uint32_t)a.vs * es, ost = (uint32_t)a.os * es;
-    const uint32_t col0 = (cb * W + wave) * 16, col = col0 + m;
+    const uint32_t col0 = (cb * kScanWaves + wave) * 16, col = col0 + m;
     const bool in = col < a.V;
     // Sixteen bytes of a row of the tile: lane's row (of each load's) and column.
     constexpr uint32_t kRowLanes = 16 * es / 16;
@@ -1087,6 +1114,7 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
     auto bring = [&](const Source& from, uint32_t i, uint32_t x, uint32_t of) {
         constexpr uint32_t kRec = sizeof(ChunkRecord) / 1024;
         constexpr uint32_t kOps = sizeof(ChunkOperands<LO, KB>) / 1024;
+        constexpr uint32_t W = kScanWaves;
         constexpr uint32_t kRecLoads = (kRec + W - 1) / W, kOpsLoads = (kOps + W - 1) / W;
         u32x4* dst = reinterpret_cast<u32x4*>(&buf[i & 1]);
 #pragma unroll
@@ -1385,13 +1413,18 @@ __global__ __launch_bounds__(64 * W, 2) void delta_scan_kernel(
         }
 }
 
-// Chunks for sequences that fill one and heads that the products' tiles take.
-constexpr uint32_t kChunkMinTokens = 24;
-
+// Chunks for heads that the products' tiles take, from the length on where one
+// chunk costs no more than its tokens one by one.  Measured over 32 heads of
+// 128 x 128, us in chunks and token by token:
+//   gates by channel, 1 / 8 / 64 sequences of 20 tokens  23, 26 | 44, 37 | 203, 195
+//                                             24 tokens  23, 30 | 44, 45 | 205, 224
+//   gates by head (16 key heads),             12 tokens  18, 16 | 27, 21 | 112, 120
+//                                             16 tokens  18, 19 | 28, 26 | 116, 149
+// (12 tokens between 8 and 16).
 bool runs_in_chunks(const k3x_hip_delta_params* p) {
     const uint32_t longest =
         p->longest ? p->longest : (p->tokens + p->sequences - 1) / p->sequences;
-    return p->key_dim <= 128 && longest >= kChunkMinTokens;
+    return p->key_dim <= 128 && longest >= (p->gate == K3X_GATE_CHANNEL ? 24u : 16u);
 }
 
 // Where a call's records and operands lie in its workspace.
@@ -1430,18 +1463,13 @@ int launch_chunks(k3x_hip_ctx* ctx, const DeltaArgs& a, void* workspace, const C
     if (vec && a.K == 32 * KB) prepare(std::true_type{});
     else prepare(std::false_type{});
     constexpr bool LO = CHANNEL || DT == K3X_DTYPE_F32;
-    const uint32_t heads = a.N * a.H;
     const uint32_t es = sizeof(typename Elem<DT>::type);
     const uint32_t rows = (a.V * es % 16 == 0 && a.vs * es % 16 == 0 && aligned(a.v, 16) ? 1 : 0) |
                           (a.V * es % 16 == 0 && a.os * es % 16 == 0 && aligned(a.out, 16) ? 2 : 0);
-    if (a.V > 64 && heads >= ctx->cu_count / 2)
-        hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB, 8>),
-                           dim3(heads * ((a.V + 127) / 128)), dim3(512),
-                           (scan_lds<DT, LO, KB, 8>()), ctx->stream, a, records, ops, rows);
-    else
-        hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB, 4>),
-                           dim3(heads * ((a.V + 63) / 64)), dim3(256),
-                           (scan_lds<DT, LO, KB, 4>()), ctx->stream, a, records, ops, rows);
+    hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB>),
+                       dim3(a.N * a.H * ((a.V + kScanCols - 1) / kScanCols)),
+                       dim3(64 * kScanWaves), (scan_lds<DT, LO, KB>()), ctx->stream, a, records,
+                       ops, rows);
     return launched(ctx, 2);
 }
 
