@@ -448,8 +448,9 @@ typedef struct k3x_hip_delta_params {
  * K3X_GATE_NONE); beta fp32 [T][Hv].  Sequence n has the rows offsets[n] ..
  * offsets[n + 1] - 1 (device u32 [N + 1]; NULL: T / N rows each), of which the
  * first limits[n] only are taken where limits (device u32 [N]) is given: rows of
- * out past them are left as they were.  So a window of drafted tokens is run with state_out NULL, and
- * run again up to the accepted count with it.
+ * out past them are left as they were.  So a window of the last token and the
+ * drafted ones is run with state_out NULL, and run again with it up to the last
+ * accepted token.
  * state_in: device fp32 [slots][Hv][K][V], 16-byte aligned, or NULL (zeros);
  * state_out: the same, state_in itself or apart from it, or NULL (not
  * written).  Sequence n has the state slot_index[n] (device u32 [N]), or n
