@@ -22,6 +22,7 @@ struct RouteArgs {
     uint32_t scoring, renorm;
     float scale;
     uint32_t G, top_groups, group_score;
+    uint32_t group, group_by;  // experts a group; 2^20 / group + 1
     uint32_t stride;
     uint32_t* ids;
     float* weights;
@@ -85,11 +86,11 @@ __device__ inline uint32_t route_check(const RouteArgs& a, float logit, float s,
 // the smaller one.
 template <int Ctrl>
 __device__ inline uint32_t dpp_max(uint32_t x) {
-    return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, Ctrl, 0xf, 0xf, false));
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, Ctrl, 0xf, 0xf, true));
 }
 template <int Ctrl>
 __device__ inline uint32_t dpp_min(uint32_t x) {
-    return min(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, Ctrl, 0xf, 0xf, false));
+    return min(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, Ctrl, 0xf, 0xf, true));
 }
 template <bool MAX>
 __device__ inline uint32_t across_rows(uint32_t x, bool halves) {
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(64) void route_lds_kernel(RouteArgs a) {
     __syncthreads();
     if (a.G > 1) {
         // Lane g ranks group g; the experts of the groups left out lose their keys.
-        const uint32_t n = E / a.G;
+        const uint32_t n = a.group;
         uint64_t gk = 0;
         if (lane < a.G) {
             uint64_t k1 = 0, k2 = 0;
@@ -256,7 +257,9 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_wave_kernel(RouteArgs 
         double e[KPL], den = 0.0;
 #pragma unroll
         for (int i = 0; i < KPL; ++i) {
-            e[i] = lane + 64u * i < E ? exp_f64((double)l[i] - mx) : 0.0;
+            // Past E the last expert's once more, and left out after: no branch.
+            const double y = exp_f64((double)l[i] - mx);
+            e[i] = lane + 64u * i < E ? y : 0.0;
             den += e[i];
         }
         const double inv = 1.0 / wave_sum(den);
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_wave_kernel(RouteArgs 
         for (int i = 0; i < KPL; ++i)
             if (lane + 64u * i < E) keys[lane + 64u * i] = ord[i];
         wave_sync();
-        const uint32_t n = E / a.G, width = 64u >> (32 - __clz(a.G - 1));  // lanes a group
+        const uint32_t n = a.group, width = 64u >> (32 - __clz(a.G - 1));  // lanes a group
         const uint32_t g = lane / width;
         uint32_t k1 = 0, k2 = 0;
         if (g < a.G)
@@ -305,19 +308,20 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_wave_kernel(RouteArgs 
         float gs = key_score((uint64_t)k1 << 32);
         if (a.group_score == K3X_GROUP_TOP2 && n > 1)
             gs = __fadd_rn(gs, key_score((uint64_t)k2 << 32));
-        const uint64_t gk = topk_key(gs, g);
+        // A group's lanes compare it with every width-th group each.
+        const uint32_t gk = (uint32_t)(topk_key(gs, 0) >> 32);
         uint32_t rank = 0;
-        for (uint32_t i = 0; i < a.G; ++i) {
-            const uint64_t o =
-                (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(gk >> 32), i * width)
-                    << 32 |
-                (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)gk, i * width);
-            rank += o > gk;
+        for (uint32_t i = 0; i < a.G; i += width) {
+            const uint32_t o = i + lane % width;
+            const uint32_t ok = (uint32_t)__shfl((int)gk, (int)(o * width & 63));
+            const uint64_t above = __ballot(o < a.G && (ok > gk || (ok == gk && o < g)));
+            rank += (uint32_t)__popcll(above >> (g * width & 63) & (~0ull >> (64 - width)));
         }
         const uint64_t kept = __ballot(g < a.G && rank < a.top_groups);
+        // e / n by a factor: e (2^20 / n + 1) 2^-20 is over it by 2^-10 <= 1 / n at most.
 #pragma unroll
         for (int i = 0; i < KPL; ++i)
-            if (!(kept >> ((lane + 64u * i) / n * width & 63) & 1)) ord[i] = 0;
+            if (!(kept >> (((lane + 64u * i) * a.group_by >> 20) * width & 63) & 1)) ord[i] = 0;
         wave_sync();
     }
     uint32_t head = 0;
@@ -415,6 +419,8 @@ int k3x_hip_route(k3x_hip_ctx* ctx, const k3x_hip_route_params* p, const void* l
     a.renorm = p->renorm;
     a.scale = p->routed_scale;
     a.G = p->top_groups == p->groups ? 1 : p->groups;  // every group stays: no groups
+    a.group = a.E / a.G;
+    a.group_by = (1u << 20) / a.group + 1;
     a.top_groups = p->top_groups;
     a.group_score = p->group_score;
     a.stride = p->logits_stride ? p->logits_stride : p->experts;
