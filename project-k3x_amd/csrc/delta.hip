@@ -1496,9 +1496,10 @@ bool delta_ok(const k3x_hip_delta_params* p) {
            (!p->k_stride || (p->k_stride >= kw && p->k_stride <= most)) &&
            (!p->v_stride || (p->v_stride >= vw && p->v_stride <= most)) &&
            (!p->out_stride || (p->out_stride >= vw && p->out_stride <= most)) &&
-           // workgroups of a launch
-           (uint64_t)p->sequences * p->value_heads * 16 < (1ull << 31) &&
-           ((uint64_t)p->tokens / 32 + p->sequences) * p->value_heads < (1ull << 31);
+           // threads of a launch
+           (uint64_t)p->sequences * p->value_heads * ((p->value_dim + 63) / 64) * 256 <
+               (1ull << 32) &&
+           ((uint64_t)p->tokens / kChunk + p->sequences) * p->value_heads * 128 < (1ull << 32);
 }
 
 }  // namespace

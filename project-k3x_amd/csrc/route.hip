@@ -218,7 +218,7 @@ __global__ __launch_bounds__(64) void route_lds_kernel(RouteArgs a) {
 // few dozen keys in place of K passes over all.
 //
 // Bound by the instructions: 30011 tokens of 256 experts (bf16, softmax, Top-8
-// in 4 of 8 groups) take 38 us, the time of some 780 a token on every SIMD, where
+// in 4 of 8 groups) take 33 us, some 600 vector instructions a token, where
 // the logits' 15 MB take 4 us; 2048 tokens of 896 experts (sigmoid) 13 us.
 // The fewest registers that hold the experts (Top-8 of sigmoid scores, 30011
 // tokens): 256 experts 23 us with 4 a lane, 33 with 8, 61 with 16; 512 experts

@@ -4,7 +4,7 @@
 //            the sum of exponentials over it (logits, and greedy choices);
 //   accept   one workgroup a sequence: every row's totals and drafted token's
 //            probabilities at once, then the walk over the drafts;
-//   draw     the row that the next token is drawn from, by parts of 4096: their
+//   draw     the row that the next token is drawn from, by the same parts: their
 //            sums, and by the sequence's last workgroup the part and the entry
 //            that the border falls in.
 //
@@ -24,8 +24,9 @@ using namespace k3x_ops;
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kEntries = 16;  // of a part, a thread
-constexpr uint32_t kPart = kThreads * kEntries;
+constexpr uint32_t kEntries = 16;  // of a part, a lane
+constexpr uint32_t kPart = 64 * kEntries;  // a wave's
+constexpr uint32_t kWaves = kThreads / 64;
 constexpr uint32_t kMaxDrafts = 64;
 
 // One part of a row; max NaN: it holds an entry that no row may.
@@ -49,12 +50,11 @@ struct VerifyArgs {
     const float *accept_u, *sample_u;
     uint32_t *accepted, *out_tokens;
     uint32_t N, D, V, stride;
-    uint32_t row_parts_of;  // a row, in waves' parts
-    uint32_t parts;         // of the draw, in workgroups' parts
+    uint32_t parts;     // of a row
     uint32_t form, greedy;
     uint32_t vec;       // rows by 16 bytes
     double rate;        // log2(e) / temperature
-    RowPart* row_parts; // [N (2 D + 1)][row_parts_of]: a sequence's target rows, then its draft's
+    RowPart* row_parts; // [N (2 D + 1)][parts]: a sequence's target rows, then its draft's
     Drawn* drawn;       // [N]
     double* sums;       // [N][parts]
     uint32_t* status;
@@ -73,7 +73,7 @@ __device__ inline const typename Elem<DT>::type* row_of(const VerifyArgs& a, uin
 }
 
 __device__ inline size_t part_index(const VerifyArgs& a, uint32_t n, uint32_t r) {
-    return ((size_t)n * (2 * a.D + 1) + r) * a.row_parts_of;
+    return ((size_t)n * (2 * a.D + 1) + r) * a.parts;
 }
 
 // The larger of two (entry, index) pairs, the lower index on a tie.
@@ -104,32 +104,37 @@ __device__ inline double exp2_f64(double y) {
     return __builtin_ldexp(p, (int)k);
 }
 
-// A thread's sixteen entries of a part of TH threads, neighbours by 16 bytes
-// where rows are, so that a wave's loads are whole lines; where() rises with j.
-template <uint32_t DT, uint32_t TH>
+// A lane's sixteen entries of a part, neighbours by 16 bytes where rows are, so
+// that a wave's loads are whole lines; where() rises with j.  By 16 bytes against
+// by one entry, all launches: 131072 and 131073 probabilities of 64 sequences 27
+// and 30 us, logits of 16 sequences of 4 drafts 47 and 52.
+template <uint32_t DT>
 struct Entries {
     typedef typename Elem<DT>::type E;
-    static constexpr uint32_t kWide = 16 / sizeof(E), kAll = TH * kEntries;
-    static __device__ inline uint32_t where(const VerifyArgs& a, uint32_t lo, uint32_t thread,
+    static constexpr uint32_t kWide = 16 / sizeof(E);
+    static __device__ inline uint32_t where(const VerifyArgs& a, uint32_t lo, uint32_t lane,
                                             int j) {
-        return a.vec ? lo + j / kWide * (TH * kWide) + thread * kWide + j % kWide
-                     : lo + j * TH + thread;
+        return a.vec ? lo + j / kWide * (64 * kWide) + lane * kWide + j % kWide
+                     : lo + j * 64 + lane;
     }
     // Past hi: `past`.
     static __device__ inline void load(const VerifyArgs& a, const E* x, uint32_t lo, uint32_t hi,
-                                       uint32_t thread, float past, float (&l)[kEntries]) {
+                                       uint32_t lane, float past, float (&l)[kEntries]) {
         typedef E Vec __attribute__((ext_vector_type(kWide)));
-        if (a.vec && lo + kAll <= hi) {
+        if (a.vec && lo + kPart <= hi) {
 #pragma unroll
             for (int j = 0; j < (int)kEntries; j += kWide) {
-                const Vec v = *reinterpret_cast<const Vec*>(x + where(a, lo, thread, j));
+                const Vec v = *reinterpret_cast<const Vec*>(x + where(a, lo, lane, j));
 #pragma unroll
                 for (int y = 0; y < (int)kWide; ++y) l[j + y] = Elem<DT>::load(v[y]);
             }
+        } else if (lo + kPart <= hi) {
+#pragma unroll
+            for (int j = 0; j < (int)kEntries; ++j) l[j] = Elem<DT>::load(x[lo + lane + j * 64]);
         } else {
 #pragma unroll
             for (int j = 0; j < (int)kEntries; ++j) {
-                const uint32_t i = where(a, lo, thread, j);
+                const uint32_t i = where(a, lo, lane, j);
                 l[j] = Elem<DT>::load(x[min(i, hi - 1)]);
                 if (i >= hi) l[j] = past;
             }
@@ -138,20 +143,20 @@ struct Entries {
 };
 
 // Parts of a row by waves, which do not wait for one another.  16 sequences of 4
-// drafts and 100003 fp32 logits (58 MB): 23 us, 2.5 TB/s; the exponentials in
+// drafts and 100003 fp32 logits (58 MB): 22 us, 2.6 TB/s; the exponentials in
 // double, some 18 operations each, take 7 us of it at the unit's rate.
 template <uint32_t DT>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a) {
     const uint32_t rows = a.draft ? 2 * a.D + 1 : a.D + 1;
-    const uint32_t blocks = (a.row_parts_of + kThreads / 64 - 1) / (kThreads / 64);
+    const uint32_t blocks = (a.parts + kWaves - 1) / kWaves;
     const uint32_t rr = blockIdx.x / blocks, n = rr / rows, r = rr % rows, lane = threadIdx.x & 63;
-    const uint32_t part = blockIdx.x % blocks * (kThreads / 64) +
+    const uint32_t part = blockIdx.x % blocks * kWaves +
                           __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t count = drafts_of(a, n);
-    if (part >= a.row_parts_of || count > a.D || (r <= a.D ? r > count : r - a.D - 1 >= count))
+    if (part >= a.parts || count > a.D || (r <= a.D ? r > count : r - a.D - 1 >= count))
         return;
-    typedef Entries<DT, 64> Mine;
-    const uint32_t lo = part * Mine::kAll, hi = min(a.V, lo + Mine::kAll);
+    typedef Entries<DT> Mine;
+    const uint32_t lo = part * kPart, hi = min(a.V, lo + kPart);
     float l[kEntries];
     Mine::load(a, row_of<DT>(a, n, r), lo, hi, lane, -__builtin_inff(), l);
     if (*(volatile uint32_t*)a.status) return;
@@ -195,7 +200,7 @@ __device__ inline bool row_total(const VerifyArgs& a, uint32_t n, uint32_t r, do
     float m = -__builtin_inff();
     uint32_t at = 0xffffffffu;
     bool nan = false;
-    for (uint32_t i = lane; i < a.row_parts_of; i += 64) {
+    for (uint32_t i = lane; i < a.parts; i += 64) {
         nan |= parts[i].max != parts[i].max;
         take_max(m, at, parts[i].max, parts[i].arg);
     }
@@ -206,7 +211,7 @@ __device__ inline bool row_total(const VerifyArgs& a, uint32_t n, uint32_t r, do
     if (m == -__builtin_inff() || (a.form == K3X_DIST_PROBS && m == 0.0f)) return false;
     double s = 0.0;
     if (!a.greedy)
-        for (uint32_t i = lane; i < a.row_parts_of; i += 64)
+        for (uint32_t i = lane; i < a.parts; i += 64)
             if (parts[i].sum > 0.0)
                 s += parts[i].sum *
                      exp2_f64(((double)parts[i].max - (double)m) * a.rate);
@@ -373,40 +378,57 @@ __device__ inline double run_start(double s, double start, double* sd) {
     return c;
 }
 
-// The token of a part that the border falls in: the last entry over 0 that the
-// cumulative sum (start before the part) has not passed the border before.  By
-// the whole workgroup, sixteen neighbours a thread; the part holds an entry
-// over 0 and start <= border.  found: 0 before.
-template <uint32_t DT>
-__device__ inline uint32_t draw_token(const VerifyArgs& a, const Rest<DT>& rest, uint32_t lo,
-                                      double start, double border, double* sd, uint32_t* found) {
-    const uint32_t b = lo + threadIdx.x * kEntries;
-    float pl[kEntries], ql[kEntries];
+// Sum over the lanes before and the lane itself.
+__device__ inline double lanes_sum(double c) {
+    const uint32_t lane = threadIdx.x & 63;
 #pragma unroll
-    for (int j = 0; j < (int)kEntries; ++j) {
-        const uint32_t i = min(b + j, a.V - 1);
-        pl[j] = Elem<DT>::load(rest.p[i]);
-        ql[j] = rest.q ? Elem<DT>::load(rest.q[i]) : 0.0f;
+    for (int d = 1; d < 64; d <<= 1) {
+        const double o = __shfl_up(c, d);
+        if (lane >= (uint32_t)d) c += o;
     }
-    double r[kEntries], s = 0.0;
-#pragma unroll
-    for (int j = 0; j < (int)kEntries; ++j) {
-        r[j] = b + j < a.V ? rest.of(a, b + j, pl[j], ql[j]) : 0.0;
-        s += r[j];
-    }
-    double c = run_start(s, start, sd);
-    uint32_t hit = 0;
-#pragma unroll
-    for (int j = 0; j < (int)kEntries; ++j) {
-        if (r[j] > 0.0 && c <= border) hit = b + j + 1;
-        c += r[j];
-    }
-    if (hit) atomicMax(found, hit);
-    __syncthreads();
-    return *found - 1;
+    return c;
 }
 
-// The same over the whole row.
+// The token of a part that the border falls in: the last entry over 0 that the
+// cumulative sum (start before the part) has not passed the border before.  By
+// a wave; the part holds an entry over 0 and start <= border.  The part's
+// chunks of W neighbours a lane, then the lanes, then the neighbours: at each
+// level the last one over 0 that starts at the border or before, and the first
+// over 0 is one, so that something is found whatever the sums' roundings.
+template <uint32_t DT, int W>
+__device__ inline uint32_t draw_token(const VerifyArgs& a, uint32_t lo,
+                                      const double (&r)[kEntries], double start, double border) {
+    const uint32_t lane = threadIdx.x & 63;
+    double mine[W] = {}, sum = 0.0, at = start;
+    uint32_t chunk = 0;
+#pragma unroll
+    for (int c = 0; c < (int)kEntries / W; ++c) {
+        double l = 0.0;
+#pragma unroll
+        for (int y = 0; y < W; ++y) l += r[c * W + y];
+        const double all = wave_sum(l);
+        if (all > 0.0 && at <= border) {
+            chunk = c;
+            start = at;
+            sum = l;
+#pragma unroll
+            for (int y = 0; y < W; ++y) mine[y] = r[c * W + y];
+        }
+        at += all;
+    }
+    double c = __shfl_up(lanes_sum(sum), 1);
+    c = lane ? start + c : start;
+    const int from = 63 - __clzll((unsigned long long)__ballot(sum > 0.0 && c <= border));
+    uint32_t hit = 0;
+#pragma unroll
+    for (int y = 0; y < W; ++y) {
+        if (mine[y] > 0.0 && c <= border) hit = y;
+        c += mine[y];
+    }
+    return lo + (chunk * 64 + from) * W + (uint32_t)__shfl((int)hit, from);
+}
+
+// The same over the whole row, by the workgroup.
 template <uint32_t DT>
 __device__ inline uint32_t draw_whole(const VerifyArgs& a, const Rest<DT>& rest, double border,
                                       double* sd, uint32_t* found) {
@@ -428,82 +450,101 @@ __device__ inline uint32_t draw_whole(const VerifyArgs& a, const Rest<DT>& rest,
 
 // The row that the next token is drawn from: sums of all parts, and the entry by
 // the last workgroup that arrives, so that no launch waits between.  64 sequences
-// of 131072 probabilities (67 MB): 31 us, of which the last workgroup's steps
-// after the sums are some 10.  Rows by 16 bytes: 40 us with the launch before, by
-// one entry 44 (131073 entries).
+// of 131072 probabilities (67 MB): 21 us, 13 of them the sums (5.2 TB/s) and the
+// others the last workgroup's loads that wait for one another, for which one
+// wave holds the part in registers (by the workgroup, runs of sixteen neighbours
+// a thread: 20 us in place of 8).
 template <uint32_t DT>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
     __shared__ double sd[kThreads / 64];
     __shared__ uint32_t found, last;
-    const uint32_t part = blockIdx.x % a.parts, n = blockIdx.x / a.parts, tid = threadIdx.x;
+    const uint32_t blocks = (a.parts + kWaves - 1) / kWaves;
+    const uint32_t n = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 63;
+    const uint32_t part = blockIdx.x % blocks * kWaves + (tid >> 6);
     if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
     const Drawn d = a.drawn[n];
     if (d.done) return;
     Rest<DT> rest(a, d, n);
-    const uint32_t lo = part * kPart, hi = min(a.V, lo + kPart);
-    {
+    const float past = a.form == K3X_DIST_PROBS ? 0.0f : -__builtin_inff();
+    typedef Entries<DT> Mine;
+    // The wave's entries of the part at lo of what is drawn from.
+    auto entries = [&](uint32_t lo, double (&r)[kEntries]) {
+        const uint32_t hi = min(a.V, lo + kPart);
         float pl[kEntries], ql[kEntries] = {};
-        const float past = a.form == K3X_DIST_PROBS ? 0.0f : -__builtin_inff();
-        typedef Entries<DT, kThreads> Mine;
-        Mine::load(a, rest.p, lo, hi, tid, past, pl);
-        if (rest.q) Mine::load(a, rest.q, lo, hi, tid, past, ql);
-        double s = 0.0;
+        Mine::load(a, rest.p, lo, hi, lane, past, pl);
+        if (rest.q) Mine::load(a, rest.q, lo, hi, lane, past, ql);
 #pragma unroll
         for (int j = 0; j < (int)kEntries; ++j)
-            s += rest.of(a, Mine::where(a, lo, tid, j), pl[j], ql[j]);
-        s = block_sum(s, sd);
-        // The sum, then the arrival, both past the caches of one die: the last
+            r[j] = rest.of(a, Mine::where(a, lo, lane, j), pl[j], ql[j]);
+    };
+    if (part < a.parts) {
+        double r[kEntries], s = 0.0;
+        entries(part * kPart, r);
+#pragma unroll
+        for (int j = 0; j < (int)kEntries; ++j) s += r[j];
+        s = wave_sum(s);
+        // The sums, then the arrival, all past the caches of one die: the last
         // workgroup sees every sum.  (A releasing add would write back the
-        // die's whole cache for each workgroup: 91 us in place of 31 for 64
-        // sequences of 131072 probabilities.)
-        if (tid == 0) {
-            found = 0;
+        // die's whole cache for each workgroup: it made 91 us of 31.)
+        if (lane == 0) {
             __hip_atomic_store(a.sums + (size_t)n * a.parts + part, s, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            last = __hip_atomic_fetch_add(&a.drawn[n].arrived, 1u, __ATOMIC_RELAXED,
-                                          __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
         }
-        __syncthreads();
-        if (!last) return;
     }
-    // Parts by lane, in order: their sums and what lies before each.
-    const uint32_t lane = tid & 63;
-    double total = 0.0, start = 0.0;
-    uint32_t bad = 0, next = 0;
+    __syncthreads();
+    if (tid == 0) {
+        found = 0;
+        last = __hip_atomic_fetch_add(&a.drawn[n].arrived, 1u, __ATOMIC_RELAXED,
+                                      __HIP_MEMORY_SCOPE_AGENT) == blocks - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    // A run of parts a lane, in order: their sums and what lies before each.
+    constexpr uint32_t kRun = (1u << 20) / kPart / 64;
+    const uint32_t run = (a.parts + 63) / 64;
     const float u = a.sample_u[n];
     uint32_t* out = a.out_tokens + (size_t)n * (a.D + 1);
-    double run[4], own[4];
+    double own[kRun], all = 0.0;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        const uint32_t i = 64 * x + lane;
-        own[x] = i < a.parts ? __hip_atomic_load(a.sums + (size_t)n * a.parts + i,
-                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-                             : 0.0;
-        double c = own[x];
-#pragma unroll
-        for (int k = 1; k < 64; k <<= 1) {
-            const double o = __shfl_up(c, k);
-            if (lane >= (uint32_t)k) c += o;
-        }
-        run[x] = total + (c - own[x]);
-        total += __shfl(c, 63);
+    for (uint32_t x = 0; x < kRun; ++x) {
+        const uint32_t i = lane * run + x;
+        own[x] = x < run && i < a.parts
+                     ? __hip_atomic_load(a.sums + (size_t)n * a.parts + i, __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT)
+                     : 0.0;
     }
+#pragma unroll
+    for (uint32_t x = 0; x < kRun; ++x) all += own[x];
+    double c = lanes_sum(all);
+    double total = __shfl(c, 63);
+    c = __shfl_up(c, 1);
+    if (lane == 0) c = 0.0;
+    uint32_t bad = 0, next = 0;
     if (!(u >= 0.0f && u < 1.0f) || !(total >= 0.0 && total < __builtin_inf())) bad = 1;
     if (!bad) {
         double border = (double)u * total;
         if (total > 0.0) {
+            if (tid >= 64) return;
             // The last part over 0 that starts at the border or before.
+            const uint64_t mask = __ballot(all > 0.0 && c <= border);
+            const int from = 63 - __clzll((unsigned long long)mask);
             uint32_t in = 0;
+            double start = 0.0;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint64_t mask = __ballot(own[x] > 0.0 && run[x] <= border);
-                if (!mask) continue;
-                const int l = 63 - __clzll((unsigned long long)mask);
-                in = 64 * x + l;
-                start = __shfl(run[x], l);
+            for (uint32_t x = 0; x < kRun; ++x) {
+                if (own[x] > 0.0 && c <= border) {
+                    in = x;
+                    start = c;
+                }
+                c += own[x];
             }
-            next = draw_token<DT>(a, rest, in * kPart, start, border, sd, &found);
+            const uint32_t lo = ((uint32_t)from * run + (uint32_t)__shfl((int)in, from)) * kPart;
+            start = __shfl(start, from);
+            double r[kEntries];
+            entries(lo, r);
+            next = a.vec ? draw_token<DT, Mine::kWide>(a, lo, r, start, border)
+                         : draw_token<DT, 1>(a, lo, r, start, border);
         } else {
             // Nothing is left over q (or of a row without its drafted token):
             // the target's own probabilities.
@@ -521,7 +562,8 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
         return;
     }
     if (tid == 0) a.accepted[n] = d.accepted;
-    for (uint32_t i = tid; i <= a.D; i += kThreads)
+    if (tid >= 64) return;
+    for (uint32_t i = tid; i <= a.D; i += 64)
         out[i] = i < d.accepted    ? a.tokens[(size_t)n * a.D + i]
                  : i == d.accepted ? next
                                    : 0xffffffffu;
@@ -533,31 +575,29 @@ int launch_verify(k3x_hip_ctx* ctx, const VerifyArgs& a) {
     const uint32_t rows = a.draft ? 2 * a.D + 1 : a.D + 1;
     if (a.form == K3X_DIST_LOGITS || a.greedy) {
         hipLaunchKernelGGL(verify_rows_kernel<DT>,
-                           dim3(a.N * rows * ((a.row_parts_of + kThreads / 64 - 1) / (kThreads / 64))),
+                           dim3(a.N * rows * ((a.parts + kWaves - 1) / kWaves)),
                            dim3(kThreads), 0, ctx->stream, a);
         ++launches;
     }
     hipLaunchKernelGGL(verify_accept_kernel<DT>, dim3(a.N), dim3(64 * std::min(rows, 16u)), 0,
                        ctx->stream, a);
     if (!a.greedy) {
-        hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3(a.N * a.parts), dim3(kThreads), 0,
-                           ctx->stream, a);
+        hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3(a.N * ((a.parts + kWaves - 1) / kWaves)),
+                           dim3(kThreads), 0, ctx->stream, a);
         ++launches;
     }
     return launched(ctx, launches);
 }
 
 uint32_t parts_of(const k3x_hip_verify_params* p) { return (p->vocab + kPart - 1) / kPart; }
-uint32_t row_parts_of(const k3x_hip_verify_params* p) {
-    return (p->vocab + 64 * kEntries - 1) / (64 * kEntries);
-}
-
 bool verify_ok(const k3x_hip_verify_params* p) {
     return p->sequences && p->sequences <= 65535 && p->drafts <= kMaxDrafts && p->vocab &&
            p->vocab <= (1u << 20) && p->dtype <= K3X_DTYPE_BF16 && p->form <= K3X_DIST_PROBS &&
            p->greedy <= 1 && std::isfinite(p->temperature) && p->temperature > 0.0f &&
            (!p->row_stride || p->row_stride >= p->vocab) &&
-           (uint64_t)p->sequences * (2 * p->drafts + 1) * parts_of(p) < (1ull << 31);
+           // threads of a launch
+           (uint64_t)p->sequences * (2 * p->drafts + 1) * ((parts_of(p) + kWaves - 1) / kWaves) *
+                   kThreads < (1ull << 32);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -569,7 +609,7 @@ extern "C" {
 size_t k3x_hip_verify_workspace(const k3x_hip_verify_params* p) {
     if (!p || !verify_ok(p)) return 0;
     const size_t n = p->sequences, parts = parts_of(p);
-    return up256(n * (2 * p->drafts + 1) * row_parts_of(p) * sizeof(RowPart)) + up256(n * sizeof(Drawn)) +
+    return up256(n * (2 * p->drafts + 1) * parts * sizeof(RowPart)) + up256(n * sizeof(Drawn)) +
            up256(n * parts * sizeof(double));
 }
 
@@ -604,14 +644,13 @@ int k3x_hip_verify_draft(k3x_hip_ctx* ctx, const k3x_hip_verify_params* p, const
     a.V = p->vocab;
     a.stride = p->row_stride ? p->row_stride : p->vocab;
     a.parts = parts_of(p);
-    a.row_parts_of = row_parts_of(p);
     a.vec = a.stride * es % 16 == 0 && aligned(target, 16) && aligned(draft, 16);
     a.form = p->form;
     a.greedy = p->greedy;
     a.rate = 1.4426950408889634 / p->temperature;
     uint8_t* w = static_cast<uint8_t*>(workspace);
     a.row_parts = reinterpret_cast<RowPart*>(w);
-    w += up256((size_t)a.N * (2 * a.D + 1) * a.row_parts_of * sizeof(RowPart));
+    w += up256((size_t)a.N * (2 * a.D + 1) * a.parts * sizeof(RowPart));
     a.drawn = reinterpret_cast<Drawn*>(w);
     w += up256((size_t)a.N * sizeof(Drawn));
     a.sums = reinterpret_cast<double*>(w);

@@ -123,6 +123,13 @@ def test_verify_refuses(lib, kw):
     assert verify(lib, **kw) == BAD
 
 
+def test_more_threads_than_a_launch(lib):
+    """Extents that are each allowed, whose product is no launch (2^32 threads)."""
+    assert delta(lib, sequences=32768, value_heads=1024, slots=32768) == BAD
+    assert delta(lib, sequences=1, tokens=1 << 24, value_heads=1024, longest=1 << 24) == BAD
+    assert verify(lib, sequences=65535, drafts=64, vocab=1 << 20) == BAD
+
+
 def test_binding_checks_tensors():
     """The binding's own checks come before any pointer is taken."""
     class Fake:
