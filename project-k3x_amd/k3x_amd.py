@@ -607,21 +607,36 @@ def _dtype(t) -> int:
     return code
 
 
-def _expect(what: str, t, shape, dtypes) -> None:
-    """A tensor of the shape and of one of the types."""
+def _expect(ctx: Context, what: str, t, shape, dtypes) -> None:
+    """A tensor of the shape and of one of the types, on the context's device."""
     if t.shape != shape or t.dtype not in dtypes:
         raise ValueError(f"{what}: expected {shape} of {dtypes}, not {tuple(t.shape)} of "
                          f"{t.dtype}")
+    at = t.get_device()
+    if at < 0 or at != ctx.device:
+        raise ValueError(f"{what}: expected a tensor on the context's device, not on {t.device}")
 
 
-def _rows(t):
-    """(device pointer, elements from row to row) of rows that are contiguous in themselves; the
-    distance is 0 where it is the row's length or there is one row."""
-    if not t.is_cuda:
-        raise ValueError("expected a device tensor")
-    if t.is_contiguous():
-        return t.data_ptr(), 0
-    return t.data_ptr(), _row_stride(t)
+def _at(ctx: Context, what: str, t, shape, dtypes) -> int:
+    """Device pointer of such a tensor, contiguous."""
+    _expect(ctx, what, t, shape, dtypes)
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous tensor")
+    return t.data_ptr()
+
+
+def _rows(ctx: Context, what: str, t, shape, dtypes):
+    """(device pointer, elements from row to row) of such a tensor, its rows contiguous in
+    themselves; the distance is 0 where it is the row's length or there is one row."""
+    _expect(ctx, what, t, shape, dtypes)
+    return t.data_ptr(), 0 if t.is_contiguous() else _row_stride(t)
+
+
+def _workspace(ctx: Context, t):
+    """(pointer, bytes) of a workspace or None."""
+    if t is None:
+        return None, 0
+    return _at(ctx, "workspace", t, t.shape, (t.dtype,)), t.numel() * t.element_size()
 
 
 def _row_stride(t) -> int:
@@ -645,15 +660,13 @@ def route(ctx: Context, params: RouteParams, logits, ids, weights, bias=None) ->
     """ids [T][K] (int32) and weights [T][K] (fp32) from router logits [T][E] (fp32 or bf16)
     and the fp32 bias [E] (k3x_hip_route)."""
     T, E, K, types = params.tokens, params.experts, params.top_k, _types()
-    _expect("logits", logits, (T, E), types["logits"])
-    if bias is not None:
-        _expect("bias", bias, (E,), types["f32"])
-    _expect("ids", ids, (T, K), types["ints"])
-    _expect("weights", weights, (T, K), types["f32"])
     p = RouteParams.from_buffer_copy(params)
-    at, p.logits_stride = _rows(logits)
+    lp, p.logits_stride = _rows(ctx, "logits", logits, (T, E), types["logits"])
     p.dtype = _dtype(logits)
-    return ctx.lib.k3x_hip_route(ctx.handle, C.byref(p), at, ptr(bias), ptr(ids), ptr(weights))
+    bp = None if bias is None else _at(ctx, "bias", bias, (E,), types["f32"])
+    return ctx.lib.k3x_hip_route(ctx.handle, C.byref(p), lp, bp,
+                                 _at(ctx, "ids", ids, (T, K), types["ints"]),
+                                 _at(ctx, "weights", weights, (T, K), types["f32"]))
 
 
 def make_delta_params(q, k, v, sequences, gate=None, scale=1.0, norm_epsilon=0.0, longest=0,
@@ -681,29 +694,28 @@ def delta_rule(ctx: Context, params: DeltaParams, q, k, v, beta, out, gate=None,
     p = DeltaParams.from_buffer_copy(params)
     T, N, H, K, V = p.tokens, p.sequences, p.value_heads, p.key_dim, p.value_dim
     types, same = _types(), (v.dtype,)
-    _expect("q", q, (T, p.key_heads, K), same)
-    _expect("k", k, (T, p.key_heads, K), same)
-    _expect("v", v, (T, H, V), same)
-    _expect("out", out, (T, H, V), same)
-    _expect("beta", beta, (T, H), types["f32"])
+    f32, ints = types["f32"], types["ints"]
+    qp, p.q_stride = _rows(ctx, "q", q, (T, p.key_heads, K), same)
+    kp, p.k_stride = _rows(ctx, "k", k, (T, p.key_heads, K), same)
+    vp, p.v_stride = _rows(ctx, "v", v, (T, H, V), same)
+    op, p.out_stride = _rows(ctx, "out", out, (T, H, V), same)
+    bp = _at(ctx, "beta", beta, (T, H), f32)
+    gp = sp = lp = ip = fp = tp = None
     if gate is not None:
-        _expect("gate", gate, (T, H, K) if p.gate == GATE_CHANNEL else (T, H), types["f32"])
-    for what, t, n in (("offsets", offsets, N + 1), ("limits", limits, N),
-                       ("slot_index", slot_index, N)):
-        if t is not None:
-            _expect(what, t, (n,), types["ints"])
-    for what, t in (("state_in", state_in), ("state_out", state_out)):
-        if t is not None:
-            _expect(what, t, (p.slots, H, K, V), types["f32"])
+        gp = _at(ctx, "gate", gate, (T, H, K) if p.gate == GATE_CHANNEL else (T, H), f32)
+    if offsets is not None:
+        sp = _at(ctx, "offsets", offsets, (N + 1,), ints)
+    if limits is not None:
+        lp = _at(ctx, "limits", limits, (N,), ints)
+    if slot_index is not None:
+        ip = _at(ctx, "slot_index", slot_index, (N,), ints)
+    if state_in is not None:
+        fp = _at(ctx, "state_in", state_in, (p.slots, H, K, V), f32)
+    if state_out is not None:
+        tp = _at(ctx, "state_out", state_out, (p.slots, H, K, V), f32)
     p.dtype = _dtype(v)
-    qp, p.q_stride = _rows(q)
-    kp, p.k_stride = _rows(k)
-    vp, p.v_stride = _rows(v)
-    op, p.out_stride = _rows(out)
-    return ctx.lib.k3x_hip_delta_rule(
-        ctx.handle, C.byref(p), qp, kp, vp, ptr(gate), ptr(beta), ptr(offsets), ptr(limits),
-        ptr(slot_index), ptr(state_in), ptr(state_out), op, ptr(workspace),
-        0 if workspace is None else workspace.numel() * workspace.element_size())
+    return ctx.lib.k3x_hip_delta_rule(ctx.handle, C.byref(p), qp, kp, vp, gp, bp, sp, lp, ip, fp,
+                                      tp, op, *_workspace(ctx, workspace))
 
 
 def make_verify_params(target, form=DIST_LOGITS, greedy=False, temperature=1.0) -> VerifyParams:
@@ -722,24 +734,24 @@ def verify_draft(ctx: Context, params: VerifyParams, target, tokens, accepted, o
     """Verifies drafted tokens [N][D] against the target's rows [N][D + 1][V]
     (k3x_hip_verify_draft): accepted [N] and out_tokens [N][D + 1] int32."""
     N, D, V, types = params.sequences, params.drafts, params.vocab, _types()
-    _expect("target", target, (N, D + 1, V), types["logits"])
-    if draft is not None:
-        _expect("draft", draft, (N, D, V), (target.dtype,))
-    _expect("tokens", tokens, (N, D), types["ints"])
-    if draft_counts is not None:
-        _expect("draft_counts", draft_counts, (N,), types["ints"])
-    if accept_u is not None:
-        _expect("accept_u", accept_u, (N, D), types["f32"])
-    if sample_u is not None:
-        _expect("sample_u", sample_u, (N,), types["f32"])
-    _expect("accepted", accepted, (N,), types["ints"])
-    _expect("out_tokens", out_tokens, (N, D + 1), types["ints"])
+    f32, ints = types["f32"], types["ints"]
+    tp = _at(ctx, "target", target, (N, D + 1, V), types["logits"])
     if _dtype(target) != params.dtype:
         raise ValueError("target: not of the parameters' type")
+    xp = _at(ctx, "tokens", tokens, (N, D), ints)
+    dp = cp = ap = sp = None
+    if draft is not None:
+        dp = _at(ctx, "draft", draft, (N, D, V), (target.dtype,))
+    if draft_counts is not None:
+        cp = _at(ctx, "draft_counts", draft_counts, (N,), ints)
+    if accept_u is not None:
+        ap = _at(ctx, "accept_u", accept_u, (N, D), f32)
+    if sample_u is not None:
+        sp = _at(ctx, "sample_u", sample_u, (N,), f32)
     return ctx.lib.k3x_hip_verify_draft(
-        ctx.handle, C.byref(params), ptr(target), ptr(draft), ptr(tokens), ptr(draft_counts),
-        ptr(accept_u), ptr(sample_u), ptr(accepted), ptr(out_tokens), ptr(workspace),
-        0 if workspace is None else workspace.numel() * workspace.element_size())
+        ctx.handle, C.byref(params), tp, dp, xp, cp, ap, sp,
+        _at(ctx, "accepted", accepted, (N,), ints),
+        _at(ctx, "out_tokens", out_tokens, (N, D + 1), ints), *_workspace(ctx, workspace))
 
 
 class Storage:
