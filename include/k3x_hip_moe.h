@@ -407,7 +407,7 @@ typedef struct k3x_hip_route_params {
  * left as they were: a score, bias or sum that is not finite, with renormalised
  * weights a sum of 0 (K3X_ERR_INVALID_STATE; with K3X_RENORM_DOUBLE and sigmoid
  * scores a logit or bias that is not finite, or the sum, as
- * K3X_ERR_INVALID_EXTENT).  The reference routes on the host
+ * K3X_ERR_INVALID_EXTENT); other tokens' outputs may then be missing.  The reference routes on the host
  * (runtime/src/routing_policy.cpp:31-160; official_moe.cpp:211-245).
  * Asynchronous. */
 int k3x_hip_route(k3x_hip_ctx* ctx, const k3x_hip_route_params* params, const void* logits,
@@ -463,9 +463,10 @@ typedef struct k3x_hip_delta_params {
  * that may, have one each.
  * Latched: offsets that fall or pass T, a slot past slots, two sequences of
  * one state with state_out (K3X_ERR_INVALID_STATE; nothing of those sequences
- * is read or written); a q, k, v, gate or beta that is not finite or a gate
- * above 0 (K3X_ERR_INVALID_MXFP4, as for the layer's input; the sequence's
- * outputs are then not defined).  Replaces the recurrence of
+ * is read or written); a q, k, v, gate or beta or a state in use that is not
+ * finite or a gate above 0 (K3X_ERR_INVALID_MXFP4, as for the layer's input).
+ * The outputs of a sequence with such values are then not defined, those of the
+ * others may be missing, and where offsets fall none are defined.  Replaces the recurrence of
  * ComputeBackend::official_kda (runtime/cuda/official_kda.cuh:11-37), batched.
  * Asynchronous. */
 int k3x_hip_delta_rule(k3x_hip_ctx* ctx, const k3x_hip_delta_params* params, const void* q,
@@ -515,7 +516,8 @@ typedef struct k3x_hip_verify_params {
  * Latched as K3X_ERR_INVALID_STATE, the sequence's outputs left as they were: a
  * drafted token past V that is reached, a used row that holds NaN, plus
  * infinity (logits) or a negative or infinite entry (probabilities) or nothing
- * but minus infinity or zeros, a uniform outside [0, 1), a draft count past D.
+ * but minus infinity or zeros, a uniform outside [0, 1), a draft count past D;
+ * other sequences' outputs may then be missing.
  * The reference verifies on the host (generate_speculative,
  * runtime/src/model.cpp:1507).  Asynchronous. */
 int k3x_hip_verify_draft(k3x_hip_ctx* ctx, const k3x_hip_verify_params* params,

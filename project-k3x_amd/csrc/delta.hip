@@ -257,6 +257,8 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
         // u of rows 0 and 1, then of every row.
         float ux = now.beta * __builtin_fmaf(-rk, x, odd ? v[1] : v[0]);
         float uy = now.beta * __builtin_fmaf(-rk, y, odd ? v[3] : v[2]);
+        z = __builtin_fmaf(ux, 0.0f, z);  // of a state that is not finite, too
+        z = __builtin_fmaf(uy, 0.0f, z);
         float any, u[4];
         swap_halves(ux, ux, &ux, &any);
         swap_halves(uy, uy, &uy, &any);

@@ -376,6 +376,17 @@ def test_values_that_are_not_finite_are_latched(hip, lens, what, value):
     check(hip, inputs(lens, 1, 2, 64, 32))
 
 
+@pytest.mark.parametrize("lens", [(1,), (4,), (70,)], ids=["one", "short", "long"])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_state_that_is_not_finite_is_latched(hip, lens, value):
+    k3x, ctx = hip
+    s = inputs(lens, 1, 2, 64, 32)
+    s["state"][0, 1, 63, 31] = value
+    st, _, _ = call(hip, s)
+    assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_MXFP4
+    check(hip, inputs(lens, 1, 2, 64, 32))
+
+
 def test_growing_gate_is_latched(hip):
     k3x, ctx = hip
     for lens in ((4,), (70,)):

@@ -147,6 +147,20 @@ def test_minus_infinity_is_a_mask(hip):
         check(hip, logits, None, 5, softmax=softmax)
 
 
+@pytest.mark.parametrize("groups,top_groups", [(1, 1), (8, 3), (3, 2), (64, 5)])
+def test_lowest_value_is_a_mask(hip, groups, top_groups):
+    """Experts whose bias is the type's lowest value come after all others; a
+    group of none but such (the sum of its two largest is minus infinity) last."""
+    E = 192
+    bias = torch.full((E,), torch.finfo(torch.float32).min, device=DEV)
+    bias[5:9], bias[100], bias[150:153] = 0.25, 0.0, -1.0
+    logits = torch.randn((5, E), device=DEV, generator=gen(12))
+    for softmax in (False, True):
+        for top2 in (False, True):
+            check(hip, logits, bias, 6, softmax=softmax, groups=groups, top_groups=top_groups,
+                  top2=top2)
+
+
 def test_negative_bias_order(hip):
     """Adjusted scores below zero, and minus zero beside zero."""
     logits = torch.randn((9, 96), device=DEV, generator=gen(8))
