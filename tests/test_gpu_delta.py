@@ -458,3 +458,43 @@ def test_two_calls_at_once(hip):
             assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2])
     for ctx in ctxs:
         ctx.close()
+
+
+@pytest.mark.parametrize("lens", [(1, 1), (3, 40)], ids=["short", "long"])
+def test_states_past_32_bits(hip, lens):
+    """2^32 elements and more of states; the last one of them and the first."""
+    k3x, ctx = hip
+    H, K, V = 32, 128, 128
+    slots = 2 ** 32 // (H * K * V) + 2
+    s = inputs(lens, 32, H, K, V, BF16)
+    index = torch.tensor([slots - 1, 0], dtype=torch.int32, device=DEV)
+    states = torch.empty((slots, H, K, V), device=DEV)
+    for n, slot in enumerate((slots - 1, 0)):
+        states[slot].copy_(s["state"][n])
+    st, out, _ = call(hip, s, slot_index=index, state_in=states, state_out=states, slots=slots)
+    assert st == 0 and ctx.synchronize() == 0
+    want, S, tol, stol = definition(s, K ** -0.5)
+    close(out, want, tol, BF16)
+    for n, slot in enumerate((slots - 1, 0)):
+        close(states[slot], S[n], stol[n])
+
+
+@pytest.mark.parametrize("lens", [(2, 3), (2, 130)], ids=["short", "long"])
+def test_rows_past_32_bits(hip, lens):
+    """Rows 2^24 elements apart, the longest stride: the long ones 2^32 bytes from end to end."""
+    T, stride = sum(lens), 2 ** 24
+    s = inputs(lens, 1, 2, 64, 64, BF16)
+    wide = torch.empty((T, stride), dtype=BF16, device=DEV)
+    at = 0
+    for x, n in (("q", 64), ("k", 64), ("v", 128)):
+        rows = wide[:, at:at + n].unflatten(1, (-1, 64))
+        rows.copy_(s[x])
+        s[x] = rows
+        at += n
+    out = wide[:, stride - 128:].unflatten(1, (2, 64))
+    k3x, ctx = hip
+    st, out, S = call(hip, s, out=out)
+    assert st == 0 and ctx.synchronize() == 0
+    want, Sw, tol, stol = definition(s, 64 ** -0.5)
+    close(out, want, tol, BF16)
+    close(S, Sw, stol)

@@ -254,3 +254,18 @@ def test_captured(hip):
             assert st == 0 and ctx.synchronize() == 0
             assert torch.equal(got[0], ids2) and torch.equal(got[1], w2)
         ctx.close()
+
+
+def test_logits_past_32_bits(hip):
+    """2^32 logits, the most tokens and experts; the last tokens' routes."""
+    k3x, ctx = hip
+    T, E, K = 1 << 20, 4096, 4
+    logits = torch.zeros((T, E), dtype=torch.bfloat16, device=DEV)
+    logits[-3:] = torch.randn((3, E), device=DEV, generator=gen(77)).bfloat16()
+    st, ids, w = call(hip, logits, None, K)
+    assert st == 0 and ctx.synchronize() == 0
+    want, weights = plain(logits[-3:], None, K)
+    assert torch.equal(ids[-3:].cpu().long(), want)
+    err = (w[-3:].cpu().double() - weights).abs()
+    assert (err <= (4 + K) * 2.0 ** -24 * weights).all()
+    assert torch.equal(ids[:-3].cpu(), torch.arange(K, dtype=torch.int32).expand(T - 3, K))

@@ -293,3 +293,24 @@ def test_captured(hip):
             assert st == 0 and ctx.synchronize() == 0
             assert torch.equal(got[0], a2) and torch.equal(got[1], o2)
         ctx.close()
+
+
+@pytest.mark.parametrize("greedy", [True, False], ids=["greedy", "sampled"])
+def test_rows_past_32_bits(hip, greedy):
+    """2^32 entries and more of the longest rows; the last sequence's tokens."""
+    k3x, ctx = hip
+    N, D, V = 1366, 2, 1 << 20
+    s = dict(target=torch.zeros((N, D + 1, V), dtype=BF16, device=DEV), draft=None,
+             tokens=torch.zeros((N, D), dtype=torch.int32, device=DEV))
+    g = gen(5)
+    s["target"][-1].copy_(torch.randn((D + 1, V), device=DEV, generator=g) * 3)
+    s["tokens"][-1, 0] = s["target"][-1, 0].float().argmax()
+    s["accept_u"] = torch.full((N, D), 2.0 ** -30, device=DEV)
+    s["sample_u"] = torch.rand((N,), device=DEV, generator=g)
+    st, accepted, out = call(hip, s, greedy=greedy)
+    assert st == 0 and ctx.synchronize() == 0
+    last = {x: None if y is None else y[-1:] for x, y in s.items()}
+    want_a, want = definition(last, False, greedy, 1.0)
+    assert torch.equal(accepted[-1:].cpu(), want_a) and torch.equal(out[-1:].cpu(), want)
+    if greedy:  # rows of equal entries: the lowest token
+        assert (accepted[:-1] == D).all() and (out[:-1] == 0).all()
