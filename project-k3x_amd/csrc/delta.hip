@@ -420,12 +420,13 @@ __device__ inline float sum_groups(float v) {
     v = fold_rows(v, v);
     return fold_halves(v, v);
 }
+// Of v >= 0, whose order is that of its bits.
 __device__ inline float max_groups(float v) {
-    float a, b;
-    swap_rows(v, v, &a, &b);
-    v = fmaxf(a, b);
-    swap_halves(v, v, &a, &b);
-    return fmaxf(a, b);
+    const uint32_t u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t x = max(r[0], r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __uint_as_float(max(h[0], h[1]));
 }
 
 // 2^-e and 2^e for the least e with |x| < 2^e (x finite); 1 and 1 for x = 0.
@@ -998,6 +999,14 @@ __device__ inline void store_one(E x, __amdgpu_buffer_rsrc_t r, uint32_t voffset
                                               0);
 }
 
+// load_lds16 at an offset of the instruction, from both addresses.
+template <int Offset>
+__device__ inline void load_lds16_at(__amdgpu_buffer_rsrc_t r, u32x4* dst, uint32_t voffset,
+                                     uint32_t soffset) {
+    typedef __attribute__((address_space(3))) void* lds_ptr_t;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, voffset, soffset, Offset, 0);
+}
+
 // Walks one sequence's chunks for 64 value columns of one head.  Each of the four
 // waves holds 16 columns of the state as the results of 2 KB products (rows by
 // 16): row 16 t + 4 (l / 16) + i and column l % 16 in register i of tile t of
@@ -1005,13 +1014,14 @@ __device__ inline void store_one(E x, __amdgpu_buffer_rsrc_t r, uint32_t voffset
 // chunk is multiplied, the next one's record, operands and values come to LDS
 // as they lie, the loads spread over the products.
 //
-// A chunk takes 2.1 us: (P k) S, U, its operand, T U and the update follow one
-// another, and one wave a SIMD issues all of them, 645 instructions of which 84
-// are products (1344 of 4900 cycles).  So a sequence of 2048 tokens takes 135 us,
-// and seven of 8192 together (448 workgroups, two a CU) 153 us.  Neither fewer
-// columns a workgroup (two waves: 136 us of the first, one: 156), nor more (eight
-// waves: 170 us of the second), nor two waves to 16 columns, each with half of
-// the channels (155 us), shorten that.
+// A chunk takes 2.0 us: (P k) S, U, its operand, T U and the update follow one
+// another, and one wave a SIMD issues all of them, some 610 instructions of
+// which 84 are products (1344 of 4700 cycles).  So a sequence of 2048 tokens
+// takes 129 us, and seven of 8192 together (448 workgroups, two a CU) 150 us.
+// Neither fewer columns a workgroup (two waves as long on the first, one 15%
+// longer), nor more (eight waves 11% longer on the second), nor two waves to 16
+// columns, each with half of the channels (15%), nor the outputs stored without
+// LDS (9%) shorten that.
 template <bool LO, int KB>
 struct ScanChunk {
     ChunkRecord r;
@@ -1115,21 +1125,25 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
     };
     auto bring = [&](const Source& from, uint32_t i, uint32_t x, uint32_t of) {
         constexpr uint32_t kRec = sizeof(ChunkRecord) / 1024;
-        constexpr uint32_t kOps = sizeof(ChunkOperands<LO, KB>) / 1024;
-        constexpr uint32_t W = kScanWaves;
-        constexpr uint32_t kRecLoads = (kRec + W - 1) / W, kOpsLoads = (kOps + W - 1) / W;
+        constexpr uint32_t kOps = sizeof(ChunkOperands<LO, KB>) / 1024 / kScanWaves;
+        constexpr uint32_t kRecLoads = (kRec + kScanWaves - 1) / kScanWaves;
         u32x4* dst = reinterpret_cast<u32x4*>(&buf[i & 1]);
+        // Neighbouring loads go by the instruction's offset, four from one base.
+        auto four = [&](__amdgpu_buffer_rsrc_t r, uint32_t first, uint32_t skip, uint32_t y) {
+            u32x4* to = dst + 64 * (skip + first);
+            if (y == 0) load_lds16_at<0>(r, to, lane * 16, first * 1024);
+            if (y == 1) load_lds16_at<1024>(r, to, lane * 16, first * 1024);
+            if (y == 2) load_lds16_at<2048>(r, to, lane * 16, first * 1024);
+            if (y == 3) load_lds16_at<3072>(r, to, lane * 16, first * 1024);
+        };
 #pragma unroll
-        for (uint32_t y = 0; y < kRecLoads + kOpsLoads; ++y) {
-            if (y % of != x) continue;
+        for (uint32_t y = 0; y < kRecLoads + kOps; ++y) {
+            if (y * of / (kRecLoads + kOps) != x) continue;
             if (y < kRecLoads) {
-                const uint32_t unit = W * y + wave;
-                if (W * (y + 1) <= kRec || unit < kRec)
-                    load_lds16(from.rec, dst + 64 * unit, lane * 16, unit * 1024);
+                if (kRecLoads * wave + y < kRec) four(from.rec, kRecLoads * wave, 0, y);
             } else {
-                const uint32_t unit = W * (y - kRecLoads) + wave;
-                if (W * (y + 1 - kRecLoads) <= kOps || unit < kOps)
-                    load_lds16(from.ops, dst + 64 * (kRec + unit), lane * 16, unit * 1024);
+                const uint32_t z = y - kRecLoads;
+                four(from.ops, kOps * wave + z / 4 * 4, kRec, z % 4);
             }
         }
     };
@@ -1185,7 +1199,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
         auto factors = [&](const float* f, int t) {
             return *reinterpret_cast<const f32x4*>(f + 16 * t + 4 * g);
         };
-        float most = 0.0f;
+        float most = 0.0f, vmost = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -1202,13 +1216,13 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 v[t][j] = __builtin_ldexpf(v[t][j], -shift);
-                most = fmaxf(most, fabsf(v[t][j]) * kOperand);
+                vmost = fmaxf(vmost, fabsf(v[t][j]));
             }
         // Column sizes near 1 leave both the products' growth and the parts
         // below hi their room.
-        most = max_groups(most);
-        const bool off = most > 32.0f * kOperand || (most < 0.5f * kOperand && most > 0.0f);
-        if (__any(off)) {
+        most = max_groups(fmaxf(most, vmost * kOperand));
+        const bool off = (most > 32.0f * kOperand) | ((most < 0.5f * kOperand) & (most > 0.0f));
+        if (__builtin_amdgcn_ballot_w64(off)) {
             const int d = off ? __builtin_amdgcn_frexp_expf(most) - 3 - 6 : 0;
             shift += d;
 #pragma unroll
@@ -1274,7 +1288,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(y[t][j]));
-            if (!__any(big > 16384.0f)) return;
+            if (!__builtin_amdgcn_ballot_w64(big > 16384.0f)) return;
             big = max_groups(big);
             const int d = big > 16384.0f ? __builtin_amdgcn_frexp_expf(big) - 5 : 0;
             shift += d;
