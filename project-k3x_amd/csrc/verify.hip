@@ -107,7 +107,7 @@ __device__ inline double exp2_f64(double y) {
 // A lane's sixteen entries of a part, neighbours by 16 bytes where rows are, so
 // that a wave's loads are whole lines; where() rises with j.  By 16 bytes against
 // by one entry, all launches: 131072 and 131073 probabilities of 64 sequences 27
-// and 30 us, logits of 16 sequences of 4 drafts 47 and 52.
+// and 30 us, logits of 16 sequences of 4 drafts 43 and 48.
 template <uint32_t DT>
 struct Entries {
     typedef typename Elem<DT>::type E;
@@ -143,7 +143,7 @@ struct Entries {
 };
 
 // Parts of a row by waves, which do not wait for one another.  16 sequences of 4
-// drafts and 100003 fp32 logits (58 MB): 22 us, 2.6 TB/s; the exponentials in
+// drafts and 100003 fp32 logits (58 MB): 17 us, 3.4 TB/s; the exponentials in
 // double, some 18 operations each, take 7 us of it at the unit's rate.
 template <uint32_t DT>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a) {
@@ -164,18 +164,23 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a) {
     uint32_t arg = 0xffffffffu;
     bool wrong = false;
 #pragma unroll
-    for (int j = 0; j < (int)kEntries; ++j) {
+    for (int j = 0; j < (int)kEntries; ++j) wrong |= !(l[j] < __builtin_inff());
+    if (!a.greedy) {
+#pragma unroll
+        for (int j = 0; j < (int)kEntries; ++j) m = fmaxf(m, l[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < (int)kEntries; ++j)
+            if (l[j] > m) {
+                m = l[j];
+                arg = Mine::where(a, lo, lane, j);
+            }
         // Past the row's end minus infinity: no entry of a row of
         // probabilities, but not one that is looked at either.
-        const uint32_t i = Mine::where(a, lo, lane, j);
-        wrong |= !(l[j] < __builtin_inff()) ||
-                 (a.form == K3X_DIST_PROBS && l[j] < 0.0f && i < hi);
-        if (!a.greedy) {
-            m = fmaxf(m, l[j]);
-        } else if (l[j] > m) {
-            m = l[j];
-            arg = i;
-        }
+        if (a.form == K3X_DIST_PROBS)
+#pragma unroll
+            for (int j = 0; j < (int)kEntries; ++j)
+                wrong |= l[j] < 0.0f && Mine::where(a, lo, lane, j) < hi;
     }
     const float top = unordered(wave_max_u32(ordered(m)));
     if (a.greedy) arg = ~wave_max_u32(m == top ? ~arg : 0u);
