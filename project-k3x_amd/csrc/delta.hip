@@ -1015,19 +1015,18 @@ __device__ inline void load_lds16_at(__amdgpu_buffer_rsrc_t r, u32x4* dst, uint3
 // as they lie, the loads spread over the products.
 //
 // A chunk takes 2.0 us: (P k) S, U, its operand, T U and the update follow one
-// another, and one wave a SIMD issues all of them, some 610 instructions of
+// another, and one wave a SIMD issues all of them, some 600 instructions of
 // which 84 are products (1344 of 4700 cycles).  So a sequence of 2048 tokens
-// takes 129 us, and seven of 8192 together (448 workgroups, two a CU) 150 us.
+// takes 126 us, and seven of 8192 together (448 workgroups, two a CU) 145 us.
 // Neither fewer columns a workgroup (two waves as long on the first, one 15%
 // longer), nor more (eight waves 11% longer on the second), nor two waves to 16
-// columns, each with half of the channels (15%), nor the outputs stored without
-// LDS (9%) shorten that.
+// columns, each with half of the channels (15%), shorten that.
 template <bool LO, int KB>
 struct ScanChunk {
     ChunkRecord r;
     ChunkOperands<LO, KB> o;
 };
-// A wave's values of a chunk, [32][16]; its outputs go out through them.
+// A wave's values of a chunk, [32][16].
 template <uint32_t DT>
 using ScanTile = typename Elem<DT>::type[kChunk][16];
 
@@ -1039,8 +1038,8 @@ constexpr size_t scan_lds() {
     return 2 * sizeof(ScanChunk<LO, KB>) + 2 * kScanWaves * sizeof(ScanTile<DT>);
 }
 
-// vec: bit 0, rows of v by 16 bytes (179 us with the operands' kernel, by one
-// element 187, of the first call above); bit 1, rows of out.
+// vec: bit 0, rows of v by 16 bytes (173 us with the operands' kernel, by one element
+// 185, of the first call above).
 template <uint32_t DT, bool CHANNEL, int KB>
 __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
     DeltaArgs a, const ChunkRecord* records,
@@ -1384,25 +1383,10 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
                                       left(ci), ost, a.V * es);
         // The next chunk is in LDS (only this one's outputs may still be on
         // their way) and every wave is done with this one.
-        if (vec & 2) {
-            ScanTile<DT>& tile = tiles[ci & 1];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    tile[16 * t + 4 * g + j][m] = Elem<DT>::store(__builtin_ldexpf(
-                        __builtin_fmaf(fp[t][j], ap[t][j], fo[t][j] * aq[t][j]), shift));
-            wave_sync();
-#pragma unroll
-            for (int x = 0; x < kTileLoads; ++x)
-                __builtin_amdgcn_raw_buffer_store_b128(
-                    reinterpret_cast<const u32x4*>(tile)[64 * x + lane], outs,
-                    tcol < a.V ? (trow + x * (64 / kRowLanes)) * ost + tcol * es : kOutside, 0, 0);
-            if (more) put_values(ci + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kTileLoads)
-                         : "memory");
-        } else {
+        // Rows of 32 bytes a wave, as they lie in the registers.  Nothing above is
+        // moved down here (without this the compiler does, and it takes 12% longer).
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int t = j / 4, i = j % 4;
@@ -1413,7 +1397,6 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
             if (more) put_values(ci + 1);
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        }
     }
     // A value that is not finite has made every row of its column NaN (the
     // products' operands hold no infinity that is not NaN in a sum).
@@ -1480,8 +1463,7 @@ int launch_chunks(k3x_hip_ctx* ctx, const DeltaArgs& a, void* workspace, const C
     else prepare(std::false_type{});
     constexpr bool LO = CHANNEL || DT == K3X_DTYPE_F32;
     const uint32_t es = sizeof(typename Elem<DT>::type);
-    const uint32_t rows = (a.V * es % 16 == 0 && a.vs * es % 16 == 0 && aligned(a.v, 16) ? 1 : 0) |
-                          (a.V * es % 16 == 0 && a.os * es % 16 == 0 && aligned(a.out, 16) ? 2 : 0);
+    const uint32_t rows = a.V * es % 16 == 0 && a.vs * es % 16 == 0 && aligned(a.v, 16) ? 1 : 0;
     hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB>),
                        dim3(a.N * a.H * ((a.V + kScanCols - 1) / kScanCols)),
                        dim3(64 * kScanWaves), (scan_lds<DT, LO, KB>()), ctx->stream, a, records,
