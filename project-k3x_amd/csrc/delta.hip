@@ -1017,7 +1017,7 @@ __device__ inline void load_lds16_at(__amdgpu_buffer_rsrc_t r, u32x4* dst, uint3
 // A chunk takes 2.0 us: (P k) S, U, its operand, T U and the update follow one
 // another, and one wave a SIMD issues all of them, some 600 instructions of
 // which 84 are products (1344 of 4700 cycles).  So a sequence of 2048 tokens
-// takes 126 us, and seven of 8192 together (448 workgroups, two a CU) 145 us.
+// takes 125 us, and seven of 8192 together (448 workgroups, two a CU) 145 us.
 // Neither fewer columns a workgroup (two waves as long on the first, one 15%
 // longer), nor more (eight waves 11% longer on the second), nor two waves to 16
 // columns, each with half of the channels (15%), shorten that.
@@ -1038,12 +1038,12 @@ constexpr size_t scan_lds() {
     return 2 * sizeof(ScanChunk<LO, KB>) + 2 * kScanWaves * sizeof(ScanTile<DT>);
 }
 
-// vec: bit 0, rows of v by 16 bytes (173 us with the operands' kernel, by one element
+// VEC: rows of v by 16 bytes (173 us with the operands' kernel, by one element
 // 185, of the first call above).
-template <uint32_t DT, bool CHANNEL, int KB>
+template <uint32_t DT, bool CHANNEL, int KB, bool VEC>
 __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
     DeltaArgs a, const ChunkRecord* records,
-    const ChunkOperands<CHANNEL || DT == K3X_DTYPE_F32, KB>* operands, uint32_t vec) {
+    const ChunkOperands<CHANNEL || DT == K3X_DTYPE_F32, KB>* operands) {
     typedef typename Elem<DT>::type E;
     constexpr bool LO = CHANNEL || DT == K3X_DTYPE_F32;
     typedef ScanChunk<LO, KB> Chunk;
@@ -1089,7 +1089,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
     E direct[8];  // a chunk's values where rows are not by 16 bytes
     auto bring_values = [&](uint32_t i) {
         const auto r = value_rows(i);
-        if (vec & 1) {
+        if (VEC) {
             // What lies past the last row or column is not used, but finite.
             const uint32_t c = tcol < a.V ? tcol * es : 0, last = left(i) - 1;
 #pragma unroll
@@ -1104,7 +1104,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
         }
     };
     auto put_values = [&](uint32_t i) {
-        if (vec & 1) return;
+        if (VEC) return;
 #pragma unroll
         for (int j = 0; j < 8; ++j) tiles[i & 1][4 * g + 16 * (j / 4) + j % 4][m] = direct[j];
     };
@@ -1463,11 +1463,14 @@ int launch_chunks(k3x_hip_ctx* ctx, const DeltaArgs& a, void* workspace, const C
     else prepare(std::false_type{});
     constexpr bool LO = CHANNEL || DT == K3X_DTYPE_F32;
     const uint32_t es = sizeof(typename Elem<DT>::type);
-    const uint32_t rows = a.V * es % 16 == 0 && a.vs * es % 16 == 0 && aligned(a.v, 16) ? 1 : 0;
-    hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB>),
-                       dim3(a.N * a.H * ((a.V + kScanCols - 1) / kScanCols)),
-                       dim3(64 * kScanWaves), (scan_lds<DT, LO, KB>()), ctx->stream, a, records,
-                       ops, rows);
+    auto scan = [&](auto by16) {
+        hipLaunchKernelGGL((delta_scan_kernel<DT, CHANNEL, KB, decltype(by16)::value>),
+                           dim3(a.N * a.H * ((a.V + kScanCols - 1) / kScanCols)),
+                           dim3(64 * kScanWaves), (scan_lds<DT, LO, KB>()), ctx->stream, a,
+                           records, ops);
+    };
+    if (a.V * es % 16 == 0 && a.vs * es % 16 == 0 && aligned(a.v, 16)) scan(std::true_type{});
+    else scan(std::false_type{});
     return launched(ctx, 2);
 }
 
