@@ -607,28 +607,30 @@ def _dtype(t) -> int:
     return code
 
 
-def _expect(ctx: Context, what: str, t, shape, dtypes) -> None:
-    """A tensor of the shape and of one of the types, on the context's device."""
+def _refuse(ctx: Context, what: str, t, shape, dtypes) -> None:
     if t.shape != shape or t.dtype not in dtypes:
         raise ValueError(f"{what}: expected {shape} of {dtypes}, not {tuple(t.shape)} of "
                          f"{t.dtype}")
-    at = t.get_device()
-    if at < 0 or at != ctx.device:
+    if t.get_device() < 0 or t.get_device() != ctx.device:
         raise ValueError(f"{what}: expected a tensor on the context's device, not on {t.device}")
+    raise ValueError(f"{what}: expected a contiguous tensor")
 
 
 def _at(ctx: Context, what: str, t, shape, dtypes) -> int:
-    """Device pointer of such a tensor, contiguous."""
-    _expect(ctx, what, t, shape, dtypes)
-    if not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous tensor")
+    """Device pointer of a contiguous tensor of the shape and of one of the types, on the
+    context's device."""
+    if (t.shape != shape or t.dtype not in dtypes or not t.is_cuda or
+            t.get_device() != ctx.device or not t.is_contiguous()):
+        _refuse(ctx, what, t, shape, dtypes)
     return t.data_ptr()
 
 
 def _rows(ctx: Context, what: str, t, shape, dtypes):
     """(device pointer, elements from row to row) of such a tensor, its rows contiguous in
     themselves; the distance is 0 where it is the row's length or there is one row."""
-    _expect(ctx, what, t, shape, dtypes)
+    if (t.shape != shape or t.dtype not in dtypes or not t.is_cuda or
+            t.get_device() != ctx.device):
+        _refuse(ctx, what, t, shape, dtypes)
     return t.data_ptr(), 0 if t.is_contiguous() else _row_stride(t)
 
 
