@@ -144,6 +144,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
     const uint32_t cb = blockIdx.x % blocks, h = blockIdx.x / blocks % a.H;
     const uint32_t n = blockIdx.x / blocks / a.H;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t status = *(volatile uint32_t*)a.status;  // with the offsets, not after them
     Sequence sq;
     uint32_t bad = find_sequence(a, n, &sq);
     if (!bad && slot_taken(a, n, sq.slot)) bad = K3X_ERR_INVALID_STATE;
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
         return;
     }
     // From here on the waves of the workgroup do not wait for one another.
-    if (*(volatile uint32_t*)a.status) return;
+    if (status) return;
     const uint32_t c0 = cb * kStepCols + wave * 16 + 4 * (lane % 4), r0 = R * (lane / 4);
     if (cb * kStepCols + wave * 16 >= a.V) return;
     const uint32_t hk = h / (a.H / a.Hk);

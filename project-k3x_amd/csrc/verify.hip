@@ -244,10 +244,11 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a) {
     __shared__ Row rows[2 * kMaxDrafts + 1];
     __shared__ uint32_t verdict;
     const uint32_t n = blockIdx.x, tid = threadIdx.x;
-    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
+    const uint32_t status = *(volatile uint32_t*)a.status;  // looked at with the rows
     const uint32_t count = drafts_of(a, n);
     uint32_t* out = a.out_tokens + (size_t)n * (a.D + 1);
     if (count > a.D) {  // left out, or out of range
+        if (__syncthreads_or(status)) return;
         if (count == K3X_VERIFY_SKIP) {
             for (uint32_t i = tid; i <= a.D; i += blockDim.x) out[i] = 0xffffffffu;
             if (tid == 0) a.accepted[n] = 0;
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(1024) void verify_accept_kernel(VerifyArgs a) {
         if (row.fit && !a.greedy) row.prob = prob(a, l, row.max, row.inv);
         if ((tid & 63) == 0) rows[i] = row;
     }
-    __syncthreads();
+    if (__syncthreads_or(status)) return;
     if (tid == 0) {
         uint32_t bad = 0, i = 0;
         for (;; ++i) {
@@ -466,8 +467,9 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
     const uint32_t blocks = (a.parts + kWaves - 1) / kWaves;
     const uint32_t n = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 63;
     const uint32_t part = blockIdx.x % blocks * kWaves + (tid >> 6);
-    if (__syncthreads_or(*(volatile uint32_t*)a.status)) return;
+    const uint32_t status = *(volatile uint32_t*)a.status;
     const Drawn d = a.drawn[n];
+    if (__syncthreads_or(status)) return;
     if (d.done) return;
     Rest<DT> rest(a, d, n);
     const float past = a.form == K3X_DIST_PROBS ? 0.0f : -__builtin_inff();
