@@ -1134,7 +1134,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
             if (y == 0) load_lds16_at<0>(r, to, lane * 16, first * 1024);
             if (y == 1) load_lds16_at<1024>(r, to, lane * 16, first * 1024);
             if (y == 2) load_lds16_at<2048>(r, to, lane * 16, first * 1024);
-            if (y == 3) load_lds16_at<3072>(r, to, lane * 16, first * 1024);
+            if (y == 3) load_lds16_at<3 * 1024>(r, to, lane * 16, first * 1024);
         };
 #pragma unroll
         for (uint32_t y = 0; y < kRecLoads + kOps; ++y) {
