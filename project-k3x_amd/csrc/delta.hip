@@ -103,6 +103,15 @@ __device__ inline float dpp(float x, float old = 0.0f) {
                                                       0xf, 0xf, false));
 }
 
+// x of lane i of the lane's four.
+__device__ inline float of_four(float x, int i) {
+    const int v = __float_as_int(x);
+    return __int_as_float(i == 0   ? __builtin_amdgcn_update_dpp(0, v, 0x00, 0xf, 0xf, true)
+                          : i == 1 ? __builtin_amdgcn_update_dpp(0, v, 0x55, 0xf, 0xf, true)
+                          : i == 2 ? __builtin_amdgcn_update_dpp(0, v, 0xaa, 0xf, 0xf, true)
+                                   : __builtin_amdgcn_update_dpp(0, v, 0xff, 0xf, 0xf, true));
+}
+
 // Four elements as they lie.
 template <typename E>
 using Vec4 = E __attribute__((ext_vector_type(4)));
@@ -130,13 +139,14 @@ __device__ inline Vec4<E> load4(const E* row, uint32_t c, uint32_t n, bool vec) 
 // are neighbours in the columns of one head and share nothing else.
 //
 // One token a sequence is the state's read and write: 64 sequences of 32 heads
-// of 128 x 128 take 48 us, 5.6 TB/s.  More tokens are bound by the sums' chain:
-// 16 tokens a sequence (8 sequences, limits) 26 us, 1.3 us a token.
+// of 128 x 128 take 48 us, 5.6 TB/s.  More tokens are bound by the vector
+// instructions of a token and the sums' chain: 16 tokens a sequence (8 sequences,
+// limits) 24 us, 1.2 us a token.
 constexpr int kStepWaves = 4;
 constexpr uint32_t kStepCols = 16 * kStepWaves;
 
-// vec: bit 0, q, k and gate by four elements (of the calls above 48 and 26 us;
-// by one 57 and 37); bit 1, v (by one 27 of the second); bit 2, states.
+// vec: bit 0, q, k and gate by several elements (of the calls above 48 and 24 us;
+// by one 55 and 34); bit 1, v (by one 50 and 26); bit 2, states.
 template <uint32_t DT, int R, uint32_t GATE>
 __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a, uint32_t vec) {
     typedef typename Elem<DT>::type E;
@@ -164,9 +174,12 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
         for (int i = 0; i < R; ++i)
             S[i] = load4(a.state_in + base + (size_t)min(r0 + i, a.K - 1) * a.V, c0, a.V, vec & 4);
     }
+    // Four lanes share their rows' gates, a quarter each.
+    constexpr int kGates = R / 4;
+    const uint32_t g0 = r0 + kGates * (lane % 4);
     struct Row {
         Vec4<E> q[R / 4], k[R / 4], v;
-        f32x4 gate[GATE == K3X_GATE_CHANNEL ? R / 4 : 1];
+        float gate[GATE == K3X_GATE_CHANNEL ? kGates : 1];
         float beta;
     } next, now;
     auto fetch = [&](uint32_t t) {
@@ -178,9 +191,19 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
         for (int i = 0; i < R / 4; ++i) {
             next.q[i] = load4(q, r0 + 4 * i, a.K, vec & 1);
             next.k[i] = load4(k, r0 + 4 * i, a.K, vec & 1);
-            if (GATE == K3X_GATE_CHANNEL) next.gate[i] = load4(g, r0 + 4 * i, a.K, vec & 1);
         }
-        if (GATE == K3X_GATE_HEAD) next.gate[0][0] = g[0];
+        if constexpr (GATE == K3X_GATE_CHANNEL) {
+            typedef float Gates __attribute__((ext_vector_type(kGates)));
+            if (kGates > 1 && (vec & 1)) {
+                const Gates x = *reinterpret_cast<const Gates*>(g + min(g0, a.K - kGates));
+#pragma unroll
+                for (int i = 0; i < kGates; ++i) next.gate[i] = x[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < kGates; ++i) next.gate[i] = g[min(g0 + i, a.K - 1)];
+            }
+        }
+        if (GATE == K3X_GATE_HEAD) next.gate[0] = g[0];
         next.v = load4(static_cast<const E*>(a.v) + row * a.vs + (size_t)h * a.V, c0, a.V, vec & 2);
         next.beta = a.beta[row * a.H + h];
     };
@@ -196,19 +219,18 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
     for (uint32_t t = 0; t < sq.len; ++t) {
         now = next;
         fetch(min(t + 1, sq.len - 1));
-        float q[R], k[R], v[4], d[R];
+        float q[R], k[R], v[4], d[kGates];
         float qq = 0.0f, kk = 0.0f, kq = 0.0f;
         f32x4 p = {}, o = {};
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             q[i] = Elem<DT>::load(now.q[i / 4][i % 4]);
             k[i] = Elem<DT>::load(now.k[i / 4][i % 4]);
-            d[i] = GATE == K3X_GATE_CHANNEL ? now.gate[i / 4][i % 4] : now.gate[0][0];
         }
         if (r0 + R > a.K) {
 #pragma unroll
             for (int i = 0; i < R; ++i)
-                if (r0 + i >= a.K) q[i] = k[i] = 0.0f, d[i] = 0.0f;
+                if (r0 + i >= a.K) q[i] = k[i] = 0.0f;
         }
         z = __builtin_fmaf(now.beta, 0.0f, z);
 #pragma unroll
@@ -216,24 +238,24 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
             v[j] = Elem<DT>::load(now.v[j]);
             z = __builtin_fmaf(v[j], 0.0f, z);
         }
-        if (GATE == K3X_GATE_HEAD) {
-            wrong |= !(now.gate[0][0] <= 0.0f);
-            d[0] = exp_decay(now.gate[0][0]);
+        if (GATE != K3X_GATE_NONE) {
+#pragma unroll
+            for (int i = 0; i < (GATE == K3X_GATE_CHANNEL ? kGates : 1); ++i) {
+                wrong |= !(now.gate[i] <= 0.0f);
+                d[i] = exp_decay(now.gate[i]);
+            }
         }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             z = __builtin_fmaf(q[i], 0.0f, z);
             z = __builtin_fmaf(k[i], 0.0f, z);
-            if (GATE == K3X_GATE_CHANNEL) {
-                wrong |= !(d[i] <= 0.0f);
-                d[i] = exp_decay(d[i]);
-            }
+            const float decay = GATE == K3X_GATE_CHANNEL ? of_four(d[i % kGates], i / kGates) : d[0];
             qq = __builtin_fmaf(q[i], q[i], qq);
             kk = __builtin_fmaf(k[i], k[i], kk);
             kq = __builtin_fmaf(k[i], q[i], kq);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (GATE != K3X_GATE_NONE) S[i][j] *= d[GATE == K3X_GATE_HEAD ? 0 : i];
+                if (GATE != K3X_GATE_NONE) S[i][j] *= decay;
                 p[j] = __builtin_fmaf(S[i][j], k[i], p[j]);
                 o[j] = __builtin_fmaf(S[i][j], q[i], o[j]);
             }
@@ -653,7 +675,7 @@ __device__ inline f16x8 by_channel(const ByChannel<KB>& tr, uint32_t tile) {
 // TB/s; one 32-channel part in registers at a time, two workgroups a SIMD pair
 // (three or four do not fit without spills).
 // WHOLE: K = 32 KB and rows by four elements, so that no load is guarded (rows
-// off by one element: 199 us in place of 179 with the scan).
+// off by one element: 189 us in place of 167 with the scan).
 template <uint32_t DT, int KB, bool WHOLE>
 __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
     DeltaArgs a, ChunkRecord* records, ChunkOperands<true, KB>* operands) {
@@ -818,7 +840,7 @@ __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
 // tokens: the products of keys and queries once, and for each value head (a
 // wave every other one) its factors exp(G_i - G_j), G the log decays summed in
 // double.  8192 tokens of 16 key and 32 value heads of 128: 72 us for 67 MB read
-// and 185 MB written, 3.5 TB/s.  WHOLE as above (242 in place of 215 us).
+// and 185 MB written, 3.5 TB/s.  WHOLE as above (237 in place of 210 us).
 template <uint32_t DT, int KB, bool WHOLE>
 __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
     DeltaArgs a, ChunkRecord* records, ChunkOperands<DT == K3X_DTYPE_F32, KB>* operands) {
@@ -1039,8 +1061,8 @@ constexpr size_t scan_lds() {
     return 2 * sizeof(ScanChunk<LO, KB>) + 2 * kScanWaves * sizeof(ScanTile<DT>);
 }
 
-// VEC: rows of v by 16 bytes (173 us with the operands' kernel, by one element
-// 185, of the first call above).
+// VEC: rows of v by 16 bytes (167 us with the operands' kernel, by one element
+// 176, of the first call above).
 template <uint32_t DT, bool CHANNEL, int KB, bool VEC>
 __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
     DeltaArgs a, const ChunkRecord* records,
@@ -1416,11 +1438,10 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
 // Chunks for heads that the products' tiles take, from the length on where one
 // chunk costs no more than its tokens one by one.  Measured over 32 heads of
 // 128 x 128, us in chunks and token by token:
-//   gates by channel, 1 / 8 / 64 sequences of 20 tokens  23, 26 | 44, 37 | 203, 195
-//                                             24 tokens  23, 30 | 44, 45 | 205, 224
-//   gates by head (16 key heads),             12 tokens  18, 16 | 27, 21 | 112, 120
-//                                             16 tokens  18, 19 | 28, 26 | 116, 149
-// (12 tokens between 8 and 16).
+//   gates by channel, 1 / 8 / 64 sequences of 20 tokens  22, 24 | 43, 35 | 196, 187
+//                                             24 tokens  22, 28 | 43, 43 | 198, 214
+//   gates by head (16 key heads),              8 tokens  17, 13 | 27, 17 | 106, 91
+//                                             16 tokens  17, 19 | 27, 27 | 113, 147
 bool runs_in_chunks(const k3x_hip_delta_params* p) {
     const uint32_t longest =
         p->longest ? p->longest : (p->tokens + p->sequences - 1) / p->sequences;

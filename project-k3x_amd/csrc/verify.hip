@@ -106,8 +106,8 @@ __device__ inline double exp2_f64(double y) {
 
 // A lane's sixteen entries of a part, neighbours by 16 bytes where rows are, so
 // that a wave's loads are whole lines; where() rises with j.  By 16 bytes against
-// by one entry, all launches: 131072 and 131073 probabilities of 64 sequences 27
-// and 30 us, logits of 16 sequences of 4 drafts 43 and 48.
+// by one entry, all launches: 131072 and 131073 probabilities of 64 sequences 26
+// and 28 us, logits of 16 sequences of 4 drafts 43 and 47.
 template <uint32_t DT>
 struct Entries {
     typedef typename Elem<DT>::type E;
