@@ -640,20 +640,16 @@ struct TokenScales {
     }
 };
 
-// Keys by channel, for the state's update: a wave's tokens into `tr` (a row a
-// channel), and from there, once all are in, as operands.
-template <int KB>
-using ByChannel = _Float16[32 * KB][kChunk + 8];
+// A part's keys by channel, for the state's update: a wave's tokens into `tr` (a
+// row a channel), and from there, once all are in, as operands.
+typedef _Float16 ByChannel[32][kChunk + 8];
 
-template <int KB>
-__device__ inline void put_by_channel(ByChannel<KB>& tr, int b, uint32_t g, uint32_t token,
-                                      const f16x8& x) {
+__device__ inline void put_by_channel(ByChannel& tr, uint32_t g, uint32_t token, const f16x8& x) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) tr[32 * b + token_of(g, j)][token] = x[j];
+    for (int j = 0; j < 8; ++j) tr[token_of(g, j)][token] = x[j];
 }
 
-template <int KB>
-__device__ inline f16x8 by_channel(const ByChannel<KB>& tr, uint32_t tile) {
+__device__ inline f16x8 by_channel(const ByChannel& tr, uint32_t tile) {
     typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const f16x4 lo = *reinterpret_cast<const f16x4*>(&tr[16 * tile + m][4 * g]);
@@ -683,7 +679,7 @@ __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
     __shared__ Tile32 Ls, Ps;
     __shared__ Pair8 cross[64];
     __shared__ float total[2][32];
-    __shared__ __attribute__((aligned(16))) ByChannel<1> tr[2];
+    __shared__ __attribute__((aligned(16))) ByChannel tr[2];
     __shared__ float beta_s[kChunk], c_s[kChunk];
     const uint32_t h = blockIdx.x % a.H, slot = blockIdx.x / a.H;
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -798,15 +794,15 @@ __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
         ops->Q[0][w][b][lane] = qp.hi;
         ops->Q[1][w][b][lane] = qp.lo;
         const Pair8 sp = split8(suf);
-        put_by_channel<1>(tr[0], 0, g, t, sp.hi);
-        put_by_channel<1>(tr[1], 0, g, t, sp.lo);
+        put_by_channel(tr[0], g, t, sp.hi);
+        put_by_channel(tr[1], g, t, sp.lo);
         if (w == 0 && m == 0) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) rec->decay[32 * b + token_of(g, j)] = tot[j] * other[j];
         }
         lds_barrier();
-        ops->Kt[0][2 * b + w][lane] = by_channel<1>(tr[0], w);
-        ops->Kt[1][2 * b + w][lane] = by_channel<1>(tr[1], w);
+        ops->Kt[0][2 * b + w][lane] = by_channel(tr[0], w);
+        ops->Kt[1][2 * b + w][lane] = by_channel(tr[1], w);
     }
     diag = sum_groups(diag);
     if (wrong || z != z) latch(a.status, K3X_ERR_INVALID_MXFP4);
@@ -848,7 +844,7 @@ __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
     constexpr bool LO = DT == K3X_DTYPE_F32;
     __shared__ Tile32 Gk, Gq, work[2];
     __shared__ Pair8 cross[64];
-    __shared__ __attribute__((aligned(16))) ByChannel<1> tr[LO ? 2 : 1];
+    __shared__ __attribute__((aligned(16))) ByChannel tr[LO ? 2 : 1];
     __shared__ float c_s[kChunk], rk_s[kChunk], rq_s[kChunk], o_s[kChunk], beta_s[2][kChunk];
     __shared__ double G_s[2][kChunk];
     const uint32_t hk = blockIdx.x % a.Hk, slot = blockIdx.x / a.Hk, per = a.H / a.Hk;
@@ -896,11 +892,11 @@ __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
         if (w == 0) cross[lane] = kp;
         ops->K[0][w][b][lane] = kp.hi;
         ops->Q[0][w][b][lane] = qp.hi;
-        put_by_channel<1>(tr[0], 0, g, t, kp.hi);
+        put_by_channel(tr[0], g, t, kp.hi);
         if (LO) {
             ops->K[LO ? 1 : 0][w][b][lane] = kp.lo;
             ops->Q[LO ? 1 : 0][w][b][lane] = qp.lo;
-            put_by_channel<1>(tr[LO ? 1 : 0], 0, g, t, kp.lo);
+            put_by_channel(tr[LO ? 1 : 0], g, t, kp.lo);
         }
         lds_barrier();
         if (w == 1) {
@@ -909,7 +905,7 @@ __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
             q21 = mfma_pairs(qp, before, q21);
         }
 #pragma unroll
-        for (int y = 0; y < (LO ? 2 : 1); ++y) ops->Kt[y][2 * b + w][lane] = by_channel<1>(tr[y], w);
+        for (int y = 0; y < (LO ? 2 : 1); ++y) ops->Kt[y][2 * b + w][lane] = by_channel(tr[y], w);
         lds_barrier();
     }
     diag = sum_groups(diag);
