@@ -407,8 +407,9 @@ typedef struct k3x_hip_route_params {
  * left as they were: a score, bias or sum that is not finite, with renormalised
  * weights a sum of 0 (K3X_ERR_INVALID_STATE; with K3X_RENORM_DOUBLE and sigmoid
  * scores a logit or bias that is not finite, or the sum, as
- * K3X_ERR_INVALID_EXTENT); other tokens' outputs may then be missing.  The reference routes on the host
- * (runtime/src/routing_policy.cpp:31-160; official_moe.cpp:211-245).
+ * K3X_ERR_INVALID_EXTENT); other tokens' outputs may then be missing.  The
+ * reference routes on the host (runtime/src/routing_policy.cpp:31-160;
+ * official_moe.cpp:211-245).
  * Asynchronous. */
 int k3x_hip_route(k3x_hip_ctx* ctx, const k3x_hip_route_params* params, const void* logits,
                   const float* bias, uint32_t* ids, float* weights);
