@@ -452,6 +452,13 @@ __device__ inline float max_groups(float v) {
     return __uint_as_float(max(h[0], h[1]));
 }
 
+__device__ inline int max_groups(int v) {
+    const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    const int x = max((int)r[0], (int)r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+    return max((int)h[0], (int)h[1]);
+}
+
 // 2^-e and 2^e for the least e with |x| < 2^e (x finite); 1 and 1 for x = 0.
 __device__ inline void unit_scale(float x, float* down, float* up) {
     int e = x > 0.0f ? __builtin_amdgcn_frexp_expf(x) : 0;
@@ -1232,26 +1239,29 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[t][j] = __builtin_ldexpf(v[t][j], -shift);
-                vmost = fmaxf(vmost, fabsf(v[t][j]));
-            }
+            for (int j = 0; j < 4; ++j) vmost = fmaxf(vmost, fabsf(v[t][j]));
         // Column sizes near 1 leave both the products' growth and the parts
-        // below hi their room.
-        most = max_groups(fmaxf(most, vmost * kOperand));
-        const bool off = (most > 32.0f * kOperand) | ((most < 0.5f * kOperand) & (most > 0.0f));
+        // below hi their room.  A size is an exponent of 2, that of the values as
+        // they came (times kOperand, as the state is held): by the shift that a
+        // state next to nothing has left behind they need not be numbers of fp32.
+        constexpr int kEmpty = -(1 << 30);
+        const int size =
+            max_groups(max(most > 0.0f ? __builtin_amdgcn_frexp_expf(most) + shift : kEmpty,
+                           vmost > 0.0f ? __builtin_amdgcn_frexp_expf(vmost) + 6 : kEmpty));
+        int d = size - shift - 3 - 6;
+        const bool off = ((d > 2) | (d < -3)) & (size > kEmpty);
         if (__builtin_amdgcn_ballot_w64(off)) {
-            const int d = off ? __builtin_amdgcn_frexp_expf(most) - 3 - 6 : 0;
+            d = off ? d : 0;
             shift += d;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[t][j] = __builtin_ldexpf(v[t][j], -d);
 #pragma unroll
             for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) S[t][i] = __builtin_ldexpf(S[t][i], -d);
         }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[t][j] = __builtin_ldexpf(v[t][j], -shift);
         // (P k) S and (P q) S; the products of one sum lie apart.
         f16x8 tf[2][2];
         f32x4 rt[2], rr[2];

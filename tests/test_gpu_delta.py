@@ -498,3 +498,59 @@ def test_rows_past_32_bits(hip, lens):
     want, Sw, tol, stol = definition(s, 64 ** -0.5)
     close(out, want, tol, BF16)
     close(S, Sw, stol)
+
+
+def quiet(s, tokens):
+    """The first `tokens` rows without values, under a decay that empties no state."""
+    s["v"][:tokens] = 0
+    if s["gate"] is not None:
+        s["gate"][:] = -0.7
+    return s
+
+
+@pytest.mark.parametrize("longest", [1, 1 << 20], ids=["tokens", "chunks"])
+@pytest.mark.parametrize("gate", ["head", "channel"])
+@pytest.mark.parametrize("tokens,decay", [(96, -1.6), (192, -0.7), (1000, -0.7)])
+def test_values_after_a_long_decay(hip, tokens, decay, gate, longest):
+    """Nothing is written for a while, so that the state all but vanishes; then values of
+    size one."""
+    s = quiet(inputs((tokens + 70,), 1, 2, 128, 48, BF16, gate), tokens)
+    s["gate"][:] = decay
+    check(hip, s, longest=longest)
+
+
+@pytest.mark.parametrize("longest", [1, 1 << 20], ids=["tokens", "chunks"])
+@pytest.mark.parametrize("gate", ["none", "head", "channel"])
+@pytest.mark.parametrize("size", [1e-30, 1e-36, 1e-40, 1e30, 1e36])
+def test_state_and_values_of_unlike_sizes(hip, size, gate, longest):
+    """A state next to nothing, or far above the values that follow; every other column as
+    large as they are."""
+    s = inputs((50,), 1, 2, 64, 48, gate=gate)
+    s["state"][..., ::2] *= size
+    check(hip, s, longest=longest)
+
+
+@pytest.mark.parametrize("longest", [1, 1 << 20], ids=["tokens", "chunks"])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("gate", ["none", "head", "channel"])
+def test_values_near_the_largest(hip, gate, dtype, longest):
+    s = quiet(inputs((90,), 1, 2, 128, 48, dtype, gate), 90)
+    for t in (5, 40):
+        s["v"][t] = (1.5e37 * (2 * torch.rand(s["v"][t].shape, device=DEV, generator=gen(t)) - 1)
+                     ).to(dtype)
+    s["state"][:] = 0
+    check(hip, s, longest=longest)
+
+
+@pytest.mark.parametrize("gate", ["head", "channel"])
+def test_long_decay_over_two_calls(hip, gate):
+    """The second call starts from the state that is left, around the smallest numbers."""
+    k3x, ctx = hip
+    whole = quiet(inputs((250,), 1, 2, 128, 48, BF16, gate), 130)
+    a = {x: whole[x][:130] if x in ("q", "k", "v", "beta", "gate") else whole[x] for x in whole}
+    b = {x: whole[x][130:] if x in ("q", "k", "v", "beta", "gate") else whole[x] for x in whole}
+    a["lens"], b["lens"] = [130], [120]
+    for part in (a, b):
+        part["offsets"] = torch.tensor([0, part["lens"][0]], dtype=torch.int32, device=DEV)
+    _, b["state"] = check(hip, a)
+    check(hip, b)
