@@ -1173,6 +1173,13 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
         }
     };
     const size_t base = ((size_t)sq.slot * a.H + h) * a.K * a.V;
+    if (!chunks) {  // the state as it is, which a column's scale need not hold
+        if (!a.state_out || !in || a.state_in == a.state_out) return;
+        for (uint32_t r = g; r < a.K; r += 4)
+            a.state_out[base + (size_t)r * a.V + col] =
+                a.state_in ? a.state_in[base + (size_t)r * a.V + col] : 0.0f;
+        return;
+    }
     // A column is held times 2^-shift, the state times kOperand besides.
     f32x4 S[2 * KB];
     int shift = 0;
@@ -1194,12 +1201,10 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
 #pragma unroll
             for (int i = 0; i < 4; ++i) S[t][i] = kOperand * __builtin_ldexpf(S[t][i], -shift);
     }
-    if (chunks) {
-        bring_values(0);
-        bring(source(), 0, 0, 1);
-        put_values(0);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    }
+    bring_values(0);
+    bring(source(), 0, 0, 1);
+    put_values(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     for (uint32_t ci = 0; ci < chunks; ++ci) {
         const ChunkRecord& rc = buf[ci & 1].r;
         const ChunkOperands<LO, KB>& o = buf[ci & 1].o;
@@ -1429,8 +1434,8 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
     }
     // A value that is not finite has made every row of its column NaN (the
     // products' operands hold no infinity that is not NaN in a sum).
-    if (chunks && !(S[0][0] - S[0][0] == 0.0f)) latch(a.status, K3X_ERR_INVALID_MXFP4);
-    if (!a.state_out || !in || (!chunks && a.state_in == a.state_out)) return;
+    if (!(S[0][0] - S[0][0] == 0.0f)) latch(a.status, K3X_ERR_INVALID_MXFP4);
+    if (!a.state_out || !in) return;
 #pragma unroll
     for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll

@@ -554,3 +554,18 @@ def test_long_decay_over_two_calls(hip, gate):
         part["offsets"] = torch.tensor([0, part["lens"][0]], dtype=torch.int32, device=DEV)
     _, b["state"] = check(hip, a)
     check(hip, b)
+
+
+@pytest.mark.parametrize("in_place", [False, True], ids=["apart", "in_place"])
+def test_sequences_of_no_tokens_keep_their_states(hip, in_place):
+    """A state is copied bit for bit, whatever its columns span, also beside long sequences
+    and where a limit leaves no token."""
+    k3x, ctx = hip
+    s = inputs((0, 80, 3, 40), 1, 2, 128, 48)
+    s["state"] *= 10.0 ** torch.linspace(-42, 36, 128, device=DEV)[:, None]
+    s["state"][0, 1, 3, 7], s["state"][0, 1, 4, 7] = math.nan, -math.inf
+    before = s["state"].clone()
+    st, _, S = call(hip, s, limits=[5, 0, 0, 7], **(dict(state_out=s["state"]) if in_place else {}))
+    assert st == 0 and ctx.synchronize() == 0
+    assert torch.equal(S[:3].view(torch.int32), before[:3].view(torch.int32))
+    assert not torch.equal(S[3], before[3])
