@@ -44,7 +44,9 @@ struct k3x_hip_ctx {
     // The wide path's smaller size classes run on side_stream beside the
     // full chunks: forked after the grouping, joined after their down GEMMs.
     hipEvent_t class_fork_ev = nullptr, class_join_ev = nullptr;
-    uint32_t* status = nullptr;  // device word, latched kernel errors
+    // Device words: latched kernel errors, and those of a delta rule call with
+    // states in place until it is done (zeroed at creation, left zero by every call).
+    uint32_t* status = nullptr;
     size_t max_lds_per_block = 65536;
     uint32_t cu_count = 256;
     // Grow-only scratch (replaces runtime/cuda/device_memory.cuh:44-61).

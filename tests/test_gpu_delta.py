@@ -569,3 +569,52 @@ def test_sequences_of_no_tokens_keep_their_states(hip, in_place):
     assert st == 0 and ctx.synchronize() == 0
     assert torch.equal(S[:3].view(torch.int32), before[:3].view(torch.int32))
     assert not torch.equal(S[3], before[3])
+
+
+FAULTS = ["q", "v", "state", "slot", "twice"]
+
+
+@pytest.mark.parametrize("fault", FAULTS)
+@pytest.mark.parametrize("length,N", [(1, 700), (40, 100)], ids=["short", "long"])
+@pytest.mark.parametrize("gate", ["head", "channel"])
+def test_a_fault_leaves_the_other_sequences_whole(hip, gate, length, N, fault):
+    """States in place: sequences beside an unfit one are those of a call without it, all
+    their heads and columns, more of them than run at once.  What is enqueued after the
+    call does nothing until the error is read."""
+    k3x, ctx = hip
+    s = inputs((length,) * N, 1, 8, 128, 128, BF16, gate)
+    pool = torch.empty((N + 3, 8, 128, 128), device=DEV)
+    pool[:N].copy_(s["state"])
+    pool[N:] = -7.0
+    clean, index = pool.clone(), torch.arange(N, dtype=torch.int32, device=DEV)
+    st, want, _ = call(hip, s, state_in=clean, state_out=clean, slots=N + 3, slot_index=index)
+    assert st == 0 and ctx.synchronize() == 0
+    fit, code = torch.ones(N, dtype=torch.bool, device=DEV), k3x.ERR_INVALID_MXFP4
+    fit[0] = False
+    if fault == "state":
+        pool[0, 3, 5] = math.inf
+    elif fault in ("slot", "twice"):
+        index[0] = N + 3 if fault == "slot" else N - 1
+        fit[N - 1] = fault == "slot"
+        code = k3x.ERR_INVALID_STATE
+    else:
+        s[fault][length // 2, 0, 2] = math.nan
+    before = pool.clone()
+    st, out, _ = call(hip, s, state_in=pool, state_out=pool, slots=N + 3, slot_index=index)
+    assert st == 0
+    later = torch.full((2, 4), -7, dtype=torch.int32, device=DEV)
+    weights = torch.full((2, 4), -7.0, device=DEV)
+    assert k3x.route(ctx, k3x.make_route_params(2, 64, 4), torch.zeros((2, 64), device=DEV), later,
+                     weights) == 0
+    st, out2, S2 = call(hip, dict(s, lens=[length], offsets=s["offsets"][:2], state=clean[:1]))
+    assert st == 0
+    assert ctx.synchronize() == code
+    assert (later == -7).all() and (weights == -7).all()
+    assert (out2 == -7).all() and (S2 == -7).all()
+    assert torch.equal(pool[:N][fit], clean[:N][fit])
+    assert torch.equal(out.unflatten(0, (N, length))[fit], want.unflatten(0, (N, length))[fit])
+    assert (pool[N:] == -7).all()
+    if code == k3x.ERR_INVALID_STATE:  # nothing of the unfit ones is written
+        assert torch.equal(pool[:N][~fit], before[:N][~fit])
+        assert (out.unflatten(0, (N, length))[~fit] == -7).all()
+    assert ctx.synchronize() == 0
