@@ -466,12 +466,13 @@ typedef struct k3x_hip_delta_params {
  * one state with state_out (K3X_ERR_INVALID_STATE; nothing of those sequences
  * is read or written); a q, k, v, gate or beta or a state in use that is not
  * finite or a gate above 0 (K3X_ERR_INVALID_MXFP4, as for the layer's input).
- * The outputs of a sequence with such values are then not defined, and where
- * offsets fall none are.  With states in place (state_out = state_in) the other
- * sequences' outputs and states are those of a call without it: such a call cannot
- * be repeated.  Of any other call they may be missing, and its state_in is what it
- * was.  Calls of one context that overlap share its status, so that an error of
- * one may leave out parts of the other.  Replaces the recurrence of
+ * The outputs of a sequence with such values are then not defined.  With states
+ * in place (state_out = state_in) the other sequences' outputs and states are
+ * those of a call without it (such a call cannot be repeated), but where offsets
+ * fall a call in chunks writes nothing.  Of any other call they may be missing,
+ * and its state_in is what it was.  Calls of one context that overlap share its
+ * status, so that an error of one may leave out parts of the other.  Replaces
+ * the recurrence of
  * ComputeBackend::official_kda (runtime/cuda/official_kda.cuh:11-37), batched.
  * Asynchronous. */
 int k3x_hip_delta_rule(k3x_hip_ctx* ctx, const k3x_hip_delta_params* params, const void* q,

@@ -1092,7 +1092,13 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
         if (threadIdx.x == 0) latch(a.errors, bad);
         return;
     }
-    if (__syncthreads_or(*(volatile const uint32_t*)a.status)) return;
+    // Where offsets fall, their sequence latches it, and nothing is done: chunks are
+    // searched for by the offsets, so that others' may not have been made.
+    uint32_t stop = *(volatile const uint32_t*)a.status;
+    if (a.offsets)
+        for (uint32_t x = threadIdx.x; x < a.N; x += blockDim.x)
+            stop |= a.offsets[x + 1] < a.offsets[x];
+    if (__syncthreads_or(stop)) return;
     const uint32_t begin = __builtin_amdgcn_readfirstlane(sq.begin);
     const uint32_t len = __builtin_amdgcn_readfirstlane(sq.len);
     const uint32_t chunks = (len + kChunk - 1) / kChunk;

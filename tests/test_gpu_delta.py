@@ -618,3 +618,19 @@ def test_a_fault_leaves_the_other_sequences_whole(hip, gate, length, N, fault):
         assert torch.equal(pool[:N][~fit], before[:N][~fit])
         assert (out.unflatten(0, (N, length))[~fit] == -7).all()
     assert ctx.synchronize() == 0
+
+
+@pytest.mark.parametrize("cu", [[0, 41, 40, 120], [120, 40, 80, 120], [0, 40, 80, 79],
+                                [1 << 31, 0, 60, 120]], ids=["middle", "first", "last", "far"])
+@pytest.mark.parametrize("gate", ["head", "channel"])
+def test_falling_offsets_in_chunks(hip, gate, cu):
+    """No sequence of the call is touched: the workspace holds what an earlier call left."""
+    k3x, ctx = hip
+    s = inputs((40, 40, 40), 1, 2, 64, 32, BF16, gate)
+    pool = s["state"].clone()
+    cu = [x - (1 << 32) if x >> 31 else x for x in cu]
+    st, out, _ = call(hip, s, state_in=pool, state_out=pool,
+                      offsets=torch.tensor(cu, dtype=torch.int32, device=DEV))
+    assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_STATE
+    assert torch.equal(pool, s["state"]) and (out == -7).all()
+    check(hip, s)
