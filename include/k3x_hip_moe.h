@@ -465,7 +465,9 @@ typedef struct k3x_hip_delta_params {
  * Latched: offsets that fall or pass T, a slot past slots, two sequences of
  * one state with state_out (K3X_ERR_INVALID_STATE; nothing of those sequences
  * is read or written); a q, k, v, gate or beta or a state in use that is not
- * finite or a gate above 0 (K3X_ERR_INVALID_MXFP4, as for the layer's input).
+ * finite, with norm_epsilon > 0 a q or k whose sum of squares is not (in fp32),
+ * or a gate above 0 (K3X_ERR_INVALID_MXFP4, as for the layer's input); token by
+ * token also a product S^T k past fp32.
  * The outputs of a sequence with such values are then not defined.  With states
  * in place (state_out = state_in) the other sequences' outputs and states are
  * those of a call without it (such a call cannot be repeated), but where offsets

@@ -216,6 +216,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
             if (r0 + i >= a.K) S[i] = f32x4{};
     }
     float z = 0.0f;  // NaN once an input is not finite
+    float longest = 0.0f;  // of the squared norms, by rows of lanes
     bool wrong = false;
     for (uint32_t t = 0; t < sq.len; ++t) {
         now = next;
@@ -272,6 +273,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
         x += dpp<0x128>(x);  // row_ror:8
         y += dpp<0x128>(y);
         w += dpp<0x128>(w);
+        longest = fmaxf(longest, w);
         const float sk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), 0));
         const float skq = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), 16));
         const float sq2 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), 32));
@@ -303,6 +305,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
 #pragma unroll
             for (int j = 0; j < 4; ++j) S[i][j] = __builtin_fmaf(k[i], u[j], S[i][j]);
     }
+    if (a.eps > 0.0f) wrong |= longest == __builtin_inff();
     if (wrong || z != z) latch(a.errors, K3X_ERR_INVALID_MXFP4);
     if (!a.state_out || (!sq.len && a.state_in == a.state_out)) return;
 #pragma unroll
@@ -616,8 +619,8 @@ struct TokenPart {
 struct TokenScales {
     float qd, qu, kd, ku;  // 2^-e and 2^e of the largest element
     float qn, kn;          // 1 / norm
-    // By the whole wave; latches an element that is not finite (here and now: a
-    // check at the end would hold every element until then).
+    // By the whole wave; latches an element, or a norm in use, that is not finite
+    // (here and now: a check at the end would hold every element until then).
     template <uint32_t DT, int KB, bool WHOLE>
     __device__ __forceinline__ void find(const DeltaArgs& a, const typename Elem<DT>::type* qr,
                                          const typename Elem<DT>::type* kr, uint32_t g) {
@@ -640,11 +643,14 @@ struct TokenScales {
                 kk = __builtin_fmaf(y[j], y[j], kk);
             }
         }
+        qq = sum_groups(qq);
+        kk = sum_groups(kk);
+        if (a.eps > 0.0f) z = __builtin_fmaf(fmaxf(qq, kk), 0.0f, z);  // too long for a norm
         if (z != z) latch(a.errors, K3X_ERR_INVALID_MXFP4);
         unit_scale(max_groups(qm), &qd, &qu);
         unit_scale(max_groups(km), &kd, &ku);
-        qn = 1.0f / sqrtf(sum_groups(qq) + a.eps);
-        kn = 1.0f / sqrtf(sum_groups(kk) + a.eps);
+        qn = 1.0f / sqrtf(qq + a.eps);
+        kn = 1.0f / sqrtf(kk + a.eps);
     }
 };
 

@@ -634,3 +634,17 @@ def test_falling_offsets_in_chunks(hip, gate, cu):
     assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_STATE
     assert torch.equal(pool, s["state"]) and (out == -7).all()
     check(hip, s)
+
+
+@pytest.mark.parametrize("what", ["q", "k"])
+@pytest.mark.parametrize("gate", ["head", "channel"])
+@pytest.mark.parametrize("longest", [1, 1 << 20], ids=["tokens", "chunks"])
+def test_norms_past_the_range_are_latched(hip, longest, gate, what):
+    """A row whose sum of squares is no fp32 number is not taken for one of length 0."""
+    k3x, ctx = hip
+    s = inputs((40,), 1, 2, 64, 32, BF16, gate)
+    s[what][20] = (s[what][20].float() * 1e20).to(BF16)
+    st, _, _ = call(hip, s, longest=longest)
+    assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_MXFP4
+    s[what][20] = (s[what][20].float() * 1e-3).to(BF16)
+    check(hip, s, longest=longest)
