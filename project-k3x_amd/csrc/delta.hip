@@ -463,10 +463,12 @@ __device__ inline int max_groups(int v) {
     return max((int)h[0], (int)h[1]);
 }
 
-// 2^-e and 2^e for the least e with |x| < 2^e (x finite); 1 and 1 for x = 0.
+// 2^-e and 2^e for the least e with |x| < 2^e (x finite), as far as both are
+// numbers of fp32: what is below 2^-100 stays below 1/2, what is above 2^127
+// below 2.  1 and 1 for x = 0.
 __device__ inline void unit_scale(float x, float* down, float* up) {
     int e = x > 0.0f ? __builtin_amdgcn_frexp_expf(x) : 0;
-    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    e = e < -100 ? -100 : e > 127 ? 127 : e;
     *down = __builtin_ldexpf(1.0f, -e);
     *up = __builtin_ldexpf(1.0f, e);
 }

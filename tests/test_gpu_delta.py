@@ -648,3 +648,13 @@ def test_norms_past_the_range_are_latched(hip, longest, gate, what):
     assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_MXFP4
     s[what][20] = (s[what][20].float() * 1e-3).to(BF16)
     check(hip, s, longest=longest)
+
+
+@pytest.mark.parametrize("gate", ["head", "channel"])
+@pytest.mark.parametrize("size", [1e-20, 1e20, 1e34])
+@pytest.mark.parametrize("longest", [1, 1 << 20], ids=["tokens", "chunks"])
+def test_queries_of_any_size_without_norm(hip, longest, size, gate):
+    s = inputs((45,), 1, 2, 64, 32, gate=gate)
+    s["k"] = s["k"] / s["k"].norm(dim=-1, keepdim=True) * 0.999
+    s["q"] *= size
+    check(hip, s, norm=False, scale=0.5, longest=longest)
