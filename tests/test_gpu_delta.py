@@ -658,3 +658,59 @@ def test_queries_of_any_size_without_norm(hip, longest, size, gate):
     s["k"] = s["k"] / s["k"].norm(dim=-1, keepdim=True) * 0.999
     s["q"] *= size
     check(hip, s, norm=False, scale=0.5, longest=longest)
+
+
+def owned_rows(lens, sequences):
+    at, rows = 0, []
+    for n, length in enumerate(lens):
+        if n in sequences:
+            rows += range(at, at + length)
+        at += length
+    return rows
+
+
+@pytest.mark.parametrize("in_place", [False, True], ids=["apart", "in_place"])
+@pytest.mark.parametrize("lens", [(2, 2), (40, 40)], ids=["short", "long"])
+@pytest.mark.parametrize("index,unfit", [([0, 4], [1]), ([-1, 2], [0]), ([3, 3], [0, 1]),
+                                         ([1 << 30, 4], [0, 1])])
+def test_slots_that_are_no_states(hip, index, unfit, lens, in_place):
+    """Rows of a sequence without a state and states without a sequence stay as they were,
+    beyond the last one of the call too."""
+    k3x, ctx = hip
+    s = inputs(lens, 1, 1, 64, 32)
+    room = torch.full((9, 1, 64, 32), -7.0, device=DEV)
+    pool = room[1:5]
+    fresh = torch.full_like(room, -7.0)
+    pool[:2].copy_(s["state"])
+    before = room.clone()
+    st, out, _ = call(hip, s, state_in=pool, state_out=pool if in_place else fresh[1:5], slots=4,
+                      slot_index=torch.tensor(index, dtype=torch.int32, device=DEV))
+    assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_STATE
+    assert (out[owned_rows(lens, unfit)] == -7).all()
+    mine = [1 + x for n, x in enumerate(index) if n not in unfit]
+    rest = [x for x in range(9) if x not in mine]
+    assert torch.equal(room[rest], before[rest])
+    assert (fresh[rest] == -7).all()
+
+
+@pytest.mark.parametrize("lens", [(2, 2), (40, 40)], ids=["short", "long"])
+def test_offsets_past_the_rows(hip, lens):
+    """Sequences that end behind the last row read and write nothing, nor do those that
+    fall; what lies around the rows and the states stays as it was."""
+    k3x, ctx = hip
+    s = inputs(lens, 1, 1, 64, 32, extra=50)
+    T = sum(lens)
+    room = dict(out=torch.full((T + 50, 1, 32), -7.0, device=DEV),
+                state=torch.full((6, 1, 64, 32), -7.0, device=DEV))
+    few = {x: y[:T] if x in ("q", "k", "v", "beta", "gate") else y for x, y in s.items()}
+    for cu, unfit in (([0, T // 2, T + 7], [1]), ([T + 1, T + 2, T + 3], [0, 1]),
+                      ([0, T + 1, T], [0, 1]), ([-9, 0, T // 2], [0])):
+        for x in room.values():
+            x[:] = -7.0
+        st, _, _ = call(hip, few, out=room["out"][:T], state_out=room["state"][:2],
+                        offsets=torch.tensor(cu, dtype=torch.int32, device=DEV))
+        assert st == 0 and ctx.synchronize() == k3x.ERR_INVALID_STATE
+        assert (room["out"][T:] == -7).all() and (room["state"][2:] == -7).all()
+        assert (room["state"][unfit] == -7).all()
+        if cu[0] == 0 and cu[1] <= cu[2]:
+            assert (room["out"][T // 2:T] == -7).all()
