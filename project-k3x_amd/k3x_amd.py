@@ -730,20 +730,45 @@ def verify_workspace_bytes(params: VerifyParams) -> int:
     return load().k3x_hip_verify_workspace(C.byref(params))
 
 
+def _vocab_rows(ctx: Context, what: str, t, shape, dtypes):
+    """(device pointer, elements from row to row) of rows [N][R][V] that lie evenly, each
+    contiguous in itself; the distance is 0 where it is the row's length, None where there is
+    one row at most."""
+    if (t.shape != shape or t.dtype not in dtypes or not t.is_cuda or
+            t.get_device() != ctx.device):
+        _refuse(ctx, what, t, shape, dtypes)
+    N, R, V = shape
+    if t.is_contiguous():
+        return t.data_ptr(), 0 if N * R > 1 else None
+    n, r, v = t.stride()
+    step = r if R > 1 else n
+    if V > 1 and v != 1:
+        raise ValueError(f"{what}: expected rows that are contiguous in themselves")
+    if N * R > 1 and (step < V or step >= 1 << 32 or (N > 1 and R > 1 and n != R * r)):
+        raise ValueError(f"{what}: expected rows that lie evenly, not strides {t.stride()}")
+    return t.data_ptr(), step if N * R > 1 else None
+
+
 def verify_draft(ctx: Context, params: VerifyParams, target, tokens, accepted, out_tokens,
                  draft=None, draft_counts=None, accept_u=None, sample_u=None,
                  workspace=None) -> int:
     """Verifies drafted tokens [N][D] against the target's rows [N][D + 1][V]
-    (k3x_hip_verify_draft): accepted [N] and out_tokens [N][D + 1] int32."""
+    (k3x_hip_verify_draft): accepted [N] and out_tokens [N][D + 1] int32.  Rows of target and
+    draft may be parts of longer ones, as far apart in both; the distance is the tensors'."""
     N, D, V, types = params.sequences, params.drafts, params.vocab, _types()
     f32, ints = types["f32"], types["ints"]
-    tp = _at(ctx, "target", target, (N, D + 1, V), types["logits"])
+    tp, step = _vocab_rows(ctx, "target", target, (N, D + 1, V), types["logits"])
     if _dtype(target) != params.dtype:
         raise ValueError("target: not of the parameters' type")
     xp = _at(ctx, "tokens", tokens, (N, D), ints)
     dp = cp = ap = sp = None
     if draft is not None:
-        dp = _at(ctx, "draft", draft, (N, D, V), (target.dtype,))
+        dp, drafted = _vocab_rows(ctx, "draft", draft, (N, D, V), (target.dtype,))
+        if drafted is not None and drafted != step and not params.greedy:
+            raise ValueError("draft: rows not as far apart as the target's")
+    if params.row_stride != (step or 0):
+        params = VerifyParams.from_buffer_copy(params)
+        params.row_stride = step or 0
     if draft_counts is not None:
         cp = _at(ctx, "draft_counts", draft_counts, (N,), ints)
     if accept_u is not None:

@@ -314,3 +314,17 @@ def test_rows_past_32_bits(hip, greedy):
     assert torch.equal(accepted[-1:].cpu(), want_a) and torch.equal(out[-1:].cpu(), want)
     if greedy:  # rows of equal entries: the lowest token
         assert (accepted[:-1] == D).all() and (out[:-1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("probs", [False, True], ids=["logits", "probs"])
+@pytest.mark.parametrize("greedy", [False, True], ids=["sampled", "greedy"])
+@pytest.mark.parametrize("pad", [3, 64])
+def test_padded_rows(hip, dtype, probs, greedy, pad):
+    """Rows of a padded vocabulary as they lie: what the padding holds is not looked at."""
+    s = inputs(3, 2, 2049, dtype, probs)
+    for x in ("target", "draft"):
+        rows = torch.full((*s[x].shape[:2], 2049 + pad), math.nan, device=DEV).to(dtype)
+        rows[..., :2049] = s[x]
+        s[x] = rows[..., :2049]
+    check(hip, s, probs, greedy)

@@ -166,3 +166,76 @@ def test_strides_of_rows():
     for bad in (wide.t(), wide.unflatten(1, (2, 15))[:, :, :5]):
         with pytest.raises(ValueError):
             k3x._row_stride(bad)
+
+
+class Recorded:
+    """A context whose library calls are kept and not made."""
+    handle, device = None, 0
+
+    def __init__(self):
+        self.lib, self.calls = self, []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append((name, a)) or 0
+
+
+class OnDevice(torch.Tensor):
+    """A tensor that says it is on device 0."""
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+def there(x):
+    return x.as_subclass(OnDevice)
+
+
+def verified(target, draft=None, params=None):
+    """The parameters that verify_draft calls the library with."""
+    N, D1, V = target.shape
+    c, ints = Recorded(), torch.zeros((N, D1), dtype=torch.int32)
+    p = k3x.make_verify_params(target) if params is None else params
+    u = torch.zeros((N, D1))
+    assert k3x.verify_draft(c, p, there(target), there(ints[:, 1:].contiguous()),
+                            there(ints[:, 0].contiguous()), there(ints),
+                            draft=None if draft is None else there(draft),
+                            accept_u=there(u[:, 1:].contiguous()),
+                            sample_u=there(u[:, 0].contiguous())) == 0
+    (name, args), = c.calls
+    assert name == "k3x_hip_verify_draft"
+    return args[1]._obj
+
+
+def test_verified_rows_lie_where_the_tensors_say():
+    """The distance of rows is the tensors' own, whatever the parameters hold: a distance set
+    there would be read past the end of packed rows."""
+    packed = torch.zeros((2, 4, 9))
+    p = k3x.make_verify_params(packed)
+    p.row_stride = 1 << 20
+    assert verified(packed, packed[:, :3].contiguous(), p).row_stride in (0, 9)
+    assert p.row_stride == 1 << 20  # the caller's own is left
+    wide = torch.zeros((2, 4, 13))[..., :9]
+    assert verified(wide).row_stride == 13
+    assert verified(wide, torch.zeros((2, 3, 13))[..., :9]).row_stride == 13
+    assert verified(torch.zeros((5, 1, 13))[..., 2:11]).row_stride == 13
+    assert verified(torch.zeros((1, 5, 13))[..., 2:11]).row_stride == 13
+    one = torch.zeros((1, 2, 13))[..., :9]  # a single drafted row lies anywhere
+    assert verified(one, torch.zeros((1, 1, 30))[..., :9]).row_stride == 13
+    assert verified(one, torch.zeros((1, 1, 9))).row_stride == 13
+
+
+@pytest.mark.parametrize("target,draft", [
+    (torch.zeros((2, 4, 13))[..., :9], torch.zeros((2, 3, 9))),
+    (torch.zeros((2, 4, 9)), torch.zeros((2, 3, 13))[..., :9]),
+    (torch.zeros((2, 5, 9))[:, :4], None),
+    (torch.zeros((4, 2, 9)).transpose(0, 1), None),
+    (torch.zeros((2, 4, 18))[..., ::2], None),
+    (torch.zeros((1, 1, 9)).expand(2, 4, 9), None),
+    (torch.zeros(40).as_strided((2, 4, 9), (16, 4, 1)), None),
+    (torch.empty((2, 4, 9), device="meta").as_strided((2, 4, 9), (1 << 34, 1 << 32, 1)), None)],
+    ids=["draft_packed", "target_packed", "gap", "transposed", "every_second", "one_row", "overlap",
+         "far"])
+def test_verified_rows_that_do_not_lie_evenly(target, draft):
+    with pytest.raises(ValueError):
+        verified(target, draft)
