@@ -663,7 +663,10 @@ def route(ctx: Context, params: RouteParams, logits, ids, weights, bias=None) ->
     and the fp32 bias [E] (k3x_hip_route)."""
     T, E, K, types = params.tokens, params.experts, params.top_k, _types()
     p = RouteParams.from_buffer_copy(params)
-    lp, p.logits_stride = _rows(ctx, "logits", logits, (T, E), types["logits"])
+    lp, step = _rows(ctx, "logits", logits, (T, E), types["logits"])
+    if step >= 1 << 32:
+        raise ValueError("logits: rows 2^32 elements apart and more")
+    p.logits_stride = step
     p.dtype = _dtype(logits)
     bp = None if bias is None else _at(ctx, "bias", bias, (E,), types["f32"])
     return ctx.lib.k3x_hip_route(ctx.handle, C.byref(p), lp, bp,

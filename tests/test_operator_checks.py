@@ -239,3 +239,19 @@ def test_verified_rows_lie_where_the_tensors_say():
 def test_verified_rows_that_do_not_lie_evenly(target, draft):
     with pytest.raises(ValueError):
         verified(target, draft)
+
+
+@pytest.mark.parametrize("far,refused", [(64, False), (80, False), ((1 << 32) - 1, False),
+                                         (1 << 32, True), ((1 << 32) + 80, True)])
+def test_distance_of_logits(far, refused):
+    """A distance past the parameter's 32 bits is refused, not cut to them."""
+    c, p = Recorded(), k3x.make_route_params(2, 64, 4)
+    logits = there(torch.empty((2, 64), device="meta").as_strided((2, 64), (far, 1)))
+    ids, weights = there(torch.zeros((2, 4), dtype=torch.int32)), there(torch.zeros((2, 4)))
+    if refused:
+        with pytest.raises(ValueError):
+            k3x.route(c, p, logits, ids, weights)
+        assert not c.calls
+    else:
+        assert k3x.route(c, p, logits, ids, weights) == 0
+        assert c.calls[0][1][1]._obj.logits_stride == (0 if far == 64 else far)
