@@ -519,7 +519,9 @@ typedef struct k3x_hip_verify_params {
  * accepted u32 [N]; out_tokens u32 [N][D + 1]: the accepted tokens, the next
  * token, then 0xffffffff.  draft_counts (device u32 [N], or NULL) gives
  * sequences fewer drafts than D (the next row is then the last), or
- * K3X_VERIFY_SKIP: accepted 0, no tokens, nothing read.
+ * K3X_VERIFY_SKIP: accepted 0, no tokens, nothing read.  So a sequence's tokens
+ * to commit (limits of k3x_hip_delta_rule) are accepted + 1, and none where
+ * out_tokens[n][0] is 0xffffffff.
  * workspace as k3x_hip_delta_rule's, k3x_hip_verify_workspace(params) bytes.
  * Latched as K3X_ERR_INVALID_STATE, the sequence's outputs left as they were: a
  * drafted token past V that is reached, a used row that holds NaN, plus

@@ -218,3 +218,43 @@ def test_captured_step(hip, D):
         one.bank.close()
         two.bank.close()
         ctx.close()
+
+
+@pytest.mark.parametrize("gate", ["head", "channel"])
+@pytest.mark.parametrize("D", [3, 30])
+def test_sequences_left_out_keep_their_states(hip, D, gate):
+    """draft_counts leaves sequences out and gives others fewer drafts: the limits made of
+    both outputs commit nothing of the former."""
+    k3x, ctx = hip
+    N = 5
+    counts = [D, -1, 0, D - 1, -1]
+    step = Step(k3x, ctx, N, D, gate, 11)
+    before = step.state.clone()
+    g = delta.gen(4)
+    step.v["target"].copy_(torch.randn(step.v["target"].shape, device=DEV, generator=g))
+    step.drafts(5)
+    v = step.v
+    assert k3x.verify_draft(
+        ctx, step.verify, v["target"], v["tokens"], step.accepted, step.tokens, draft=v["draft"],
+        draft_counts=torch.tensor(counts, dtype=torch.int32, device=DEV),
+        accept_u=v["accept_u"], sample_u=v["sample_u"], workspace=step.verify_ws) == 0
+    step.limits = torch.where(step.tokens[:, 0] == -1, 0, step.accepted + 1)
+    assert step.limits.dtype == torch.int32
+    step.rule(step.again, limits=step.limits, commit=True)
+    assert ctx.synchronize() == 0
+    accepted, tokens = verify.definition(v, False, False, 0.9, counts)
+    assert torch.equal(step.accepted.cpu(), accepted) and torch.equal(step.tokens.cpu(), tokens)
+    limits = [0 if c == -1 else int(a) + 1 for c, a in zip(counts, accepted)]
+    assert step.limits.tolist() == limits
+    out, state, tol, stol = delta.definition(step.s, K ** -0.5, limits=limits)
+    delta.close(step.state, state, stol)
+    for n in range(N):
+        at = n * (D + 1)
+        rows = slice(at, at + limits[n])
+        delta.close(step.again[rows], out[rows], tol[rows], BF16)
+        assert (step.again[at + limits[n]:at + D + 1] == -7).all()
+        if counts[n] == -1:
+            assert torch.equal(step.state[n], before[n])
+        else:
+            assert not torch.equal(step.state[n], before[n])
+    step.bank.close()
