@@ -5,6 +5,10 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import os
+import re
+from decimal import Decimal, localcontext
+from fractions import Fraction
 
 import pytest
 
@@ -255,3 +259,27 @@ def test_distance_of_logits(far, refused):
     else:
         assert k3x.route(c, p, logits, ids, weights) == 0
         assert c.calls[0][1][1]._obj.logits_stride == (0 if far == 64 else far)
+
+
+def test_bound_of_the_exponential_in_verification():
+    """The series of verify.hip's 2^f against 60 digits over |f| <= 1/2, exactly as its
+    coefficients are held: within the bound that its comment states."""
+    path = os.path.join(os.path.dirname(k3x.__file__), "csrc", "verify.hip")
+    with open(path) as f:
+        source = f.read()
+    at = source.index("inline double exp2_f64")
+    bound = float(re.findall(r"([0-9.]+e-[0-9]+) of it at most", source[:at])[-1])
+    body = source[at:source.index("ldexp", at)]
+    series = [Fraction(float(x or y)) for x, y in
+              re.findall(r"double p = ([0-9.e+-]+);|p, f, ([0-9.e+-]+)\)", body)]
+    assert len(series) == 12
+    worst = 0.0
+    with localcontext() as digits:
+        digits.prec = 60
+        for i in range(-256, 257):
+            f, p = Fraction(i, 512), Fraction(0)
+            for c in series:
+                p = p * f + c
+            want = (Decimal(2).ln() * f.numerator / f.denominator).exp()
+            worst = max(worst, abs(float(Decimal(p.numerator) / p.denominator / want - 1)))
+    assert worst <= bound, worst
