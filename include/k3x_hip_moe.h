@@ -510,8 +510,8 @@ typedef struct k3x_hip_verify_params {
  * temperature), or the rows themselves), draft i is accepted while
  *   accept_u[n][i] q_i(x_i) < p_i(x_i)
  * and the next token is drawn from max(p_i - q_i, 0) at the first draft i that
- * is not, or from p_D: the first token whose cumulative sum is over
- * sample_u[n] times the whole.  draft (device [N][D][V]) NULL: q_i is 1 at x_i.
+ * is not (p_i itself where that is 0 everywhere), or from p_D: the first token
+ * whose cumulative sum is over sample_u[n] times the whole.  draft (device [N][D][V]) NULL: q_i is 1 at x_i.
  * accept_u fp32 [N][D], sample_u fp32 [N], in [0, 1).  greedy: accepted while
  * x_i is the largest entry of the target's row i, and the next token is the
  * largest of its row (draft, accept_u and sample_u are not read).
@@ -527,7 +527,9 @@ typedef struct k3x_hip_verify_params {
  * drafted token past V that is reached, a used row that holds NaN, plus
  * infinity (logits) or a negative or infinite entry (probabilities) or nothing
  * but minus infinity or zeros, a uniform outside [0, 1), a draft count past D;
- * other sequences' outputs may then be missing.
+ * other sequences' outputs may then be missing.  Rows past the first draft that
+ * is not accepted are not used; of probabilities, unless greedy, the rows before
+ * it only at the drafted token.
  * The reference verifies on the host (generate_speculative,
  * runtime/src/model.cpp:1507).  Asynchronous. */
 int k3x_hip_verify_draft(k3x_hip_ctx* ctx, const k3x_hip_verify_params* params,

@@ -328,3 +328,29 @@ def test_padded_rows(hip, dtype, probs, greedy, pad):
         rows[..., :2049] = s[x]
         s[x] = rows[..., :2049]
     check(hip, s, probs, greedy)
+
+
+def test_entries_that_are_not_used(hip):
+    """Probabilities of accepted rows are looked at for the drafted token only, rows past the
+    first draft that is not accepted not at all."""
+    s = inputs(2, 4, 3000, probs=True)
+    s["accept_u"][:] = 0
+    s["accept_u"][:, 2] = 1 - 2.0 ** -24
+    at = torch.arange(2, device=DEV)
+    x = s["tokens"][:, 2].long()
+    s["draft"][at, 2, x], s["target"][at, 2, x] = 1.0, 1e-9  # not accepted
+    clean = {k: v.clone() for k, v in s.items()}
+    for i in range(2):
+        for name in ("target", "draft"):
+            keep = s[name][at, i, s["tokens"][:, i].long()].clone()
+            s[name][:, i] = math.nan
+            s[name][at, i, s["tokens"][:, i].long()] = keep
+    s["target"][:, 3:] = math.inf
+    s["draft"][:, 3:] = -1.0
+    s["tokens"][:, 3] = -1
+    k3x, ctx = hip
+    assert (check(hip, clean, True) == 2).all()
+    st, accepted, out = call(hip, s, True)
+    st2, accepted2, out2 = call(hip, clean, True)
+    assert st == st2 == 0 and ctx.synchronize() == 0
+    assert torch.equal(accepted, accepted2) and torch.equal(out, out2)
