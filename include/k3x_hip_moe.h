@@ -467,7 +467,7 @@ typedef struct k3x_hip_delta_params {
  * is read or written); a q, k, v, gate or beta or a state in use that is not
  * finite, with norm_epsilon > 0 a q or k whose sum of squares is not (in fp32),
  * or a gate above 0 (K3X_ERR_INVALID_MXFP4, as for the layer's input); token by
- * token also a product S^T k past fp32.
+ * token also a product of the state with a k or q as given past fp32.
  * The outputs of a sequence with such values are then not defined.  With states
  * in place (state_out = state_in) the other sequences' outputs and states are
  * those of a call without it (such a call cannot be repeated), but where offsets
