@@ -430,8 +430,9 @@ typedef struct k3x_hip_delta_params {
     uint32_t gate;        /* enum k3x_gate */
     float scale;          /* of the queries */
     float norm_epsilon;   /* > 0: q and k each over sqrt(sum of squares + epsilon); 0: as given */
-    uint32_t longest;     /* tokens of the longest sequence if known, 0: not.  Chooses the
-                             kernels only: results hold whatever it says. */
+    uint32_t longest;     /* tokens of the longest sequence if known, 0: not (then the
+                             average).  Chooses the kernels only, token by token or in
+                             chunks: results hold whatever it says. */
     uint32_t slots;       /* states in state_in and state_out */
     /* Elements from token to token of q, k, v and out (q, k and v may be
      * parts of one projection's rows), 2^24 at most; 0: packed. */
@@ -458,10 +459,12 @@ typedef struct k3x_hip_delta_params {
  * without slot_index (then slots >= N).  A sequence of no tokens has its state
  * copied.
  * One token a sequence and short sequences run token by token; longer ones in
- * chunks whose writes are solved for at once.  workspace: device, 256-byte
- * aligned, k3x_hip_delta_workspace(params) bytes (NULL where that is 0), the
- * call's own until it is done: calls that may overlap, and captured graphs
- * that may, have one each.
+ * chunks of 32 whose writes are solved for at once; there an output is also off
+ * by up to 2^-29 |q| scale times the largest value that its column takes in the
+ * chunk, later tokens' too.
+ * workspace: device, 256-byte aligned, k3x_hip_delta_workspace(params) bytes
+ * (NULL where that is 0), the call's own until it is done: calls that may
+ * overlap, and captured graphs that may, have one each.
  * Latched: offsets that fall or pass T, a slot past slots, two sequences of
  * one state with state_out (K3X_ERR_INVALID_STATE; nothing of those sequences
  * is read or written); a q, k, v, gate or beta or a state in use that is not

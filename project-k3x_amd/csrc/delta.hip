@@ -1065,6 +1065,12 @@ struct ScanChunk {
 template <uint32_t DT>
 using ScanTile = typename Elem<DT>::type[kChunk][16];
 
+// A column's largest is brought below 2^kHeld, as the state is held, once it is
+// out of 2^(kHeld - 4) .. 2^(kHeld + 1).  As large as f16 allows: parts of an
+// operand end at 2^-24, so that a value is held to 2^-25 / 2^(kHeld - 10) of the
+// column's largest at worst, also of a later token of its chunk.
+constexpr int kHeld = 14;
+
 constexpr int kScanWaves = 4;
 constexpr uint32_t kScanCols = 16 * kScanWaves;
 
@@ -1210,7 +1216,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
                 most = fmaxf(most, fabsf(S[t][i]));
             }
         most = max_groups(most);
-        if (most > 0.0f) shift = __builtin_amdgcn_frexp_expf(most) - 3;
+        if (most > 0.0f) shift = __builtin_amdgcn_frexp_expf(most) + 6 - kHeld;
 #pragma unroll
         for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
@@ -1260,16 +1266,15 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j) vmost = fmaxf(vmost, fabsf(v[t][j]));
-        // Column sizes near 1 leave both the products' growth and the parts
-        // below hi their room.  A size is an exponent of 2, that of the values as
+        // A column's size is an exponent of 2, that of the values as
         // they came (times kOperand, as the state is held): by the shift that a
         // state next to nothing has left behind they need not be numbers of fp32.
         constexpr int kEmpty = -(1 << 30);
         const int size =
             max_groups(max(most > 0.0f ? __builtin_amdgcn_frexp_expf(most) + shift : kEmpty,
                            vmost > 0.0f ? __builtin_amdgcn_frexp_expf(vmost) + 6 : kEmpty));
-        int d = size - shift - 3 - 6;
-        const bool off = ((d > 2) | (d < -3)) & (size > kEmpty);
+        int d = size - shift - kHeld;
+        const bool off = ((d > 1) | (d < -3)) & (size > kEmpty);
         if (__builtin_amdgcn_ballot_w64(off)) {
             d = off ? d : 0;
             shift += d;
@@ -1338,7 +1343,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
                 for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(y[t][j]));
             if (!__builtin_amdgcn_ballot_w64(big > 16384.0f)) return;
             big = max_groups(big);
-            const int d = big > 16384.0f ? __builtin_amdgcn_frexp_expf(big) - 5 : 0;
+            const int d = big > 16384.0f ? __builtin_amdgcn_frexp_expf(big) - 12 : 0;
             shift += d;
 #pragma unroll
             for (int t = 0; t < 2; ++t)

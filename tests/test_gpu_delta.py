@@ -714,3 +714,17 @@ def test_offsets_past_the_rows(hip, lens):
         assert (room["state"][unfit] == -7).all()
         if cu[0] == 0 and cu[1] <= cu[2]:
             assert (room["out"][T // 2:T] == -7).all()
+
+
+@pytest.mark.parametrize("gate", ["none", "head", "channel"])
+@pytest.mark.parametrize("norm", [True, False], ids=["norm", "given"])
+def test_values_that_grow_within_a_chunk(hip, gate, norm):
+    """Tokens before larger ones of their chunk, up to 2^13 times as large: within the bound
+    that their own and earlier sizes give."""
+    s = inputs((96,), 1, 2, 64, 48, gate=gate)
+    if not norm:
+        s["k"] = s["k"] / s["k"].norm(dim=-1, keepdim=True) * 0.999
+    s["state"][:] = 0
+    s["v"] = s["v"].sign() * (1 + s["v"].abs().clamp(max=1))
+    s["v"] *= (2.0 ** (torch.arange(96, device=DEV) % 32 * 0.4))[:, None, None]
+    check(hip, s, norm=norm)
