@@ -147,7 +147,7 @@ constexpr int kStepWaves = 4;
 constexpr uint32_t kStepCols = 16 * kStepWaves;
 
 // vec: bit 0, q, k and gate by several elements (of the calls above 48 and 24 us;
-// by one 55 and 34); bit 1, v (by one 50 and 26); bit 2, states.
+// by one 55 and 33); bit 1, v (by one 49 and 26); bit 2, states.
 template <uint32_t DT, int R, uint32_t GATE>
 __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a, uint32_t vec) {
     typedef typename Elem<DT>::type E;
@@ -687,7 +687,7 @@ __device__ inline f16x8 by_channel(const ByChannel& tr, uint32_t tile) {
 // TB/s; one 32-channel part in registers at a time, two workgroups a SIMD pair
 // (three or four do not fit without spills).
 // WHOLE: K = 32 KB and rows by four elements, so that no load is guarded (rows
-// off by one element: 189 us in place of 167 with the scan).
+// off by one element: 191 us in place of 165 with the scan, on warm inputs).
 template <uint32_t DT, int KB, bool WHOLE>
 __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
     DeltaArgs a, ChunkRecord* records, ChunkOperands<true, KB>* operands) {
@@ -851,8 +851,8 @@ __global__ __launch_bounds__(128, 2) void delta_prep_channel_kernel(
 // One chunk of one key head under a decay a value head, by two waves of 16
 // tokens: the products of keys and queries once, and for each value head (a
 // wave every other one) its factors exp(G_i - G_j), G the log decays summed in
-// double.  8192 tokens of 16 key and 32 value heads of 128: 72 us for 67 MB read
-// and 185 MB written, 3.5 TB/s.  WHOLE as above (237 in place of 210 us).
+// double.  8192 tokens of 16 key and 32 value heads of 128: 77 us for 67 MB read
+// and 185 MB written, 3.3 TB/s.  WHOLE as above (242 in place of 203 us).
 template <uint32_t DT, int KB, bool WHOLE>
 __global__ __launch_bounds__(128, 2) void delta_prep_head_kernel(
     DeltaArgs a, ChunkRecord* records, ChunkOperands<DT == K3X_DTYPE_F32, KB>* operands) {
@@ -1049,10 +1049,10 @@ __device__ inline void load_lds16_at(__amdgpu_buffer_rsrc_t r, u32x4* dst, uint3
 // chunk is multiplied, the next one's record, operands and values come to LDS
 // as they lie, the loads spread over the products.
 //
-// A chunk takes 2.0 us: (P k) S, U, its operand, T U and the update follow one
-// another, and one wave a SIMD issues all of them, some 600 instructions of
-// which 84 are products (1344 of 4700 cycles).  So a sequence of 2048 tokens
-// takes 125 us, and seven of 8192 together (448 workgroups, two a CU) 145 us.
+// A chunk takes 1.9 us: (P k) S, U, its operand, T U and the update follow one
+// another, and one wave a SIMD issues all of them, some 580 instructions of
+// which 84 are products (1344 of 4400 cycles).  So a sequence of 2048 tokens
+// takes 124 us, and seven of 8192 together (448 workgroups, two a CU) 150 us.
 // Neither fewer columns a workgroup (two waves as long on the first, one 15%
 // longer), nor more (eight waves 11% longer on the second), nor two waves to 16
 // columns, each with half of the channels (15%), shorten that.
@@ -1079,8 +1079,8 @@ constexpr size_t scan_lds() {
     return 2 * sizeof(ScanChunk<LO, KB>) + 2 * kScanWaves * sizeof(ScanTile<DT>);
 }
 
-// VEC: rows of v by 16 bytes (167 us with the operands' kernel, by one element
-// 176, of the first call above).
+// VEC: rows of v by 16 bytes (165 us with the operands' kernel, by one element
+// 177, of the first call above on warm inputs).
 template <uint32_t DT, bool CHANNEL, int KB, bool VEC>
 __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
     DeltaArgs a, const ChunkRecord* records,
@@ -1435,22 +1435,22 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
         const auto outs = rows_buffer(static_cast<E*>(a.out) +
                                           (begin + (size_t)ci * kChunk) * a.os + (size_t)h * a.V,
                                       left(ci), ost, a.V * es);
-        // The next chunk is in LDS (only this one's outputs may still be on
-        // their way) and every wave is done with this one.
-        // Rows of 32 bytes a wave, as they lie in the registers.  Nothing above is
-        // moved down here (without this the compiler does, and it takes 12% longer).
+        // Outputs of 32 bytes a row and wave, as they lie in the registers.  Nothing above
+        // is moved down here (without this the compiler does, and it takes 12% longer).
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int t = j / 4, i = j % 4;
-                const float y = __builtin_fmaf(fp[t][i], ap[t][i], fo[t][i] * aq[t][i]);
-                store_one<E>(Elem<DT>::store(__builtin_ldexpf(y, shift)), outs,
-                             in ? (4 * g + 16 * t + i) * ost + col * es : kOutside, 0);
-            }
-            if (more) put_values(ci + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int j = 0; j < 8; ++j) {
+            const int t = j / 4, i = j % 4;
+            const float y = __builtin_fmaf(fp[t][i], ap[t][i], fo[t][i] * aq[t][i]);
+            store_one<E>(Elem<DT>::store(__builtin_ldexpf(y, shift)), outs,
+                         in ? (4 * g + 16 * t + i) * ost + col * es : kOutside, 0);
+        }
+        if (more) put_values(ci + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        // The next chunk is in LDS (only these eight stores may still be on their
+        // way) and every wave is done with this one.
+        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
     // A value that is not finite has made every row of its column NaN (the
     // products' operands hold no infinity that is not NaN in a sum).

@@ -456,7 +456,7 @@ __device__ inline uint32_t draw_whole(const VerifyArgs& a, const Rest<DT>& rest,
 
 // The row that the next token is drawn from: sums of all parts, and the entry by
 // the last workgroup that arrives, so that no launch waits between.  64 sequences
-// of 131072 probabilities (67 MB): 21 us, 13 of them the sums (5.2 TB/s) and the
+// of 131072 probabilities (67 MB): 20 us, 13 of them the sums (5.2 TB/s) and the
 // others the last workgroup's loads that wait for one another, for which one
 // wave holds the part in registers (by the workgroup, runs of sixteen neighbours
 // a thread: 20 us in place of 8).
