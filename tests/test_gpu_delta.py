@@ -728,3 +728,51 @@ def test_values_that_grow_within_a_chunk(hip, gate, norm):
     s["v"] = s["v"].sign() * (1 + s["v"].abs().clamp(max=1))
     s["v"] *= (2.0 ** (torch.arange(96, device=DEV) % 32 * 0.4))[:, None, None]
     check(hip, s, norm=norm)
+
+
+@pytest.mark.parametrize("lens", [(1,) * 5, (75, 40, 33)], ids=["short", "long"])
+def test_captured_in_place(hip, lens):
+    """Replays move the states on; one that meets an unfit sequence moves the others', the
+    next does nothing until the error is read, and those after it run again."""
+    k3x, _ = hip
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ctx = k3x.Context(0)
+        s = inputs(lens, 1, 2, 128, 64, BF16)
+        p = k3x.make_delta_params(s["q"], s["k"], s["v"], len(lens), gate=s["gate"], scale=0.1,
+                                  norm_epsilon=EPS, longest=max(lens))
+        need = k3x.delta_workspace_bytes(p)
+        ws = torch.empty((need,), dtype=torch.uint8, device=DEV) if need else None
+        one, two = s["state"].clone(), s["state"].clone()
+        out, out2 = torch.zeros_like(s["v"]), torch.zeros_like(s["v"])
+
+        def run(state, out):
+            return k3x.delta_rule(ctx, p, s["q"], s["k"], s["v"], s["beta"], out, gate=s["gate"],
+                                  offsets=s["offsets"], state_in=state, state_out=state,
+                                  workspace=ws)
+
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            assert run(one, out) == 0
+        for i in range(5):
+            s["v"].copy_(torch.randn(s["v"].shape, device=DEV, generator=gen(60 + i)))
+            kept = s["v"][0].clone()
+            assert run(two, out2) == 0 and ctx.synchronize() == 0
+            if i == 2:
+                s["v"][0, 0, 0] = math.nan
+            graph.replay()
+            if i != 2:
+                assert ctx.synchronize() == 0
+                assert torch.equal(one, two) and torch.equal(out, out2)
+                continue
+            s["v"][0].copy_(kept)
+            after = one.clone()
+            graph.replay()
+            assert ctx.synchronize() == k3x.ERR_INVALID_MXFP4
+            assert torch.equal(one[1:], two[1:]) and torch.equal(one[1:], after[1:])
+            assert torch.equal(out[lens[0]:], out2[lens[0]:])
+            one[0].copy_(two[0])
+            out.copy_(out2)
+        del graph
+        ctx.close()
