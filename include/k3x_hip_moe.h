@@ -460,8 +460,8 @@ typedef struct k3x_hip_delta_params {
  * copied.
  * One token a sequence and short sequences run token by token; longer ones in
  * chunks of 32 whose writes are solved for at once; there an output is also off
- * by up to 2^-29 |q| scale times the largest value that its column takes in the
- * chunk, later tokens' too.
+ * by up to 2^-28 |q| scale times the largest value that its column takes in the
+ * chunk, later tokens' too, for each of the chunk's tokens up to its own.
  * workspace: device, 256-byte aligned, k3x_hip_delta_workspace(params) bytes
  * (NULL where that is 0), the call's own until it is done: calls that may
  * overlap, and captured graphs that may, have one each.
@@ -477,8 +477,8 @@ typedef struct k3x_hip_delta_params {
  * fall a call in chunks writes nothing.  Of any other call they may be missing,
  * and its state_in is what it was.  Calls of one context that overlap share its
  * status, so that an error of one may leave out parts of the other.  Replaces
- * the recurrence of
- * ComputeBackend::official_kda (runtime/cuda/official_kda.cuh:11-37), batched.
+ * the recurrence of ComputeBackend::official_kda
+ * (runtime/cuda/official_kda.cuh:11-37), batched.
  * Asynchronous. */
 int k3x_hip_delta_rule(k3x_hip_ctx* ctx, const k3x_hip_delta_params* params, const void* q,
                        const void* k, const void* v, const float* gate, const float* beta,
@@ -514,7 +514,8 @@ typedef struct k3x_hip_verify_params {
  *   accept_u[n][i] q_i(x_i) < p_i(x_i)
  * and the next token is drawn from max(p_i - q_i, 0) at the first draft i that
  * is not (p_i itself where that is 0 everywhere), or from p_D: the first token
- * whose cumulative sum is over sample_u[n] times the whole.  draft (device [N][D][V]) NULL: q_i is 1 at x_i.
+ * whose cumulative sum is over sample_u[n] times the whole.  draft (device
+ * [N][D][V]) NULL: q_i is 1 at x_i.
  * accept_u fp32 [N][D], sample_u fp32 [N], in [0, 1).  greedy: accepted while
  * x_i is the largest entry of the target's row i, and the next token is the
  * largest of its row (draft, accept_u and sample_u are not read).

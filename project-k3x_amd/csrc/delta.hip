@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void delta_step_kernel(DeltaArgs a
     const uint32_t cb = blockIdx.x % blocks, h = blockIdx.x / blocks % a.H;
     const uint32_t n = blockIdx.x / blocks / a.H;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t status = *(volatile const uint32_t*)a.status;  // with the offsets, not after them
+    const uint32_t status = *(volatile const uint32_t*)a.status;  // with the offsets, not after
     Sequence sq;
     uint32_t bad = find_sequence(a, n, &sq);
     if (!bad && slot_taken(a, n, sq.slot)) bad = K3X_ERR_INVALID_STATE;
@@ -1266,9 +1266,9 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void delta_scan_kernel(
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j) vmost = fmaxf(vmost, fabsf(v[t][j]));
-        // A column's size is an exponent of 2, that of the values as
-        // they came (times kOperand, as the state is held): by the shift that a
-        // state next to nothing has left behind they need not be numbers of fp32.
+        // A column's size is an exponent of 2, that of the values as they came (times
+        // kOperand, as the state is held): by the shift that a state next to nothing
+        // has left behind they need not be numbers of fp32.
         constexpr int kEmpty = -(1 << 30);
         const int size =
             max_groups(max(most > 0.0f ? __builtin_amdgcn_frexp_expf(most) + shift : kEmpty,
