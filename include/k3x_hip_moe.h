@@ -543,6 +543,186 @@ int k3x_hip_verify_draft(k3x_hip_ctx* ctx, const k3x_hip_verify_params* params,
                          void* workspace, size_t workspace_bytes);
 size_t k3x_hip_verify_workspace(const k3x_hip_verify_params* params);
 
+/* ---- adjustment of logits --------------------------------------------------- */
+
+/* mask_index of a row that no mask applies to. */
+#define K3X_NO_MASK 0xffffffffu
+
+typedef struct k3x_hip_logits_params {
+    uint32_t sequences;     /* N, 1 .. 65535 */
+    uint32_t drafts;        /* D, drafted tokens a sequence, 0 .. 64 */
+    uint32_t vocab;         /* V, 1 .. 2^20 */
+    uint32_t dtype;         /* of logits and out: K3X_DTYPE_F32 or K3X_DTYPE_BF16 */
+    uint32_t row_stride;    /* elements from row to row of logits, >= V; 0: V */
+    uint32_t out_stride;    /* the same of out */
+    uint32_t history_width; /* tokens from row to row of history */
+    uint32_t biases;        /* entries of bias_tokens and bias_values */
+    uint32_t masks;         /* rows of masks */
+    uint32_t mask_stride;   /* words from row to row of masks, >= ceil(V / 32); 0: that */
+} k3x_hip_logits_params;
+
+/* Adjusts the rows that k3x_hip_verify_draft takes (device [N][D + 1][V]; row i
+ * follows i drafted tokens) before anything is drawn from them.  With c the
+ * number of times that a token stands in the sequence's answer, the history past
+ * its prompt and the drafted tokens before the row, each logit l becomes, in fp32
+ * and in this order,
+ *   l > 0 ? l / repetition : l * repetition   where the token stands in the
+ *                                             prompt or the answer
+ *   l - frequency c, then l - presence        where c > 0
+ *   l + its bias
+ *   minus infinity                            where the row's mask bit is 0
+ * and is rounded to its type once.  out (device [N][D + 1][V]) may be logits.
+ * history: device u32 [N][history_width], of which sequence n has
+ * history_lens[n] tokens and of those prompt_lens[n] (NULL: 0) in its prompt;
+ * drafts as k3x_hip_verify_draft's tokens, u32 [N][D], and draft_counts: rows of
+ * sequences that are left out and rows past a sequence's drafts are left as they
+ * were.  repetition, frequency, presence: fp32 [N]; NULL leaves a step out.
+ * Biases: entries bias_offsets[n] .. bias_offsets[n + 1] - 1 (device u32 [N + 1])
+ * of bias_tokens (u32) and bias_values (fp32) are sequence n's; of several for one
+ * token the last holds.  masks: device u32 [masks][mask_stride], bit t % 32 of word
+ * t / 32 set where token t is allowed; row i of sequence n has the mask
+ * mask_index[n][i] (u32 [N][D + 1]) or K3X_NO_MASK.  history, bias_offsets and
+ * masks may each be NULL, with what belongs to them; without a history drafted
+ * tokens count all the same.
+ * Latched as K3X_ERR_INVALID_STATE: a history longer than its row, a prompt longer
+ * than its history, a token of the history, a draft or a bias past V, bias offsets
+ * that fall or pass `biases`, a mask past `masks`, a draft count past D, a
+ * repetition that is not a number above 0, a frequency or presence that is not
+ * finite; rows of that sequence may then be missing or hold some of the steps.
+ * Logits and biases may hold anything and go through the arithmetic as they are.
+ * Asynchronous. */
+int k3x_hip_adjust_logits(k3x_hip_ctx* ctx, const k3x_hip_logits_params* params,
+                          const void* logits, const uint32_t* history,
+                          const uint32_t* history_lens, const uint32_t* prompt_lens,
+                          const uint32_t* drafts, const uint32_t* draft_counts,
+                          const float* repetition, const float* frequency,
+                          const float* presence, const uint32_t* bias_offsets,
+                          const uint32_t* bias_tokens, const float* bias_values,
+                          const uint32_t* masks, const uint32_t* mask_index, void* out);
+
+/* ---- latent attention -------------------------------------------------------- */
+
+/* How a cached token's latent is held: 16-bit values of the call's type, or E4M3
+ * or E2M1 codes with one E8M0 scale for 32 of them. */
+enum k3x_cache_format { K3X_CACHE_16BIT = 0, K3X_CACHE_MXFP8 = 1, K3X_CACHE_MXFP4 = 2 };
+
+/* A cache of latents in pages, and the tokens of a call.
+ *
+ * pool: device, 256-byte aligned, [pages][page_size] rows of
+ * k3x_hip_mla_row_bytes() bytes, each
+ *   the latent: L 16-bit values, L E4M3 codes, or L / 2 bytes of E2M1 codes, low
+ *   nibble first;
+ *   the rotary part: R 16-bit values;
+ *   with codes: L / 32 scale bytes (2^(b - 127)) and zeros up to 16.
+ * table: device u32 [N][table_width]: position p of sequence n is row p %
+ * page_size of page table[n][p / page_size].  Pages may be shared between
+ * sequences; entries past the last used one are not read.
+ * lens: device u32 [N], the positions of each sequence with the call's own
+ * tokens: sequence n has the rows offsets[n] .. offsets[n + 1] - 1 of the call's
+ * tensors (device u32 [N + 1]; NULL: T / N rows each), and they are its last
+ * positions, lens[n] - (offsets[n + 1] - offsets[n]) .. lens[n] - 1.  Rows at
+ * positions below 0 (a padded sequence has lens[n] = 0) are not written, read or
+ * seen.  Rows past offsets[N] are left as they were.
+ * Latched as K3X_ERR_INVALID_STATE by every call, which then reads and writes
+ * nothing outside its tensors and the pool, and leaves outputs undefined: offsets
+ * that fall or pass T, a length past table_width * page_size, a page in use that is
+ * not below `pages`, more tokens in a sequence than `longest`. */
+typedef struct k3x_hip_mla_params {
+    uint32_t sequences;    /* N, 1 .. 65535 */
+    uint32_t tokens;       /* T, 0 .. 2^22 */
+    uint32_t heads;        /* H, 1 .. 1024 (k3x_hip_mla_attention) */
+    uint32_t latent;       /* L, a multiple of 32, 32 .. 512 */
+    uint32_t rotary;       /* R, a multiple of 8, 0 .. 64 */
+    uint32_t dtype;        /* K3X_DTYPE_BF16, or K3X_DTYPE_F16 with K3X_CACHE_16BIT */
+    uint32_t cache_format; /* enum k3x_cache_format */
+    uint32_t page_size;    /* 1 .. 65536 */
+    uint32_t pages;        /* of the pool, pages * page_size at most 2^31 */
+    uint32_t table_width;  /* 1 .. 2^20 */
+    uint32_t longest;      /* tokens of the call in a sequence at most; 0: T */
+    float scale;           /* of the scores, > 0 (k3x_hip_mla_attention) */
+    float norm_epsilon;    /* >= 0, with gamma (k3x_hip_mla_store) */
+    /* Elements from token to token of latent, rotary, q and out; 0: packed. */
+    uint64_t latent_stride, rotary_stride, q_stride, out_stride;
+} k3x_hip_mla_params;
+
+/* Bytes of a cached row; 0 for parameters that the calls refuse. */
+size_t k3x_hip_mla_row_bytes(const k3x_hip_mla_params* params);
+
+/* Writes the call's tokens to their pages: latent device [T][L], rotary [T][R]
+ * (NULL with R = 0), both of the call's type.  gamma (device fp32 [L], or NULL):
+ * the latent is normalised first, x / sqrt(mean(x^2) + norm_epsilon) * gamma,
+ * formed in double and rounded to the call's type.  Codes are rounded to nearest,
+ * ties to even, with the least scale (2^-110 at least) by which the largest of its
+ * 32 is at most 448 (E4M3) or 6 (E2M1), so that nothing saturates.  Tokens of
+ * sequences that share the page of their last positions overwrite one another.
+ * Also latched, as K3X_ERR_INVALID_MXFP4, the token's row left as it was: a latent
+ * or rotary part that is not finite as it is written.  Asynchronous. */
+int k3x_hip_mla_store(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const void* latent,
+                      const void* rotary, const float* gamma, const uint32_t* table,
+                      const uint32_t* offsets, const uint32_t* lens, void* pool);
+
+/* Reads the call's tokens back from their pages, as the values that they stand
+ * for: latent device [T][L], rotary [T][R] (NULL: not read), of the call's type
+ * (codes times their scales are bf16 numbers).  A whole prefix of n tokens is a
+ * call with n rows and lens n.  Asynchronous. */
+int k3x_hip_mla_load(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const void* pool,
+                     const uint32_t* table, const uint32_t* offsets, const uint32_t* lens,
+                     void* latent, void* rotary);
+
+/* Attention over the cached latents with the up-projections absorbed: q device
+ * [T][H][L + R], the latent part of each query multiplied by its head's key
+ * projection already; a token's key is its row of L + R values for every head and
+ * its value the first L of them.  A token at position p sees positions 0 .. p:
+ *   out = sum softmax(scale q . key) latent    (device [T][H][L], of the call's type)
+ * and lse (device fp32 [T][H], or NULL) is the logarithm of the softmax's sum.  A
+ * token that sees nothing has zeros and minus infinity.  Sums are held in fp32;
+ * a key's weight is rounded to the call's type before it multiplies the latent.
+ * q, out and pool 16-byte aligned, strides of q and out multiples of 8 elements.
+ * workspace as k3x_hip_delta_rule's, k3x_hip_mla_attention_workspace(params)
+ * bytes.  Also latched, as K3X_ERR_INVALID_MXFP4: an output that is not finite
+ * (for a query or a cached row that is not).  Replaces the attention of
+ * reference/k3x_ref/mla.py, batched.  Asynchronous. */
+int k3x_hip_mla_attention(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const void* q,
+                          const void* pool, const uint32_t* table, const uint32_t* offsets,
+                          const uint32_t* lens, void* out, float* lse, void* workspace,
+                          size_t workspace_bytes);
+size_t k3x_hip_mla_attention_workspace(const k3x_hip_mla_params* params);
+
+typedef struct k3x_hip_mla_prompt_params {
+    uint32_t sequences; /* N, 1 .. 65535 */
+    uint32_t tokens;    /* T rows of q and out, 0 .. 2^22 */
+    uint32_t keys;      /* S rows of k, v and rotary, 0 .. 2^22 */
+    uint32_t heads;     /* H, 1 .. 1024 */
+    uint32_t key_dim;   /* Dn of a head of its own, a multiple of 8, 8 .. 128 */
+    uint32_t rotary;    /* R, a multiple of 8, 0 .. 64 */
+    uint32_t value_dim; /* Dv, a multiple of 8, 8 .. 128 */
+    uint32_t dtype;     /* K3X_DTYPE_BF16 or K3X_DTYPE_F16 */
+    uint32_t causal;    /* 1: the last query sees every key, each before it one less */
+    uint32_t longest;   /* queries of the longest sequence if known, 0: not (then T).  Only
+                           how the work is laid out: results hold whatever it says. */
+    float scale;        /* of the scores, > 0 */
+    /* Elements from row to row, and of k and v from head to head (k and v may be
+     * parts of one projection's rows); multiples of 8; 0: packed. */
+    uint64_t q_stride, k_stride, v_stride, rotary_stride, out_stride;
+    uint64_t k_head_stride, v_head_stride;
+} k3x_hip_mla_prompt_params;
+
+/* Attention of prompts over expanded keys and values: q device [T][H][Dn + R], k
+ * [S][H][Dn], v [S][H][Dv], rotary [S][R] (the part of a key that all heads share;
+ * NULL with R = 0):
+ *   out = sum softmax(scale q . (k, rotary)) v    (device [T][H][Dv])
+ * Sequence n has the queries offsets[n] .. offsets[n + 1] - 1 and the keys
+ * key_offsets[n] .. key_offsets[n + 1] - 1 (device u32 [N + 1] each; NULL: T / N and
+ * S / N rows each), a cached prefix's first.  causal: query i of m sees the first
+ * n - m + i + 1 of n keys.  lse, empty rows, sums and weights as for
+ * k3x_hip_mla_attention.  q, k, v, rotary and out 16-byte aligned.
+ * Latched: offsets that fall, pass T or S (K3X_ERR_INVALID_STATE; nothing of such
+ * a sequence is read), an output that is not finite (K3X_ERR_INVALID_MXFP4).
+ * Asynchronous. */
+int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* params, const void* q,
+                       const void* k, const void* v, const void* rotary, const uint32_t* offsets,
+                       const uint32_t* key_offsets, void* out, float* lse);
+
 /* ---- official K3 MoE FFN (Stable LatentMoE) ------------------------------ */
 
 /* The official layer wraps a bank of experts that run at the latent width L

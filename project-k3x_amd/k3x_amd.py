@@ -31,6 +31,8 @@ GROUP_MAX, GROUP_TOP2 = 0, 1
 GATE_NONE, GATE_HEAD, GATE_CHANNEL = 0, 1, 2
 DIST_LOGITS, DIST_PROBS = 0, 1
 VERIFY_SKIP = 0xffffffff
+NO_MASK = 0xffffffff
+CACHE_16BIT, CACHE_MXFP8, CACHE_MXFP4 = 0, 1, 2
 MATRIX_GATE, MATRIX_UP, MATRIX_DOWN = 0, 1, 2
 
 STREAM_GATE_CODES = 1
@@ -136,6 +138,29 @@ class VerifyParams(C.Structure):
                [("temperature", C.c_float), ("row_stride", C.c_uint32)]
 
 
+class LogitsParams(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("sequences", "drafts", "vocab", "dtype", "row_stride",
+                                         "out_stride", "history_width", "biases", "masks",
+                                         "mask_stride")]
+
+
+class MlaParams(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("sequences", "tokens", "heads", "latent", "rotary",
+                                         "dtype", "cache_format", "page_size", "pages",
+                                         "table_width", "longest")] + \
+               [("scale", C.c_float), ("norm_epsilon", C.c_float)] + \
+               [(n, C.c_uint64) for n in ("latent_stride", "rotary_stride", "q_stride",
+                                          "out_stride")]
+
+
+class MlaPromptParams(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("sequences", "tokens", "keys", "heads", "key_dim",
+                                         "rotary", "value_dim", "dtype", "causal", "longest")] + \
+               [("scale", C.c_float)] + \
+               [(n, C.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "rotary_stride",
+                                          "out_stride", "k_head_stride", "v_head_stride")]
+
+
 class Stats(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in ("forward_calls", "kernel_launches", "scratch_bytes",
                                          "resident_weight_bytes", "weight_h2d_bytes",
@@ -195,6 +220,13 @@ _SIGS = {
     "k3x_hip_delta_workspace": (C.c_size_t, [C.POINTER(DeltaParams)]),
     "k3x_hip_verify_draft": (C.c_int, [_vp, C.POINTER(VerifyParams)] + [_vp] * 9 + [C.c_size_t]),
     "k3x_hip_verify_workspace": (C.c_size_t, [C.POINTER(VerifyParams)]),
+    "k3x_hip_adjust_logits": (C.c_int, [_vp, C.POINTER(LogitsParams)] + [_vp] * 15),
+    "k3x_hip_mla_row_bytes": (C.c_size_t, [C.POINTER(MlaParams)]),
+    "k3x_hip_mla_store": (C.c_int, [_vp, C.POINTER(MlaParams)] + [_vp] * 7),
+    "k3x_hip_mla_load": (C.c_int, [_vp, C.POINTER(MlaParams)] + [_vp] * 6),
+    "k3x_hip_mla_attention": (C.c_int, [_vp, C.POINTER(MlaParams)] + [_vp] * 8 + [C.c_size_t]),
+    "k3x_hip_mla_attention_workspace": (C.c_size_t, [C.POINTER(MlaParams)]),
+    "k3x_hip_mla_prompt": (C.c_int, [_vp, C.POINTER(MlaPromptParams)] + [_vp] * 8),
     "k3x_hip_official_create": (C.c_int, [_vp, _vp, C.POINTER(OfficialDesc), C.POINTER(_vp)]),
     "k3x_hip_official_destroy": (C.c_int, [_vp]),
     "k3x_hip_official_upload_ffn": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
@@ -596,7 +628,7 @@ def _types() -> dict:
         _TYPES.update(
             codes={torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16},
             ints=(torch.int32, torch.uint32), f32=(torch.float32,),
-            logits=(torch.float32, torch.bfloat16))
+            logits=(torch.float32, torch.bfloat16), bytes=(torch.uint8,))
     return _TYPES
 
 
@@ -782,6 +814,198 @@ def verify_draft(ctx: Context, params: VerifyParams, target, tokens, accepted, o
         ctx.handle, C.byref(params), tp, dp, xp, cp, ap, sp,
         _at(ctx, "accepted", accepted, (N,), ints),
         _at(ctx, "out_tokens", out_tokens, (N, D + 1), ints), *_workspace(ctx, workspace))
+
+
+def make_logits_params(logits) -> LogitsParams:
+    """Parameters of adjust_logits for rows [N][D + 1][V]."""
+    N, D1, V = logits.shape
+    return LogitsParams(N, D1 - 1, V, _dtype(logits), 0, 0, 0, 0, 0, 0)
+
+
+def adjust_logits(ctx: Context, params: LogitsParams, logits, out, history=None,
+                  history_lens=None, prompt_lens=None, drafts=None, draft_counts=None,
+                  repetition=None, frequency=None, presence=None, bias=None, masks=None,
+                  mask_index=None) -> int:
+    """Penalties, biases and masks on rows [N][D + 1][V] (k3x_hip_adjust_logits): out of
+    logits' type, or logits itself.  history [N][width] with history_lens and prompt_lens [N],
+    drafts [N][D], draft_counts [N], masks [M][words] with mask_index [N][D + 1], all int32;
+    repetition, frequency, presence [N] fp32; bias (offsets [N + 1], tokens [B], values [B]).
+    Rows of logits, out and masks may be parts of longer ones."""
+    p = LogitsParams.from_buffer_copy(params)
+    N, D, V, types = p.sequences, p.drafts, p.vocab, _types()
+    f32, ints = types["f32"], types["ints"]
+    xp, step = _vocab_rows(ctx, "logits", logits, (N, D + 1, V), types["logits"])
+    yp, out_step = _vocab_rows(ctx, "out", out, (N, D + 1, V), (logits.dtype,))
+    p.row_stride, p.out_stride = step or 0, out_step or 0
+    p.dtype = _dtype(logits)
+    if yp == xp and p.row_stride != p.out_stride:
+        raise ValueError("out: the memory of logits, but rows elsewhere")
+
+    def each(what, t, dtypes):
+        return None if t is None else _at(ctx, what, t, (N,), dtypes)
+    hp = op = tp = vp = mp = ip = None
+    if history is not None:
+        p.history_width = history.shape[-1]
+        hp = _at(ctx, "history", history, (N, p.history_width), ints)
+    if bias is not None:
+        offsets, tokens, values = bias
+        p.biases = tokens.shape[0]
+        op = _at(ctx, "bias offsets", offsets, (N + 1,), ints)
+        tp = _at(ctx, "bias tokens", tokens, (p.biases,), ints)
+        vp = _at(ctx, "bias values", values, (p.biases,), f32)
+    if masks is not None:
+        p.masks = masks.shape[0]
+        mp, words = _rows(ctx, "masks", masks, (p.masks, (V + 31) // 32), ints)
+        if words >= 1 << 32:
+            raise ValueError("masks: rows 2^32 words apart and more")
+        p.mask_stride = words
+    if mask_index is not None:
+        ip = _at(ctx, "mask_index", mask_index, (N, D + 1), ints)
+    return ctx.lib.k3x_hip_adjust_logits(
+        ctx.handle, C.byref(p), xp, hp, each("history_lens", history_lens, ints),
+        each("prompt_lens", prompt_lens, ints),
+        _at(ctx, "drafts", drafts, (N, D), ints) if drafts is not None else None,
+        each("draft_counts", draft_counts, ints), each("repetition", repetition, f32),
+        each("frequency", frequency, f32), each("presence", presence, f32), op, tp, vp, mp, ip,
+        yp)
+
+
+def make_mla_params(pool, table, tokens, latent, rotary=0, heads=1, cache_format=CACHE_16BIT,
+                    dtype=None, scale=1.0, norm_epsilon=0.0, longest=0) -> MlaParams:
+    """Parameters of the mla_* calls over a pool [pages][page_size][row bytes] (uint8) and a
+    table [N][width] (int32): tokens rows of the call, dtype torch.bfloat16 (None) or float16."""
+    pages, page_size, _ = pool.shape
+    N, width = table.shape
+    code = DTYPE_BF16 if dtype is None else _types()["codes"].get(dtype, 255)
+    return MlaParams(N, tokens, heads, latent, rotary, code, cache_format, page_size, pages,
+                     width, longest, scale, norm_epsilon, 0, 0, 0, 0)
+
+
+def mla_row_bytes(latent, rotary=0, cache_format=CACHE_16BIT) -> int:
+    """Bytes of a cached token."""
+    p = MlaParams(1, 0, 1, latent, rotary, DTYPE_BF16, cache_format, 1, 1, 1, 0, 1.0, 0.0, 0, 0, 0,
+                  0)
+    n = load().k3x_hip_mla_row_bytes(C.byref(p))
+    if not n:
+        raise ValueError(f"no cache of latents of {latent} and {rotary} in format {cache_format}")
+    return n
+
+
+def _mla_dtypes(p: MlaParams):
+    return tuple(t for t, code in _types()["codes"].items() if code == p.dtype)
+
+
+def _mla_pages(ctx: Context, p: MlaParams, pool, table, lens, offsets):
+    """(pool, table, offsets, lens) pointers of an mla_* call."""
+    ints = _types()["ints"]
+    row = ctx.lib.k3x_hip_mla_row_bytes(C.byref(p))
+    # Parameters that the call refuses have no rows to compare.
+    shape = (p.pages, p.page_size, row) if row else pool.shape
+    return (_at(ctx, "pool", pool, shape, _types()["bytes"]),
+            _at(ctx, "table", table, (p.sequences, p.table_width), ints),
+            None if offsets is None else _at(ctx, "offsets", offsets, (p.sequences + 1,), ints),
+            _at(ctx, "lens", lens, (p.sequences,), ints))
+
+
+def mla_store(ctx: Context, params: MlaParams, latent, pool, table, lens, rotary=None,
+              offsets=None, gamma=None) -> int:
+    """Writes rows latent [T][L] and rotary [T][R] to their pages, with gamma [L] (fp32)
+    normalised first (k3x_hip_mla_store); lens [N] with these tokens, offsets [N + 1]."""
+    p = MlaParams.from_buffer_copy(params)
+    same = _mla_dtypes(p)
+    lp, p.latent_stride = _rows(ctx, "latent", latent, (p.tokens, p.latent), same)
+    rp = gp = None
+    if rotary is not None:
+        rp, p.rotary_stride = _rows(ctx, "rotary", rotary, (p.tokens, p.rotary), same)
+    if gamma is not None:
+        gp = _at(ctx, "gamma", gamma, (p.latent,), _types()["f32"])
+    pp, tp, op, np_ = _mla_pages(ctx, p, pool, table, lens, offsets)
+    return ctx.lib.k3x_hip_mla_store(ctx.handle, C.byref(p), lp, rp, gp, tp, op, np_, pp)
+
+
+def mla_load(ctx: Context, params: MlaParams, pool, table, lens, latent, rotary=None,
+             offsets=None) -> int:
+    """Reads the call's rows back as values: latent [T][L], rotary [T][R]
+    (k3x_hip_mla_load)."""
+    p = MlaParams.from_buffer_copy(params)
+    same = _mla_dtypes(p)
+    lp, p.latent_stride = _rows(ctx, "latent", latent, (p.tokens, p.latent), same)
+    rp = None
+    if rotary is not None:
+        rp, p.rotary_stride = _rows(ctx, "rotary", rotary, (p.tokens, p.rotary), same)
+    pp, tp, op, np_ = _mla_pages(ctx, p, pool, table, lens, offsets)
+    return ctx.lib.k3x_hip_mla_load(ctx.handle, C.byref(p), pp, tp, op, np_, lp, rp)
+
+
+def mla_attention_workspace_bytes(params: MlaParams) -> int:
+    return load().k3x_hip_mla_attention_workspace(C.byref(params))
+
+
+def mla_attention(ctx: Context, params: MlaParams, q, pool, table, lens, out, offsets=None,
+                  lse=None, workspace=None) -> int:
+    """Attention of absorbed queries [T][H][L + R] over the cache, out [T][H][L], lse [T][H]
+    fp32 (k3x_hip_mla_attention)."""
+    p = MlaParams.from_buffer_copy(params)
+    T, H, same = p.tokens, p.heads, _mla_dtypes(p)
+    qp, p.q_stride = _rows(ctx, "q", q, (T, H, p.latent + p.rotary), same)
+    yp, p.out_stride = _rows(ctx, "out", out, (T, H, p.latent), same)
+    ep = None if lse is None else _at(ctx, "lse", lse, (T, H), _types()["f32"])
+    pp, tp, op, np_ = _mla_pages(ctx, p, pool, table, lens, offsets)
+    return ctx.lib.k3x_hip_mla_attention(ctx.handle, C.byref(p), qp, pp, tp, op, np_, yp, ep,
+                                         *_workspace(ctx, workspace))
+
+
+def make_mla_prompt_params(q, k, v, sequences, rotary=None, causal=True, scale=1.0,
+                           longest=0) -> MlaPromptParams:
+    """Parameters of mla_prompt for q [T][H][Dn + R], k [S][H][Dn], v [S][H][Dv] and rotary
+    [S][R]."""
+    S, H, Dn = k.shape
+    return MlaPromptParams(sequences, q.shape[0], S, H, Dn,
+                           0 if rotary is None else rotary.shape[1], v.shape[2], _dtype(q),
+                           int(causal), longest, scale, 0, 0, 0, 0, 0, 0, 0)
+
+
+def _head_rows(ctx: Context, what: str, t, shape, dtypes):
+    """(device pointer, elements from row to row, from head to head) of rows [S][H][D] whose
+    heads are contiguous in themselves; 0 where a distance is the packed one."""
+    if (t.shape != shape or t.dtype not in dtypes or not t.is_cuda or
+            t.get_device() != ctx.device):
+        _refuse(ctx, what, t, shape, dtypes)
+    S, H, D = shape
+    if t.is_contiguous() or not t.numel():
+        return t.data_ptr(), 0, 0
+    s, h, d = t.stride()
+    # A distance that nothing is read at is the packed one.
+    s, h = s if S > 1 else 0, h if H > 1 else 0
+    if (D > 1 and d != 1) or (H > 1 and h < D) or (S > 1 and s < D):
+        raise ValueError(f"{what}: expected heads that are contiguous in themselves and apart, "
+                         f"not strides {t.stride()}")
+    return t.data_ptr(), s, h
+
+
+def mla_prompt(ctx: Context, params: MlaPromptParams, q, k, v, out, rotary=None, offsets=None,
+               key_offsets=None, lse=None) -> int:
+    """Attention of prompts over expanded keys and values: out [T][H][Dv], lse [T][H] fp32
+    (k3x_hip_mla_prompt); offsets and key_offsets [N + 1] int32.  k and v may be parts of one
+    projection's rows."""
+    p = MlaPromptParams.from_buffer_copy(params)
+    T, S, H, N, same = p.tokens, p.keys, p.heads, p.sequences, (q.dtype,)
+    ints = _types()["ints"]
+    p.dtype = _dtype(q)
+    qp, p.q_stride = _rows(ctx, "q", q, (T, H, p.key_dim + p.rotary), same)
+    kp, p.k_stride, p.k_head_stride = _head_rows(ctx, "k", k, (S, H, p.key_dim), same)
+    vp, p.v_stride, p.v_head_stride = _head_rows(ctx, "v", v, (S, H, p.value_dim), same)
+    yp, p.out_stride = _rows(ctx, "out", out, (T, H, p.value_dim), same)
+    rp = op = fp = ep = None
+    if rotary is not None:
+        rp, p.rotary_stride = _rows(ctx, "rotary", rotary, (S, p.rotary), same)
+    if offsets is not None:
+        op = _at(ctx, "offsets", offsets, (N + 1,), ints)
+    if key_offsets is not None:
+        fp = _at(ctx, "key_offsets", key_offsets, (N + 1,), ints)
+    if lse is not None:
+        ep = _at(ctx, "lse", lse, (T, H), _types()["f32"])
+    return ctx.lib.k3x_hip_mla_prompt(ctx.handle, C.byref(p), qp, kp, vp, rp, op, fp, yp, ep)
 
 
 class Storage:
