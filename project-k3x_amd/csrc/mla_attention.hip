@@ -1,6 +1,22 @@
 // mla_attention.hip -- attention over the cached latents, the up-projections
 // absorbed into queries and outputs.
+//
+// All heads of a token read the same row of L + R values as the key and its
+// first L as the value, so the rows (token, head) of a sequence are one operand:
+// S^T = K Q^T and O^T = K[:, :L]^T P^T on the matrix cores, 32 cached tokens at a
+// time, with the running maximum and sum of a softmax.  Both products take the
+// tile of K from LDS, where it lies once for all rows of a workgroup.  S^T is
+// computed with tokens as its rows because its result then already is, lane for
+// lane, the operand P^T of the second product (a lane holds four neighbouring
+// tokens of one row; the tokens of that product's depth are taken in the order
+// that this leaves), and a row's maximum and sum lie in one lane of each half.
+//
+// The cached tokens of all sequences, in tiles of 32, are one line that is cut
+// into equal ranges for the workgroups: a sequence that falls into several
+// ranges is joined by a second launch.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "k3x_mla.hpp"
 
@@ -11,6 +27,15 @@ using namespace k3x_mla;
 namespace {
 
 constexpr uint32_t kThreads = 256;
+constexpr uint32_t kTile = 32;       // cached tokens a step
+constexpr uint32_t kLeast = 2;       // tiles of a range at least
+constexpr uint32_t kGroup = kTile * 128;  // bytes of 64 columns of a tile in LDS
+
+// A sequence that begins in range w and ends in another.
+struct Split {
+    uint32_t pieces;  // ranges that it lies in; 0: none to join
+    uint32_t w, begin, count;
+};
 
 struct AttentionArgs {
     Pages pages;
@@ -18,103 +43,730 @@ struct AttentionArgs {
     const uint8_t* pool;
     void* out;
     float* lse;
-    uint32_t H, L, R, F;
+    uint32_t H, L, R;
     uint64_t qs, os;
-    float scale;
+    float rate;  // scale * log2(e)
+    uint32_t G, RB;  // ranges, row blocks of a sequence at most
+    Split* splits;   // [N], or where there are more sequences than ranges [G], by range
+    float2* sums;    // [G][RB][2][rows]: maximum (log2) and sum of a piece
+    float4* parts;   // [G][RB][2][rows * LP / 4]: its outputs, as the lanes hold them
     uint32_t* status;
 };
 
+// Which columns of 16 bytes are exchanged in token t of a tile's 64-column group,
+// so that neither product's reads of it meet in a bank: eight tokens' same column
+// (keys), and four tokens' two neighbours (values).
+__device__ inline uint32_t swizzle(uint32_t t) { return (t & 3) << 1 | (t >> 2 & 1); }
+
+// Rows a wave and how the waves lie: WM row blocks by WD parts of the latent.
+template <int HT_, int WM_, int WD_>
+struct Shape {
+    static constexpr int HT = HT_, WM = WM_, WD = WD_;
+    static constexpr int rows = HT * WM;
+};
+
+template <uint32_t DT, int HT>
+struct Mma;
 template <uint32_t DT>
-__device__ inline float cached(const AttentionArgs& a, const uint8_t* row, uint32_t d) {
-    typedef typename Elem<DT>::type E;
-    if (d >= a.L) return Elem<DT>::load(reinterpret_cast<const E*>(row + a.pages.row.codes)[d - a.L]);
-    if (a.F == K3X_CACHE_16BIT) return Elem<DT>::load(reinterpret_cast<const E*>(row)[d]);
-    const float s = e8m0_to_f32(row[a.pages.row.scales + d / 32]);
-    if (a.F == K3X_CACHE_MXFP8)
-        return (float)mxfp8_8(uint2{row[d], 0u}, s)[0];
-    return (float)dequant8(row[d / 2] >> (d & 1 ? 4 : 0), s)[0];
+struct Mma<DT, 32> {
+    typedef __attribute__((ext_vector_type(16))) float Acc;
+    static __device__ inline Acc run(u32x4 a, u32x4 b, Acc c) {
+        typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+        if constexpr (DT == K3X_DTYPE_BF16)
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                           __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                          __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <uint32_t DT>
+struct Mma<DT, 16> {
+    typedef f32x4 Acc;
+    static __device__ inline Acc run(u32x4 a, u32x4 b, Acc c) {
+        typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+        if constexpr (DT == K3X_DTYPE_BF16)
+            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                           __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                          __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+// Two values as the type's bits, the first in the low half.
+template <uint32_t DT>
+__device__ inline uint32_t pack2(float a, float b) {
+    typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+    if constexpr (DT == K3X_DTYPE_BF16)
+        return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+    else
+        return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
 }
 
-// A workgroup a token and head: 256 keys at a time.
-template <uint32_t DT>
-__global__ __launch_bounds__(kThreads) void mla_attention_kernel(AttentionArgs a) {
-    typedef typename Elem<DT>::type E;
-    __shared__ float q[576], w[kThreads], red[kThreads];
-    const uint32_t tid = threadIdx.x, t = blockIdx.x / a.H, h = blockIdx.x % a.H;
+// Over the lanes that hold one row's scores: the halves, and for 16 rows the
+// 16-lane rows too.
+template <int HT, typename Op>
+__device__ inline float across(float x, Op op) {
+    const uint32_t u = __float_as_uint(x);
+    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    x = op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    if constexpr (HT == 16) {
+        const uint32_t w = __float_as_uint(x);
+        const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+        x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    return x;
+}
+
+// o *= k.  Results that fill half of the register file and more stay in its
+// accumulators, which no other instruction multiplies: each goes through one
+// register in between.  (Left to the compiler, the branch around this makes it
+// hold them twice, and 700 registers go to memory.)  The products that wrote them
+// have ended: those of the next tile's scores lie between.
+template <int OT, typename Acc>
+__device__ __forceinline__ void scale_all(Acc (&o)[OT], float k) {
+    constexpr int W = sizeof(Acc) / 4;
+    if constexpr (OT * W < 128) {
+#pragma unroll
+        for (int i = 0; i < OT; ++i) o[i] *= k;
+    } else {
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                float x = o[i][j], t;
+                asm volatile(
+                    "v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\t"
+                    "v_accvgpr_write_b32 %0, %1"
+                    : "+a"(x), "=&v"(t) : "v"(k));
+                o[i][j] = x;
+            }
+        asm volatile("s_nop 15" ::: "memory");
+    }
+}
+
+// x, as a value that is not computed ahead of the place and held until then.
+__device__ inline uint32_t opaque(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+typedef __attribute__((address_space(3))) uint8_t lds_byte;
+
+__device__ inline u32x4 lds16(const lds_byte* p) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(p);
+}
+// Of a 16-lane row's four tokens by 16 columns, its lane's column.
+__device__ inline uint2 lds_transposed(const lds_byte* p) {
+    typedef __attribute__((ext_vector_type(4))) short s16x4;
+    return __builtin_bit_cast(
+        uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                   (__attribute__((address_space(3))) s16x4*)const_cast<lds_byte*>(p)));
+}
+
+template <int N>
+__device__ inline void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ inline void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Tiles of a sequence in the line; an empty one takes one, in which its rows are
+// written as empty.
+__device__ inline uint32_t tiles_of(const Pages& a, uint32_t n) {
+    Tokens s;
+    if (!tokens_of(a, n, &s) || !s.count) return 0;
+    return max(1u, (s.len + kTile - 1) / kTile);
+}
+
+// FULL: L is LP (else the columns past L are zeros, and not brought or written) and
+// a page holds whole eights of tokens.
+template <uint32_t DT, uint32_t F, int LP, typename S, int BUFS, bool FULL>
+__global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention_kernel(AttentionArgs a) {
+    constexpr int HT = S::HT, WD = S::WD, CG = LP / 64 + 1;
+    constexpr uint32_t kBuffer = CG * kGroup;
+    constexpr int KS = HT == 32 ? 4 : 2;        // products over 64 columns
+    constexpr int OT = LP / HT / WD;            // tiles of the latent, a wave
+    typedef Mma<DT, HT> M;
+    typedef typename M::Acc Acc;
+    // One array: with several the compiler tells them apart, and waits for all direct
+    // loads to LDS before any read of theirs.
+    __shared__ __attribute__((aligned(256))) uint8_t smem[BUFS * kBuffer];
+    uint32_t* const scan = reinterpret_cast<uint32_t*>(smem);  // before the first tile
+    uint32_t* const at_s = scan + 4;
+    lds_byte* const lds = (lds_byte*)smem;
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Row blocks of one range lie on one die, eight ranges beside each other.
+    uint32_t w, rb;
+    if (a.G % 8 == 0) {
+        const uint32_t x = blockIdx.x / 8;
+        w = x / a.RB * 8 + blockIdx.x % 8;
+        rb = x % a.RB;
+    } else {
+        w = blockIdx.x / a.RB;
+        rb = blockIdx.x % a.RB;
+    }
     if (*(volatile uint32_t*)a.status) return;
     if (blockIdx.x == 0) check_sequences(a.pages, a.status);
-    const uint32_t n = sequence_of(a.pages, t);
-    Tokens s;
-    if (n >= a.pages.N || !tokens_of(a.pages, n, &s) || t < s.begin || t - s.begin >= s.count)
-        return;
-    const int64_t p = (int64_t)s.len - s.count + (t - s.begin);
-    const uint32_t sees = p < 0 ? 0 : (uint32_t)p + 1;
-    const E* qr = static_cast<const E*>(a.q) + t * a.qs + (size_t)h * (a.L + a.R);
-    for (uint32_t d = tid; d < a.L + a.R; d += kThreads) q[d] = Elem<DT>::load(qr[d]);
-    float m = -3.4e38f, l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (uint32_t at = 0; at < sees; at += kThreads) {
-        const uint32_t k = at + tid;
+
+    // ---- the line and this workgroup's range of it --------------------------
+    // Tiles before and in sequences base .. base + 255, a sequence a thread.
+    auto scan_tiles = [&](uint32_t base, uint32_t* mine) {
+        const uint32_t n = base + tid;
+        uint32_t c = *mine = n < a.pages.N ? tiles_of(a.pages, n) : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(c, d);
+            if (lane >= (uint32_t)d) c += o;
+        }
         __syncthreads();
-        float x = -__builtin_inff();
-        if (k < sees) {
-            const uint8_t* row = cached_row(a.pages, const_cast<uint8_t*>(a.pool), n, k);
-            if (row) {
-                x = 0.0f;
-                for (uint32_t d = 0; d < a.L + a.R; ++d)
-                    x = __builtin_fmaf(q[d], cached<DT>(a, row, d), x);
-                x *= a.scale;
-            } else {
-                latch(a.status, K3X_ERR_INVALID_STATE);
+        if (lane == 63) scan[wave] = c;
+        __syncthreads();
+        uint32_t before = 0;
+        for (uint32_t i = 0; i < wave; ++i) before += scan[i];
+        return before + c;  // with the thread's own
+    };
+    const bool by_sequence = a.pages.N <= a.G;
+    uint32_t total = 0, own, upto = 0;
+    for (uint32_t base = 0; base < a.pages.N; base += kThreads) {
+        upto = scan_tiles(base, &own);
+        total += scan[0] + scan[1] + scan[2] + scan[3];
+        if (by_sequence && blockIdx.x == 0 && !own && base + tid < a.pages.N)
+            a.splits[base + tid].pieces = 0;  // in no range
+    }
+    const uint32_t chunk = max(kLeast, (total + a.G - 1) / a.G);
+    const uint64_t from64 = (uint64_t)w * chunk;
+    if (!by_sequence && rb == 0 && tid == 0) a.splits[w].pieces = 0;
+    if (from64 >= total) return;
+    const uint32_t from = (uint32_t)from64, to = min(total, from + chunk);
+    // The sequence that tile `from` is in, and the tiles before it.
+    uint32_t carry = 0;
+    for (uint32_t base = 0; base < a.pages.N; base += kThreads) {
+        if (a.pages.N > kThreads) upto = scan_tiles(base, &own);
+        if (own && from >= carry + upto - own && from < carry + upto) {
+            at_s[0] = base + tid;
+            at_s[1] = carry + upto - own;
+        }
+        carry += scan[0] + scan[1] + scan[2] + scan[3];
+        if (carry > from) break;
+    }
+    __syncthreads();
+    uint32_t n = at_s[0], first = at_s[1];
+    __syncthreads();
+
+    // What is not brought to LDS stays zero there.
+    if (!FULL || a.R < 64) {
+        for (uint32_t i = tid * 16; i < BUFS * kBuffer; i += kThreads * 16)
+            *reinterpret_cast<u32x4*>(smem + i) = u32x4{};
+        __syncthreads();
+    }
+
+    const uint32_t wm = wave / WD, wd = wave % WD;
+    const uint32_t col = lane % HT, g = lane / HT;
+    // Where the lane reads its operands in a tile: keys, and values of a 16-lane
+    // row's four tokens.  Other columns of a 64-column group are an exclusive or away.
+    const uint32_t kat0 = col * 128 + (g ^ swizzle(col)) * 16;
+    const uint32_t i16 = lane & 15, vrow = 4 * g + i16 / 4;
+    const uint32_t vat0 = vrow * 128 +
+                          (((HT == 32 ? 2 * (lane >> 4 & 1) : 0) + (i16 & 3) / 2) ^ swizzle(vrow)) * 16 +
+                          (i16 & 1) * 8;
+    // What the lane brings of each tile: token 8 wave + lane / 8, the columns of 16
+    // bytes (codes: the 16 bytes) lane % 8 of each group.
+    const uint32_t btok = 8 * wave + lane / 8, bcol = lane % 8;
+    const uint32_t bput = bcol ^ swizzle(lane / 8);
+
+    bool bad_page = false, bad_value = false;
+    while (true) {
+        Tokens s;
+        const uint32_t tiles = tiles_of(a.pages, n);
+        tokens_of(a.pages, n, &s);
+        if (!tiles) {
+            ++n;
+            continue;
+        }
+        const uint32_t rows = s.count * a.H;
+        const uint32_t t0 = max(from, first) - first, t1 = min(to - first, tiles);
+        const bool whole = t0 == 0 && t1 == tiles;
+        if (rb == 0 && tid == 0 && t0 == 0 && (by_sequence || t1 < tiles))
+            a.splits[by_sequence ? n : w] =
+                Split{t1 < tiles ? (first + tiles - 1) / chunk - w + 1 : 0, w, s.begin, s.count};
+        const uint32_t r0 = rb * S::rows;
+        if (r0 < rows) {
+            // The row of this lane, and how many tokens it sees.
+            const uint32_t r = min(r0 + wm * HT + col, rows - 1), ri = r / a.H;
+            const int32_t sees = (int32_t)s.len - (int32_t)s.count + (int32_t)ri + 1;
+            const int32_t sees_least = (int32_t)s.len - (int32_t)s.count + (int32_t)(r0 / a.H) + 1;
+            const int32_t sees_most = (int32_t)s.len - (int32_t)s.count +
+                                      (int32_t)(min(r0 + S::rows - 1, rows - 1) / a.H) + 1;
+            const uint32_t seen = sees_most > 0 ? (uint32_t)sees_most : 0;
+            const uint32_t end = min(t1, (seen + kTile - 1) / kTile);
+            u32x4 qf[CG * KS];
+            {
+                const uint8_t* q = static_cast<const uint8_t*>(a.q) +
+                                   2 * ((uint64_t)(s.begin + ri) * a.qs +
+                                        (uint64_t)(r % a.H) * (a.L + a.R));
+#pragma unroll
+                for (int c = 0; c < CG; ++c)
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        // Columns of the latent, then of the rotary part.
+                        const uint32_t d = (c < CG - 1 ? c * 64 : 0) + (i * (8 / KS) + g) * 8;
+                        const bool in = c < CG - 1 ? FULL || d < a.L : d < a.R;
+                        const u32x4 x = *reinterpret_cast<const u32x4*>(
+                            q + (in ? 2 * (c < CG - 1 ? d : a.L + d) : 0));
+                        qf[c * KS + i] = x & (in ? 0xffffffffu : 0u);
+                    }
+            }
+            Acc o[OT];
+#pragma unroll
+            for (int i = 0; i < OT; ++i) o[i] = Acc{};
+            float m = -3.4028235e38f, l = 0.0f;
+
+            // ---- bringing tiles ---------------------------------------------
+            constexpr bool DIRECT = F == K3X_CACHE_16BIT && FULL;
+            // The wave's eight tokens of a tile, where a page holds whole eights.
+            auto eight = [&](uint32_t t) {
+                return __builtin_amdgcn_readfirstlane(min(t * kTile + 8 * wave, s.len - 1) & ~7u);
+            };
+            auto position = [&](uint32_t t) { return min(t * kTile + btok, s.len - 1); };
+            auto page_of = [&](uint32_t t) {
+                const uint32_t p = DIRECT ? eight(t) : position(t);
+                return a.pages.table[(size_t)n * a.pages.width + p / a.pages.page];
+            };
+            auto row_of = [&](uint32_t p, uint32_t id) {
+                bad_page |= id >= a.pages.pages;
+                if (id >= a.pages.pages) id = 0;
+                return a.pool + ((size_t)id * a.pages.page + p % a.pages.page) * a.pages.row.bytes;
+            };
+            constexpr int UNITS = F == K3X_CACHE_MXFP8   ? LP / 128
+                                  : F == K3X_CACHE_MXFP4 ? LP / 256
+                                  : DIRECT               ? 1
+                                                         : LP / 64;
+            u32x4 codes[UNITS], scales, turned;
+            // Loads of a tile: straight to buffer b, or to registers.
+            auto bring = [&](uint32_t t, uint32_t b, uint32_t id) {
+                if constexpr (DIRECT) {
+                    // Eight tokens a wave, each load 128 bytes of every one.
+                    const uint32_t p = eight(t);
+                    const uint8_t* row = row_of(p, __builtin_amdgcn_readfirstlane(id));
+                    const auto rows8 = __builtin_amdgcn_make_buffer_rsrc(
+                        const_cast<uint8_t*>(row), 0, 8 * a.pages.row.bytes, 0x00020000);
+                    const uint32_t from = (position(t) - p) * a.pages.row.bytes + bput * 16;
+                    u32x4* dst = reinterpret_cast<u32x4*>(smem + b * kBuffer + wave * 1024);
+#pragma unroll
+                    for (int c = 0; c < CG - 1; ++c)
+                        load_lds16(rows8, dst + c * (kGroup / 16), from, c * 128);
+                    if (bput < a.R / 8)
+                        load_lds16(rows8, dst + (CG - 1) * (kGroup / 16), from, LP * 2);
+                } else {
+                    const uint8_t* row = row_of(position(t), id);
+#pragma unroll
+                    for (int k = 0; k < UNITS; ++k) {
+                        const uint32_t u = bcol + 8 * k;
+                        codes[k] = FULL || u * 16 < a.pages.row.codes
+                                       ? *reinterpret_cast<const u32x4*>(row + u * 16) : u32x4{};
+                    }
+                    if constexpr (F != K3X_CACHE_16BIT)
+                        scales = *reinterpret_cast<const u32x4*>(row + a.pages.row.scales);
+                    if (bcol < a.R / 8)
+                        turned = *reinterpret_cast<const u32x4*>(row + a.pages.row.codes + bcol * 16);
+                }
+            };
+            // Codes in registers to the values that they stand for in buffer b.
+            auto put = [&](uint32_t b) {
+                if constexpr (!DIRECT) {
+                    uint8_t* dst = smem + b * kBuffer + btok * 128;
+                    const uint32_t z = swizzle(lane / 8);
+#pragma unroll
+                    for (int k = 0; k < UNITS; ++k) {
+                        const uint32_t u = bcol + 8 * k;
+                        if constexpr (F == K3X_CACHE_16BIT) {
+                            if (u * 8 < a.L)
+                                *reinterpret_cast<u32x4*>(dst + k * kGroup + (bcol ^ z) * 16) = codes[k];
+                        } else if constexpr (F == K3X_CACHE_MXFP8) {
+                            const float sc = e8m0_to_f32(scales[k] >> (bcol / 2 * 8) & 0xff);
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const uint32_t x = 2 * (u % 4) + j;
+                                if (FULL || u * 16 < a.L)
+                                    *reinterpret_cast<bf16x8*>(dst + u / 4 * kGroup + (x ^ z) * 16) =
+                                        mxfp8_8(uint2{codes[k][2 * j], codes[k][2 * j + 1]}, sc);
+                            }
+                        } else {
+                            const uint32_t dw = bcol / 4 ? scales[2 * k + 1] : scales[2 * k];
+                            const float sc = e8m0_to_f32(dw >> (bcol % 4 * 8) & 0xff);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const uint32_t x = 4 * (u % 2) + j;
+                                if (FULL || u * 32 < a.L)
+                                    *reinterpret_cast<bf16x8*>(dst + u / 2 * kGroup + (x ^ z) * 16) =
+                                        dequant8(codes[k][j], sc);
+                            }
+                        }
+                    }
+                    if (bcol < a.R / 8)
+                        *reinterpret_cast<u32x4*>(dst + (CG - 1) * kGroup + (bcol ^ z) * 16) = turned;
+                }
+            };
+
+            // ---- one tile ---------------------------------------------------
+            auto tile = [&](uint32_t t, uint32_t b) {
+                const lds_byte* kb = lds + b * kBuffer;
+                // Operands of the next group of columns (or tile of the latent) are read
+                // beside the products of this one, and no further ahead: the scheduler
+                // would read all of them first, past the registers there are.
+                constexpr int XT = HT == 32 ? 1 : 2;
+                Acc sc[XT];
+#pragma unroll
+                for (int i = 0; i < XT; ++i) sc[i] = Acc{};
+                u32x4 kf[2][KS][XT];
+                const uint32_t kat = opaque(kat0);
+                auto keys = [&](int c) {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i)
+#pragma unroll
+                        for (int x = 0; x < XT; ++x)
+                            kf[c & 1][i][x] = lds16(kb + c * kGroup + x * 2048 + (kat ^ i * (128 / KS)));
+                };
+                auto products = [&](int c) {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i)
+#pragma unroll
+                        for (int x = 0; x < XT; ++x)
+                            sc[x] = M::run(kf[c & 1][i][x], qf[c * KS + i], sc[x]);
+                };
+                if (a.R) {
+                    keys(CG - 1);
+                    products(CG - 1);
+                }
+                keys(0);
+#pragma unroll
+                for (int c = 0; c < CG - 1; ++c) {
+                    if (c + 1 < CG - 1) keys(c + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    products(c);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                constexpr int NV = HT == 32 ? 16 : 8;
+                float x[NV];
+#pragma unroll
+                for (int i = 0; i < NV; ++i) x[i] = HT == 32 ? sc[0][i] : sc[i / 4][i % 4];
+                if ((int32_t)((t + 1) * kTile) > sees_least) {
+                    // Past what the row sees.
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        const int32_t tok = (int32_t)(t * kTile) +
+                                            (HT == 32 ? 8 * (i / 4) + 4 * (int)g + i % 4
+                                                      : 16 * (i / 4) + 4 * (int)g + i % 4);
+                        if (tok >= sees) x[i] = -__builtin_inff();
+                    }
+                }
+                float top = x[0];
+#pragma unroll
+                for (int i = 1; i < NV; ++i) top = fmaxf(top, x[i]);
+                top = across<HT>(top, [](float p, float r) { return fmaxf(p, r); }) * a.rate;
+                // The maximum that weights are taken from may lag by 2^8: sums and
+                // outputs keep their bits, and are seldom multiplied again.
+                if (__any(top > m + 8.0f)) {
+                    const float up = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - up);
+                    m = up;
+                    l *= keep;
+                    scale_all<OT>(o, keep);
+                }
+                uint32_t p[NV / 2];
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NV; i += 2) {
+                    const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.rate, -m));
+                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], a.rate, -m));
+                    sum += u + v;
+                    p[i / 2] = pack2<DT>(u, v);
+                }
+                l += sum;
+                constexpr int HV = HT == 32 ? 2 : 1;
+                u32x4 vf[2][HV];
+                const uint32_t vat = opaque(vat0);
+                auto values = [&](int y) {
+                    const uint32_t d = y + wd * OT;  // tile of HT columns of the latent
+                    const lds_byte* vb = kb + d * HT / 64 * kGroup + (vat ^ y % (64 / HT) * (HT * 2));
+#pragma unroll
+                    for (int h = 0; h < HV; ++h) {
+                        // Tokens 16 h .. 16 h + 15 (or all 32), by fours of each half.
+                        const uint2 v0 = lds_transposed(vb + h * 2048);
+                        const uint2 v1 = lds_transposed(vb + h * 2048 + (HT == 32 ? 1024 : 2048));
+                        vf[y & 1][h] = u32x4{v0.x, v0.y, v1.x, v1.y};
+                    }
+                };
+                values(0);
+#pragma unroll
+                for (int y = 0; y < OT; ++y) {
+                    if (y + 1 < OT) values(y + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int h = 0; h < HV; ++h)
+                        o[y] = M::run(vf[y & 1][h],
+                                      u32x4{p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]},
+                                      o[y]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+
+            // ---- the piece's tiles --------------------------------------------
+            if (t0 < end) {
+                if constexpr (DIRECT) {
+                    // BUFS - 1 tiles on their way.  When one is used, the loads of the
+                    // later ones may be outstanding, and no others are behind its own.
+                    uint32_t id = page_of(t0), next;
+#pragma unroll
+                    for (uint32_t i = 0; i < BUFS - 1; ++i) {
+                        next = page_of(min(t0 + i + 1, end - 1));
+                        bring(min(t0 + i, end - 1), i, id);
+                        id = next;
+                    }
+                    uint32_t b = 0;
+                    for (uint32_t t = t0; t < end; ++t) {
+                        if (a.R) wait_loads<(BUFS - 2) * CG>();
+                        else wait_loads<(BUFS - 2) * (CG - 1)>();
+                        barrier();
+                        next = page_of(min(t + BUFS, end - 1));
+                        bring(min(t + BUFS - 1, end - 1), b >= 1 ? b - 1 : BUFS - 1, id);
+                        id = next;
+                        tile(t, b);
+                        b = b + 1 == BUFS ? 0 : b + 1;
+                    }
+                    wait_loads<0>();
+                    barrier();
+                } else {
+                    uint32_t id = page_of(t0), next = page_of(min(t0 + 1, end - 1));
+                    bring(t0, 0, id);
+                    put(0);
+                    bring(min(t0 + 1, end - 1), 0, next);
+                    next = page_of(min(t0 + 2, end - 1));
+                    uint32_t b = 0;
+                    for (uint32_t t = t0; t < end; ++t) {
+                        barrier();
+                        put(b ^ 1);
+                        bring(min(t + 2, end - 1), 0, next);
+                        next = page_of(min(t + 3, end - 1));
+                        tile(t, b);
+                        b ^= 1;
+                    }
+                    barrier();
+                }
+            }
+
+            // ---- out ----------------------------------------------------------
+            l = across<HT>(l, [](float p, float r) { return p + r; });
+            const bool live = r0 + wm * HT + col < rows;
+            const float inv = !whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+            const uint32_t re = min(r0 + wm * HT + opaque(col), rows - 1);
+            const uint64_t row = s.begin + re / a.H;
+            const uint32_t head = re % a.H;
+            uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.os + (uint64_t)head * a.L;
+            const size_t piece = ((size_t)w * a.RB + rb) * 2 + (t0 ? 0 : 1);
+            constexpr int Q = HT == 32 ? 4 : 1;
+            float4* part = a.parts + piece * (S::rows * LP / 4) + wave * OT * Q * 64 + lane;
+            float check = l * 0.0f;  // NaN once something is not finite
+#pragma unroll
+            for (int y = 0; y < OT; ++y) {
+#pragma unroll
+                for (int i = 0; i < Q; ++i) {
+                    const uint32_t d = (y + wd * OT) * HT + 8 * i + 4 * g;
+                    const float4 v{o[y][4 * i] * inv, o[y][4 * i + 1] * inv,
+                                   o[y][4 * i + 2] * inv, o[y][4 * i + 3] * inv};
+                    if (FULL || d < a.L) {
+                        check = __builtin_fmaf(v.x, 0.0f, check);
+                        check = __builtin_fmaf(v.y, 0.0f, check);
+                        check = __builtin_fmaf(v.z, 0.0f, check);
+                        check = __builtin_fmaf(v.w, 0.0f, check);
+                        if (!whole) part[(y * Q + i) * 64] = v;
+                        else if (live)
+                            *reinterpret_cast<uint2*>(out + d) =
+                                uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            bad_value |= live && !(check == 0.0f);
+            if (g == 0 && wd == 0) {
+                if (!whole)
+                    a.sums[piece * S::rows + wm * HT + col] = float2{m, l};
+                else if (a.lse && live)
+                    a.lse[row * a.H + head] =
+                        l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
+                                 : -__builtin_inff();
             }
         }
-        red[tid] = x;
-        __syncthreads();
-        float top = m;
-        for (uint32_t i = 0; i < kThreads; ++i) top = fmaxf(top, red[i]);
-        w[tid] = expf(x - top);
-        __syncthreads();
-        const float keep = expf(m - top);
-        m = top;
-        l *= keep;
-        o[0] *= keep;
-        o[1] *= keep;
-        for (uint32_t i = 0; i < min(kThreads, sees - at); ++i) {
-            l += w[i];
-            const uint8_t* row = cached_row(a.pages, const_cast<uint8_t*>(a.pool), n, at + i);
-            if (!row) continue;
-            for (uint32_t j = 0; j < 2; ++j)
-                if (tid + j * kThreads < a.L)
-                    o[j] = __builtin_fmaf(w[i], cached<DT>(a, row, tid + j * kThreads), o[j]);
+        first += tiles;
+        ++n;
+        if (first >= to) break;
+    }
+    if (bad_page) latch(a.status, K3X_ERR_INVALID_STATE);
+    if (bad_value) latch(a.status, K3X_ERR_INVALID_MXFP4);
+}
+
+// Joins the pieces of a sequence that lies in several ranges, 64 float4 as a
+// wave of the first launch held them: a wave each, or (FOUR, for many pieces) four
+// waves, each every fourth piece.
+template <uint32_t DT, int LP, typename S, bool FOUR>
+__global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
+    constexpr int HT = S::HT, WD = S::WD;
+    constexpr uint32_t kSlices = S::rows * LP / (FOUR ? 256 : 1024);
+    constexpr uint32_t NF = LP / HT / WD * (HT == 32 ? 4 : 1);
+    __shared__ float4 os[FOUR ? 4 : 1][64];
+    __shared__ float ls[FOUR ? 4 : 1][64];
+    const uint32_t slice = blockIdx.x % kSlices, x = blockIdx.x / kSlices;
+    const uint32_t rb = x % a.RB, lane = threadIdx.x & 63, quarter = threadIdx.x / 64;
+    if (*(volatile uint32_t*)a.status) return;
+    const Split s = a.splits[x / a.RB];
+    const uint32_t rows = s.count * a.H;
+    if (!s.pieces || rb * S::rows >= rows) return;
+    const uint32_t f = FOUR ? slice : slice * 4 + quarter, wave = f / NF, i = f % NF;
+    const uint32_t wm = wave / WD, wd = wave % WD;
+    const uint32_t at = wm * HT + lane % HT, r = rb * S::rows + at;
+    const uint32_t d = HT == 32 ? wd * (LP / WD) + i / 4 * 32 + i % 4 * 8 + lane / 32 * 4
+                                : wd * (LP / WD) + i * 16 + lane / 16 * 4;
+    const bool live = r < rows && d < a.L;
+    auto piece = [&](uint32_t p) { return ((size_t)(s.w + p) * a.RB + rb) * 2 + (p ? 0 : 1); };
+    float m = -3.4028235e38f;
+    for (uint32_t p = 0; p < s.pieces; ++p) m = fmaxf(m, a.sums[piece(p) * S::rows + at].x);
+    float l = 0.0f;
+    float4 o{};
+    constexpr uint32_t kStep = FOUR ? 4 : 1, kAhead = 4;
+    for (uint32_t p0 = FOUR ? quarter : 0; p0 < s.pieces; p0 += kStep * kAhead) {
+        float2 ml[kAhead];
+        float4 v[kAhead];
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            const size_t q = piece(min(p0 + j * kStep, s.pieces - 1));
+            ml[j] = a.sums[q * S::rows + at];
+            v[j] = live ? a.parts[q * (S::rows * LP / 4) + f * 64 + lane] : float4{};
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            // A piece that the row does not see has no sum, and may hold no outputs.
+            if (p0 + j * kStep >= s.pieces || !(ml[j].y > 0.0f)) continue;
+            const float k = __builtin_amdgcn_exp2f(ml[j].x - m);
+            l = __builtin_fmaf(ml[j].y, k, l);
+            o.x = __builtin_fmaf(v[j].x, k, o.x);
+            o.y = __builtin_fmaf(v[j].y, k, o.y);
+            o.z = __builtin_fmaf(v[j].z, k, o.z);
+            o.w = __builtin_fmaf(v[j].w, k, o.w);
         }
     }
-    E* out = static_cast<E*>(a.out) + t * a.os + (size_t)h * a.L;
-    for (uint32_t j = 0; j < 2; ++j)
-        if (tid + j * kThreads < a.L) {
-            const float v = sees ? o[j] / l : 0.0f;
-            if (!(fabsf(v) < __builtin_inff())) latch(a.status, K3X_ERR_INVALID_MXFP4);
-            out[tid + j * kThreads] = Elem<DT>::store(v);
+    if constexpr (FOUR) {
+        os[quarter][lane] = o;
+        ls[quarter][lane] = l;
+        __syncthreads();
+        if (quarter) return;
+#pragma unroll
+        for (int j = 1; j < 4; ++j) {
+            l += ls[j][lane];
+            o.x += os[j][lane].x;
+            o.y += os[j][lane].y;
+            o.z += os[j][lane].z;
+            o.w += os[j][lane].w;
         }
-    if (a.lse && tid == 0)
-        a.lse[(size_t)t * a.H + h] = sees ? m + logf(l) : -__builtin_inff();
+    }
+    if (!live) return;
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const uint64_t t = s.begin + r / a.H;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.os + (uint64_t)(r % a.H) * a.L + d;
+    *reinterpret_cast<uint2*>(out) = uint2{pack2<DT>(o.x * inv, o.y * inv),
+                                           pack2<DT>(o.z * inv, o.w * inv)};
+    if (a.lse && d == 0)
+        a.lse[t * a.H + r % a.H] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
+                                            : -__builtin_inff();
+}
+
+// How a call is laid out: rows of a workgroup, ranges, row blocks.
+struct Plan {
+    uint32_t rows, G, RB, LP;
+    bool full;
+};
+Plan plan_of(const k3x_hip_mla_params* p) {
+    Plan x;
+    const uint64_t most = (uint64_t)(p->longest ? p->longest : p->tokens) * p->heads;
+    x.LP = p->latent <= 256 ? 256 : 512;
+    x.rows = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : 128;
+    x.full = p->latent == x.LP && (p->cache_format != K3X_CACHE_16BIT || p->page_size % 8 == 0);
+    if (!x.full && x.rows > 16) x.rows = 64;  // the others: two shapes
+    x.RB = (uint32_t)std::max<uint64_t>(1, (most + x.rows - 1) / x.rows);
+    // Two workgroups a compute unit where registers and LDS allow.
+    const uint32_t places = x.rows == 16 ? 512 : 256;
+    x.G = std::max(1u, places / x.RB);
+    if (x.G >= 8) x.G -= x.G % 8;
+    return x;
+}
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+template <uint32_t DT, uint32_t F, int LP, typename S, bool FULL>
+int launch(k3x_hip_ctx* ctx, const AttentionArgs& a) {
+    constexpr int BUFS = F == K3X_CACHE_16BIT && FULL && S::rows > 16 ? 3 : 2;
+    hipLaunchKernelGGL((mla_attention_kernel<DT, F, LP, S, BUFS, FULL>), dim3(a.G * a.RB),
+                       dim3(kThreads), 0, ctx->stream, a);
+    const uint32_t splits = std::min(a.G, a.pages.N) * a.RB;
+    if (a.G / a.pages.N >= 8)
+        hipLaunchKernelGGL((mla_join_kernel<DT, LP, S, true>), dim3(splits * (S::rows * LP / 256)),
+                           dim3(kThreads), 0, ctx->stream, a);
+    else
+        hipLaunchKernelGGL((mla_join_kernel<DT, LP, S, false>),
+                           dim3(splits * (S::rows * LP / 1024)), dim3(kThreads), 0, ctx->stream, a);
+    return launched(ctx, 2);
+}
+
+template <uint32_t DT, uint32_t F, int LP>
+int launch_shape(k3x_hip_ctx* ctx, const AttentionArgs& a, const Plan& x) {
+    if (!x.full)
+        return x.rows == 16 ? launch<DT, F, LP, Shape<16, 1, 4>, false>(ctx, a)
+                            : launch<DT, F, LP, Shape<32, 2, 2>, false>(ctx, a);
+    switch (x.rows) {
+        case 16: return launch<DT, F, LP, Shape<16, 1, 4>, true>(ctx, a);
+        case 32: return launch<DT, F, LP, Shape<32, 1, 4>, true>(ctx, a);
+        case 64: return launch<DT, F, LP, Shape<32, 2, 2>, true>(ctx, a);
+        default: return launch<DT, F, LP, Shape<32, 4, 1>, true>(ctx, a);
+    }
+}
+template <uint32_t DT, uint32_t F>
+int launch_width(k3x_hip_ctx* ctx, const AttentionArgs& a, const Plan& x) {
+    return x.LP == 256 ? launch_shape<DT, F, 256>(ctx, a, x) : launch_shape<DT, F, 512>(ctx, a, x);
+}
+
+bool attention_ok(const k3x_hip_mla_params* p) {
+    if (!mla_ok(p)) return false;
+    const Plan x = plan_of(p);
+    return (uint64_t)x.G * x.RB * (x.rows * x.LP / 256) * kThreads < (1ull << 32);
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t k3x_hip_mla_attention_workspace(const k3x_hip_mla_params* p) { return 0; }
+size_t k3x_hip_mla_attention_workspace(const k3x_hip_mla_params* p) {
+    if (!p || !attention_ok(p)) return 0;
+    const Plan x = plan_of(p);
+    const size_t pieces = (size_t)x.G * x.RB * 2;
+    return up256(x.G * sizeof(Split)) + up256(pieces * x.rows * sizeof(float2)) +
+           pieces * x.rows * x.LP * sizeof(float);
+}
 
 int k3x_hip_mla_attention(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const void* q,
                           const void* pool, const uint32_t* table, const uint32_t* offsets,
                           const uint32_t* lens, void* out, float* lse, void* workspace,
                           size_t workspace_bytes) {
-    if (!ctx || !p || !mla_ok(p) || !q || !pool || !table || !lens || !out ||
+    if (!ctx || !p || !attention_ok(p) || !q || !pool || !table || !lens || !out ||
         p->q_stride % 8 || p->out_stride % 8)
         return K3X_ERR_INVALID_EXTENT;
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(pool, 256) || !aligned(table, 4) ||
         !aligned(offsets, 4) || !aligned(lens, 4) || !aligned(lse, 4))
         return K3X_ERR_INVALID_EXTENT;
+    if (!workspace || !aligned(workspace, 256) ||
+        workspace_bytes < k3x_hip_mla_attention_workspace(p))
+        return K3X_ERR_INVALID_EXTENT;
     if (hipSetDevice(ctx->device) != hipSuccess) return K3X_ERR_BACKEND_UNAVAILABLE;
+    const Plan x = plan_of(p);
     AttentionArgs a{};
     a.pages = pages_of(p, table, offsets, lens);
     a.q = q;
@@ -124,18 +776,26 @@ int k3x_hip_mla_attention(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const v
     a.H = p->heads;
     a.L = p->latent;
     a.R = p->rotary;
-    a.F = p->cache_format;
     a.qs = p->q_stride ? p->q_stride : (uint64_t)p->heads * (p->latent + p->rotary);
     a.os = p->out_stride ? p->out_stride : (uint64_t)p->heads * p->latent;
-    a.scale = p->scale;
+    a.rate = p->scale * 1.4426950408889634f;
+    a.G = x.G;
+    a.RB = x.RB;
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    const size_t pieces = (size_t)x.G * x.RB * 2;
+    a.splits = reinterpret_cast<Split*>(w);
+    w += up256(x.G * sizeof(Split));
+    a.sums = reinterpret_cast<float2*>(w);
+    w += up256(pieces * x.rows * sizeof(float2));
+    a.parts = reinterpret_cast<float4*>(w);
     a.status = ctx->status;
     if (!p->tokens) return K3X_OK;
-    const dim3 grid(p->tokens * p->heads), block(kThreads);
-    if (p->dtype == K3X_DTYPE_F16)
-        hipLaunchKernelGGL(mla_attention_kernel<K3X_DTYPE_F16>, grid, block, 0, ctx->stream, a);
-    else
-        hipLaunchKernelGGL(mla_attention_kernel<K3X_DTYPE_BF16>, grid, block, 0, ctx->stream, a);
-    return launched(ctx, 1);
+    if (p->dtype == K3X_DTYPE_F16) return launch_width<K3X_DTYPE_F16, K3X_CACHE_16BIT>(ctx, a, x);
+    switch (p->cache_format) {
+        case K3X_CACHE_16BIT: return launch_width<K3X_DTYPE_BF16, K3X_CACHE_16BIT>(ctx, a, x);
+        case K3X_CACHE_MXFP8: return launch_width<K3X_DTYPE_BF16, K3X_CACHE_MXFP8>(ctx, a, x);
+        default: return launch_width<K3X_DTYPE_BF16, K3X_CACHE_MXFP4>(ctx, a, x);
+    }
 }
 
 }  // extern "C"
