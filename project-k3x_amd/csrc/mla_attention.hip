@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "k3x_mla.hpp"
+#include "k3x_mla_mma.hpp"
 
 using namespace k3x_dev;
 using namespace k3x_ops;
@@ -53,71 +54,12 @@ struct AttentionArgs {
     uint32_t* status;
 };
 
-// Which columns of 16 bytes are exchanged in token t of a tile's 64-column group,
-// so that neither product's reads of it meet in a bank: eight tokens' same column
-// (keys), and four tokens' two neighbours (values).
-__device__ inline uint32_t swizzle(uint32_t t) { return (t & 3) << 1 | (t >> 2 & 1); }
-
 // Rows a wave and how the waves lie: WM row blocks by WD parts of the latent.
 template <int HT_, int WM_, int WD_>
 struct Shape {
     static constexpr int HT = HT_, WM = WM_, WD = WD_;
     static constexpr int rows = HT * WM;
 };
-
-template <uint32_t DT, int HT>
-struct Mma;
-template <uint32_t DT>
-struct Mma<DT, 32> {
-    typedef __attribute__((ext_vector_type(16))) float Acc;
-    static __device__ inline Acc run(u32x4 a, u32x4 b, Acc c) {
-        typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
-        if constexpr (DT == K3X_DTYPE_BF16)
-            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                           __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-        else
-            return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
-                                                          __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    }
-};
-template <uint32_t DT>
-struct Mma<DT, 16> {
-    typedef f32x4 Acc;
-    static __device__ inline Acc run(u32x4 a, u32x4 b, Acc c) {
-        typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
-        if constexpr (DT == K3X_DTYPE_BF16)
-            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                           __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-        else
-            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
-                                                          __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    }
-};
-
-// Two values as the type's bits, the first in the low half.
-template <uint32_t DT>
-__device__ inline uint32_t pack2(float a, float b) {
-    typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-    if constexpr (DT == K3X_DTYPE_BF16)
-        return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
-    else
-        return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
-}
-
-// Over the lanes that hold one row's scores: the halves, and for 16 rows the
-// 16-lane rows too.
-template <int HT, typename Op>
-__device__ inline float across(float x, Op op) {
-    const uint32_t u = __float_as_uint(x);
-    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    x = op(__uint_as_float(h[0]), __uint_as_float(h[1]));
-    if constexpr (HT == 16) {
-        const uint32_t w = __float_as_uint(x);
-        const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-        x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    }
-    return x;
-}
 
 // o *= k.  Results that fill half of the register file and more stay in its
 // accumulators, which no other instruction multiplies: each goes through one
@@ -146,31 +88,6 @@ __device__ __forceinline__ void scale_all(Acc (&o)[OT], float k) {
         asm volatile("s_nop 15" ::: "memory");
     }
 }
-
-// x, as a value that is not computed ahead of the place and held until then.
-__device__ inline uint32_t opaque(uint32_t x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
-
-typedef __attribute__((address_space(3))) uint8_t lds_byte;
-
-__device__ inline u32x4 lds16(const lds_byte* p) {
-    return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(p);
-}
-// Of a 16-lane row's four tokens by 16 columns, its lane's column.
-__device__ inline uint2 lds_transposed(const lds_byte* p) {
-    typedef __attribute__((ext_vector_type(4))) short s16x4;
-    return __builtin_bit_cast(
-        uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                   (__attribute__((address_space(3))) s16x4*)const_cast<lds_byte*>(p)));
-}
-
-template <int N>
-__device__ inline void wait_loads() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-__device__ inline void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Tiles of a sequence in the line; an empty one takes one, in which its rows are
 // written as empty.

@@ -1,24 +1,36 @@
 // mla_prompt.hip -- attention of prompts over expanded keys and values, with a
 // part of the key that all heads share.
+//
+// S^T = K Q^T and O^T = V^T P^T on the matrix cores, as in mla_attention.hip: the
+// result of the first product is, lane for lane, the second one's operand.  A
+// wave holds 32 queries of one head and their outputs; the tiles of K and V of a
+// workgroup's head lie in LDS, brought straight from memory a tile ahead.  Blocks
+// of queries run from the last to the first, whose work under a causal mask is
+// the least.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "k3x_mla.hpp"
+#include "k3x_mla_mma.hpp"
 
 using namespace k3x_dev;
 using namespace k3x_ops;
+using namespace k3x_mla;
 
 namespace {
 
 constexpr uint32_t kThreads = 256;
+constexpr uint32_t kRows = 128;  // queries a workgroup
 
 struct PromptArgs {
     const void *q, *k, *v, *rotary;
     const uint32_t *offsets, *key_offsets;
     void* out;
     float* lse;
-    uint32_t N, T, S, H, Dn, R, Dv, causal;
+    uint32_t N, T, S, H, Dn, R, Dv, causal, blocks;
     uint64_t qs, ks, vs, rs, os, kh, vh;
-    float scale;
+    float rate;  // scale * log2(e)
     uint32_t* status;
 };
 
@@ -46,66 +58,240 @@ __device__ inline bool ranges_of(const PromptArgs& a, uint32_t n, Ranges* r) {
     return e >= b && e <= a.T && g >= f && g <= a.S;
 }
 
-// A workgroup a query and head: 256 keys at a time.
-template <uint32_t DT>
-__global__ __launch_bounds__(kThreads) void mla_prompt_kernel(PromptArgs a) {
-    typedef typename Elem<DT>::type E;
-    __shared__ float q[192], w[kThreads], red[kThreads];
-    __shared__ uint32_t owner;
-    const uint32_t tid = threadIdx.x, t = blockIdx.x / a.H, h = blockIdx.x % a.H;
+// KD columns of a key and VD of a value at most, in groups of 64 in LDS.  FULL:
+// Dn and R are whole groups and Dv is VD, so that nothing is left out.
+template <uint32_t DT, int KD, int VD, int TILE, bool FULL>
+__global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
+    constexpr int KG = KD / 64, VG = VD / 64, ST = TILE / 32, OT = VD / 32;
+    constexpr uint32_t kGroup = TILE * 128;      // bytes of a group
+    constexpr uint32_t kBuffer = (KG + VG) * kGroup;
+    typedef Mma<DT, 32> M;
+    typedef typename M::Acc Acc;
+    // One array: see mla_attention.hip.
+    __shared__ __attribute__((aligned(256))) uint8_t smem[2 * kBuffer];
+    uint32_t* const scan = reinterpret_cast<uint32_t*>(smem);  // before the first tile
+    uint32_t* const found = scan + 4;
+    lds_byte* const lds = (lds_byte*)smem;
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t h = blockIdx.x % a.H;
+    const uint32_t block = a.blocks - 1 - blockIdx.x / a.H;
     if (*(volatile uint32_t*)a.status) return;
-    if (tid == 0) owner = a.N;
-    __syncthreads();
-    for (uint32_t n = tid; n < a.N; n += kThreads) {
-        Ranges r;
-        if (!ranges_of(a, n, &r)) latch(a.status, K3X_ERR_INVALID_STATE);
-        else if (t >= r.q && t - r.q < r.m) atomicMin(&owner, n);
+
+    // The sequence that the block is in: blocks of 128 queries, sequence by sequence.
+    if (tid == 0) found[0] = a.N;
+    uint32_t carry = 0;
+    bool bad = false;
+    for (uint32_t base = 0; base < a.N; base += kThreads) {
+        const uint32_t n = base + tid;
+        Ranges r{};
+        if (n < a.N && !ranges_of(a, n, &r)) {
+            bad = true;
+            r.m = 0;
+        }
+        const uint32_t own = (r.m + kRows - 1) / kRows;
+        uint32_t c = own;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(c, d);
+            if (lane >= (uint32_t)d) c += o;
+        }
+        __syncthreads();
+        if (lane == 63) scan[wave] = c;
+        __syncthreads();
+        for (uint32_t i = 0; i < wave; ++i) c += scan[i];
+        c += carry;  // with the thread's own
+        if (own && block >= c - own && block < c) {
+            found[0] = n;
+            found[1] = block - (c - own);
+        }
+        carry += scan[0] + scan[1] + scan[2] + scan[3];
     }
+    if (blockIdx.x == 0 && bad) latch(a.status, K3X_ERR_INVALID_STATE);
     __syncthreads();
-    if (owner >= a.N) return;
+    const uint32_t n = found[0], i0 = found[1] * kRows;
+    if (n >= a.N) return;
     Ranges s;
-    ranges_of(a, owner, &s);
-    const int64_t p = a.causal ? (int64_t)s.n - s.m + (t - s.q) + 1 : s.n;
-    const uint32_t sees = p < 0 ? 0 : (uint32_t)p;
-    const uint32_t D = a.Dn + a.R;
-    const E* qr = static_cast<const E*>(a.q) + t * a.qs + (size_t)h * D;
-    for (uint32_t d = tid; d < D; d += kThreads) q[d] = Elem<DT>::load(qr[d]);
-    float m = -3.4e38f, l = 0.0f, o = 0.0f;
-    for (uint32_t at = 0; at < sees; at += kThreads) {
+    ranges_of(a, n, &s);
+    __syncthreads();
+    if (!FULL) {  // columns that are not brought stay zero
+        for (uint32_t i = tid * 16; i < 2 * kBuffer; i += kThreads * 16)
+            *reinterpret_cast<u32x4*>(smem + i) = u32x4{};
         __syncthreads();
-        float x = -__builtin_inff();
-        if (at + tid < sees) {
-            const size_t row = s.k + at + tid;
-            const E* k = static_cast<const E*>(a.k) + row * a.ks + h * a.kh;
-            const E* r = static_cast<const E*>(a.rotary) + row * a.rs;
-            x = 0.0f;
-            for (uint32_t d = 0; d < D; ++d)
-                x = __builtin_fmaf(q[d], Elem<DT>::load(d < a.Dn ? k[d] : r[d - a.Dn]), x);
-            x *= a.scale;
+    }
+
+    const uint32_t col = lane & 31, g = lane >> 5;
+    const uint32_t i = min(i0 + 32 * wave + col, s.m - 1);  // the lane's query
+    const int32_t hidden = a.causal ? (int32_t)(s.m - 1) : 0;  // keys of the first query's future
+    auto sees_of = [&](uint32_t x) {
+        return a.causal ? (int32_t)s.n - hidden + (int32_t)x : (int32_t)s.n;
+    };
+    const int32_t sees = sees_of(i);
+    const int32_t least = sees_of(min(i0 + 32 * wave, s.m - 1));  // of the wave
+    const int32_t most = sees_of(min(i0 + kRows - 1, s.m - 1));   // of the workgroup
+    const uint32_t tiles = most > 0 ? ((uint32_t)most + TILE - 1) / TILE : 0;
+
+    const uint32_t kat0 = col * 128 + (g ^ swizzle(col)) * 16;
+    const uint32_t i16 = lane & 15, vrow = 4 * g + i16 / 4;
+    const uint32_t vat0 = vrow * 128 + ((2 * (lane >> 4 & 1) + (i16 & 3) / 2) ^ swizzle(vrow)) * 16 +
+                          (i16 & 1) * 8;
+    // What the lane brings: token 8 (wave + 4 x) + lane / 8 of a tile, 16 bytes a group.
+    const uint32_t btok = 8 * wave + lane / 8, bput = lane % 8 ^ swizzle(lane / 8);
+
+    u32x4 qf[KG * 4];
+    {
+        const uint8_t* q = static_cast<const uint8_t*>(a.q) +
+                           2 * ((uint64_t)(s.q + i) * a.qs + (uint64_t)h * (a.Dn + a.R));
+        // Groups of the head's own columns, then those of the rotary part.
+        const uint32_t own = (a.Dn + 63) / 64;
+#pragma unroll
+        for (int c = 0; c < KG; ++c)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const bool mine = (uint32_t)c < own;
+                const uint32_t d = (mine ? c * 64 : (c - own) * 64) + x * 16 + g * 8;
+                const bool in = FULL ? mine || d < a.R : d < (mine ? a.Dn : a.R);
+                const u32x4 y = *reinterpret_cast<const u32x4*>(
+                    q + (in ? 2 * (mine ? d : a.Dn + d) : 0));
+                qf[c * 4 + x] = y & (in ? 0xffffffffu : 0u);
+            }
+    }
+    Acc o[OT];
+#pragma unroll
+    for (int x = 0; x < OT; ++x) o[x] = Acc{};
+    float m = -3.4028235e38f, l = 0.0f;
+
+    const uint32_t own = (a.Dn + 63) / 64;
+    auto bring = [&](uint32_t t, uint32_t b) {
+#pragma unroll
+        for (int x = 0; x < TILE / 32; ++x) {
+            // Eight tokens a wave and load, from the first of the eight.
+            const uint32_t p = min(t * TILE + 32 * x + 8 * wave, s.n - 1);
+            const uint32_t to = min(t * TILE + 32 * x + btok, s.n - 1) - p;
+            const uint64_t row = s.k + p;
+            u32x4* dst = reinterpret_cast<u32x4*>(smem + b * kBuffer + x * 4096 + wave * 1024);
+            auto rows8 = [&](const void* base, uint64_t stride, uint64_t at) {
+                return __builtin_amdgcn_make_buffer_rsrc(
+                    static_cast<uint8_t*>(const_cast<void*>(base)) + 2 * (row * stride + at), 0,
+                    0xffffffffu, 0x00020000);
+            };
+            const auto kr = rows8(a.k, a.ks, h * a.kh), vr = rows8(a.v, a.vs, h * a.vh);
+            const uint32_t kf = to * (uint32_t)(2 * a.ks) + bput * 16;
+            const uint32_t vf = to * (uint32_t)(2 * a.vs) + bput * 16;
+#pragma unroll
+            for (int c = 0; c < KG; ++c)
+                if ((uint32_t)c < own && (FULL || c * 8 + bput < a.Dn / 8))
+                    load_lds16(kr, dst + c * (kGroup / 16), kf, c * 128);
+            if (bput < a.R / 8) {
+                const auto rr = rows8(a.rotary, a.rs, 0);
+                load_lds16(rr, dst + own * (kGroup / 16), to * (uint32_t)(2 * a.rs) + bput * 16, 0);
+            }
+#pragma unroll
+            for (int c = 0; c < VG; ++c)
+                if (FULL || c * 8 + bput < a.Dv / 8)
+                    load_lds16(vr, dst + (KG + c) * (kGroup / 16), vf, c * 128);
         }
-        red[tid] = x;
-        __syncthreads();
-        float top = m;
-        for (uint32_t i = 0; i < kThreads; ++i) top = fmaxf(top, red[i]);
-        w[tid] = expf(x - top);
-        __syncthreads();
-        const float keep = expf(m - top);
-        m = top;
-        l *= keep;
-        o *= keep;
-        for (uint32_t i = 0; i < min(kThreads, sees - at); ++i) {
-            l += w[i];
-            if (tid < a.Dv)
-                o = __builtin_fmaf(w[i], Elem<DT>::load((static_cast<const E*>(a.v) + (size_t)(s.k + at + i) * a.vs + h * a.vh)[tid]), o);
+    };
+
+    auto tile = [&](uint32_t t, uint32_t b) {
+        const lds_byte* kb = lds + b * kBuffer;
+        Acc sc[ST];
+#pragma unroll
+        for (int x = 0; x < ST; ++x) sc[x] = Acc{};
+#pragma unroll
+        for (int c = 0; c < KG; ++c)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int x = 0; x < ST; ++x)
+                    sc[x] = M::run(lds16(kb + c * kGroup + x * 4096 + (kat0 ^ y * 32)),
+                                   qf[c * 4 + y], sc[x]);
+        if ((int32_t)((t + 1) * TILE) > least) {
+            // Past what the query sees.
+#pragma unroll
+            for (int x = 0; x < ST; ++x)
+#pragma unroll
+                for (int y = 0; y < 16; ++y)
+                    if ((int32_t)(t * TILE + 32 * x + 8 * (y / 4) + 4 * g + y % 4) >= sees)
+                        sc[x][y] = -__builtin_inff();
+        }
+        float top = sc[0][0];
+#pragma unroll
+        for (int x = 0; x < ST; ++x)
+#pragma unroll
+            for (int y = 0; y < 16; ++y) top = fmaxf(top, sc[x][y]);
+        top = across<32>(top, [](float p, float r) { return fmaxf(p, r); }) * a.rate;
+        // The maximum may lag by 2^8: see mla_attention.hip.
+        if (__any(top > m + 8.0f)) {
+            const float up = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - up);
+            m = up;
+            l *= keep;
+#pragma unroll
+            for (int x = 0; x < OT; ++x) o[x] *= keep;
+        }
+        uint32_t p[ST][8];
+        float sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < ST; ++x)
+#pragma unroll
+            for (int y = 0; y < 16; y += 2) {
+                const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][y], a.rate, -m));
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][y + 1], a.rate, -m));
+                sum += u + v;
+                p[x][y / 2] = pack2<DT>(u, v);
+            }
+        l += sum;
+#pragma unroll
+        for (int x = 0; x < ST; ++x)
+#pragma unroll
+            for (int y = 0; y < OT; ++y)
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    const lds_byte* vb = kb + (KG + y / 2) * kGroup + x * 4096 + z * 2048 +
+                                         (vat0 ^ y % 2 * 64);
+                    const uint2 v0 = lds_transposed(vb), v1 = lds_transposed(vb + 1024);
+                    o[y] = M::run(u32x4{v0.x, v0.y, v1.x, v1.y},
+                                  u32x4{p[x][4 * z], p[x][4 * z + 1], p[x][4 * z + 2],
+                                        p[x][4 * z + 3]}, o[y]);
+                }
+    };
+
+    if (tiles) {
+        bring(0, 0);
+        for (uint32_t t = 0; t < tiles; ++t) {
+            wait_loads<0>();
+            barrier();
+            if (t + 1 < tiles) bring(t + 1, (t + 1) & 1);
+            tile(t, t & 1);
         }
     }
-    if (tid < a.Dv) {
-        const float v = sees ? o / l : 0.0f;
-        if (!(fabsf(v) < __builtin_inff())) latch(a.status, K3X_ERR_INVALID_MXFP4);
-        (static_cast<E*>(a.out) + t * a.os + (size_t)h * a.Dv)[tid] = Elem<DT>::store(v);
-    }
-    if (a.lse && tid == 0)
-        a.lse[(size_t)t * a.H + h] = sees ? m + logf(l) : -__builtin_inff();
+    l = across<32>(l, [](float p, float r) { return p + r; });
+    const bool live = i0 + 32 * wave + col < s.m;
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const uint64_t row = s.q + i;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.os + (uint64_t)h * a.Dv;
+    float check = l * 0.0f;  // NaN once something is not finite
+#pragma unroll
+    for (int y = 0; y < OT; ++y)
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            const uint32_t d = y * 32 + 8 * z + 4 * g;
+            const float4 v{o[y][4 * z] * inv, o[y][4 * z + 1] * inv, o[y][4 * z + 2] * inv,
+                           o[y][4 * z + 3] * inv};
+            if (FULL || d < a.Dv) {
+                check = __builtin_fmaf(v.x, 0.0f, check);
+                check = __builtin_fmaf(v.y, 0.0f, check);
+                check = __builtin_fmaf(v.z, 0.0f, check);
+                check = __builtin_fmaf(v.w, 0.0f, check);
+                if (live)
+                    *reinterpret_cast<uint2*>(out + d) =
+                        uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+            }
+        }
+    if (live && !(check == 0.0f)) latch(a.status, K3X_ERR_INVALID_MXFP4);
+    if (a.lse && live && g == 0)
+        a.lse[row * a.H + h] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
+                                        : -__builtin_inff();
 }
 
 bool prompt_ok(const k3x_hip_mla_prompt_params* p) {
@@ -124,6 +310,19 @@ bool prompt_ok(const k3x_hip_mla_prompt_params* p) {
            fits(p->rotary_stride, p->rotary) && fits(p->out_stride, H * p->value_dim);
 }
 
+template <uint32_t DT>
+int launch(k3x_hip_ctx* ctx, const PromptArgs& a) {
+    const dim3 grid(a.blocks * a.H), block(kThreads);
+    const bool whole = a.Dn % 64 == 0 && a.R % 64 == 0;
+    if (whole && a.Dn + a.R == 192 && a.Dv == 128)
+        hipLaunchKernelGGL((mla_prompt_kernel<DT, 192, 128, 32, true>), grid, block, 0, ctx->stream, a);
+    else if (whole && a.Dn + a.R == 128 && a.Dv == 128)
+        hipLaunchKernelGGL((mla_prompt_kernel<DT, 128, 128, 32, true>), grid, block, 0, ctx->stream, a);
+    else
+        hipLaunchKernelGGL((mla_prompt_kernel<DT, 192, 128, 32, false>), grid, block, 0, ctx->stream, a);
+    return launched(ctx, 1);
+}
+
 }  // namespace
 
 extern "C" {
@@ -136,7 +335,6 @@ int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* p, con
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(rotary, 16) ||
         !aligned(out, 16) || !aligned(offsets, 4) || !aligned(key_offsets, 4) || !aligned(lse, 4))
         return K3X_ERR_INVALID_EXTENT;
-    if (hipSetDevice(ctx->device) != hipSuccess) return K3X_ERR_BACKEND_UNAVAILABLE;
     PromptArgs a{};
     a.q = q;
     a.k = k;
@@ -161,15 +359,18 @@ int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* p, con
     a.vs = p->v_stride ? p->v_stride : a.H * a.vh;
     a.rs = p->rotary_stride ? p->rotary_stride : a.R;
     a.os = p->out_stride ? p->out_stride : (uint64_t)a.H * a.Dv;
-    a.scale = p->scale;
+    a.rate = p->scale * 1.4426950408889634f;
     a.status = ctx->status;
+    // Blocks of all sequences at most, each with one that is not full; the threads
+    // of a launch, and eight rows apart within 32 bits.
+    a.blocks = a.T / kRows + std::min(a.N, a.T);
+    if ((uint64_t)a.blocks * a.H * kThreads >= (1ull << 32) || a.ks > (1u << 27) ||
+        a.vs > (1u << 27) || a.rs > (1u << 27))
+        return K3X_ERR_INVALID_EXTENT;
+    if (hipSetDevice(ctx->device) != hipSuccess) return K3X_ERR_BACKEND_UNAVAILABLE;
     if (!a.T) return K3X_OK;
-    const dim3 grid(a.T * a.H), block(kThreads);
-    if (p->dtype == K3X_DTYPE_F16)
-        hipLaunchKernelGGL(mla_prompt_kernel<K3X_DTYPE_F16>, grid, block, 0, ctx->stream, a);
-    else
-        hipLaunchKernelGGL(mla_prompt_kernel<K3X_DTYPE_BF16>, grid, block, 0, ctx->stream, a);
-    return launched(ctx, 1);
+    return p->dtype == K3X_DTYPE_F16 ? launch<K3X_DTYPE_F16>(ctx, a)
+                                     : launch<K3X_DTYPE_BF16>(ctx, a);
 }
 
 }  // extern "C"
