@@ -625,8 +625,8 @@ enum k3x_cache_format { K3X_CACHE_16BIT = 0, K3X_CACHE_MXFP8 = 1, K3X_CACHE_MXFP
  * seen.  Rows past offsets[N] are left as they were.
  * Latched as K3X_ERR_INVALID_STATE by every call, which then reads and writes
  * nothing outside its tensors and the pool, and leaves outputs undefined: offsets
- * that fall or pass T, a length past table_width * page_size, a page in use that is
- * not below `pages`, more tokens in a sequence than `longest`. */
+ * that fall or pass T, a length past table_width * page_size or 2^29, a page in use
+ * that is not below `pages`, more tokens in a sequence than `longest`. */
 typedef struct k3x_hip_mla_params {
     uint32_t sequences;    /* N, 1 .. 65535 */
     uint32_t tokens;       /* T, 0 .. 2^22 */
@@ -701,8 +701,9 @@ typedef struct k3x_hip_mla_prompt_params {
     uint32_t longest;   /* queries of the longest sequence if known, 0: not (then T).  Only
                            how the work is laid out: results hold whatever it says. */
     float scale;        /* of the scores, > 0 */
-    /* Elements from row to row, and of k and v from head to head (k and v may be
-     * parts of one projection's rows); multiples of 8; 0: packed. */
+    /* Elements from row to row (of k, v and rotary 2^27 at most), and of k and v from
+     * head to head (k and v may be parts of one projection's rows); multiples of 8;
+     * 0: packed. */
     uint64_t q_stride, k_stride, v_stride, rotary_stride, out_stride;
     uint64_t k_head_stride, v_head_stride;
 } k3x_hip_mla_prompt_params;

@@ -3,6 +3,7 @@
 // cache and the rows in them.
 #pragma once
 
+#include <algorithm>
 #include <cmath>
 
 #include "k3x_ops.hpp"
@@ -27,8 +28,14 @@ inline __host__ __device__ RowLayout row_layout(uint32_t format, uint32_t L, uin
 // The sequences of a call and their pages.
 struct Pages {
     const uint32_t *table, *offsets, *lens;
-    uint32_t N, T, page, pages, width, longest;
+    uint32_t N, T, page, pages, width, longest, most;  // most: positions of a sequence
+    uint32_t page_by, page_shift;  // page_of
     RowLayout row;
+    // p / page for p < 2^31: page_by = ceil(2^page_shift / page) with 2^(page_shift - 31)
+    // >= page, so that its product is off by less than p / 2^page_shift <= 1 / page.
+    __device__ inline uint32_t page_of(uint32_t p) const {
+        return (uint32_t)((uint64_t)p * page_by >> page_shift);
+    }
 };
 
 // Sequence n's rows of the call; false: offsets or length are not fit (latched
@@ -49,7 +56,7 @@ __device__ inline bool tokens_of(const Pages& a, uint32_t n, Tokens* s) {
     s->begin = b;
     s->count = e - b;
     s->len = a.lens[n];
-    return e >= b && e <= a.T && e - b <= a.longest && s->len <= (uint64_t)a.width * a.page;
+    return e >= b && e <= a.T && e - b <= a.longest && s->len <= a.most;
 }
 
 // Latches what tokens_of refuses, by the whole workgroup, which is one of the
@@ -86,9 +93,9 @@ __device__ inline uint32_t sequence_of(const Pages& a, uint32_t t) {
 // Row of position p (below the sequence's length) of a sequence's pages; null
 // where the page is not one of the pool.
 __device__ inline uint8_t* cached_row(const Pages& a, uint8_t* pool, uint32_t n, uint32_t p) {
-    const uint32_t id = a.table[(size_t)n * a.width + p / a.page];
+    const uint32_t page = a.page_of(p), id = a.table[(size_t)n * a.width + page];
     if (id >= a.pages) return nullptr;
-    return pool + ((size_t)id * a.page + p % a.page) * a.row.bytes;
+    return pool + ((size_t)id * a.page + (p - page * a.page)) * a.row.bytes;
 }
 
 // Eight E4M3 codes times a power of two as bf16, exact (four significant bits).
@@ -127,9 +134,13 @@ inline Pages pages_of(const k3x_hip_mla_params* p, const uint32_t* table, const 
     a.N = p->sequences;
     a.T = p->tokens;
     a.page = p->page_size;
+    a.page_shift = 31;
+    while (1ull << (a.page_shift - 31) < a.page) ++a.page_shift;
+    a.page_by = (uint32_t)(((1ull << a.page_shift) + a.page - 1) / a.page);
     a.pages = p->pages;
     a.width = p->table_width;
     a.longest = p->longest ? p->longest : p->tokens;
+    a.most = (uint32_t)std::min<uint64_t>((uint64_t)a.width * a.page, 1u << 29);
     a.row = row_layout(p->cache_format, p->latent, p->rotary);
     return a;
 }

@@ -9,10 +9,13 @@ namespace k3x_mla {
 
 using namespace k3x_dev;
 
-// Which columns of 16 bytes are exchanged in token t of a tile's 64-column group,
-// so that neither product's reads of it meet in a bank: eight tokens' same column
-// (keys), and four tokens' two neighbours (values).
-__device__ inline uint32_t swizzle(uint32_t t) { return (t & 3) << 1 | (t >> 2 & 1); }
+// Which columns of 16 bytes are exchanged in token t of a tile's 64-column group
+// (128 bytes a token), so that reads do not meet in a bank: 64 banks hold two
+// tokens, keys are read sixteen tokens at a time at one column, values four or
+// eight tokens at four or two columns.  So the bits of t / 2, reversed.
+__device__ inline uint32_t swizzle(uint32_t t) {
+    return (t << 1 & 4) | (t >> 1 & 2) | (t >> 3 & 1);
+}
 
 template <uint32_t DT, int HT>
 struct Mma;

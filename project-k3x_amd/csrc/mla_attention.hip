@@ -91,10 +91,9 @@ __device__ __forceinline__ void scale_all(Acc (&o)[OT], float k) {
 
 // Tiles of a sequence in the line; an empty one takes one, in which its rows are
 // written as empty.
-__device__ inline uint32_t tiles_of(const Pages& a, uint32_t n) {
-    Tokens s;
-    if (!tokens_of(a, n, &s) || !s.count) return 0;
-    return max(1u, (s.len + kTile - 1) / kTile);
+__device__ inline uint32_t tiles_in(const Tokens& s) { return max(1u, (s.len + kTile - 1) / kTile); }
+__device__ inline uint32_t tiles_of(const Pages& a, uint32_t n, Tokens* s) {
+    return tokens_of(a, n, s) && s->count ? tiles_in(*s) : 0;
 }
 
 // FULL: L is LP (else the columns past L are zeros, and not brought or written) and
@@ -115,24 +114,15 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     lds_byte* const lds = (lds_byte*)smem;
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // Row blocks of one range lie on one die, eight ranges beside each other.
-    uint32_t w, rb;
-    if (a.G % 8 == 0) {
-        const uint32_t x = blockIdx.x / 8;
-        w = x / a.RB * 8 + blockIdx.x % 8;
-        rb = x % a.RB;
-    } else {
-        w = blockIdx.x / a.RB;
-        rb = blockIdx.x % a.RB;
-    }
-    if (*(volatile uint32_t*)a.status) return;
+    const uint32_t status = *(volatile uint32_t*)a.status;  // looked at with the lengths
     if (blockIdx.x == 0) check_sequences(a.pages, a.status);
 
     // ---- the line and this workgroup's range of it --------------------------
     // Tiles before and in sequences base .. base + 255, a sequence a thread.
-    auto scan_tiles = [&](uint32_t base, uint32_t* mine) {
+    Tokens mine;
+    auto scan_tiles = [&](uint32_t base, uint32_t* own) {
         const uint32_t n = base + tid;
-        uint32_t c = *mine = n < a.pages.N ? tiles_of(a.pages, n) : 0;
+        uint32_t c = *own = n < a.pages.N ? tiles_of(a.pages, n, &mine) : 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t o = __shfl_up(c, d);
@@ -146,18 +136,35 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         return before + c;  // with the thread's own
     };
     const bool by_sequence = a.pages.N <= a.G;
-    uint32_t total = 0, own, upto = 0;
+    uint64_t all = 0;
+    uint32_t own, upto = 0;
     for (uint32_t base = 0; base < a.pages.N; base += kThreads) {
         upto = scan_tiles(base, &own);
-        total += scan[0] + scan[1] + scan[2] + scan[3];
+        all += (uint64_t)scan[0] + scan[1] + scan[2] + scan[3];
         if (by_sequence && blockIdx.x == 0 && !own && base + tid < a.pages.N)
             a.splits[base + tid].pieces = 0;  // in no range
     }
+    if (status) return;
+    if (all >> 32) {
+        if (tid == 0) latch(a.status, K3X_ERR_INVALID_STATE);
+        return;
+    }
+    const uint32_t total = (uint32_t)all;
     const uint32_t chunk = max(kLeast, (total + a.G - 1) / a.G);
-    const uint64_t from64 = (uint64_t)w * chunk;
+    const uint32_t ranges = (total + chunk - 1) / chunk;  // in use, G at most
+    // Consecutive ranges, and a range's row blocks, lie on one die: they share cached
+    // tokens and queries.
+    uint32_t w = blockIdx.x / a.RB, rb = blockIdx.x % a.RB;
+    if (!by_sequence && rb == 0 && tid == 0 && w >= ranges) a.splits[w].pieces = 0;
+    if (a.G % 8 == 0) {
+        const uint32_t each = (ranges + 7) / 8, x = blockIdx.x / 8;
+        if (x / a.RB >= each) return;
+        w = blockIdx.x % 8 * each + x / a.RB;
+        rb = x % a.RB;
+    }
+    if (w >= ranges) return;
     if (!by_sequence && rb == 0 && tid == 0) a.splits[w].pieces = 0;
-    if (from64 >= total) return;
-    const uint32_t from = (uint32_t)from64, to = min(total, from + chunk);
+    const uint32_t from = w * chunk, to = min(total, from + chunk);
     // The sequence that tile `from` is in, and the tiles before it.
     uint32_t carry = 0;
     for (uint32_t base = 0; base < a.pages.N; base += kThreads) {
@@ -165,12 +172,17 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         if (own && from >= carry + upto - own && from < carry + upto) {
             at_s[0] = base + tid;
             at_s[1] = carry + upto - own;
+            at_s[2] = mine.begin;
+            at_s[3] = mine.count;
+            at_s[4] = mine.len;
         }
         carry += scan[0] + scan[1] + scan[2] + scan[3];
         if (carry > from) break;
     }
     __syncthreads();
-    uint32_t n = at_s[0], first = at_s[1];
+    auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane(x); };
+    uint32_t n = uniform(at_s[0]), first = uniform(at_s[1]);
+    Tokens s{uniform(at_s[2]), uniform(at_s[3]), uniform(at_s[4])};
     __syncthreads();
 
     // What is not brought to LDS stays zero there.
@@ -189,20 +201,17 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     const uint32_t vat0 = vrow * 128 +
                           (((HT == 32 ? 2 * (lane >> 4 & 1) : 0) + (i16 & 3) / 2) ^ swizzle(vrow)) * 16 +
                           (i16 & 1) * 8;
-    // What the lane brings of each tile: token 8 wave + lane / 8, the columns of 16
-    // bytes (codes: the 16 bytes) lane % 8 of each group.
-    const uint32_t btok = 8 * wave + lane / 8, bcol = lane % 8;
-    const uint32_t bput = bcol ^ swizzle(lane / 8);
+    // What the lane brings of each tile: one of eight columns of 16 bytes (codes: 16
+    // bytes) of a token.  Direct loads fill LDS lane by lane, eight tokens a wave;
+    // through registers sixteen lanes write sixteen tokens, which do not meet in a bank.
+    constexpr bool DIRECT = F == K3X_CACHE_16BIT && FULL;
+    const uint32_t btok = DIRECT ? 8 * wave + lane / 8 : 16 * (wave / 2) + lane % 16;
+    const uint32_t bcol = DIRECT ? lane % 8 : lane / 16 + 4 * (wave % 2);
+    const uint32_t bput = bcol ^ swizzle(btok);
 
     bool bad_page = false, bad_value = false;
     while (true) {
-        Tokens s;
-        const uint32_t tiles = tiles_of(a.pages, n);
-        tokens_of(a.pages, n, &s);
-        if (!tiles) {
-            ++n;
-            continue;
-        }
+        const uint32_t tiles = tiles_in(s);
         const uint32_t rows = s.count * a.H;
         const uint32_t t0 = max(from, first) - first, t1 = min(to - first, tiles);
         const bool whole = t0 == 0 && t1 == tiles;
@@ -212,7 +221,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         const uint32_t r0 = rb * S::rows;
         if (r0 < rows) {
             // The row of this lane, and how many tokens it sees.
-            const uint32_t r = min(r0 + wm * HT + col, rows - 1), ri = r / a.H;
+            const uint32_t r = min(r0 + wm * HT + opaque(col), rows - 1), ri = r / a.H;
             const int32_t sees = (int32_t)s.len - (int32_t)s.count + (int32_t)ri + 1;
             const int32_t sees_least = (int32_t)s.len - (int32_t)s.count + (int32_t)(r0 / a.H) + 1;
             const int32_t sees_most = (int32_t)s.len - (int32_t)s.count +
@@ -220,29 +229,17 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
             const uint32_t seen = sees_most > 0 ? (uint32_t)sees_most : 0;
             const uint32_t end = min(t1, (seen + kTile - 1) / kTile);
             u32x4 qf[CG * KS];
-            {
-                const uint8_t* q = static_cast<const uint8_t*>(a.q) +
-                                   2 * ((uint64_t)(s.begin + ri) * a.qs +
-                                        (uint64_t)(r % a.H) * (a.L + a.R));
-#pragma unroll
-                for (int c = 0; c < CG; ++c)
-#pragma unroll
-                    for (int i = 0; i < KS; ++i) {
-                        // Columns of the latent, then of the rotary part.
-                        const uint32_t d = (c < CG - 1 ? c * 64 : 0) + (i * (8 / KS) + g) * 8;
-                        const bool in = c < CG - 1 ? FULL || d < a.L : d < a.R;
-                        const u32x4 x = *reinterpret_cast<const u32x4*>(
-                            q + (in ? 2 * (c < CG - 1 ? d : a.L + d) : 0));
-                        qf[c * KS + i] = x & (in ? 0xffffffffu : 0u);
-                    }
-            }
             Acc o[OT];
+            {
+                const float zero = __uint_as_float(opaque(0));
 #pragma unroll
-            for (int i = 0; i < OT; ++i) o[i] = Acc{};
+                for (int i = 0; i < OT; ++i)
+#pragma unroll
+                    for (int j = 0; j < (int)(sizeof(Acc) / 4); ++j) o[i][j] = zero;
+            }
             float m = -3.4028235e38f, l = 0.0f;
 
             // ---- bringing tiles ---------------------------------------------
-            constexpr bool DIRECT = F == K3X_CACHE_16BIT && FULL;
             // The wave's eight tokens of a tile, where a page holds whole eights.
             auto eight = [&](uint32_t t) {
                 return __builtin_amdgcn_readfirstlane(min(t * kTile + 8 * wave, s.len - 1) & ~7u);
@@ -250,12 +247,13 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
             auto position = [&](uint32_t t) { return min(t * kTile + btok, s.len - 1); };
             auto page_of = [&](uint32_t t) {
                 const uint32_t p = DIRECT ? eight(t) : position(t);
-                return a.pages.table[(size_t)n * a.pages.width + p / a.pages.page];
+                return a.pages.table[(size_t)n * a.pages.width + a.pages.page_of(p)];
             };
             auto row_of = [&](uint32_t p, uint32_t id) {
                 bad_page |= id >= a.pages.pages;
                 if (id >= a.pages.pages) id = 0;
-                return a.pool + ((size_t)id * a.pages.page + p % a.pages.page) * a.pages.row.bytes;
+                const uint32_t in = p - a.pages.page_of(p) * a.pages.page;
+                return a.pool + ((size_t)id * a.pages.page + in) * a.pages.row.bytes;
             };
             constexpr int UNITS = F == K3X_CACHE_MXFP8   ? LP / 128
                                   : F == K3X_CACHE_MXFP4 ? LP / 256
@@ -295,7 +293,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
             auto put = [&](uint32_t b) {
                 if constexpr (!DIRECT) {
                     uint8_t* dst = smem + b * kBuffer + btok * 128;
-                    const uint32_t z = swizzle(lane / 8);
+                    const uint32_t z = swizzle(btok);
 #pragma unroll
                     for (int k = 0; k < UNITS; ++k) {
                         const uint32_t u = bcol + 8 * k;
@@ -328,6 +326,24 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                 }
             };
 
+            auto load_queries = [&] {
+                const uint32_t half = opaque(g);
+                const uint8_t* q = static_cast<const uint8_t*>(a.q) +
+                                   2 * ((uint64_t)(s.begin + ri) * a.qs +
+                                        (uint64_t)(r - ri * a.H) * (a.L + a.R));
+#pragma unroll
+                for (int c = 0; c < CG; ++c)
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        // Columns of the latent, then of the rotary part.
+                        const uint32_t d = (c < CG - 1 ? c * 64 : 0) + (i * (8 / KS) + half) * 8;
+                        const bool in = c < CG - 1 ? FULL || d < a.L : d < a.R;
+                        const u32x4 x = *reinterpret_cast<const u32x4*>(
+                            q + (in ? 2 * (c < CG - 1 ? d : a.L + d) : 0));
+                        qf[c * KS + i] = x & (in ? 0xffffffffu : 0u);
+                    }
+            };
+
             // ---- one tile ---------------------------------------------------
             auto tile = [&](uint32_t t, uint32_t b) {
                 const lds_byte* kb = lds + b * kBuffer;
@@ -354,18 +370,32 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                         for (int x = 0; x < XT; ++x)
                             sc[x] = M::run(kf[c & 1][i][x], qf[c * KS + i], sc[x]);
                 };
-                if (a.R) {
-                    keys(CG - 1);
-                    products(CG - 1);
-                }
+                // (Without a rotary part its group is zeros.)
                 keys(0);
 #pragma unroll
-                for (int c = 0; c < CG - 1; ++c) {
-                    if (c + 1 < CG - 1) keys(c + 1);
+                for (int c = 0; c < CG; ++c) {
+                    if (c + 1 < CG) keys(c + 1);
                     __builtin_amdgcn_sched_barrier(0);
                     products(c);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                constexpr int HV = HT == 32 ? 2 : 1;
+                u32x4 vf[2][HV];
+                const uint32_t vat = opaque(vat0);
+                auto values = [&](int y) {
+                    const uint32_t d = y + wd * OT;  // tile of HT columns of the latent
+                    const lds_byte* vb = kb + d * HT / 64 * kGroup;
+                    const uint32_t at = vat ^ y % (64 / HT) * (HT * 2);
+#pragma unroll
+                    for (int h = 0; h < HV; ++h) {
+                        // Tokens 16 h .. 16 h + 15 (or all 32), by fours of each half.
+                        const uint2 v0 = lds_transposed(vb + h * 2048 + at);
+                        const uint2 v1 = HT == 32 ? lds_transposed(vb + h * 2048 + 1024 + (at ^ 16))
+                                                  : lds_transposed(vb + 2048 + at);
+                        vf[y & 1][h] = u32x4{v0.x, v0.y, v1.x, v1.y};
+                    }
+                };
+                values(0);  // on their way while weights are formed
                 constexpr int NV = HT == 32 ? 16 : 8;
                 float x[NV];
 #pragma unroll
@@ -390,7 +420,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     const float up = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - up);
                     m = up;
                     l *= keep;
-                    scale_all<OT>(o, keep);
+                    if (t != t0) scale_all<OT>(o, keep);
                 }
                 uint32_t p[NV / 2];
                 float sum = 0.0f;
@@ -402,21 +432,6 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     p[i / 2] = pack2<DT>(u, v);
                 }
                 l += sum;
-                constexpr int HV = HT == 32 ? 2 : 1;
-                u32x4 vf[2][HV];
-                const uint32_t vat = opaque(vat0);
-                auto values = [&](int y) {
-                    const uint32_t d = y + wd * OT;  // tile of HT columns of the latent
-                    const lds_byte* vb = kb + d * HT / 64 * kGroup + (vat ^ y % (64 / HT) * (HT * 2));
-#pragma unroll
-                    for (int h = 0; h < HV; ++h) {
-                        // Tokens 16 h .. 16 h + 15 (or all 32), by fours of each half.
-                        const uint2 v0 = lds_transposed(vb + h * 2048);
-                        const uint2 v1 = lds_transposed(vb + h * 2048 + (HT == 32 ? 1024 : 2048));
-                        vf[y & 1][h] = u32x4{v0.x, v0.y, v1.x, v1.y};
-                    }
-                };
-                values(0);
 #pragma unroll
                 for (int y = 0; y < OT; ++y) {
                     if (y + 1 < OT) values(y + 1);
@@ -442,6 +457,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                         bring(min(t0 + i, end - 1), i, id);
                         id = next;
                     }
+                    load_queries();
                     uint32_t b = 0;
                     for (uint32_t t = t0; t < end; ++t) {
                         if (a.R) wait_loads<(BUFS - 2) * CG>();
@@ -458,6 +474,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                 } else {
                     uint32_t id = page_of(t0), next = page_of(min(t0 + 1, end - 1));
                     bring(t0, 0, id);
+                    load_queries();
                     put(0);
                     bring(min(t0 + 1, end - 1), 0, next);
                     next = page_of(min(t0 + 2, end - 1));
@@ -486,26 +503,30 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
             constexpr int Q = HT == 32 ? 4 : 1;
             float4* part = a.parts + piece * (S::rows * LP / 4) + wave * OT * Q * 64 + lane;
             float check = l * 0.0f;  // NaN once something is not finite
+            auto each = [&](auto put4) {
 #pragma unroll
-            for (int y = 0; y < OT; ++y) {
+                for (int y = 0; y < OT; ++y) {
 #pragma unroll
-                for (int i = 0; i < Q; ++i) {
-                    const uint32_t d = (y + wd * OT) * HT + 8 * i + 4 * g;
-                    const float4 v{o[y][4 * i] * inv, o[y][4 * i + 1] * inv,
-                                   o[y][4 * i + 2] * inv, o[y][4 * i + 3] * inv};
-                    if (FULL || d < a.L) {
+                    for (int i = 0; i < Q; ++i) {
+                        const uint32_t d = (y + wd * OT) * HT + 8 * i + 4 * g;
+                        const float4 v{o[y][4 * i] * inv, o[y][4 * i + 1] * inv,
+                                       o[y][4 * i + 2] * inv, o[y][4 * i + 3] * inv};
+                        if (!FULL && d >= a.L) continue;
                         check = __builtin_fmaf(v.x, 0.0f, check);
                         check = __builtin_fmaf(v.y, 0.0f, check);
                         check = __builtin_fmaf(v.z, 0.0f, check);
                         check = __builtin_fmaf(v.w, 0.0f, check);
-                        if (!whole) part[(y * Q + i) * 64] = v;
-                        else if (live)
-                            *reinterpret_cast<uint2*>(out + d) =
-                                uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+                        put4(y * Q + i, d, v);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            };
+            if (!whole)
+                each([&](int f, uint32_t, float4 v) { part[f * 64] = v; });
+            else if (live)
+                each([&](int, uint32_t d, float4 v) {
+                    *reinterpret_cast<uint2*>(out + d) = uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+                });
             bad_value |= live && !(check == 0.0f);
             if (g == 0 && wd == 0) {
                 if (!whole)
@@ -517,8 +538,10 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
             }
         }
         first += tiles;
-        ++n;
         if (first >= to) break;
+        do ++n;
+        while (n < a.pages.N && !tiles_of(a.pages, n, &s));
+        if (n == a.pages.N) break;
     }
     if (bad_page) latch(a.status, K3X_ERR_INVALID_STATE);
     if (bad_value) latch(a.status, K3X_ERR_INVALID_MXFP4);
@@ -533,13 +556,13 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
     constexpr uint32_t kSlices = S::rows * LP / (FOUR ? 256 : 1024);
     constexpr uint32_t NF = LP / HT / WD * (HT == 32 ? 4 : 1);
     __shared__ float4 os[FOUR ? 4 : 1][64];
-    __shared__ float ls[FOUR ? 4 : 1][64];
+    __shared__ float2 ls[FOUR ? 4 : 1][64];
     const uint32_t slice = blockIdx.x % kSlices, x = blockIdx.x / kSlices;
     const uint32_t rb = x % a.RB, lane = threadIdx.x & 63, quarter = threadIdx.x / 64;
-    if (*(volatile uint32_t*)a.status) return;
+    const uint32_t status = *(volatile uint32_t*)a.status;
     const Split s = a.splits[x / a.RB];
     const uint32_t rows = s.count * a.H;
-    if (!s.pieces || rb * S::rows >= rows) return;
+    if (status || !s.pieces || rb * S::rows >= rows) return;
     const uint32_t f = FOUR ? slice : slice * 4 + quarter, wave = f / NF, i = f % NF;
     const uint32_t wm = wave / WD, wd = wave % WD;
     const uint32_t at = wm * HT + lane % HT, r = rb * S::rows + at;
@@ -547,9 +570,7 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
                                 : wd * (LP / WD) + i * 16 + lane / 16 * 4;
     const bool live = r < rows && d < a.L;
     auto piece = [&](uint32_t p) { return ((size_t)(s.w + p) * a.RB + rb) * 2 + (p ? 0 : 1); };
-    float m = -3.4028235e38f;
-    for (uint32_t p = 0; p < s.pieces; ++p) m = fmaxf(m, a.sums[piece(p) * S::rows + at].x);
-    float l = 0.0f;
+    float m = -3.4028235e38f, l = 0.0f;
     float4 o{};
     constexpr uint32_t kStep = FOUR ? 4 : 1, kAhead = 4;
     for (uint32_t p0 = FOUR ? quarter : 0; p0 < s.pieces; p0 += kStep * kAhead) {
@@ -561,6 +582,13 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
             ml[j] = a.sums[q * S::rows + at];
             v[j] = live ? a.parts[q * (S::rows * LP / 4) + f * 64 + lane] : float4{};
         }
+        float top = m;
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) top = fmaxf(top, ml[j].x);
+        const float keep = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= keep;
+        o = float4{o.x * keep, o.y * keep, o.z * keep, o.w * keep};
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
             // A piece that the row does not see has no sum, and may hold no outputs.
@@ -575,16 +603,21 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
     }
     if constexpr (FOUR) {
         os[quarter][lane] = o;
-        ls[quarter][lane] = l;
+        ls[quarter][lane] = float2{m, l};
         __syncthreads();
         if (quarter) return;
+        for (int j = 1; j < 4; ++j) m = fmaxf(m, ls[j][lane].x);
+        l = 0.0f;
+        o = float4{};
 #pragma unroll
-        for (int j = 1; j < 4; ++j) {
-            l += ls[j][lane];
-            o.x += os[j][lane].x;
-            o.y += os[j][lane].y;
-            o.z += os[j][lane].z;
-            o.w += os[j][lane].w;
+        for (int j = 0; j < 4; ++j) {
+            const float k = __builtin_amdgcn_exp2f(ls[j][lane].x - m);
+            const float4 v = os[j][lane];
+            l = __builtin_fmaf(ls[j][lane].y, k, l);
+            o.x = __builtin_fmaf(v.x, k, o.x);
+            o.y = __builtin_fmaf(v.y, k, o.y);
+            o.z = __builtin_fmaf(v.z, k, o.z);
+            o.w = __builtin_fmaf(v.w, k, o.w);
         }
     }
     if (!live) return;

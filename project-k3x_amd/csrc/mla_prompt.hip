@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
     const uint32_t vat0 = vrow * 128 + ((2 * (lane >> 4 & 1) + (i16 & 3) / 2) ^ swizzle(vrow)) * 16 +
                           (i16 & 1) * 8;
     // What the lane brings: token 8 (wave + 4 x) + lane / 8 of a tile, 16 bytes a group.
-    const uint32_t btok = 8 * wave + lane / 8, bput = lane % 8 ^ swizzle(lane / 8);
+    const uint32_t btok = 8 * wave + lane / 8, bput = lane % 8 ^ swizzle(btok);
 
     u32x4 qf[KG * 4];
     {
@@ -247,9 +247,10 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
             for (int y = 0; y < OT; ++y)
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
-                    const lds_byte* vb = kb + (KG + y / 2) * kGroup + x * 4096 + z * 2048 +
-                                         (vat0 ^ y % 2 * 64);
-                    const uint2 v0 = lds_transposed(vb), v1 = lds_transposed(vb + 1024);
+                    const lds_byte* vb = kb + (KG + y / 2) * kGroup + x * 4096 + z * 2048;
+                    const uint32_t at = vat0 ^ y % 2 * 64;
+                    const uint2 v0 = lds_transposed(vb + at);
+                    const uint2 v1 = lds_transposed(vb + 1024 + (at ^ 16));
                     o[y] = M::run(u32x4{v0.x, v0.y, v1.x, v1.y},
                                   u32x4{p[x][4 * z], p[x][4 * z + 1], p[x][4 * z + 2],
                                         p[x][4 * z + 3]}, o[y]);
