@@ -1,9 +1,10 @@
 // mla_cache.hip -- the paged cache of latent attention: rows written with their
 // norm and quantisation, and read back.
 //
-// A wave a token: eight neighbours of the latent a lane, so that a block of 32
-// is four lanes, its largest two exchanges within them, and a row one load and
-// one store a lane.
+// A wave a token at a time: eight neighbours of the latent a lane, so that a block
+// of 32 is four lanes, its largest two exchanges within them, and a row one load and
+// one store a lane.  Of many tokens a wave takes eight, looked up together, with
+// their loads on their way together.
 #include <hip/hip_runtime.h>
 
 #include "k3x_mla.hpp"
@@ -56,34 +57,61 @@ __device__ inline uint16_t bits(float v) {
     return __builtin_bit_cast(uint16_t, Elem<DT>::store(v));
 }
 
-// Row t's sequence and position; false: it has none that is cached.
-__device__ inline bool locate(const Pages& a, uint32_t t, uint32_t* n, uint32_t* pos) {
-    *n = sequence_of(a, t);
+// Cached rows of the call's tokens t0 .. t0 + TP - 1, token i's in lane i; null: it
+// has none (or its page is none of the pool, which is latched).  By a wave.
+template <int TP>
+__device__ inline uint8_t* find_rows(const CacheArgs& a, uint32_t t0) {
+    const Pages& p = a.pages;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t n = sequence_of(p, t0);
+    if (TP > 1) {
+        if (p.offsets) {
+            // Of the 64 sequences from the first token's on (the first ones, where it lies
+            // before them all); another search past them.
+            const uint32_t from = n < p.N ? n : 0, o = p.offsets[min(from + lane, p.N)];
+#pragma unroll
+            for (int i = 1; i < TP; ++i) {
+                const uint32_t k = __popcll(__ballot(from + lane < p.N && o <= t0 + i));
+                uint32_t m = from + max(k, 1u) - 1;
+                if (k == 64) m = sequence_of(p, t0 + i);
+                if (lane == (uint32_t)i) n = m;
+            }
+        } else if (n < p.N) {
+            n = (t0 + min(lane, (uint32_t)TP - 1)) / (p.T / p.N);
+        }
+    }
+    const uint32_t t = t0 + lane;
     Tokens s;
-    if (*n >= a.N || !tokens_of(a, *n, &s) || t < s.begin || t - s.begin >= s.count) return false;
-    const int64_t p = (int64_t)s.len - s.count + (t - s.begin);
-    *pos = (uint32_t)p;
-    return p >= 0;
+    if (lane >= TP || t >= p.T || n >= p.N || !tokens_of(p, n, &s) || t < s.begin ||
+        t - s.begin >= s.count)
+        return nullptr;
+    const int64_t pos = (int64_t)s.len - s.count + (t - s.begin);
+    if (pos < 0) return nullptr;
+    uint8_t* row = cached_row(p, a.pool, n, (uint32_t)pos);
+    if (!row) latch(a.status, K3X_ERR_INVALID_STATE);
+    return row;
+}
+// Lane i's pointer, in every lane.
+__device__ inline uint8_t* row_of(uint8_t* mine, int i) {
+    const uint64_t v = reinterpret_cast<uint64_t>(mine);
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, i);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), i);
+    return reinterpret_cast<uint8_t*>((uint64_t)hi << 32 | lo);
+}
+
+// 1 / sqrt(x) in double: an estimate of 24 bits or so, and Newton's step twice.
+__device__ inline double rsqrt_f64(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = y * __builtin_fma(-0.5 * x * y, y, 1.5);
+    return y;
 }
 
 template <uint32_t DT, uint32_t F>
-__global__ __launch_bounds__(kThreads) void mla_store_kernel(CacheArgs a) {
+__device__ inline void store_row(const CacheArgs& a, uint8_t* row, u16x8 v, u16x8 r,
+                                 const float (&gamma)[8]) {
     const uint32_t lane = threadIdx.x & 63;
-    const uint32_t t = blockIdx.x * (kThreads / 64) +
-                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (*(volatile uint32_t*)a.status) return;
-    if (blockIdx.x == 0) check_sequences(a.pages, a.status);
-    uint32_t n, pos;
-    if (t >= a.pages.T || !locate(a.pages, t, &n, &pos)) return;
-    uint8_t* row = cached_row(a.pages, a.pool, n, pos);
-    if (!row) {
-        if (lane == 0) latch(a.status, K3X_ERR_INVALID_STATE);
-        return;
-    }
     const bool mine = 8 * lane < a.L, turns = 8 * lane < a.R;
-    u16x8 v{}, r{};
-    if (mine) v = load8(static_cast<const uint16_t*>(a.latent) + t * a.ls + 8 * lane, a.vec);
-    if (turns) r = load8(static_cast<const uint16_t*>(a.rotary) + t * a.rs + 8 * lane, a.vec);
     float x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = value<DT>(v[j]);
@@ -92,13 +120,12 @@ __global__ __launch_bounds__(kThreads) void mla_store_kernel(CacheArgs a) {
         // side that the formula says.
         double s = 0.0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += (double)x[j] * (double)x[j];
+        for (int j = 0; j < 8; ++j) s = __builtin_fma((double)x[j], (double)x[j], s);
         s = wave_sum(s);
-        const double inv = 1.0 / sqrt(s / a.L + a.eps);
+        const double inv = rsqrt_f64(s / a.L + a.eps);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float g = mine ? a.gamma[8 * lane + j] : 0.0f;
-            v[j] = bits<DT>((float)((double)x[j] * inv * (double)g));
+            v[j] = bits<DT>((float)((double)x[j] * inv * (double)gamma[j]));
             x[j] = value<DT>(v[j]);
         }
     }
@@ -150,36 +177,77 @@ __global__ __launch_bounds__(kThreads) void mla_store_kernel(CacheArgs a) {
     }
 }
 
-template <uint32_t DT, uint32_t F>
+template <uint32_t DT, uint32_t F, int TP>
+__global__ __launch_bounds__(kThreads) void mla_store_kernel(CacheArgs a) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t t0 = (blockIdx.x * (kThreads / 64) +
+                         __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * TP;
+    const uint32_t status = *(volatile uint32_t*)a.status;
+    if (blockIdx.x == 0) check_sequences(a.pages, a.status);
+    if (t0 >= a.pages.T) return;
+    u16x8 v[TP]{}, r[TP]{};
+#pragma unroll
+    for (int i = 0; i < TP; ++i) {
+        const size_t t = min(t0 + i, a.pages.T - 1);
+        if (8 * lane < a.L)
+            v[i] = load8(static_cast<const uint16_t*>(a.latent) + t * a.ls + 8 * lane, a.vec);
+        if (8 * lane < a.R)
+            r[i] = load8(static_cast<const uint16_t*>(a.rotary) + t * a.rs + 8 * lane, a.vec);
+    }
+    float gamma[8] = {};
+    if (a.gamma && 8 * lane < a.L)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) gamma[j] = a.gamma[8 * lane + j];
+    uint8_t* const rows = find_rows<TP>(a, t0);
+    if (status) return;
+#pragma unroll
+    for (int i = 0; i < TP; ++i)
+        if (uint8_t* row = row_of(rows, i)) store_row<DT, F>(a, row, v[i], r[i], gamma);
+}
+
+template <uint32_t F, int TP>
 __global__ __launch_bounds__(kThreads) void mla_load_kernel(CacheArgs a) {
     const uint32_t lane = threadIdx.x & 63;
-    const uint32_t t = blockIdx.x * (kThreads / 64) +
-                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (*(volatile uint32_t*)a.status) return;
+    const uint32_t t0 = (blockIdx.x * (kThreads / 64) +
+                         __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * TP;
+    const uint32_t status = *(volatile uint32_t*)a.status;
     if (blockIdx.x == 0) check_sequences(a.pages, a.status);
-    uint32_t n, pos;
-    if (t >= a.pages.T || !locate(a.pages, t, &n, &pos)) return;
-    const uint8_t* row = cached_row(a.pages, a.pool, n, pos);
-    if (!row) {
-        if (lane == 0) latch(a.status, K3X_ERR_INVALID_STATE);
-        return;
-    }
+    if (t0 >= a.pages.T) return;
+    uint8_t* const rows = find_rows<TP>(a, t0);
+    if (status) return;
     const RowLayout& at = a.pages.row;
-    if (a.rotary && 8 * lane < a.R)
-        store8(static_cast<uint16_t*>(a.rotary) + t * a.rs + 8 * lane,
-               *reinterpret_cast<const u16x8*>(row + at.codes + 16 * lane), a.vec);
-    if (8 * lane >= a.L) return;
-    u16x8 v;
-    if constexpr (F == K3X_CACHE_16BIT) {
-        v = *reinterpret_cast<const u16x8*>(row + 16 * lane);
-    } else {
-        const float scale = e8m0_to_f32(row[at.scales + lane / 4]);
-        bf16x8 w;
-        if constexpr (F == K3X_CACHE_MXFP8) w = mxfp8_8(*reinterpret_cast<const uint2*>(row + 8 * lane), scale);
-        else w = dequant8(*reinterpret_cast<const uint32_t*>(row + 4 * lane), scale);
-        v = __builtin_bit_cast(u16x8, w);
+    const bool mine = 8 * lane < a.L, turns = a.rotary && 8 * lane < a.R;
+    u16x8 v[TP], r[TP];
+    uint2 codes[TP];
+    uint32_t scale[TP];
+#pragma unroll
+    for (int i = 0; i < TP; ++i) {
+        const uint8_t* row = row_of(rows, i);
+        if (!row) continue;
+        if (turns) r[i] = *reinterpret_cast<const u16x8*>(row + at.codes + 16 * lane);
+        if (!mine) continue;
+        if constexpr (F == K3X_CACHE_16BIT) {
+            v[i] = *reinterpret_cast<const u16x8*>(row + 16 * lane);
+        } else {
+            scale[i] = row[at.scales + lane / 4];
+            if constexpr (F == K3X_CACHE_MXFP8)
+                codes[i] = *reinterpret_cast<const uint2*>(row + 8 * lane);
+            else
+                codes[i].x = *reinterpret_cast<const uint32_t*>(row + 4 * lane);
+        }
     }
-    store8(static_cast<uint16_t*>(a.latent) + t * a.ls + 8 * lane, v, a.vec);
+#pragma unroll
+    for (int i = 0; i < TP; ++i) {
+        if (!row_of(rows, i)) continue;
+        const size_t t = t0 + i;
+        if (turns) store8(static_cast<uint16_t*>(a.rotary) + t * a.rs + 8 * lane, r[i], a.vec);
+        if (!mine) continue;
+        if constexpr (F == K3X_CACHE_MXFP8)
+            v[i] = __builtin_bit_cast(u16x8, mxfp8_8(codes[i], e8m0_to_f32(scale[i])));
+        else if constexpr (F == K3X_CACHE_MXFP4)
+            v[i] = __builtin_bit_cast(u16x8, dequant8(codes[i].x, e8m0_to_f32(scale[i])));
+        store8(static_cast<uint16_t*>(a.latent) + t * a.ls + 8 * lane, v[i], a.vec);
+    }
 }
 
 // What both calls share; 0 or the status to return.
@@ -206,7 +274,26 @@ int cache_args(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const void* latent
     return K3X_OK;
 }
 
-dim3 grid_of(const CacheArgs& a) { return dim3(a.pages.T ? (a.pages.T + 3) / 4 : 1); }
+// Eight tokens a wave once there are more than the waves that are held at once.
+// SPLIT
+template <uint32_t DT, uint32_t F>
+int launch_store(k3x_hip_ctx* ctx, const CacheArgs& a) {
+    const uint32_t T = a.pages.T;
+    if (T > 8192)
+        hipLaunchKernelGGL((mla_store_kernel<DT, F, 8>), dim3((T + 31) / 32), dim3(kThreads), 0, ctx->stream, a);
+    else
+        hipLaunchKernelGGL((mla_store_kernel<DT, F, 1>), dim3((T + 3) / 4 + !T), dim3(kThreads), 0, ctx->stream, a);
+    return launched(ctx, 1);
+}
+template <uint32_t F>
+int launch_load(k3x_hip_ctx* ctx, const CacheArgs& a) {
+    const uint32_t T = a.pages.T;
+    if (T > 8192)
+        hipLaunchKernelGGL((mla_load_kernel<F, 8>), dim3((T + 31) / 32), dim3(kThreads), 0, ctx->stream, a);
+    else
+        hipLaunchKernelGGL((mla_load_kernel<F, 1>), dim3((T + 3) / 4 + !T), dim3(kThreads), 0, ctx->stream, a);
+    return launched(ctx, 1);
+}
 
 }  // namespace
 
@@ -225,16 +312,12 @@ int k3x_hip_mla_store(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const void*
     if (st != K3X_OK) return st;
     a.gamma = gamma;
     a.eps = p->norm_epsilon;
-    const dim3 grid = grid_of(a), block(kThreads);
-    if (p->dtype == K3X_DTYPE_F16)
-        hipLaunchKernelGGL((mla_store_kernel<K3X_DTYPE_F16, K3X_CACHE_16BIT>), grid, block, 0, ctx->stream, a);
-    else if (p->cache_format == K3X_CACHE_16BIT)
-        hipLaunchKernelGGL((mla_store_kernel<K3X_DTYPE_BF16, K3X_CACHE_16BIT>), grid, block, 0, ctx->stream, a);
-    else if (p->cache_format == K3X_CACHE_MXFP8)
-        hipLaunchKernelGGL((mla_store_kernel<K3X_DTYPE_BF16, K3X_CACHE_MXFP8>), grid, block, 0, ctx->stream, a);
-    else
-        hipLaunchKernelGGL((mla_store_kernel<K3X_DTYPE_BF16, K3X_CACHE_MXFP4>), grid, block, 0, ctx->stream, a);
-    return launched(ctx, 1);
+    if (p->dtype == K3X_DTYPE_F16) return launch_store<K3X_DTYPE_F16, K3X_CACHE_16BIT>(ctx, a);
+    switch (p->cache_format) {
+        case K3X_CACHE_16BIT: return launch_store<K3X_DTYPE_BF16, K3X_CACHE_16BIT>(ctx, a);
+        case K3X_CACHE_MXFP8: return launch_store<K3X_DTYPE_BF16, K3X_CACHE_MXFP8>(ctx, a);
+        default: return launch_store<K3X_DTYPE_BF16, K3X_CACHE_MXFP4>(ctx, a);
+    }
 }
 
 int k3x_hip_mla_load(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const void* pool,
@@ -243,14 +326,11 @@ int k3x_hip_mla_load(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const void* 
     CacheArgs a{};
     const int st = cache_args(ctx, p, latent, rotary, table, offsets, lens, pool, &a);
     if (st != K3X_OK) return st;
-    const dim3 grid = grid_of(a), block(kThreads);
-    if (p->cache_format == K3X_CACHE_16BIT)  // bits as they are, of either type
-        hipLaunchKernelGGL((mla_load_kernel<K3X_DTYPE_BF16, K3X_CACHE_16BIT>), grid, block, 0, ctx->stream, a);
-    else if (p->cache_format == K3X_CACHE_MXFP8)
-        hipLaunchKernelGGL((mla_load_kernel<K3X_DTYPE_BF16, K3X_CACHE_MXFP8>), grid, block, 0, ctx->stream, a);
-    else
-        hipLaunchKernelGGL((mla_load_kernel<K3X_DTYPE_BF16, K3X_CACHE_MXFP4>), grid, block, 0, ctx->stream, a);
-    return launched(ctx, 1);
+    switch (p->cache_format) {
+        case K3X_CACHE_16BIT: return launch_load<K3X_CACHE_16BIT>(ctx, a);  // bits as they are
+        case K3X_CACHE_MXFP8: return launch_load<K3X_CACHE_MXFP8>(ctx, a);
+        default: return launch_load<K3X_CACHE_MXFP4>(ctx, a);
+    }
 }
 
 }  // extern "C"

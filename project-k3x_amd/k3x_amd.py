@@ -628,7 +628,8 @@ def _types() -> dict:
         _TYPES.update(
             codes={torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16},
             ints=(torch.int32, torch.uint32), f32=(torch.float32,),
-            logits=(torch.float32, torch.bfloat16), bytes=(torch.uint8,))
+            logits=(torch.float32, torch.bfloat16), bytes=(torch.uint8,),
+            of={DTYPE_BF16: (torch.bfloat16,), DTYPE_F16: (torch.float16,)})
     return _TYPES
 
 
@@ -892,19 +893,44 @@ def mla_row_bytes(latent, rotary=0, cache_format=CACHE_16BIT) -> int:
 
 
 def _mla_dtypes(p: MlaParams):
-    return tuple(t for t, code in _types()["codes"].items() if code == p.dtype)
+    return _types()["of"].get(p.dtype, ())
+
+
+def _row_step(t) -> int:
+    """Elements from row to row of a tensor whose rows are contiguous in themselves; 0 where it is
+    the row's length or there is one row."""
+    if t.is_contiguous():
+        return 0
+    shape, stride, step = t.shape, t.stride(), 1
+    for i in range(len(shape) - 1, 0, -1):
+        if shape[i] != 1 and stride[i] != step:
+            raise ValueError("expected rows that are contiguous in themselves")
+        step *= shape[i]
+    if shape[0] <= 1:
+        return 0
+    if stride[0] < step:
+        raise ValueError("expected rows that do not overlap")
+    return stride[0]
+
+
+def _mla_rows(ctx: Context, what: str, t, shape, dtypes):
+    """(device pointer, elements from row to row) of an operator's rows."""
+    if (t.shape != shape or t.dtype not in dtypes or not t.is_cuda or
+            t.get_device() != ctx.device):
+        _refuse(ctx, what, t, shape, dtypes)
+    return t.data_ptr(), _row_step(t)
 
 
 def _mla_pages(ctx: Context, p: MlaParams, pool, table, lens, offsets):
     """(pool, table, offsets, lens) pointers of an mla_* call."""
-    ints = _types()["ints"]
-    row = ctx.lib.k3x_hip_mla_row_bytes(C.byref(p))
-    # Parameters that the call refuses have no rows to compare.
-    shape = (p.pages, p.page_size, row) if row else pool.shape
-    return (_at(ctx, "pool", pool, shape, _types()["bytes"]),
-            _at(ctx, "table", table, (p.sequences, p.table_width), ints),
-            None if offsets is None else _at(ctx, "offsets", offsets, (p.sequences + 1,), ints),
-            _at(ctx, "lens", lens, (p.sequences,), ints))
+    types, N, L = _types(), p.sequences, p.latent
+    ints = types["ints"]
+    row = 2 * p.rotary + (2 * L if p.cache_format == CACHE_16BIT else
+                          16 + (L if p.cache_format == CACHE_MXFP8 else L // 2))
+    return (_at(ctx, "pool", pool, (p.pages, p.page_size, row), types["bytes"]),
+            _at(ctx, "table", table, (N, p.table_width), ints),
+            None if offsets is None else _at(ctx, "offsets", offsets, (N + 1,), ints),
+            _at(ctx, "lens", lens, (N,), ints))
 
 
 def mla_store(ctx: Context, params: MlaParams, latent, pool, table, lens, rotary=None,
@@ -913,10 +939,10 @@ def mla_store(ctx: Context, params: MlaParams, latent, pool, table, lens, rotary
     normalised first (k3x_hip_mla_store); lens [N] with these tokens, offsets [N + 1]."""
     p = MlaParams.from_buffer_copy(params)
     same = _mla_dtypes(p)
-    lp, p.latent_stride = _rows(ctx, "latent", latent, (p.tokens, p.latent), same)
+    lp, p.latent_stride = _mla_rows(ctx, "latent", latent, (p.tokens, p.latent), same)
     rp = gp = None
     if rotary is not None:
-        rp, p.rotary_stride = _rows(ctx, "rotary", rotary, (p.tokens, p.rotary), same)
+        rp, p.rotary_stride = _mla_rows(ctx, "rotary", rotary, (p.tokens, p.rotary), same)
     if gamma is not None:
         gp = _at(ctx, "gamma", gamma, (p.latent,), _types()["f32"])
     pp, tp, op, np_ = _mla_pages(ctx, p, pool, table, lens, offsets)
@@ -929,10 +955,10 @@ def mla_load(ctx: Context, params: MlaParams, pool, table, lens, latent, rotary=
     (k3x_hip_mla_load)."""
     p = MlaParams.from_buffer_copy(params)
     same = _mla_dtypes(p)
-    lp, p.latent_stride = _rows(ctx, "latent", latent, (p.tokens, p.latent), same)
+    lp, p.latent_stride = _mla_rows(ctx, "latent", latent, (p.tokens, p.latent), same)
     rp = None
     if rotary is not None:
-        rp, p.rotary_stride = _rows(ctx, "rotary", rotary, (p.tokens, p.rotary), same)
+        rp, p.rotary_stride = _mla_rows(ctx, "rotary", rotary, (p.tokens, p.rotary), same)
     pp, tp, op, np_ = _mla_pages(ctx, p, pool, table, lens, offsets)
     return ctx.lib.k3x_hip_mla_load(ctx.handle, C.byref(p), pp, tp, op, np_, lp, rp)
 
@@ -947,8 +973,8 @@ def mla_attention(ctx: Context, params: MlaParams, q, pool, table, lens, out, of
     fp32 (k3x_hip_mla_attention)."""
     p = MlaParams.from_buffer_copy(params)
     T, H, same = p.tokens, p.heads, _mla_dtypes(p)
-    qp, p.q_stride = _rows(ctx, "q", q, (T, H, p.latent + p.rotary), same)
-    yp, p.out_stride = _rows(ctx, "out", out, (T, H, p.latent), same)
+    qp, p.q_stride = _mla_rows(ctx, "q", q, (T, H, p.latent + p.rotary), same)
+    yp, p.out_stride = _mla_rows(ctx, "out", out, (T, H, p.latent), same)
     ep = None if lse is None else _at(ctx, "lse", lse, (T, H), _types()["f32"])
     pp, tp, op, np_ = _mla_pages(ctx, p, pool, table, lens, offsets)
     return ctx.lib.k3x_hip_mla_attention(ctx.handle, C.byref(p), qp, pp, tp, op, np_, yp, ep,
@@ -992,13 +1018,13 @@ def mla_prompt(ctx: Context, params: MlaPromptParams, q, k, v, out, rotary=None,
     T, S, H, N, same = p.tokens, p.keys, p.heads, p.sequences, (q.dtype,)
     ints = _types()["ints"]
     p.dtype = _dtype(q)
-    qp, p.q_stride = _rows(ctx, "q", q, (T, H, p.key_dim + p.rotary), same)
+    qp, p.q_stride = _mla_rows(ctx, "q", q, (T, H, p.key_dim + p.rotary), same)
     kp, p.k_stride, p.k_head_stride = _head_rows(ctx, "k", k, (S, H, p.key_dim), same)
     vp, p.v_stride, p.v_head_stride = _head_rows(ctx, "v", v, (S, H, p.value_dim), same)
-    yp, p.out_stride = _rows(ctx, "out", out, (T, H, p.value_dim), same)
+    yp, p.out_stride = _mla_rows(ctx, "out", out, (T, H, p.value_dim), same)
     rp = op = fp = ep = None
     if rotary is not None:
-        rp, p.rotary_stride = _rows(ctx, "rotary", rotary, (S, p.rotary), same)
+        rp, p.rotary_stride = _mla_rows(ctx, "rotary", rotary, (S, p.rotary), same)
     if offsets is not None:
         op = _at(ctx, "offsets", offsets, (N + 1,), ints)
     if key_offsets is not None:
