@@ -82,8 +82,10 @@ typedef __attribute__((address_space(3))) uint8_t lds_byte;
 __device__ inline u32x4 lds16(const lds_byte* p) {
     return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(p);
 }
-// Of a 16-lane row's four tokens by 16 columns, its lane's column.
-__device__ inline uint2 lds_transposed(const lds_byte* p) {
+// Of a 16-lane row's four tokens by 16 columns, its lane's column.  __restrict__: read
+// without it the compiler waits for every direct load to LDS before, those of later
+// tiles too; what may be read is settled by the tile's own wait and barrier.
+__device__ inline uint2 lds_transposed(const lds_byte* __restrict__ p) {
     typedef __attribute__((ext_vector_type(4))) short s16x4;
     return __builtin_bit_cast(
         uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -95,5 +97,34 @@ __device__ inline void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 __device__ inline void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// o[FROM .. FROM + N - 1] *= k.  HELD: the kernel's results fill so much of the
+// register file that they stay in its accumulators, which no other instruction
+// multiplies: each goes through one register in between.  (Left to the compiler, the
+// branch around this makes it hold them twice: in mla_attention.hip 700 registers go to
+// memory.)  The products that wrote them have ended: those of the next tile's scores lie
+// between, and the waits here cover what the compiler does not see.
+template <bool HELD, int FROM, int N, int OT, typename Acc>
+__device__ __forceinline__ void scale_tiles(Acc (&o)[OT], float k) {
+    constexpr int W = sizeof(Acc) / 4;
+    if constexpr (!HELD) {
+#pragma unroll
+        for (int i = FROM; i < FROM + N; ++i) o[i] *= k;
+    } else {
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+        for (int i = FROM; i < FROM + N; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                float x = o[i][j], t;
+                asm volatile(
+                    "v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\t"
+                    "v_accvgpr_write_b32 %0, %1"
+                    : "+a"(x), "=&v"(t) : "v"(k));
+                o[i][j] = x;
+            }
+        asm volatile("s_nop 15" ::: "memory");
+    }
+}
 
 }  // namespace k3x_mla

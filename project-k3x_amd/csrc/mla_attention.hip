@@ -61,34 +61,6 @@ struct Shape {
     static constexpr int rows = HT * WM;
 };
 
-// o *= k.  Results that fill half of the register file and more stay in its
-// accumulators, which no other instruction multiplies: each goes through one
-// register in between.  (Left to the compiler, the branch around this makes it
-// hold them twice, and 700 registers go to memory.)  The products that wrote them
-// have ended: those of the next tile's scores lie between.
-template <int OT, typename Acc>
-__device__ __forceinline__ void scale_all(Acc (&o)[OT], float k) {
-    constexpr int W = sizeof(Acc) / 4;
-    if constexpr (OT * W < 128) {
-#pragma unroll
-        for (int i = 0; i < OT; ++i) o[i] *= k;
-    } else {
-        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-        for (int i = 0; i < OT; ++i)
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                float x = o[i][j], t;
-                asm volatile(
-                    "v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\t"
-                    "v_accvgpr_write_b32 %0, %1"
-                    : "+a"(x), "=&v"(t) : "v"(k));
-                o[i][j] = x;
-            }
-        asm volatile("s_nop 15" ::: "memory");
-    }
-}
-
 // Tiles of a sequence in the line; an empty one takes one, in which its rows are
 // written as empty.
 __device__ inline uint32_t tiles_in(const Tokens& s) { return max(1u, (s.len + kTile - 1) / kTile); }
@@ -104,6 +76,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     constexpr uint32_t kBuffer = CG * kGroup;
     constexpr int KS = HT == 32 ? 4 : 2;        // products over 64 columns
     constexpr int OT = LP / HT / WD;            // tiles of the latent, a wave
+    constexpr int AHEAD = F != K3X_CACHE_16BIT && S::rows == 128 ? 4 : 8;  // operands on their way
     typedef Mma<DT, HT> M;
     typedef typename M::Acc Acc;
     // One array: with several the compiler tells them apart, and waits for all direct
@@ -186,7 +159,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     __syncthreads();
 
     // What is not brought to LDS stays zero there.
-    if (!FULL || a.R < 64) {
+    if (!FULL) {
         for (uint32_t i = tid * 16; i < BUFS * kBuffer; i += kThreads * 16)
             *reinterpret_cast<u32x4*>(smem + i) = u32x4{};
         __syncthreads();
@@ -260,69 +233,91 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                                   : DIRECT               ? 1
                                                          : LP / 64;
             u32x4 codes[UNITS], scales, turned;
-            // Loads of a tile: straight to buffer b, or to registers.
-            auto bring = [&](uint32_t t, uint32_t b, uint32_t id) {
+            // A tile's loads, straight to a buffer or to registers, in steps that can stand
+            // between products: 0 finds the rows, the others load.
+            struct {
+                __amdgpu_buffer_rsrc_t rows8;
+                uint32_t from, turn;
+                u32x4* dst;
+                const uint8_t* row;
+            } src;
+            constexpr int kBring = DIRECT ? CG + 1 : UNITS + 3;
+            auto bring = [&](int step, uint32_t t, uint32_t b, uint32_t id) {
                 if constexpr (DIRECT) {
                     // Eight tokens a wave, each load 128 bytes of every one.
-                    const uint32_t p = eight(t);
-                    const uint8_t* row = row_of(p, __builtin_amdgcn_readfirstlane(id));
-                    const auto rows8 = __builtin_amdgcn_make_buffer_rsrc(
-                        const_cast<uint8_t*>(row), 0, 8 * a.pages.row.bytes, 0x00020000);
-                    const uint32_t from = (position(t) - p) * a.pages.row.bytes + bput * 16;
-                    u32x4* dst = reinterpret_cast<u32x4*>(smem + b * kBuffer + wave * 1024);
-#pragma unroll
-                    for (int c = 0; c < CG - 1; ++c)
-                        load_lds16(rows8, dst + c * (kGroup / 16), from, c * 128);
-                    if (bput < a.R / 8)
-                        load_lds16(rows8, dst + (CG - 1) * (kGroup / 16), from, LP * 2);
-                } else {
-                    const uint8_t* row = row_of(position(t), id);
-#pragma unroll
-                    for (int k = 0; k < UNITS; ++k) {
-                        const uint32_t u = bcol + 8 * k;
-                        codes[k] = FULL || u * 16 < a.pages.row.codes
-                                       ? *reinterpret_cast<const u32x4*>(row + u * 16) : u32x4{};
+                    if (step == 0) {
+                        const uint32_t p = eight(t);
+                        const uint8_t* row = row_of(p, __builtin_amdgcn_readfirstlane(id));
+                        src.rows8 = __builtin_amdgcn_make_buffer_rsrc(
+                            const_cast<uint8_t*>(row), 0, 8 * a.pages.row.bytes, 0x00020000);
+                        src.from = (position(t) - p) * a.pages.row.bytes + bput * 16;
+                        // Columns without a rotary part meet zeros of the queries: any
+                        // number will do there.
+                        src.turn = bput < a.R / 8 ? LP * 2 : 0;
+                        src.dst = reinterpret_cast<u32x4*>(smem + b * kBuffer + wave * 1024);
+                    } else if (step < CG) {
+                        load_lds16(src.rows8, src.dst + (step - 1) * (kGroup / 16), src.from,
+                                   (step - 1) * 128);
+                    } else {
+                        load_lds16(src.rows8, src.dst + (CG - 1) * (kGroup / 16),
+                                   src.from + src.turn, 0);
                     }
-                    if constexpr (F != K3X_CACHE_16BIT)
-                        scales = *reinterpret_cast<const u32x4*>(row + a.pages.row.scales);
-                    if (bcol < a.R / 8)
-                        turned = *reinterpret_cast<const u32x4*>(row + a.pages.row.codes + bcol * 16);
+                } else {
+                    if (step == 0) {
+                        src.row = row_of(position(t), id);
+                    } else if (step <= UNITS) {
+                        const uint32_t u = bcol + 8 * (step - 1);
+                        codes[step - 1] = FULL || u * 16 < a.pages.row.codes
+                                              ? *reinterpret_cast<const u32x4*>(src.row + u * 16)
+                                              : u32x4{};
+                    } else if (step == UNITS + 1) {
+                        if constexpr (F != K3X_CACHE_16BIT)
+                            scales = *reinterpret_cast<const u32x4*>(src.row + a.pages.row.scales);
+                    } else {
+                        turned = *reinterpret_cast<const u32x4*>(
+                            src.row + (bcol < a.R / 8 ? a.pages.row.codes + bcol * 16 : 0));
+                    }
                 }
             };
-            // Codes in registers to the values that they stand for in buffer b.
-            auto put = [&](uint32_t b) {
+            auto bring_all = [&](uint32_t t, uint32_t b, uint32_t id) {
+#pragma unroll
+                for (int i = 0; i < kBring; ++i) bring(i, t, b, id);
+            };
+            // Codes in registers to the values that they stand for in buffer b, in steps.
+            constexpr int kPut = DIRECT ? 0 : UNITS + 1;
+            auto put = [&](int k, uint32_t b) {
                 if constexpr (!DIRECT) {
                     uint8_t* dst = smem + b * kBuffer + btok * 128;
                     const uint32_t z = swizzle(btok);
+                    if (k == UNITS) {
+                        *reinterpret_cast<u32x4*>(dst + (CG - 1) * kGroup + (bcol ^ z) * 16) =
+                            turned & (bcol < a.R / 8 ? 0xffffffffu : 0u);
+                        return;
+                    }
+                    const uint32_t u = bcol + 8 * k;
+                    if constexpr (F == K3X_CACHE_16BIT) {
+                        if (u * 8 < a.L)
+                            *reinterpret_cast<u32x4*>(dst + k * kGroup + (bcol ^ z) * 16) = codes[k];
+                    } else if constexpr (F == K3X_CACHE_MXFP8) {
+                        const float sc = e8m0_to_f32(scales[k] >> (bcol / 2 * 8) & 0xff);
 #pragma unroll
-                    for (int k = 0; k < UNITS; ++k) {
-                        const uint32_t u = bcol + 8 * k;
-                        if constexpr (F == K3X_CACHE_16BIT) {
-                            if (u * 8 < a.L)
-                                *reinterpret_cast<u32x4*>(dst + k * kGroup + (bcol ^ z) * 16) = codes[k];
-                        } else if constexpr (F == K3X_CACHE_MXFP8) {
-                            const float sc = e8m0_to_f32(scales[k] >> (bcol / 2 * 8) & 0xff);
+                        for (int j = 0; j < 2; ++j) {
+                            const uint32_t x = 2 * (u % 4) + j;
+                            if (FULL || u * 16 < a.L)
+                                *reinterpret_cast<bf16x8*>(dst + u / 4 * kGroup + (x ^ z) * 16) =
+                                    mxfp8_8(uint2{codes[k][2 * j], codes[k][2 * j + 1]}, sc);
+                        }
+                    } else {
+                        const uint32_t dw = bcol / 4 ? scales[2 * k + 1] : scales[2 * k];
+                        const float sc = e8m0_to_f32(dw >> (bcol % 4 * 8) & 0xff);
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const uint32_t x = 2 * (u % 4) + j;
-                                if (FULL || u * 16 < a.L)
-                                    *reinterpret_cast<bf16x8*>(dst + u / 4 * kGroup + (x ^ z) * 16) =
-                                        mxfp8_8(uint2{codes[k][2 * j], codes[k][2 * j + 1]}, sc);
-                            }
-                        } else {
-                            const uint32_t dw = bcol / 4 ? scales[2 * k + 1] : scales[2 * k];
-                            const float sc = e8m0_to_f32(dw >> (bcol % 4 * 8) & 0xff);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint32_t x = 4 * (u % 2) + j;
-                                if (FULL || u * 32 < a.L)
-                                    *reinterpret_cast<bf16x8*>(dst + u / 2 * kGroup + (x ^ z) * 16) =
-                                        dequant8(codes[k][j], sc);
-                            }
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t x = 4 * (u % 2) + j;
+                            if (FULL || u * 32 < a.L)
+                                *reinterpret_cast<bf16x8*>(dst + u / 2 * kGroup + (x ^ z) * 16) =
+                                    dequant8(codes[k][j], sc);
                         }
                     }
-                    if (bcol < a.R / 8)
-                        *reinterpret_cast<u32x4*>(dst + (CG - 1) * kGroup + (bcol ^ z) * 16) = turned;
                 }
             };
 
@@ -345,57 +340,53 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
             };
 
             // ---- one tile ---------------------------------------------------
-            auto tile = [&](uint32_t t, uint32_t b) {
+            // Beside its products the loads of a later tile: direct ones to buffer nb; through
+            // registers, tile t + 1 from them to the other buffer, then tile t + 2 to them.
+            auto tile = [&](uint32_t t, uint32_t b, uint32_t nb, uint32_t id) {
                 const lds_byte* kb = lds + b * kBuffer;
-                // Operands of the next group of columns (or tile of the latent) are read
-                // beside the products of this one, and no further ahead: the scheduler
-                // would read all of them first, past the registers there are.
-                constexpr int XT = HT == 32 ? 1 : 2;
+                // Operands are read a few products ahead: LDS takes some 200 cycles for four
+                // waves at once, a product 32.  (Left to itself the scheduler reads all of
+                // them first, past the registers there are.)
+                constexpr int XT = HT == 32 ? 1 : 2, HV = HT == 32 ? 2 : 1;
+                constexpr int NK = CG * KS * XT, NW = OT * HV;
                 Acc sc[XT];
 #pragma unroll
                 for (int i = 0; i < XT; ++i) sc[i] = Acc{};
-                u32x4 kf[2][KS][XT];
+                u32x4 kf[AHEAD];
                 const uint32_t kat = opaque(kat0);
-                auto keys = [&](int c) {
-#pragma unroll
-                    for (int i = 0; i < KS; ++i)
-#pragma unroll
-                        for (int x = 0; x < XT; ++x)
-                            kf[c & 1][i][x] = lds16(kb + c * kGroup + x * 2048 + (kat ^ i * (128 / KS)));
-                };
-                auto products = [&](int c) {
-#pragma unroll
-                    for (int i = 0; i < KS; ++i)
-#pragma unroll
-                        for (int x = 0; x < XT; ++x)
-                            sc[x] = M::run(kf[c & 1][i][x], qf[c * KS + i], sc[x]);
+                auto keys = [&](int i) {
+                    const int c = i / (KS * XT), y = i / XT % KS, x = i % XT;
+                    kf[i % AHEAD] = lds16(kb + c * kGroup + x * 2048 + (kat ^ y * (128 / KS)));
                 };
                 // (Without a rotary part its group is zeros.)
-                keys(0);
 #pragma unroll
-                for (int c = 0; c < CG; ++c) {
-                    if (c + 1 < CG) keys(c + 1);
+                for (int i = 0; i < AHEAD - 1; ++i) keys(i);
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    if (i + AHEAD - 1 < NK) keys(i + AHEAD - 1);
+                    if constexpr (DIRECT)
+#pragma unroll
+                        for (int x = 0; x < kBring; ++x)
+                            if (x * NK / kBring == i) bring(x, min(t + BUFS - 1, end - 1), nb, id);
                     __builtin_amdgcn_sched_barrier(0);
-                    products(c);
+                    sc[i % XT] = M::run(kf[i % AHEAD], qf[i / XT], sc[i % XT]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                constexpr int HV = HT == 32 ? 2 : 1;
-                u32x4 vf[2][HV];
+                u32x4 vf[AHEAD];
                 const uint32_t vat = opaque(vat0);
-                auto values = [&](int y) {
+                auto values = [&](int i) {
+                    const int y = i / HV, h = i % HV;
                     const uint32_t d = y + wd * OT;  // tile of HT columns of the latent
-                    const lds_byte* vb = kb + d * HT / 64 * kGroup;
+                    const lds_byte* vb = kb + d * HT / 64 * kGroup + h * 2048;
                     const uint32_t at = vat ^ y % (64 / HT) * (HT * 2);
-#pragma unroll
-                    for (int h = 0; h < HV; ++h) {
-                        // Tokens 16 h .. 16 h + 15 (or all 32), by fours of each half.
-                        const uint2 v0 = lds_transposed(vb + h * 2048 + at);
-                        const uint2 v1 = HT == 32 ? lds_transposed(vb + h * 2048 + 1024 + (at ^ 16))
-                                                  : lds_transposed(vb + 2048 + at);
-                        vf[y & 1][h] = u32x4{v0.x, v0.y, v1.x, v1.y};
-                    }
+                    // Tokens 16 h .. 16 h + 15 (or all 32), by fours of each half.
+                    const uint2 v0 = lds_transposed(vb + at);
+                    const uint2 v1 = HT == 32 ? lds_transposed(vb + 1024 + (at ^ 16))
+                                              : lds_transposed(vb + 2048 + at);
+                    vf[i % AHEAD] = u32x4{v0.x, v0.y, v1.x, v1.y};
                 };
-                values(0);  // on their way while weights are formed
+#pragma unroll
+                for (int i = 0; i < AHEAD - 1; ++i) values(i);  // while weights are formed
                 constexpr int NV = HT == 32 ? 16 : 8;
                 float x[NV];
 #pragma unroll
@@ -420,7 +411,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     const float up = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - up);
                     m = up;
                     l *= keep;
-                    if (t != t0) scale_all<OT>(o, keep);
+                    if (t != t0) scale_tiles<OT * sizeof(Acc) >= 512, 0, OT>(o, keep);
                 }
                 uint32_t p[NV / 2];
                 float sum = 0.0f;
@@ -433,14 +424,19 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                 }
                 l += sum;
 #pragma unroll
-                for (int y = 0; y < OT; ++y) {
-                    if (y + 1 < OT) values(y + 1);
-                    __builtin_amdgcn_sched_barrier(0);
+                for (int i = 0; i < NW; ++i) {
+                    if (i + AHEAD - 1 < NW) values(i + AHEAD - 1);
+                    if constexpr (!DIRECT)
 #pragma unroll
-                    for (int h = 0; h < HV; ++h)
-                        o[y] = M::run(vf[y & 1][h],
-                                      u32x4{p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]},
-                                      o[y]);
+                        for (int x = 0; x < kPut + kBring; ++x)
+                            if (x * NW / (kPut + kBring) == i) {
+                                if (x < kPut) put(x, nb);
+                                else bring(x - kPut, min(t + 2, end - 1), 0, id);
+                            }
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int y = i / HV, h = i % HV;
+                    o[y] = M::run(vf[i % AHEAD],
+                                  u32x4{p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]}, o[y]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
@@ -454,37 +450,36 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
 #pragma unroll
                     for (uint32_t i = 0; i < BUFS - 1; ++i) {
                         next = page_of(min(t0 + i + 1, end - 1));
-                        bring(min(t0 + i, end - 1), i, id);
+                        bring_all(min(t0 + i, end - 1), i, id);
                         id = next;
                     }
                     load_queries();
                     uint32_t b = 0;
                     for (uint32_t t = t0; t < end; ++t) {
-                        if (a.R) wait_loads<(BUFS - 2) * CG>();
-                        else wait_loads<(BUFS - 2) * (CG - 1)>();
+                        wait_loads<(BUFS - 2) * CG>();
                         barrier();
                         next = page_of(min(t + BUFS, end - 1));
-                        bring(min(t + BUFS - 1, end - 1), b >= 1 ? b - 1 : BUFS - 1, id);
+                        tile(t, b, b >= 1 ? b - 1 : BUFS - 1, id);
                         id = next;
-                        tile(t, b);
                         b = b + 1 == BUFS ? 0 : b + 1;
                     }
                     wait_loads<0>();
                     barrier();
                 } else {
-                    uint32_t id = page_of(t0), next = page_of(min(t0 + 1, end - 1));
-                    bring(t0, 0, id);
+                    const uint32_t id = page_of(t0);
+                    uint32_t next = page_of(min(t0 + 1, end - 1));
+                    bring_all(t0, 0, id);
                     load_queries();
-                    put(0);
-                    bring(min(t0 + 1, end - 1), 0, next);
+#pragma unroll
+                    for (int i = 0; i < kPut; ++i) put(i, 0);
+                    bring_all(min(t0 + 1, end - 1), 0, next);
                     next = page_of(min(t0 + 2, end - 1));
                     uint32_t b = 0;
                     for (uint32_t t = t0; t < end; ++t) {
                         barrier();
-                        put(b ^ 1);
-                        bring(min(t + 2, end - 1), 0, next);
+                        const uint32_t now = next;
                         next = page_of(min(t + 3, end - 1));
-                        tile(t, b);
+                        tile(t, b, b ^ 1, now);
                         b ^= 1;
                     }
                     barrier();

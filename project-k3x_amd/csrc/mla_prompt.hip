@@ -21,14 +21,13 @@ using namespace k3x_mla;
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kRows = 128;  // queries a workgroup
 
 struct PromptArgs {
     const void *q, *k, *v, *rotary;
     const uint32_t *offsets, *key_offsets;
     void* out;
     float* lse;
-    uint32_t N, T, S, H, Dn, R, Dv, causal, blocks;
+    uint32_t N, T, S, H, Dn, R, Dv, causal, blocks, flip;
     uint64_t qs, ks, vs, rs, os, kh, vh;
     float rate;  // scale * log2(e)
     uint32_t* status;
@@ -58,11 +57,14 @@ __device__ inline bool ranges_of(const PromptArgs& a, uint32_t n, Ranges* r) {
     return e >= b && e <= a.T && g >= f && g <= a.S;
 }
 
-// KD columns of a key and VD of a value at most, in groups of 64 in LDS.  FULL:
-// Dn and R are whole groups and Dv is VD, so that nothing is left out.
-template <uint32_t DT, int KD, int VD, int TILE, bool FULL>
-__global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
+// RT tiles of 32 queries a wave.  KD columns of a key and VD of a value at most, in
+// groups of 64 in LDS; TILE keys a step.  OWN > 0: Dn is OWN whole groups, R the
+// others and Dv is VD, so that nothing is left out.
+template <uint32_t DT, int RT, int KD, int VD, int TILE, int OWN>
+__global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(PromptArgs a) {
+    constexpr bool FULL = OWN > 0;
     constexpr int KG = KD / 64, VG = VD / 64, ST = TILE / 32, OT = VD / 32;
+    constexpr uint32_t kRows = 128 * RT;         // queries a workgroup
     constexpr uint32_t kGroup = TILE * 128;      // bytes of a group
     constexpr uint32_t kBuffer = (KG + VG) * kGroup;
     typedef Mma<DT, 32> M;
@@ -75,7 +77,8 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t h = blockIdx.x % a.H;
-    const uint32_t block = a.blocks - 1 - blockIdx.x / a.H;
+    const uint32_t at = blockIdx.x / a.H, half = a.blocks / 2;
+    const uint32_t block = a.flip && at >= a.blocks - half ? at - (a.blocks - half) : a.blocks - 1 - at;
     if (*(volatile uint32_t*)a.status) return;
 
     // The sequence that the block is in: blocks of 128 queries, sequence by sequence.
@@ -121,14 +124,14 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
     }
 
     const uint32_t col = lane & 31, g = lane >> 5;
-    const uint32_t i = min(i0 + 32 * wave + col, s.m - 1);  // the lane's query
+    const uint32_t w0 = i0 + 32 * RT * wave;                   // the wave's first query
     const int32_t hidden = a.causal ? (int32_t)(s.m - 1) : 0;  // keys of the first query's future
+    auto query = [&](int x) { return min(w0 + 32 * x + col, s.m - 1); };  // the lane's
     auto sees_of = [&](uint32_t x) {
         return a.causal ? (int32_t)s.n - hidden + (int32_t)x : (int32_t)s.n;
     };
-    const int32_t sees = sees_of(i);
-    const int32_t least = sees_of(min(i0 + 32 * wave, s.m - 1));  // of the wave
-    const int32_t most = sees_of(min(i0 + kRows - 1, s.m - 1));   // of the workgroup
+    const int32_t least = sees_of(min(w0, s.m - 1));             // of the wave
+    const int32_t most = sees_of(min(i0 + kRows - 1, s.m - 1));  // of the workgroup
     const uint32_t tiles = most > 0 ? ((uint32_t)most + TILE - 1) / TILE : 0;
 
     const uint32_t kat0 = col * 128 + (g ^ swizzle(col)) * 16;
@@ -137,162 +140,214 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
                           (i16 & 1) * 8;
     // What the lane brings: token 8 (wave + 4 x) + lane / 8 of a tile, 16 bytes a group.
     const uint32_t btok = 8 * wave + lane / 8, bput = lane % 8 ^ swizzle(btok);
+    const uint32_t own = FULL ? OWN : (a.Dn + 63) / 64;  // groups of a head's own columns, then the rotary part's
 
-    u32x4 qf[KG * 4];
-    {
-        const uint8_t* q = static_cast<const uint8_t*>(a.q) +
-                           2 * ((uint64_t)(s.q + i) * a.qs + (uint64_t)h * (a.Dn + a.R));
-        // Groups of the head's own columns, then those of the rotary part.
-        const uint32_t own = (a.Dn + 63) / 64;
-#pragma unroll
-        for (int c = 0; c < KG; ++c)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const bool mine = (uint32_t)c < own;
-                const uint32_t d = (mine ? c * 64 : (c - own) * 64) + x * 16 + g * 8;
-                const bool in = FULL ? mine || d < a.R : d < (mine ? a.Dn : a.R);
-                const u32x4 y = *reinterpret_cast<const u32x4*>(
-                    q + (in ? 2 * (mine ? d : a.Dn + d) : 0));
-                qf[c * 4 + x] = y & (in ? 0xffffffffu : 0u);
-            }
-    }
-    Acc o[OT];
-#pragma unroll
-    for (int x = 0; x < OT; ++x) o[x] = Acc{};
-    float m = -3.4028235e38f, l = 0.0f;
-
-    const uint32_t own = (a.Dn + 63) / 64;
-    auto bring = [&](uint32_t t, uint32_t b) {
-#pragma unroll
-        for (int x = 0; x < TILE / 32; ++x) {
-            // Eight tokens a wave and load, from the first of the eight.
-            const uint32_t p = min(t * TILE + 32 * x + 8 * wave, s.n - 1);
-            const uint32_t to = min(t * TILE + 32 * x + btok, s.n - 1) - p;
-            const uint64_t row = s.k + p;
-            u32x4* dst = reinterpret_cast<u32x4*>(smem + b * kBuffer + x * 4096 + wave * 1024);
-            auto rows8 = [&](const void* base, uint64_t stride, uint64_t at) {
-                return __builtin_amdgcn_make_buffer_rsrc(
-                    static_cast<uint8_t*>(const_cast<void*>(base)) + 2 * (row * stride + at), 0,
-                    0xffffffffu, 0x00020000);
-            };
-            const auto kr = rows8(a.k, a.ks, h * a.kh), vr = rows8(a.v, a.vs, h * a.vh);
-            const uint32_t kf = to * (uint32_t)(2 * a.ks) + bput * 16;
-            const uint32_t vf = to * (uint32_t)(2 * a.vs) + bput * 16;
-#pragma unroll
-            for (int c = 0; c < KG; ++c)
-                if ((uint32_t)c < own && (FULL || c * 8 + bput < a.Dn / 8))
-                    load_lds16(kr, dst + c * (kGroup / 16), kf, c * 128);
-            if (bput < a.R / 8) {
-                const auto rr = rows8(a.rotary, a.rs, 0);
-                load_lds16(rr, dst + own * (kGroup / 16), to * (uint32_t)(2 * a.rs) + bput * 16, 0);
-            }
-#pragma unroll
-            for (int c = 0; c < VG; ++c)
-                if (FULL || c * 8 + bput < a.Dv / 8)
-                    load_lds16(vr, dst + (KG + c) * (kGroup / 16), vf, c * 128);
+    // A tile's loads in pieces, each 128 bytes of eight tokens a wave: they take long to
+    // be issued, so they are spread over the products.
+    struct Source {
+        __amdgpu_buffer_rsrc_t k, v, r;
+        uint32_t kf, vf, rf;
+        u32x4* dst;
+    };
+    auto source = [&](uint32_t t, uint32_t b, int x) {
+        const uint32_t p = min(t * TILE + 32 * x + 8 * wave, s.n - 1);
+        const uint32_t to = min(t * TILE + 32 * x + btok, s.n - 1) - p;
+        const uint64_t row = s.k + p;
+        auto from = [&](const void* base, uint64_t stride, uint64_t at) {
+            return __builtin_amdgcn_make_buffer_rsrc(
+                static_cast<uint8_t*>(const_cast<void*>(base)) + 2 * (row * stride + at), 0,
+                0xffffffffu, 0x00020000);
+        };
+        return Source{from(a.k, a.ks, h * a.kh), from(a.v, a.vs, h * a.vh),
+                      from(a.rotary, a.rs, 0), to * (uint32_t)(2 * a.ks) + bput * 16,
+                      to * (uint32_t)(2 * a.vs) + bput * 16, to * (uint32_t)(2 * a.rs) + bput * 16,
+                      reinterpret_cast<u32x4*>(smem + b * kBuffer + x * 4096 + wave * 1024)};
+    };
+    constexpr int kPieces = KG + VG;
+    auto bring = [&](const Source& f, int c) {
+        if (c >= KG) {
+            if (FULL || (c - KG) * 8 + bput < a.Dv / 8)
+                load_lds16(f.v, f.dst + c * (kGroup / 16), f.vf, (c - KG) * 128);
+        } else if ((uint32_t)c < own) {
+            if (FULL || c * 8 + bput < a.Dn / 8)
+                load_lds16(f.k, f.dst + c * (kGroup / 16), f.kf, c * 128);
+        } else if ((uint32_t)c == own && (FULL || bput < a.R / 8)) {
+            load_lds16(f.r, f.dst + c * (kGroup / 16), f.rf, 0);
         }
     };
 
-    auto tile = [&](uint32_t t, uint32_t b) {
-        const lds_byte* kb = lds + b * kBuffer;
-        Acc sc[ST];
+    u32x4 qf[RT][KG * 4];
 #pragma unroll
-        for (int x = 0; x < ST; ++x) sc[x] = Acc{};
+    for (int x = 0; x < RT; ++x) {
+        const uint8_t* q = static_cast<const uint8_t*>(a.q) +
+                           2 * ((uint64_t)(s.q + query(x)) * a.qs + (uint64_t)h * (a.Dn + a.R));
 #pragma unroll
         for (int c = 0; c < KG; ++c)
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+            for (int y = 0; y < 4; ++y) {
+                const bool mine = (uint32_t)c < own;
+                const uint32_t d = (mine ? c * 64 : (c - own) * 64) + y * 16 + g * 8;
+                const bool in = FULL || d < (mine ? a.Dn : a.R);
+                const u32x4 z = *reinterpret_cast<const u32x4*>(
+                    q + (in ? 2 * (mine ? d : a.Dn + d) : 0));
+                qf[x][c * 4 + y] = z & (in ? 0xffffffffu : 0u);
+            }
+    }
+    Acc o[RT * OT];
+#pragma unroll
+    for (int x = 0; x < RT * OT; ++x) o[x] = Acc{};
+    float m[RT], l[RT];
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+        m[x] = -3.4028235e38f;
+        l[x] = 0.0f;
+    }
+
+    // Tile t in buffer b; the next one's loads (the last one's again) to the other.
+    auto tile = [&](uint32_t t, uint32_t b) {
+        const lds_byte* kb = lds + b * kBuffer;
+        Source next[ST];
+#pragma unroll
+        for (int x = 0; x < ST; ++x) next[x] = source(min(t + 1, tiles - 1), b ^ 1, x);
+        Acc sc[RT][ST];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int x = 0; x < ST; ++x) sc[r][x] = Acc{};
+        // Operands are read a few products ahead: LDS takes some 200 cycles, four waves
+        // at once, a product 32.
+        constexpr int NK = KG * 4 * ST, kAhead = 8;
+        u32x4 kf[kAhead];
+        auto keys = [&](int i) {
+            const int y = i / ST, x = i % ST;
+            kf[i % kAhead] = lds16(kb + y / 4 * kGroup + x * 4096 + (kat0 ^ y % 4 * 32));
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; ++i) keys(i);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            if (i + kAhead - 1 < NK) keys(i + kAhead - 1);
+            if (i % 2 == 0 && i / 2 < ST * kPieces) bring(next[i / 2 % ST], i / 2 / ST);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                sc[r][i % ST] = M::run(kf[i % kAhead], qf[r][i / ST], sc[r][i % ST]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        static_assert(2 * ST * kPieces <= NK + 1, "pieces within the products");
+        // The first values are on their way while weights are formed.
+        constexpr int NF = ST * OT * 2;
+        u32x4 vf[kAhead];
+        auto values = [&](int i) {  // i: 32 keys, 32 columns, 16 of the keys
+            const int x = i / (2 * OT), y = i / 2 % OT, z = i % 2;
+            const lds_byte* vb = kb + (KG + y / 2) * kGroup + x * 4096 + z * 2048;
+            const uint32_t c = vat0 ^ y % 2 * 64;
+            const uint2 v0 = lds_transposed(vb + c), v1 = lds_transposed(vb + 1024 + (c ^ 16));
+            vf[i % kAhead] = u32x4{v0.x, v0.y, v1.x, v1.y};
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; ++i) values(i);
+        uint32_t p[RT][ST][8];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            if ((int32_t)((t + 1) * TILE) > least) {
+                // Past what the query sees.
+                const int32_t sees = sees_of(query(r));
 #pragma unroll
                 for (int x = 0; x < ST; ++x)
-                    sc[x] = M::run(lds16(kb + c * kGroup + x * 4096 + (kat0 ^ y * 32)),
-                                   qf[c * 4 + y], sc[x]);
-        if ((int32_t)((t + 1) * TILE) > least) {
-            // Past what the query sees.
+#pragma unroll
+                    for (int y = 0; y < 16; ++y)
+                        if ((int32_t)(t * TILE + 32 * x + 8 * (y / 4) + 4 * g + y % 4) >= sees)
+                            sc[r][x][y] = -__builtin_inff();
+            }
+            float top = sc[r][0][0];
 #pragma unroll
             for (int x = 0; x < ST; ++x)
 #pragma unroll
-                for (int y = 0; y < 16; ++y)
-                    if ((int32_t)(t * TILE + 32 * x + 8 * (y / 4) + 4 * g + y % 4) >= sees)
-                        sc[x][y] = -__builtin_inff();
-        }
-        float top = sc[0][0];
-#pragma unroll
-        for (int x = 0; x < ST; ++x)
-#pragma unroll
-            for (int y = 0; y < 16; ++y) top = fmaxf(top, sc[x][y]);
-        top = across<32>(top, [](float p, float r) { return fmaxf(p, r); }) * a.rate;
-        // The maximum may lag by 2^8: see mla_attention.hip.
-        if (__any(top > m + 8.0f)) {
-            const float up = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - up);
-            m = up;
-            l *= keep;
-#pragma unroll
-            for (int x = 0; x < OT; ++x) o[x] *= keep;
-        }
-        uint32_t p[ST][8];
-        float sum = 0.0f;
-#pragma unroll
-        for (int x = 0; x < ST; ++x)
-#pragma unroll
-            for (int y = 0; y < 16; y += 2) {
-                const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][y], a.rate, -m));
-                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][y + 1], a.rate, -m));
-                sum += u + v;
-                p[x][y / 2] = pack2<DT>(u, v);
+                for (int y = 0; y < 16; ++y) top = fmaxf(top, sc[r][x][y]);
+            top = across<32>(top, [](float u, float v) { return fmaxf(u, v); }) * a.rate;
+            // The maximum may lag by 2^8: see mla_attention.hip.
+            if (__any(top > m[r] + 8.0f)) {
+                const float up = fmaxf(m[r], top), keep = __builtin_amdgcn_exp2f(m[r] - up);
+                m[r] = up;
+                l[r] *= keep;
+                if (r == 0) scale_tiles<RT == 2, 0, OT>(o, keep);
+                else scale_tiles<RT == 2, (RT - 1) * OT, OT>(o, keep);
             }
-        l += sum;
+            float sum = 0.0f;
 #pragma unroll
-        for (int x = 0; x < ST; ++x)
+            for (int x = 0; x < ST; ++x)
 #pragma unroll
-            for (int y = 0; y < OT; ++y)
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                    const lds_byte* vb = kb + (KG + y / 2) * kGroup + x * 4096 + z * 2048;
-                    const uint32_t at = vat0 ^ y % 2 * 64;
-                    const uint2 v0 = lds_transposed(vb + at);
-                    const uint2 v1 = lds_transposed(vb + 1024 + (at ^ 16));
-                    o[y] = M::run(u32x4{v0.x, v0.y, v1.x, v1.y},
-                                  u32x4{p[x][4 * z], p[x][4 * z + 1], p[x][4 * z + 2],
-                                        p[x][4 * z + 3]}, o[y]);
+                for (int y = 0; y < 16; y += 2) {
+                    const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][x][y], a.rate, -m[r]));
+                    const float v =
+                        __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][x][y + 1], a.rate, -m[r]));
+                    sum += u + v;
+                    p[r][x][y / 2] = pack2<DT>(u, v);
                 }
+            l[r] += sum;
+        }
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            if (i + kAhead - 1 < NF) values(i + kAhead - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const int x = i / (2 * OT), y = i / 2 % OT, z = i % 2;
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                o[r * OT + y] = M::run(vf[i % kAhead],
+                                       u32x4{p[r][x][4 * z], p[r][x][4 * z + 1],
+                                             p[r][x][4 * z + 2], p[r][x][4 * z + 3]},
+                                       o[r * OT + y]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
     if (tiles) {
-        bring(0, 0);
+#pragma unroll
+        for (int x = 0; x < ST; ++x) {
+            const Source f = source(0, 0, x);
+#pragma unroll
+            for (int c = 0; c < kPieces; ++c) bring(f, c);
+        }
         for (uint32_t t = 0; t < tiles; ++t) {
             wait_loads<0>();
             barrier();
-            if (t + 1 < tiles) bring(t + 1, (t + 1) & 1);
             tile(t, t & 1);
         }
+        wait_loads<0>();
     }
-    l = across<32>(l, [](float p, float r) { return p + r; });
-    const bool live = i0 + 32 * wave + col < s.m;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const uint64_t row = s.q + i;
-    uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.os + (uint64_t)h * a.Dv;
-    float check = l * 0.0f;  // NaN once something is not finite
 #pragma unroll
-    for (int y = 0; y < OT; ++y)
+    for (int r = 0; r < RT; ++r) {
+        const float sum = across<32>(l[r], [](float u, float v) { return u + v; });
+        const bool live = w0 + 32 * r + col < s.m;
+        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const uint64_t row = s.q + query(r);
+        uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.os + (uint64_t)h * a.Dv;
+        float check = sum * 0.0f;  // NaN once something is not finite
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-            const uint32_t d = y * 32 + 8 * z + 4 * g;
-            const float4 v{o[y][4 * z] * inv, o[y][4 * z + 1] * inv, o[y][4 * z + 2] * inv,
-                           o[y][4 * z + 3] * inv};
-            if (FULL || d < a.Dv) {
-                check = __builtin_fmaf(v.x, 0.0f, check);
-                check = __builtin_fmaf(v.y, 0.0f, check);
-                check = __builtin_fmaf(v.z, 0.0f, check);
-                check = __builtin_fmaf(v.w, 0.0f, check);
-                if (live)
-                    *reinterpret_cast<uint2*>(out + d) =
-                        uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+        for (int y = 0; y < OT; ++y)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const uint32_t d = y * 32 + 8 * z + 4 * g;
+                const Acc& x = o[r * OT + y];
+                const float4 v{x[4 * z] * inv, x[4 * z + 1] * inv, x[4 * z + 2] * inv,
+                               x[4 * z + 3] * inv};
+                if (FULL || d < a.Dv) {
+                    check = __builtin_fmaf(v.x, 0.0f, check);
+                    check = __builtin_fmaf(v.y, 0.0f, check);
+                    check = __builtin_fmaf(v.z, 0.0f, check);
+                    check = __builtin_fmaf(v.w, 0.0f, check);
+                    if (live)
+                        *reinterpret_cast<uint2*>(out + d) =
+                            uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+                }
             }
-        }
-    if (live && !(check == 0.0f)) latch(a.status, K3X_ERR_INVALID_MXFP4);
-    if (a.lse && live && g == 0)
-        a.lse[row * a.H + h] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
-                                        : -__builtin_inff();
+        if (live && !(check == 0.0f)) latch(a.status, K3X_ERR_INVALID_MXFP4);
+        if (a.lse && live && g == 0)
+            a.lse[row * a.H + h] = sum > 0.0f
+                                       ? (m[r] + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f
+                                       : -__builtin_inff();
+    }
 }
 
 bool prompt_ok(const k3x_hip_mla_prompt_params* p) {
@@ -311,17 +366,24 @@ bool prompt_ok(const k3x_hip_mla_prompt_params* p) {
            fits(p->rotary_stride, p->rotary) && fits(p->out_stride, H * p->value_dim);
 }
 
+template <uint32_t DT, int RT, int KD, int TILE, int OWN>
+int launch_as(k3x_hip_ctx* ctx, PromptArgs a) {
+    // Blocks of all sequences at most, each with one that is not full.
+    a.blocks = a.T / (128 * RT) + std::min(a.N, a.T);
+    a.flip = a.blocks * a.H <= 640;
+    hipLaunchKernelGGL((mla_prompt_kernel<DT, RT, KD, 128, TILE, OWN>), dim3(a.blocks * a.H),
+                       dim3(kThreads), 0, ctx->stream, a);
+    return launched(ctx, 1);
+}
 template <uint32_t DT>
 int launch(k3x_hip_ctx* ctx, const PromptArgs& a) {
-    const dim3 grid(a.blocks * a.H), block(kThreads);
-    const bool whole = a.Dn % 64 == 0 && a.R % 64 == 0;
-    if (whole && a.Dn + a.R == 192 && a.Dv == 128)
-        hipLaunchKernelGGL((mla_prompt_kernel<DT, 192, 128, 32, true>), grid, block, 0, ctx->stream, a);
-    else if (whole && a.Dn + a.R == 128 && a.Dv == 128)
-        hipLaunchKernelGGL((mla_prompt_kernel<DT, 128, 128, 32, true>), grid, block, 0, ctx->stream, a);
-    else
-        hipLaunchKernelGGL((mla_prompt_kernel<DT, 192, 128, 32, false>), grid, block, 0, ctx->stream, a);
-    return launched(ctx, 1);
+    const bool whole = a.Dn % 64 == 0 && a.R % 64 == 0 && a.Dv == 128;
+    const bool many = (uint64_t)a.T * a.H >= (1ull << 60);
+    if (whole && a.Dn == 128 && a.R == 64)
+        return many ? launch_as<DT, 2, 192, 32, 2>(ctx, a) : launch_as<DT, 1, 192, 64, 2>(ctx, a);
+    if (whole && a.Dn == 128)
+        return many ? launch_as<DT, 2, 128, 32, 2>(ctx, a) : launch_as<DT, 1, 128, 64, 2>(ctx, a);
+    return launch_as<DT, 1, 192, 32, 0>(ctx, a);
 }
 
 }  // namespace
@@ -362,11 +424,9 @@ int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* p, con
     a.os = p->out_stride ? p->out_stride : (uint64_t)a.H * a.Dv;
     a.rate = p->scale * 1.4426950408889634f;
     a.status = ctx->status;
-    // Blocks of all sequences at most, each with one that is not full; the threads
-    // of a launch, and eight rows apart within 32 bits.
-    a.blocks = a.T / kRows + std::min(a.N, a.T);
-    if ((uint64_t)a.blocks * a.H * kThreads >= (1ull << 32) || a.ks > (1u << 27) ||
-        a.vs > (1u << 27) || a.rs > (1u << 27))
+    // The threads of a launch, and eight rows apart within 32 bits.
+    if ((a.T / 128 + (uint64_t)std::min(a.N, a.T)) * a.H * kThreads >= (1ull << 32) ||
+        a.ks > (1u << 27) || a.vs > (1u << 27) || a.rs > (1u << 27))
         return K3X_ERR_INVALID_EXTENT;
     if (hipSetDevice(ctx->device) != hipSuccess) return K3X_ERR_BACKEND_UNAVAILABLE;
     if (!a.T) return K3X_OK;

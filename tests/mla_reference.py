@@ -99,27 +99,25 @@ def softmax_rows(q, k, v, sees, scale, dtype, d_extra=4):
     score and the largest), by 2^-21 for the exponential itself and by half a step of its type;
     the sum over n weights by n 2^-23 of itself, and so is the product with v.  The output is
     rounded once more."""
-    m, n = q.shape[0], k.shape[0]
-    out = torch.zeros((m, v.shape[1]), dtype=torch.float64)
-    lse = torch.full((m,), -torch.inf, dtype=torch.float64)
-    tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
-    half = HALF[dtype]
-    for i in range(m):
-        s = max(0, min(n, int(sees[i])))
-        if not s:
-            continue
-        x = (k[:s] @ q[i]) * scale
-        size = (k[:s].abs() @ q[i].abs()).max() * scale
-        lse[i] = torch.logsumexp(x, 0)
-        w = (x - lse[i]).exp()
-        out[i] = w @ v[:s]
-        ds = float(size) * (q.shape[1] + d_extra) * 2.0 ** -23 + float(x.abs().max()) * 2.0 ** -22
-        off = half + 2 * ds + 2 * (s + 8) * 2.0 ** -23 + 2.0 ** -20
-        tol[i] = half * out[i].abs() + (1 + half) * off * (w @ v[:s].abs()) + 2.0 ** -126
-        if dtype == torch.float16:
-            tol[i] += 2.0 ** -25  # half a step of its subnormal numbers
-        ltol[i] = ds + (s + 8) * 2.0 ** -23 + 2.0 ** -20 + abs(float(lse[i])) * 2.0 ** -23
-    return out, lse, tol, ltol
+    n, half = k.shape[0], HALF[dtype]
+    sees = sees.clamp(0, n)
+    hidden = torch.arange(n) >= sees[:, None]
+    x = (q @ k.t() * scale).masked_fill(hidden, -torch.inf)
+    lse = torch.logsumexp(x, 1) if n else torch.full((len(q),), -torch.inf, dtype=torch.float64)
+    empty = (sees == 0)[:, None]
+    w = (x - lse[:, None]).exp().masked_fill(hidden | empty, 0.0)
+    out = w @ v
+    if not n:
+        return out, lse, torch.zeros_like(out), torch.zeros_like(lse)
+    size = ((q.abs() @ k.abs().t()) * scale).masked_fill(hidden, 0.0).amax(1)
+    far = x.abs().masked_fill(hidden, 0.0).amax(1)
+    ds = size * (q.shape[1] + d_extra) * 2.0 ** -23 + far * 2.0 ** -22
+    off = half + 2 * ds + 2 * (sees + 8) * 2.0 ** -23 + 2.0 ** -20
+    tol = half * out.abs() + (1 + half) * off[:, None] * (w @ v.abs()) + 2.0 ** -126
+    if dtype == torch.float16:
+        tol += 2.0 ** -25  # half a step of its subnormal numbers
+    ltol = ds + (sees + 8) * 2.0 ** -23 + 2.0 ** -20 + lse.abs() * 2.0 ** -23
+    return out, lse, tol.masked_fill(empty, 0.0), ltol.masked_fill(empty[:, 0], 0.0)
 
 
 def attention(cache, q, counts, scale):

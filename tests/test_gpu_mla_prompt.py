@@ -100,6 +100,14 @@ def test_long(hip):
     case(hip, [3, 200], [1500, 900], 1)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("Dn,R", [(128, 64), (128, 0), (64, 64)])
+def test_many_rows(hip, dtype, Dn, R):
+    """Enough rows of all heads for two tiles of queries a wave."""
+    case(hip, [300, 1, 0, 257, 40, 140], [300, 77, 5, 400, 39, 140], 256, Dn, R, 128, dtype)
+    case(hip, [1100], [1300], 128, Dn, R, 128, dtype, causal=False)
+
+
 def test_many_sequences(hip):
     counts = [n % 5 for n in range(150)]
     case(hip, counts, [c + n % 7 for n, c in enumerate(counts)], 2, 64, 32, 64)
