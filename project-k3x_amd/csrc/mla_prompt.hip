@@ -4,9 +4,7 @@
 // S^T = K Q^T and O^T = V^T P^T on the matrix cores, as in mla_attention.hip: the
 // result of the first product is, lane for lane, the second one's operand.  A
 // wave holds 32 queries of one head and their outputs; the tiles of K and V of a
-// workgroup's head lie in LDS, brought straight from memory a tile ahead.  Blocks
-// of queries run from the last to the first, whose work under a causal mask is
-// the least.
+// workgroup's head lie in LDS, brought straight from memory a tile ahead.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -21,6 +19,7 @@ using namespace k3x_mla;
 namespace {
 
 constexpr uint32_t kThreads = 256;
+constexpr uint32_t kRows = 128;  // queries a workgroup
 
 struct PromptArgs {
     const void *q, *k, *v, *rotary;
@@ -57,14 +56,13 @@ __device__ inline bool ranges_of(const PromptArgs& a, uint32_t n, Ranges* r) {
     return e >= b && e <= a.T && g >= f && g <= a.S;
 }
 
-// RT tiles of 32 queries a wave.  KD columns of a key and VD of a value at most, in
-// groups of 64 in LDS; TILE keys a step.  OWN > 0: Dn is OWN whole groups, R the
-// others and Dv is VD, so that nothing is left out.
-template <uint32_t DT, int RT, int KD, int VD, int TILE, int OWN>
-__global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(PromptArgs a) {
+// KD columns of a key and VD of a value at most, in groups of 64 in LDS; TILE keys a
+// step.  OWN > 0: Dn is OWN whole groups, R the others and Dv is VD, so that nothing is
+// left out.
+template <uint32_t DT, int KD, int VD, int TILE, int OWN>
+__global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
     constexpr bool FULL = OWN > 0;
     constexpr int KG = KD / 64, VG = VD / 64, ST = TILE / 32, OT = VD / 32;
-    constexpr uint32_t kRows = 128 * RT;         // queries a workgroup
     constexpr uint32_t kGroup = TILE * 128;      // bytes of a group
     constexpr uint32_t kBuffer = (KG + VG) * kGroup;
     typedef Mma<DT, 32> M;
@@ -77,44 +75,93 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(P
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t h = blockIdx.x % a.H;
-    const uint32_t at = blockIdx.x / a.H, half = a.blocks / 2;
-    const uint32_t block = a.flip && at >= a.blocks - half ? at - (a.blocks - half) : a.blocks - 1 - at;
     if (*(volatile uint32_t*)a.status) return;
 
-    // The sequence that the block is in: blocks of 128 queries, sequence by sequence.
-    if (tid == 0) found[0] = a.N;
-    uint32_t carry = 0;
+    // The workgroup's block of queries.  Blocks of up to 64 sequences are taken from those
+    // with the most keys to those with the fewest, in 64 classes, so that no long one begins
+    // last; of one sequence, and of more than 64, from the last to the first.
+    // blocks_of(r, k): the blocks of a sequence with at least k keys, which are its last ones.
+    auto blocks_of = [&](const Ranges& r, uint32_t k) -> uint32_t {
+        const uint32_t all = (r.m + kRows - 1) / kRows;
+        if (k == 0) return all;
+        if (r.n < k) return 0;
+        // The i-th block's last query sees n - m + min(m, kRows (i + 1)) keys.
+        const uint32_t more = r.n - k;
+        return a.causal && r.m > more ? all + 1 - (r.m - more + kRows - 1) / kRows : all;
+    };
+    uint32_t at = blockIdx.x / a.H, n = a.N, i0 = 0;
     bool bad = false;
-    for (uint32_t base = 0; base < a.N; base += kThreads) {
-        const uint32_t n = base + tid;
-        Ranges r{};
-        if (n < a.N && !ranges_of(a, n, &r)) {
+    Ranges s{};
+    auto load = [&](uint32_t x) {
+        s = Ranges{};
+        if (x < a.N && !ranges_of(a, x, &s)) {
             bad = true;
-            r.m = 0;
+            s = Ranges{};
         }
-        const uint32_t own = (r.m + kRows - 1) / kRows;
-        uint32_t c = own;
+    };
+    auto scan_lanes = [&](uint32_t c) {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t o = __shfl_up(c, d);
             if (lane >= (uint32_t)d) c += o;
         }
-        __syncthreads();
-        if (lane == 63) scan[wave] = c;
-        __syncthreads();
-        for (uint32_t i = 0; i < wave; ++i) c += scan[i];
-        c += carry;  // with the thread's own
-        if (own && block >= c - own && block < c) {
-            found[0] = n;
-            found[1] = block - (c - own);
+        return c;
+    };
+    if (a.N <= 64) {  // every wave for itself
+        load(lane);
+        const uint32_t unit = a.N == 1 ? a.S + 1 : a.S / 64 + 1;
+        uint32_t count = 0;  // blocks with at least lane * unit keys
+        for (uint32_t x = 0; x < a.N; ++x) {
+            Ranges r{};
+            r.m = __builtin_amdgcn_readlane(s.m, x);
+            r.n = __builtin_amdgcn_readlane(s.n, x);
+            count += blocks_of(r, lane * unit);
         }
-        carry += scan[0] + scan[1] + scan[2] + scan[3];
+        const uint32_t blocks = __builtin_amdgcn_readfirstlane(count);
+        // Up to two workgroups a compute unit all begin at once: then the second half goes
+        // the other way, so that a long and a short one share a unit.
+        if (a.flip && at < blocks && at >= blocks - blocks / 2)
+            at = 2 * blocks - 1 - blocks / 2 - at;
+        const uint64_t above = __ballot(count > at);
+        if (above) {
+            // A class falls with its number of keys: the last one that `at` is below.
+            const uint32_t c = 63 - __builtin_clzll(above);
+            const uint32_t before = c < 63 ? __builtin_amdgcn_readlane(count, c + 1 & 63) : 0;
+            const uint32_t more = c < 63 ? blocks_of(s, (c + 1) * unit) : 0;
+            const uint32_t own = blocks_of(s, c * unit) - more, end = before + scan_lanes(own);
+            const uint64_t mine = __ballot(at < end && at >= end - own);
+            if (mine) {
+                const uint32_t x = __builtin_ctzll(mine);
+                const uint32_t i = (s.m + kRows - 1) / kRows - 1 - more - (at - (end - own));
+                n = x;
+                i0 = __builtin_amdgcn_readlane(i, x) * kRows;
+            }
+        }
+    } else {
+        if (tid == 0) found[0] = a.N;
+        at = a.blocks - 1 - at;
+        uint32_t carry = 0;
+        for (uint32_t base = 0; base < a.N; base += kThreads) {
+            load(base + tid);
+            const uint32_t own = blocks_of(s, 0);
+            uint32_t c = scan_lanes(own);
+            __syncthreads();
+            if (lane == 63) scan[wave] = c;
+            __syncthreads();
+            for (uint32_t i = 0; i < wave; ++i) c += scan[i];
+            c += carry;  // with the thread's own
+            if (own && at >= c - own && at < c) {
+                found[0] = base + tid;
+                found[1] = at - (c - own);
+            }
+            carry += scan[0] + scan[1] + scan[2] + scan[3];
+        }
+        __syncthreads();
+        n = __builtin_amdgcn_readfirstlane(found[0]);
+        i0 = __builtin_amdgcn_readfirstlane(found[1]) * kRows;
     }
     if (blockIdx.x == 0 && bad) latch(a.status, K3X_ERR_INVALID_STATE);
-    __syncthreads();
-    const uint32_t n = found[0], i0 = found[1] * kRows;
     if (n >= a.N) return;
-    Ranges s;
     ranges_of(a, n, &s);
     __syncthreads();
     if (!FULL) {  // columns that are not brought stay zero
@@ -124,9 +171,9 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(P
     }
 
     const uint32_t col = lane & 31, g = lane >> 5;
-    const uint32_t w0 = i0 + 32 * RT * wave;                   // the wave's first query
+    const uint32_t w0 = i0 + 32 * wave;                        // the wave's first query
     const int32_t hidden = a.causal ? (int32_t)(s.m - 1) : 0;  // keys of the first query's future
-    auto query = [&](int x) { return min(w0 + 32 * x + col, s.m - 1); };  // the lane's
+    const uint32_t query = min(w0 + col, s.m - 1);             // the lane's
     auto sees_of = [&](uint32_t x) {
         return a.causal ? (int32_t)s.n - hidden + (int32_t)x : (int32_t)s.n;
     };
@@ -176,11 +223,10 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(P
         }
     };
 
-    u32x4 qf[RT][KG * 4];
-#pragma unroll
-    for (int x = 0; x < RT; ++x) {
+    u32x4 qf[KG * 4];
+    {
         const uint8_t* q = static_cast<const uint8_t*>(a.q) +
-                           2 * ((uint64_t)(s.q + query(x)) * a.qs + (uint64_t)h * (a.Dn + a.R));
+                           2 * ((uint64_t)(s.q + query) * a.qs + (uint64_t)h * (a.Dn + a.R));
 #pragma unroll
         for (int c = 0; c < KG; ++c)
 #pragma unroll
@@ -190,18 +236,14 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(P
                 const bool in = FULL || d < (mine ? a.Dn : a.R);
                 const u32x4 z = *reinterpret_cast<const u32x4*>(
                     q + (in ? 2 * (mine ? d : a.Dn + d) : 0));
-                qf[x][c * 4 + y] = z & (in ? 0xffffffffu : 0u);
+                qf[c * 4 + y] = z & (in ? 0xffffffffu : 0u);
             }
     }
-    Acc o[RT * OT];
+    Acc o[OT];
 #pragma unroll
-    for (int x = 0; x < RT * OT; ++x) o[x] = Acc{};
-    float m[RT], l[RT];
-#pragma unroll
-    for (int x = 0; x < RT; ++x) {
-        m[x] = -3.4028235e38f;
-        l[x] = 0.0f;
-    }
+    for (int x = 0; x < OT; ++x) o[x] = Acc{};
+    float m = -3.4028235e38f, l = 0.0f;
+    const int32_t sees = sees_of(query);
 
     // Tile t in buffer b; the next one's loads (the last one's again) to the other.
     auto tile = [&](uint32_t t, uint32_t b) {
@@ -209,11 +251,9 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(P
         Source next[ST];
 #pragma unroll
         for (int x = 0; x < ST; ++x) next[x] = source(min(t + 1, tiles - 1), b ^ 1, x);
-        Acc sc[RT][ST];
+        Acc sc[ST];
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int x = 0; x < ST; ++x) sc[r][x] = Acc{};
+        for (int x = 0; x < ST; ++x) sc[x] = Acc{};
         // Operands are read a few products ahead: LDS takes some 200 cycles, four waves
         // at once, a product 32.
         constexpr int NK = KG * 4 * ST, kAhead = 8;
@@ -229,9 +269,7 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(P
             if (i + kAhead - 1 < NK) keys(i + kAhead - 1);
             if (i % 2 == 0 && i / 2 < ST * kPieces) bring(next[i / 2 % ST], i / 2 / ST);
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-                sc[r][i % ST] = M::run(kf[i % kAhead], qf[r][i / ST], sc[r][i % ST]);
+            sc[i % ST] = M::run(kf[i % kAhead], qf[i / ST], sc[i % ST]);
             __builtin_amdgcn_sched_barrier(0);
         }
         static_assert(2 * ST * kPieces <= NK + 1, "pieces within the products");
@@ -247,57 +285,48 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(P
         };
 #pragma unroll
         for (int i = 0; i < kAhead - 1; ++i) values(i);
-        uint32_t p[RT][ST][8];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            if ((int32_t)((t + 1) * TILE) > least) {
-                // Past what the query sees.
-                const int32_t sees = sees_of(query(r));
-#pragma unroll
-                for (int x = 0; x < ST; ++x)
-#pragma unroll
-                    for (int y = 0; y < 16; ++y)
-                        if ((int32_t)(t * TILE + 32 * x + 8 * (y / 4) + 4 * g + y % 4) >= sees)
-                            sc[r][x][y] = -__builtin_inff();
-            }
-            float top = sc[r][0][0];
+        if ((int32_t)((t + 1) * TILE) > least) {
+            // Past what the query sees.
 #pragma unroll
             for (int x = 0; x < ST; ++x)
 #pragma unroll
-                for (int y = 0; y < 16; ++y) top = fmaxf(top, sc[r][x][y]);
-            top = across<32>(top, [](float u, float v) { return fmaxf(u, v); }) * a.rate;
-            // The maximum may lag by 2^8: see mla_attention.hip.
-            if (__any(top > m[r] + 8.0f)) {
-                const float up = fmaxf(m[r], top), keep = __builtin_amdgcn_exp2f(m[r] - up);
-                m[r] = up;
-                l[r] *= keep;
-                if (r == 0) scale_tiles<RT == 2, 0, OT>(o, keep);
-                else scale_tiles<RT == 2, (RT - 1) * OT, OT>(o, keep);
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int x = 0; x < ST; ++x)
-#pragma unroll
-                for (int y = 0; y < 16; y += 2) {
-                    const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][x][y], a.rate, -m[r]));
-                    const float v =
-                        __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][x][y + 1], a.rate, -m[r]));
-                    sum += u + v;
-                    p[r][x][y / 2] = pack2<DT>(u, v);
-                }
-            l[r] += sum;
+                for (int y = 0; y < 16; ++y)
+                    if ((int32_t)(t * TILE + 32 * x + 8 * (y / 4) + 4 * g + y % 4) >= sees)
+                        sc[x][y] = -__builtin_inff();
         }
+        float top = sc[0][0];
+#pragma unroll
+        for (int x = 0; x < ST; ++x)
+#pragma unroll
+            for (int y = 0; y < 16; ++y) top = fmaxf(top, sc[x][y]);
+        top = across<32>(top, [](float u, float v) { return fmaxf(u, v); }) * a.rate;
+        // The maximum may lag by 2^8: see mla_attention.hip.
+        if (__any(top > m + 8.0f)) {
+            const float up = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - up);
+            m = up;
+            l *= keep;
+            scale_tiles<false, 0, OT>(o, keep);
+        }
+        uint32_t p[ST][8];
+        float sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < ST; ++x)
+#pragma unroll
+            for (int y = 0; y < 16; y += 2) {
+                const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][y], a.rate, -m));
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][y + 1], a.rate, -m));
+                sum += u + v;
+                p[x][y / 2] = pack2<DT>(u, v);
+            }
+        l += sum;
 #pragma unroll
         for (int i = 0; i < NF; ++i) {
             if (i + kAhead - 1 < NF) values(i + kAhead - 1);
             __builtin_amdgcn_sched_barrier(0);
             const int x = i / (2 * OT), y = i / 2 % OT, z = i % 2;
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-                o[r * OT + y] = M::run(vf[i % kAhead],
-                                       u32x4{p[r][x][4 * z], p[r][x][4 * z + 1],
-                                             p[r][x][4 * z + 2], p[r][x][4 * z + 3]},
-                                       o[r * OT + y]);
+            o[y] = M::run(vf[i % kAhead],
+                          u32x4{p[x][4 * z], p[x][4 * z + 1], p[x][4 * z + 2], p[x][4 * z + 3]},
+                          o[y]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -316,38 +345,33 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void mla_prompt_kernel(P
         }
         wait_loads<0>();
     }
+    l = across<32>(l, [](float u, float v) { return u + v; });
+    const bool live = w0 + col < s.m;
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const uint64_t row = s.q + query;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.os + (uint64_t)h * a.Dv;
+    float check = l * 0.0f;  // NaN once something is not finite
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const float sum = across<32>(l[r], [](float u, float v) { return u + v; });
-        const bool live = w0 + 32 * r + col < s.m;
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-        const uint64_t row = s.q + query(r);
-        uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.os + (uint64_t)h * a.Dv;
-        float check = sum * 0.0f;  // NaN once something is not finite
+    for (int y = 0; y < OT; ++y)
 #pragma unroll
-        for (int y = 0; y < OT; ++y)
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const uint32_t d = y * 32 + 8 * z + 4 * g;
-                const Acc& x = o[r * OT + y];
-                const float4 v{x[4 * z] * inv, x[4 * z + 1] * inv, x[4 * z + 2] * inv,
-                               x[4 * z + 3] * inv};
-                if (FULL || d < a.Dv) {
-                    check = __builtin_fmaf(v.x, 0.0f, check);
-                    check = __builtin_fmaf(v.y, 0.0f, check);
-                    check = __builtin_fmaf(v.z, 0.0f, check);
-                    check = __builtin_fmaf(v.w, 0.0f, check);
-                    if (live)
-                        *reinterpret_cast<uint2*>(out + d) =
-                            uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
-                }
+        for (int z = 0; z < 4; ++z) {
+            const uint32_t d = y * 32 + 8 * z + 4 * g;
+            const float4 v{o[y][4 * z] * inv, o[y][4 * z + 1] * inv, o[y][4 * z + 2] * inv,
+                           o[y][4 * z + 3] * inv};
+            if (FULL || d < a.Dv) {
+                check = __builtin_fmaf(v.x, 0.0f, check);
+                check = __builtin_fmaf(v.y, 0.0f, check);
+                check = __builtin_fmaf(v.z, 0.0f, check);
+                check = __builtin_fmaf(v.w, 0.0f, check);
+                if (live)
+                    *reinterpret_cast<uint2*>(out + d) =
+                        uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
             }
-        if (live && !(check == 0.0f)) latch(a.status, K3X_ERR_INVALID_MXFP4);
-        if (a.lse && live && g == 0)
-            a.lse[row * a.H + h] = sum > 0.0f
-                                       ? (m[r] + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f
-                                       : -__builtin_inff();
-    }
+        }
+    if (live && !(check == 0.0f)) latch(a.status, K3X_ERR_INVALID_MXFP4);
+    if (a.lse && live && g == 0)
+        a.lse[row * a.H + h] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
+                                        : -__builtin_inff();
 }
 
 bool prompt_ok(const k3x_hip_mla_prompt_params* p) {
@@ -366,24 +390,16 @@ bool prompt_ok(const k3x_hip_mla_prompt_params* p) {
            fits(p->rotary_stride, p->rotary) && fits(p->out_stride, H * p->value_dim);
 }
 
-template <uint32_t DT, int RT, int KD, int TILE, int OWN>
-int launch_as(k3x_hip_ctx* ctx, PromptArgs a) {
-    // Blocks of all sequences at most, each with one that is not full.
-    a.blocks = a.T / (128 * RT) + std::min(a.N, a.T);
-    a.flip = a.blocks * a.H <= 640;
-    hipLaunchKernelGGL((mla_prompt_kernel<DT, RT, KD, 128, TILE, OWN>), dim3(a.blocks * a.H),
-                       dim3(kThreads), 0, ctx->stream, a);
-    return launched(ctx, 1);
-}
 template <uint32_t DT>
 int launch(k3x_hip_ctx* ctx, const PromptArgs& a) {
-    const bool whole = a.Dn % 64 == 0 && a.R % 64 == 0 && a.Dv == 128;
-    const bool many = (uint64_t)a.T * a.H >= (1ull << 60);
-    if (whole && a.Dn == 128 && a.R == 64)
-        return many ? launch_as<DT, 2, 192, 32, 2>(ctx, a) : launch_as<DT, 1, 192, 64, 2>(ctx, a);
-    if (whole && a.Dn == 128)
-        return many ? launch_as<DT, 2, 128, 32, 2>(ctx, a) : launch_as<DT, 1, 128, 64, 2>(ctx, a);
-    return launch_as<DT, 1, 192, 32, 0>(ctx, a);
+    const dim3 grid(a.blocks * a.H), block(kThreads);
+    if (a.Dn == 128 && a.R == 64 && a.Dv == 128)
+        hipLaunchKernelGGL((mla_prompt_kernel<DT, 192, 128, 64, 2>), grid, block, 0, ctx->stream, a);
+    else if (a.Dn == 128 && a.R == 0 && a.Dv == 128)
+        hipLaunchKernelGGL((mla_prompt_kernel<DT, 128, 128, 64, 2>), grid, block, 0, ctx->stream, a);
+    else
+        hipLaunchKernelGGL((mla_prompt_kernel<DT, 192, 128, 32, 0>), grid, block, 0, ctx->stream, a);
+    return launched(ctx, 1);
 }
 
 }  // namespace
@@ -424,8 +440,11 @@ int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* p, con
     a.os = p->out_stride ? p->out_stride : (uint64_t)a.H * a.Dv;
     a.rate = p->scale * 1.4426950408889634f;
     a.status = ctx->status;
-    // The threads of a launch, and eight rows apart within 32 bits.
-    if ((a.T / 128 + (uint64_t)std::min(a.N, a.T)) * a.H * kThreads >= (1ull << 32) ||
+    // Blocks of all sequences at most, each with one that is not full; the threads of a
+    // launch, and eight rows apart within 32 bits.
+    a.blocks = a.T / kRows + std::min(a.N, a.T);
+    a.flip = a.blocks * a.H <= 640;
+    if ((uint64_t)a.blocks * a.H * kThreads >= (1ull << 32) ||
         a.ks > (1u << 27) || a.vs > (1u << 27) || a.rs > (1u << 27))
         return K3X_ERR_INVALID_EXTENT;
     if (hipSetDevice(ctx->device) != hipSuccess) return K3X_ERR_BACKEND_UNAVAILABLE;
