@@ -623,6 +623,7 @@ enum k3x_cache_format { K3X_CACHE_16BIT = 0, K3X_CACHE_MXFP8 = 1, K3X_CACHE_MXFP
  * positions, lens[n] - (offsets[n + 1] - offsets[n]) .. lens[n] - 1.  Rows at
  * positions below 0 (a padded sequence has lens[n] = 0) are not written, read or
  * seen.  Rows past offsets[N] are left as they were.
+ * Tensors of a call without tokens may be NULL.
  * Latched as K3X_ERR_INVALID_STATE by every call, which then reads and writes
  * nothing outside its tensors and the pool, and leaves outputs undefined: offsets
  * that fall or pass T, a length past table_width * page_size or 2^29, a page in use
@@ -716,7 +717,8 @@ typedef struct k3x_hip_mla_prompt_params {
  * key_offsets[n] .. key_offsets[n + 1] - 1 (device u32 [N + 1] each; NULL: T / N and
  * S / N rows each), a cached prefix's first.  causal: query i of m sees the first
  * n - m + i + 1 of n keys.  lse, empty rows, sums and weights as for
- * k3x_hip_mla_attention.  q, k, v, rotary and out 16-byte aligned.
+ * k3x_hip_mla_attention.  q, k, v, rotary and out 16-byte aligned, those without rows
+ * may be NULL.
  * Latched: offsets that fall, pass T or S (K3X_ERR_INVALID_STATE; nothing of such
  * a sequence is read), an output that is not finite (K3X_ERR_INVALID_MXFP4).
  * Asynchronous. */

@@ -701,8 +701,8 @@ int k3x_hip_mla_attention(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const v
                           const void* pool, const uint32_t* table, const uint32_t* offsets,
                           const uint32_t* lens, void* out, float* lse, void* workspace,
                           size_t workspace_bytes) {
-    if (!ctx || !p || !attention_ok(p) || !q || !pool || !table || !lens || !out ||
-        p->q_stride % 8 || p->out_stride % 8)
+    if (!ctx || !p || !attention_ok(p) || (p->tokens && (!q || !out)) || !pool || !table ||
+        !lens || p->q_stride % 8 || p->out_stride % 8)
         return K3X_ERR_INVALID_EXTENT;
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(pool, 256) || !aligned(table, 4) ||
         !aligned(offsets, 4) || !aligned(lens, 4) || !aligned(lse, 4))

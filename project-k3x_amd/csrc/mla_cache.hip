@@ -254,7 +254,7 @@ __global__ __launch_bounds__(kThreads) void mla_load_kernel(CacheArgs a) {
 int cache_args(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const void* latent,
                const void* rotary, const uint32_t* table, const uint32_t* offsets,
                const uint32_t* lens, const void* pool, CacheArgs* a) {
-    if (!ctx || !p || !mla_ok(p) || !latent || !table || !lens || !pool)
+    if (!ctx || !p || !mla_ok(p) || (p->tokens && !latent) || !table || !lens || !pool)
         return K3X_ERR_INVALID_EXTENT;
     if (!aligned(latent, 2) || !aligned(rotary, 2) || !aligned(table, 4) ||
         !aligned(offsets, 4) || !aligned(lens, 4) || !aligned(pool, 256))
@@ -306,7 +306,7 @@ size_t k3x_hip_mla_row_bytes(const k3x_hip_mla_params* p) {
 int k3x_hip_mla_store(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const void* latent,
                       const void* rotary, const float* gamma, const uint32_t* table,
                       const uint32_t* offsets, const uint32_t* lens, void* pool) {
-    if (!p || (p->rotary && !rotary) || !aligned(gamma, 4)) return K3X_ERR_INVALID_EXTENT;
+    if (!p || (p->tokens && p->rotary && !rotary) || !aligned(gamma, 4)) return K3X_ERR_INVALID_EXTENT;
     CacheArgs a{};
     const int st = cache_args(ctx, p, latent, rotary, table, offsets, lens, pool, &a);
     if (st != K3X_OK) return st;

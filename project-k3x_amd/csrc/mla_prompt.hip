@@ -409,7 +409,8 @@ extern "C" {
 int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* p, const void* q,
                        const void* k, const void* v, const void* rotary, const uint32_t* offsets,
                        const uint32_t* key_offsets, void* out, float* lse) {
-    if (!ctx || !p || !prompt_ok(p) || !q || !k || !v || (p->rotary && !rotary) || !out)
+    if (!ctx || !p || !prompt_ok(p) || (p->tokens && (!q || !out)) ||
+        (p->keys && (!k || !v || (p->rotary && !rotary))))
         return K3X_ERR_INVALID_EXTENT;
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(rotary, 16) ||
         !aligned(out, 16) || !aligned(offsets, 4) || !aligned(key_offsets, 4) || !aligned(lse, 4))
