@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "k3x_mla.hpp"
 #include "k3x_mla_mma.hpp"
@@ -28,9 +29,7 @@ using namespace k3x_mla;
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kTile = 32;       // cached tokens a step
-constexpr uint32_t kLeast = 2;       // tiles of a range at least
-constexpr uint32_t kGroup = kTile * 128;  // bytes of 64 columns of a tile in LDS
+constexpr uint32_t kLeast = 64;  // cached tokens of a range at least
 
 // A sequence that begins in range w and ends in another.
 struct Split {
@@ -54,26 +53,39 @@ struct AttentionArgs {
     uint32_t* status;
 };
 
-// Rows a wave and how the waves lie: WM row blocks by WD parts of the latent.
-template <int HT_, int WM_, int WD_>
+// How four waves share a tile of TILE cached tokens.  WM row blocks by WD parts of the
+// latent; RT blocks of HT rows a wave.  Of 32 tokens each wave forms the scores of its own
+// rows.  Of 64 (JOINT) it forms those of one block of rows and half of the tokens, and
+// all waves take the weights from LDS: each part of a tile is read from there fewer times.
+template <int HT_, int WM_, int WD_, int RT_, int TILE_>
 struct Shape {
-    static constexpr int HT = HT_, WM = WM_, WD = WD_;
-    static constexpr int rows = HT * WM;
+    static constexpr int HT = HT_, WM = WM_, WD = WD_, RT = RT_, TILE = TILE_;
+    static constexpr int rows = HT * WM * RT;
+    static constexpr bool JOINT = TILE == 64;
 };
 
 // Tiles of a sequence in the line; an empty one takes one, in which its rows are
 // written as empty.
-__device__ inline uint32_t tiles_in(const Tokens& s) { return max(1u, (s.len + kTile - 1) / kTile); }
+template <uint32_t TILE>
+__device__ inline uint32_t tiles_in(const Tokens& s) { return max(1u, (s.len + TILE - 1) / TILE); }
+template <uint32_t TILE>
 __device__ inline uint32_t tiles_of(const Pages& a, uint32_t n, Tokens* s) {
-    return tokens_of(a, n, s) && s->count ? tiles_in(*s) : 0;
+    return tokens_of(a, n, s) && s->count ? tiles_in<TILE>(*s) : 0;
 }
 
 // FULL: L is LP (else the columns past L are zeros, and not brought or written) and
 // a page holds whole eights of tokens.
 template <uint32_t DT, uint32_t F, int LP, typename S, int BUFS, bool FULL>
 __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention_kernel(AttentionArgs a) {
-    constexpr int HT = S::HT, WD = S::WD, CG = LP / 64 + 1;
+    constexpr int HT = S::HT, WD = S::WD, RT = S::RT, CG = LP / 64 + 1;
+    constexpr bool JOINT = S::JOINT;
+    constexpr uint32_t kTile = S::TILE;
+    constexpr int XB = kTile / 32;              // eights of tokens a wave brings
+    constexpr uint32_t kGroup = kTile * 128;    // bytes of 64 columns of a tile in LDS
     constexpr uint32_t kBuffer = CG * kGroup;
+    // Behind the buffers, where waves share them: weights, a row's largest scores, flags.
+    constexpr uint32_t kWeights = BUFS * kBuffer, kTops = kWeights + RT * 4096,
+                       kFlags = kTops + RT * 256;
     constexpr int KS = HT == 32 ? 4 : 2;        // products over 64 columns
     constexpr int OT = LP / HT / WD;            // tiles of the latent, a wave
     constexpr int AHEAD = F != K3X_CACHE_16BIT && S::rows == 128 ? 4 : 8;  // operands on their way
@@ -81,7 +93,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     typedef typename M::Acc Acc;
     // One array: with several the compiler tells them apart, and waits for all direct
     // loads to LDS before any read of theirs.
-    __shared__ __attribute__((aligned(256))) uint8_t smem[BUFS * kBuffer];
+    __shared__ __attribute__((aligned(256))) uint8_t smem[JOINT ? kFlags + 16 : kWeights];
     uint32_t* const scan = reinterpret_cast<uint32_t*>(smem);  // before the first tile
     uint32_t* const at_s = scan + 4;
     lds_byte* const lds = (lds_byte*)smem;
@@ -95,7 +107,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     Tokens mine;
     auto scan_tiles = [&](uint32_t base, uint32_t* own) {
         const uint32_t n = base + tid;
-        uint32_t c = *own = n < a.pages.N ? tiles_of(a.pages, n, &mine) : 0;
+        uint32_t c = *own = n < a.pages.N ? tiles_of<kTile>(a.pages, n, &mine) : 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t o = __shfl_up(c, d);
@@ -123,7 +135,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         return;
     }
     const uint32_t total = (uint32_t)all;
-    const uint32_t chunk = max(kLeast, (total + a.G - 1) / a.G);
+    const uint32_t chunk = max(kLeast / kTile, (total + a.G - 1) / a.G);
     const uint32_t ranges = (total + chunk - 1) / chunk;  // in use, G at most
     // Consecutive ranges, and a range's row blocks, lie on one die: they share cached
     // tokens and queries.
@@ -167,6 +179,8 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
 
     const uint32_t wm = wave / WD, wd = wave % WD;
     const uint32_t col = lane % HT, g = lane / HT;
+    // The block of rows and the 32 tokens of a tile that the wave forms scores of.
+    const uint32_t srow = JOINT ? wave / 2 % RT : wm, side = JOINT ? wave % 2 : 0;
     // Where the lane reads its operands in a tile: keys, and values of a 16-lane
     // row's four tokens.  Other columns of a 64-column group are an exclusive or away.
     const uint32_t kat0 = col * 128 + (g ^ swizzle(col)) * 16;
@@ -184,7 +198,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
 
     bool bad_page = false, bad_value = false;
     while (true) {
-        const uint32_t tiles = tiles_in(s);
+        const uint32_t tiles = tiles_in<kTile>(s);
         const uint32_t rows = s.count * a.H;
         const uint32_t t0 = max(from, first) - first, t1 = min(to - first, tiles);
         const bool whole = t0 == 0 && t1 == tiles;
@@ -194,7 +208,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         const uint32_t r0 = rb * S::rows;
         if (r0 < rows) {
             // The row of this lane, and how many tokens it sees.
-            const uint32_t r = min(r0 + wm * HT + opaque(col), rows - 1), ri = r / a.H;
+            const uint32_t r = min(r0 + srow * HT + opaque(col), rows - 1), ri = r / a.H;
             const int32_t sees = (int32_t)s.len - (int32_t)s.count + (int32_t)ri + 1;
             const int32_t sees_least = (int32_t)s.len - (int32_t)s.count + (int32_t)(r0 / a.H) + 1;
             const int32_t sees_most = (int32_t)s.len - (int32_t)s.count +
@@ -202,25 +216,38 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
             const uint32_t seen = sees_most > 0 ? (uint32_t)sees_most : 0;
             const uint32_t end = min(t1, (seen + kTile - 1) / kTile);
             u32x4 qf[CG * KS];
-            Acc o[OT];
+            Acc o[RT * OT];
             {
                 const float zero = __uint_as_float(opaque(0));
 #pragma unroll
-                for (int i = 0; i < OT; ++i)
+                for (int i = 0; i < RT * OT; ++i)
 #pragma unroll
                     for (int j = 0; j < (int)(sizeof(Acc) / 4); ++j) o[i][j] = zero;
             }
-            float m = -3.4028235e38f, l = 0.0f;
+            float m[RT], l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) m[i] = -3.4028235e38f;
 
             // ---- bringing tiles ---------------------------------------------
-            // The wave's eight tokens of a tile, where a page holds whole eights.
-            auto eight = [&](uint32_t t) {
-                return __builtin_amdgcn_readfirstlane(min(t * kTile + 8 * wave, s.len - 1) & ~7u);
+            // The wave's eight tokens of a tile's x-th 32, where a page holds whole eights.
+            auto eight = [&](uint32_t t, int x) {
+                return __builtin_amdgcn_readfirstlane(
+                    min(t * kTile + 32 * x + 8 * wave, s.len - 1) & ~7u);
             };
-            auto position = [&](uint32_t t) { return min(t * kTile + btok, s.len - 1); };
+            auto position = [&](uint32_t t, int x) {
+                return min(t * kTile + 32 * x + btok, s.len - 1);
+            };
+            struct Ids {
+                uint32_t of[XB];
+            };
             auto page_of = [&](uint32_t t) {
-                const uint32_t p = DIRECT ? eight(t) : position(t);
-                return a.pages.table[(size_t)n * a.pages.width + a.pages.page_of(p)];
+                Ids id;
+#pragma unroll
+                for (int x = 0; x < XB; ++x) {
+                    const uint32_t p = DIRECT ? eight(t, x) : position(t, x);
+                    id.of[x] = a.pages.table[(size_t)n * a.pages.width + a.pages.page_of(p)];
+                }
+                return id;
             };
             auto row_of = [&](uint32_t p, uint32_t id) {
                 bad_page |= id >= a.pages.pages;
@@ -232,29 +259,31 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                                   : F == K3X_CACHE_MXFP4 ? LP / 256
                                   : DIRECT               ? 1
                                                          : LP / 64;
-            u32x4 codes[UNITS], scales, turned;
+            u32x4 codes[XB][UNITS], scales[XB], turned[XB];
             // A tile's loads, straight to a buffer or to registers, in steps that can stand
-            // between products: 0 finds the rows, the others load.
+            // between products: of each 32 tokens the first finds the rows, the others load.
             struct {
                 __amdgpu_buffer_rsrc_t rows8;
                 uint32_t from, turn;
                 u32x4* dst;
                 const uint8_t* row;
             } src;
-            constexpr int kBring = DIRECT ? CG + 1 : UNITS + 3;
-            auto bring = [&](int step, uint32_t t, uint32_t b, uint32_t id) {
+            constexpr int kSteps = DIRECT ? CG + 1 : UNITS + 3, kBring = XB * kSteps;
+            auto bring = [&](int at, uint32_t t, uint32_t b, const Ids& id) {
+                const int x = at / kSteps, step = at % kSteps;
                 if constexpr (DIRECT) {
                     // Eight tokens a wave, each load 128 bytes of every one.
                     if (step == 0) {
-                        const uint32_t p = eight(t);
-                        const uint8_t* row = row_of(p, __builtin_amdgcn_readfirstlane(id));
+                        const uint32_t p = eight(t, x);
+                        const uint8_t* row = row_of(p, __builtin_amdgcn_readfirstlane(id.of[x]));
                         src.rows8 = __builtin_amdgcn_make_buffer_rsrc(
                             const_cast<uint8_t*>(row), 0, 8 * a.pages.row.bytes, 0x00020000);
-                        src.from = (position(t) - p) * a.pages.row.bytes + bput * 16;
+                        src.from = (position(t, x) - p) * a.pages.row.bytes + bput * 16;
                         // Columns without a rotary part meet zeros of the queries: any
                         // number will do there.
                         src.turn = bput < a.R / 8 ? LP * 2 : 0;
-                        src.dst = reinterpret_cast<u32x4*>(smem + b * kBuffer + wave * 1024);
+                        src.dst = reinterpret_cast<u32x4*>(smem + b * kBuffer + x * 4096 +
+                                                           wave * 1024);
                     } else if (step < CG) {
                         load_lds16(src.rows8, src.dst + (step - 1) * (kGroup / 16), src.from,
                                    (step - 1) * 128);
@@ -264,59 +293,59 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     }
                 } else {
                     if (step == 0) {
-                        src.row = row_of(position(t), id);
+                        src.row = row_of(position(t, x), id.of[x]);
                     } else if (step <= UNITS) {
                         const uint32_t u = bcol + 8 * (step - 1);
-                        codes[step - 1] = FULL || u * 16 < a.pages.row.codes
-                                              ? *reinterpret_cast<const u32x4*>(src.row + u * 16)
-                                              : u32x4{};
+                        codes[x][step - 1] = FULL || u * 16 < a.pages.row.codes
+                                                 ? *reinterpret_cast<const u32x4*>(src.row + u * 16)
+                                                 : u32x4{};
                     } else if (step == UNITS + 1) {
                         if constexpr (F != K3X_CACHE_16BIT)
-                            scales = *reinterpret_cast<const u32x4*>(src.row + a.pages.row.scales);
+                            scales[x] =
+                                *reinterpret_cast<const u32x4*>(src.row + a.pages.row.scales);
                     } else {
-                        turned = *reinterpret_cast<const u32x4*>(
+                        turned[x] = *reinterpret_cast<const u32x4*>(
                             src.row + (bcol < a.R / 8 ? a.pages.row.codes + bcol * 16 : 0));
                     }
                 }
             };
-            auto bring_all = [&](uint32_t t, uint32_t b, uint32_t id) {
+            auto bring_all = [&](uint32_t t, uint32_t b, const Ids& id) {
 #pragma unroll
                 for (int i = 0; i < kBring; ++i) bring(i, t, b, id);
             };
             // Codes in registers to the values that they stand for in buffer b, in steps.
-            constexpr int kPut = DIRECT ? 0 : UNITS + 1;
-            auto put = [&](int k, uint32_t b) {
+            // 16 bytes of values a step, so that each passes beside one product.
+            constexpr int PER = F == K3X_CACHE_MXFP4 ? 4 : F == K3X_CACHE_MXFP8 ? 2 : 1;
+            constexpr int kPutSteps = UNITS * PER + 1, kPut = DIRECT ? 0 : XB * kPutSteps;
+            auto put = [&](int at, uint32_t b) {
                 if constexpr (!DIRECT) {
-                    uint8_t* dst = smem + b * kBuffer + btok * 128;
+                    const int i = at / kPutSteps, step = at % kPutSteps;
+                    uint8_t* dst = smem + b * kBuffer + i * 4096 + btok * 128;
                     const uint32_t z = swizzle(btok);
-                    if (k == UNITS) {
+                    if (step == UNITS * PER) {
                         *reinterpret_cast<u32x4*>(dst + (CG - 1) * kGroup + (bcol ^ z) * 16) =
-                            turned & (bcol < a.R / 8 ? 0xffffffffu : 0u);
+                            turned[i] & (bcol < a.R / 8 ? 0xffffffffu : 0u);
                         return;
                     }
+                    const int k = step / PER, j = step % PER;
                     const uint32_t u = bcol + 8 * k;
                     if constexpr (F == K3X_CACHE_16BIT) {
                         if (u * 8 < a.L)
-                            *reinterpret_cast<u32x4*>(dst + k * kGroup + (bcol ^ z) * 16) = codes[k];
+                            *reinterpret_cast<u32x4*>(dst + k * kGroup + (bcol ^ z) * 16) =
+                                codes[i][k];
                     } else if constexpr (F == K3X_CACHE_MXFP8) {
-                        const float sc = e8m0_to_f32(scales[k] >> (bcol / 2 * 8) & 0xff);
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const uint32_t x = 2 * (u % 4) + j;
-                            if (FULL || u * 16 < a.L)
-                                *reinterpret_cast<bf16x8*>(dst + u / 4 * kGroup + (x ^ z) * 16) =
-                                    mxfp8_8(uint2{codes[k][2 * j], codes[k][2 * j + 1]}, sc);
-                        }
+                        const float sc = e8m0_to_f32(scales[i][k] >> (bcol / 2 * 8) & 0xff);
+                        const uint32_t x = 2 * (u % 4) + j;
+                        if (FULL || u * 16 < a.L)
+                            *reinterpret_cast<bf16x8*>(dst + u / 4 * kGroup + (x ^ z) * 16) =
+                                mxfp8_8(uint2{codes[i][k][2 * j], codes[i][k][2 * j + 1]}, sc);
                     } else {
-                        const uint32_t dw = bcol / 4 ? scales[2 * k + 1] : scales[2 * k];
+                        const uint32_t dw = bcol / 4 ? scales[i][2 * k + 1] : scales[i][2 * k];
                         const float sc = e8m0_to_f32(dw >> (bcol % 4 * 8) & 0xff);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t x = 4 * (u % 2) + j;
-                            if (FULL || u * 32 < a.L)
-                                *reinterpret_cast<bf16x8*>(dst + u / 2 * kGroup + (x ^ z) * 16) =
-                                    dequant8(codes[k][j], sc);
-                        }
+                        const uint32_t x = 4 * (u % 2) + j;
+                        if (FULL || u * 32 < a.L)
+                            *reinterpret_cast<bf16x8*>(dst + u / 2 * kGroup + (x ^ z) * 16) =
+                                dequant8(codes[i][k][j], sc);
                     }
                 }
             };
@@ -342,21 +371,33 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
             // ---- one tile ---------------------------------------------------
             // Beside its products the loads of a later tile: direct ones to buffer nb; through
             // registers, tile t + 1 from them to the other buffer, then tile t + 2 to them.
-            auto tile = [&](uint32_t t, uint32_t b, uint32_t nb, uint32_t id) {
+            auto tile = [&](uint32_t t, uint32_t b, uint32_t nb, const Ids& id) {
                 const lds_byte* kb = lds + b * kBuffer;
+                const lds_byte* sb = kb + side * 4096;
                 // Operands are read a few products ahead: LDS takes some 200 cycles for four
                 // waves at once, a product 32.  (Left to itself the scheduler reads all of
                 // them first, past the registers there are.)
-                constexpr int XT = HT == 32 ? 1 : 2, HV = HT == 32 ? 2 : 1;
-                constexpr int NK = CG * KS * XT, NW = OT * HV;
+                constexpr int XT = HT == 32 ? 1 : 2, HV = HT == 32 ? kTile / 16 : kTile / 32;
+                constexpr int NK = CG * KS * XT, NW = OT * HV * RT;
                 Acc sc[XT];
 #pragma unroll
                 for (int i = 0; i < XT; ++i) sc[i] = Acc{};
+                // A later tile's loads beside product i of both: direct ones beside the scores',
+                // those through registers, with what is done to codes, beside all.
+                auto beside = [&](int i) {
+                    constexpr int n = DIRECT ? NK : NK + NW;
+#pragma unroll
+                    for (int x = 0; x < kPut + kBring; ++x)
+                        if (x * n / (kPut + kBring) == i) {
+                            if (x < kPut) put(x, nb);
+                            else bring(x - kPut, min(t + (DIRECT ? BUFS - 1 : 2), end - 1), nb, id);
+                        }
+                };
                 u32x4 kf[AHEAD];
                 const uint32_t kat = opaque(kat0);
                 auto keys = [&](int i) {
                     const int c = i / (KS * XT), y = i / XT % KS, x = i % XT;
-                    kf[i % AHEAD] = lds16(kb + c * kGroup + x * 2048 + (kat ^ y * (128 / KS)));
+                    kf[i % AHEAD] = lds16(sb + c * kGroup + x * 2048 + (kat ^ y * (128 / KS)));
                 };
                 // (Without a rotary part its group is zeros.)
 #pragma unroll
@@ -364,10 +405,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
 #pragma unroll
                 for (int i = 0; i < NK; ++i) {
                     if (i + AHEAD - 1 < NK) keys(i + AHEAD - 1);
-                    if constexpr (DIRECT)
-#pragma unroll
-                        for (int x = 0; x < kBring; ++x)
-                            if (x * NK / kBring == i) bring(x, min(t + BUFS - 1, end - 1), nb, id);
+                    beside(i);
                     __builtin_amdgcn_sched_barrier(0);
                     sc[i % XT] = M::run(kf[i % AHEAD], qf[i / XT], sc[i % XT]);
                     __builtin_amdgcn_sched_barrier(0);
@@ -395,7 +433,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     // Past what the row sees.
 #pragma unroll
                     for (int i = 0; i < NV; ++i) {
-                        const int32_t tok = (int32_t)(t * kTile) +
+                        const int32_t tok = (int32_t)(t * kTile + side * 32) +
                                             (HT == 32 ? 8 * (i / 4) + 4 * (int)g + i % 4
                                                       : 16 * (i / 4) + 4 * (int)g + i % 4);
                         if (tok >= sees) x[i] = -__builtin_inff();
@@ -407,36 +445,91 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                 top = across<HT>(top, [](float p, float r) { return fmaxf(p, r); }) * a.rate;
                 // The maximum that weights are taken from may lag by 2^8: sums and
                 // outputs keep their bits, and are seldom multiplied again.
-                if (__any(top > m + 8.0f)) {
-                    const float up = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - up);
-                    m = up;
-                    l *= keep;
-                    if (t != t0) scale_tiles<OT * sizeof(Acc) >= 512, 0, OT>(o, keep);
-                }
+                constexpr bool HELD = RT * OT * sizeof(Acc) >= 512;
+                float now = RT > 1 && srow ? m[RT - 1] : m[0];
+                const bool over = __any(top > now + 8.0f);
                 uint32_t p[NV / 2];
-                float sum = 0.0f;
+                float sum;
+                auto weights = [&] {
+                    sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < NV; i += 2) {
-                    const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.rate, -m));
-                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], a.rate, -m));
-                    sum += u + v;
-                    p[i / 2] = pack2<DT>(u, v);
+                    for (int i = 0; i < NV; i += 2) {
+                        const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], a.rate, -now));
+                        const float v =
+                            __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], a.rate, -now));
+                        sum += u + v;
+                        p[i / 2] = pack2<DT>(u, v);
+                    }
+                };
+                u32x4 pf[RT * HV];  // weights as the operands of the second products
+                if constexpr (JOINT) {
+                    // The wave's weights to all waves, formed again if for any the maximum
+                    // is passed.
+                    auto share = [&] {
+                        weights();
+                        if (wave / 2 < RT)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                *reinterpret_cast<u32x4*>(
+                                    smem + kWeights + (srow * 4 + side * 2 + h) * 1024 +
+                                    lane * 16) =
+                                    u32x4{p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]};
+                    };
+                    share();
+                    auto take = [&] {
+#pragma unroll
+                        for (int i = 0; i < RT * HV; ++i)
+                            pf[i] = lds16(lds + kWeights + i * 1024 + lane * 16);
+                    };
+                    if (g == 0)
+                        *reinterpret_cast<float*>(smem + kTops + (srow * 2 + side) * 128 +
+                                                  col * 4) = top;
+                    if (lane == 0) *reinterpret_cast<uint32_t*>(smem + kFlags + wave * 4) = over;
+                    barrier();
+                    const u32x4 flags = lds16(lds + kFlags);
+                    take();
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (__builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] |
+                                                       flags[3])) {
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) {
+                            const float* tops = reinterpret_cast<const float*>(smem + kTops);
+                            const float up = fmaxf(m[i], fmaxf(tops[i * 64 + col],
+                                                               tops[i * 64 + 32 + col]));
+                            const float keep = __builtin_amdgcn_exp2f(m[i] - up);
+                            m[i] = up;
+                            if ((uint32_t)i == srow) l *= keep;
+                            if (t != t0) {
+                                if (i == 0) scale_tiles<HELD, 0, OT>(o, keep);
+                                else scale_tiles<HELD, (RT - 1) * OT, OT>(o, keep);
+                            }
+                        }
+                        now = RT > 1 && srow ? m[RT - 1] : m[0];
+                        share();
+                        barrier();
+                        take();
+                    }
+                    l += sum;
+                } else {
+                    if (over) {
+                        const float up = fmaxf(m[0], top), keep = __builtin_amdgcn_exp2f(m[0] - up);
+                        m[0] = now = up;
+                        l *= keep;
+                        if (t != t0) scale_tiles<HELD, 0, OT>(o, keep);
+                    }
+                    weights();
+                    l += sum;
+#pragma unroll
+                    for (int h = 0; h < HV; ++h)
+                        pf[h] = u32x4{p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]};
                 }
-                l += sum;
 #pragma unroll
                 for (int i = 0; i < NW; ++i) {
-                    if (i + AHEAD - 1 < NW) values(i + AHEAD - 1);
-                    if constexpr (!DIRECT)
-#pragma unroll
-                        for (int x = 0; x < kPut + kBring; ++x)
-                            if (x * NW / (kPut + kBring) == i) {
-                                if (x < kPut) put(x, nb);
-                                else bring(x - kPut, min(t + 2, end - 1), 0, id);
-                            }
+                    const int v = i / RT, z = i % RT, y = v / HV, h = v % HV;
+                    if (z == 0 && v + AHEAD - 1 < NW / RT) values(v + AHEAD - 1);
+                    beside(NK + i);
                     __builtin_amdgcn_sched_barrier(0);
-                    const int y = i / HV, h = i % HV;
-                    o[y] = M::run(vf[i % AHEAD],
-                                  u32x4{p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]}, o[y]);
+                    o[z * OT + y] = M::run(vf[v % AHEAD], pf[z * HV + h], o[z * OT + y]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
@@ -446,7 +539,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                 if constexpr (DIRECT) {
                     // BUFS - 1 tiles on their way.  When one is used, the loads of the
                     // later ones may be outstanding, and no others are behind its own.
-                    uint32_t id = page_of(t0), next;
+                    Ids id = page_of(t0), next;
 #pragma unroll
                     for (uint32_t i = 0; i < BUFS - 1; ++i) {
                         next = page_of(min(t0 + i + 1, end - 1));
@@ -466,8 +559,8 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     wait_loads<0>();
                     barrier();
                 } else {
-                    const uint32_t id = page_of(t0);
-                    uint32_t next = page_of(min(t0 + 1, end - 1));
+                    const Ids id = page_of(t0);
+                    Ids next = page_of(min(t0 + 1, end - 1));
                     bring_all(t0, 0, id);
                     load_queries();
 #pragma unroll
@@ -477,7 +570,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     uint32_t b = 0;
                     for (uint32_t t = t0; t < end; ++t) {
                         barrier();
-                        const uint32_t now = next;
+                        const Ids now = next;
                         next = page_of(min(t + 3, end - 1));
                         tile(t, b, b ^ 1, now);
                         b ^= 1;
@@ -488,54 +581,77 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
 
             // ---- out ----------------------------------------------------------
             l = across<HT>(l, [](float p, float r) { return p + r; });
-            const bool live = r0 + wm * HT + col < rows;
-            const float inv = !whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
-            const uint32_t re = min(r0 + wm * HT + opaque(col), rows - 1);
-            const uint64_t row = s.begin + re / a.H;
-            const uint32_t head = re % a.H;
-            uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.os + (uint64_t)head * a.L;
+            float ls[RT];
+            ls[0] = l;
+            if constexpr (JOINT) {
+                // Of both halves of the tokens, for all waves.
+                float* sums = reinterpret_cast<float*>(smem + kTops);
+                barrier();
+                if (g == 0) sums[(srow * 2 + side) * 32 + col] = l;
+                barrier();
+#pragma unroll
+                for (int i = 0; i < RT; ++i) ls[i] = sums[i * 64 + col] + sums[i * 64 + 32 + col];
+                barrier();
+            }
             const size_t piece = ((size_t)w * a.RB + rb) * 2 + (t0 ? 0 : 1);
             constexpr int Q = HT == 32 ? 4 : 1;
-            float4* part = a.parts + piece * (S::rows * LP / 4) + wave * OT * Q * 64 + lane;
-            float check = l * 0.0f;  // NaN once something is not finite
-            auto each = [&](auto put4) {
+            auto block = [&](auto which) {
+                constexpr int z = decltype(which)::value;
+                const uint32_t at = (wm * RT + z) * HT;  // of the workgroup's rows
+                const float m1 = m[z], l1 = ls[z];
+                const bool live = r0 + at + col < rows;
+                const float inv = !whole ? 1.0f : l1 > 0.0f ? 1.0f / l1 : 0.0f;
+                const uint32_t re = min(r0 + at + opaque(col), rows - 1);
+                const uint64_t row = s.begin + re / a.H;
+                const uint32_t head = re % a.H;
+                uint16_t* out =
+                    static_cast<uint16_t*>(a.out) + row * a.os + (uint64_t)head * a.L;
+                float4* part = a.parts + piece * (S::rows * LP / 4) +
+                               (wave * RT + z) * OT * Q * 64 + lane;
+                float check = l1 * 0.0f;  // NaN once something is not finite
+                auto each = [&](auto put4) {
 #pragma unroll
-                for (int y = 0; y < OT; ++y) {
+                    for (int y = 0; y < OT; ++y) {
 #pragma unroll
-                    for (int i = 0; i < Q; ++i) {
-                        const uint32_t d = (y + wd * OT) * HT + 8 * i + 4 * g;
-                        const float4 v{o[y][4 * i] * inv, o[y][4 * i + 1] * inv,
-                                       o[y][4 * i + 2] * inv, o[y][4 * i + 3] * inv};
-                        if (!FULL && d >= a.L) continue;
-                        check = __builtin_fmaf(v.x, 0.0f, check);
-                        check = __builtin_fmaf(v.y, 0.0f, check);
-                        check = __builtin_fmaf(v.z, 0.0f, check);
-                        check = __builtin_fmaf(v.w, 0.0f, check);
-                        put4(y * Q + i, d, v);
+                        for (int i = 0; i < Q; ++i) {
+                            const uint32_t d = (y + wd * OT) * HT + 8 * i + 4 * g;
+                            const Acc& u = o[z * OT + y];
+                            const float4 v{u[4 * i] * inv, u[4 * i + 1] * inv, u[4 * i + 2] * inv,
+                                           u[4 * i + 3] * inv};
+                            if (!FULL && d >= a.L) continue;
+                            check = __builtin_fmaf(v.x, 0.0f, check);
+                            check = __builtin_fmaf(v.y, 0.0f, check);
+                            check = __builtin_fmaf(v.z, 0.0f, check);
+                            check = __builtin_fmaf(v.w, 0.0f, check);
+                            put4(y * Q + i, d, v);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
+                };
+                if (!whole)
+                    each([&](int f, uint32_t, float4 v) { part[f * 64] = v; });
+                else if (live)
+                    each([&](int, uint32_t d, float4 v) {
+                        *reinterpret_cast<uint2*>(out + d) =
+                            uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+                    });
+                bad_value |= live && !(check == 0.0f);
+                if (g == 0 && wd == 0) {
+                    if (!whole)
+                        a.sums[piece * S::rows + at + col] = float2{m1, l1};
+                    else if (a.lse && live)
+                        a.lse[row * a.H + head] =
+                            l1 > 0.0f ? (m1 + __builtin_amdgcn_logf(l1)) * 0.69314718055994531f
+                                      : -__builtin_inff();
                 }
             };
-            if (!whole)
-                each([&](int f, uint32_t, float4 v) { part[f * 64] = v; });
-            else if (live)
-                each([&](int, uint32_t d, float4 v) {
-                    *reinterpret_cast<uint2*>(out + d) = uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
-                });
-            bad_value |= live && !(check == 0.0f);
-            if (g == 0 && wd == 0) {
-                if (!whole)
-                    a.sums[piece * S::rows + wm * HT + col] = float2{m, l};
-                else if (a.lse && live)
-                    a.lse[row * a.H + head] =
-                        l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
-                                 : -__builtin_inff();
-            }
+            block(std::integral_constant<int, 0>{});
+            if constexpr (RT > 1) block(std::integral_constant<int, 1>{});
         }
         first += tiles;
         if (first >= to) break;
         do ++n;
-        while (n < a.pages.N && !tiles_of(a.pages, n, &s));
+        while (n < a.pages.N && !tiles_of<kTile>(a.pages, n, &s));
         if (n == a.pages.N) break;
     }
     if (bad_page) latch(a.status, K3X_ERR_INVALID_STATE);
@@ -547,7 +663,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
 // waves, each every fourth piece.
 template <uint32_t DT, int LP, typename S, bool FOUR>
 __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
-    constexpr int HT = S::HT, WD = S::WD;
+    constexpr int HT = S::HT, WD = S::WD, RT = S::RT;
     constexpr uint32_t kSlices = S::rows * LP / (FOUR ? 256 : 1024);
     constexpr uint32_t NF = LP / HT / WD * (HT == 32 ? 4 : 1);
     __shared__ float4 os[FOUR ? 4 : 1][64];
@@ -559,8 +675,8 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
     const uint32_t rows = s.count * a.H;
     if (status || !s.pieces || rb * S::rows >= rows) return;
     const uint32_t f = FOUR ? slice : slice * 4 + quarter, wave = f / NF, i = f % NF;
-    const uint32_t wm = wave / WD, wd = wave % WD;
-    const uint32_t at = wm * HT + lane % HT, r = rb * S::rows + at;
+    const uint32_t wd = wave / RT % WD;  // (wave: with its block of rows)
+    const uint32_t at = (wave / RT / WD * RT + wave % RT) * HT + lane % HT, r = rb * S::rows + at;
     const uint32_t d = HT == 32 ? wd * (LP / WD) + i / 4 * 32 + i % 4 * 8 + lane / 32 * 4
                                 : wd * (LP / WD) + i * 16 + lane / 16 * 4;
     const bool live = r < rows && d < a.L;
@@ -649,7 +765,7 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <uint32_t DT, uint32_t F, int LP, typename S, bool FULL>
 int launch(k3x_hip_ctx* ctx, const AttentionArgs& a) {
-    constexpr int BUFS = F == K3X_CACHE_16BIT && FULL && S::rows > 16 ? 3 : 2;
+    constexpr int BUFS = F == K3X_CACHE_16BIT && FULL && S::rows == 128 ? 3 : 2;
     hipLaunchKernelGGL((mla_attention_kernel<DT, F, LP, S, BUFS, FULL>), dim3(a.G * a.RB),
                        dim3(kThreads), 0, ctx->stream, a);
     const uint32_t splits = std::min(a.G, a.pages.N) * a.RB;
@@ -665,13 +781,13 @@ int launch(k3x_hip_ctx* ctx, const AttentionArgs& a) {
 template <uint32_t DT, uint32_t F, int LP>
 int launch_shape(k3x_hip_ctx* ctx, const AttentionArgs& a, const Plan& x) {
     if (!x.full)
-        return x.rows == 16 ? launch<DT, F, LP, Shape<16, 1, 4>, false>(ctx, a)
-                            : launch<DT, F, LP, Shape<32, 2, 2>, false>(ctx, a);
+        return x.rows == 16 ? launch<DT, F, LP, Shape<16, 1, 4, 1, 32>, false>(ctx, a)
+                            : launch<DT, F, LP, Shape<32, 2, 2, 1, 32>, false>(ctx, a);
     switch (x.rows) {
-        case 16: return launch<DT, F, LP, Shape<16, 1, 4>, true>(ctx, a);
-        case 32: return launch<DT, F, LP, Shape<32, 1, 4>, true>(ctx, a);
-        case 64: return launch<DT, F, LP, Shape<32, 2, 2>, true>(ctx, a);
-        default: return launch<DT, F, LP, Shape<32, 4, 1>, true>(ctx, a);
+        case 16: return launch<DT, F, LP, Shape<16, 1, 4, 1, 32>, true>(ctx, a);
+        case 32: return launch<DT, F, LP, Shape<32, 1, 4, 1, 64>, true>(ctx, a);
+        case 64: return launch<DT, F, LP, Shape<32, 1, 4, 2, 64>, true>(ctx, a);
+        default: return launch<DT, F, LP, Shape<32, 4, 1, 1, 32>, true>(ctx, a);
     }
 }
 template <uint32_t DT, uint32_t F>

@@ -98,7 +98,11 @@ def softmax_rows(q, k, v, sees, scale, dtype, d_extra=4):
     exponential's argument a few more: ds.  A weight is then off by a factor of exp(2 ds) (its own
     score and the largest), by 2^-21 for the exponential itself and by half a step of its type;
     the sum over n weights by n 2^-23 of itself, and so is the product with v.  The output is
-    rounded once more."""
+    rounded once more.
+
+    Below 2^-126 numbers may become zeros: the output, each weight (taken from a maximum that is
+    not above the row's, so that the largest weight and the sum that divides are 1 or more), which
+    then misses 2^-126 of its value at most, and each product of a weight and a value."""
     n, half = k.shape[0], HALF[dtype]
     sees = sees.clamp(0, n)
     hidden = torch.arange(n) >= sees[:, None]
@@ -113,7 +117,8 @@ def softmax_rows(q, k, v, sees, scale, dtype, d_extra=4):
     far = x.abs().masked_fill(hidden, 0.0).amax(1)
     ds = size * (q.shape[1] + d_extra) * 2.0 ** -23 + far * 2.0 ** -22
     off = half + 2 * ds + 2 * (sees + 8) * 2.0 ** -23 + 2.0 ** -20
-    tol = half * out.abs() + (1 + half) * off[:, None] * (w @ v.abs()) + 2.0 ** -126
+    tol = half * out.abs() + (1 + half) * off[:, None] * (w @ v.abs())
+    tol += 2.0 ** -126 * (1 + (~hidden).double() @ (v.abs() + 1))
     if dtype == torch.float16:
         tol += 2.0 ** -25  # half a step of its subnormal numbers
     ltol = ds + (sees + 8) * 2.0 ** -23 + 2.0 ** -20 + lse.abs() * 2.0 ** -23

@@ -373,6 +373,41 @@ def test_graphs_that_share_a_workspace(hip):
 
 
 @pytest.mark.parametrize("fmt", ["16bit", "mxfp8", "mxfp4"])
+@pytest.mark.parametrize("H", [3, 29, 50, 64, 100, 300])
+def test_rising_and_falling_scores(hip, fmt, H):
+    """Largest scores that rise by hundreds within a tile and from tile to tile, each row's with a
+    slope and a sign of its own, and rows whose largest is in one half of a tile's tokens."""
+    k3x, ctx = hip
+    n, wide = 3000, 256
+    print(f"[gpu-test] rising scores H={H} {fmt}", flush=True)
+    c = ref.make_cache([n, 130], wide, 0, 16, fmt, seed=H)
+    g = ref.gen(H)
+    for i, m in enumerate([n, 130]):
+        rows = torch.randn((m, wide), generator=g)
+        pos = torch.arange(m)
+        rows[:, 0] = torch.linspace(-30, 30, m)
+        rows[:, 1] = -torch.linspace(-20, 20, m).abs()
+        rows[:, 2] = torch.where(pos // 32 % 2 == 1, 16.0, -16.0)
+        none = torch.zeros((m, 0), dtype=BF16)
+        data, values = ref.encode(rows.to(BF16), none, fmt)
+        c["pool"][c["table"][i][pos // 16].long(), pos % 16] = data
+        c["rows"][i] = (values, none.double())
+    q = torch.randn((3, H, wide), generator=g) * 0.1
+    q[..., :3] = torch.randn((3, H, 3), generator=g) * 8
+    q = q.to(BF16)
+    d = mla.to_device(c)
+    p = mla.params(k3x, d, 3, H, 1.0, longest=2)
+    out = torch.empty((3, H, wide), dtype=BF16, device=DEV)
+    lse = torch.empty((3, H), device=DEV)
+    ws = torch.empty((k3x.mla_attention_workspace_bytes(p),), dtype=torch.uint8, device=DEV)
+    assert k3x.mla_attention(ctx, p, q.to(DEV), d["pool"], d["table"], mla.ints([n, 130]), out,
+                             offsets=mla.offsets_of([1, 2]), lse=lse, workspace=ws) == 0
+    assert ctx.synchronize() == 0
+    want, wl, tol, ltol = ref.attention(c, q, [1, 2], 1.0)
+    assert ref.close(out, want, tol) <= 1 and ref.close(lse, wl, ltol) <= 1
+
+
+@pytest.mark.parametrize("fmt", ["16bit", "mxfp8", "mxfp4"])
 @pytest.mark.parametrize("norm", [True, False], ids=["norm", "plain"])
 def test_many_tokens(hip, fmt, norm):
     """More tokens than one a wave, with empty sequences, ones padded to the left, first rows that
