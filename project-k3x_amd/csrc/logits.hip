@@ -16,6 +16,7 @@ using namespace k3x_ops;
 namespace {
 
 constexpr uint32_t kThreads = 256;
+constexpr uint32_t kPart = 2048;  // tokens of the vocabulary a workgroup
 constexpr uint32_t kInPrompt = 1u << 31;
 
 // 16 bytes of elements at any element's address: rows of an odd vocabulary are not
@@ -44,12 +45,11 @@ struct LogitsArgs {
 // before it is adjusted; counts and biases of the thread's tokens stay in registers.
 // 64 sequences of 4 drafts and 100003 fp32 logits with histories of 8000 (259 MB):
 // TIME.
-template <uint32_t DT, int KE>
+template <uint32_t DT>
 __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
     typedef typename Wide<DT>::E E;
     typedef typename Wide<DT>::Vec Vec;
-    constexpr int W = Wide<DT>::W, NV = KE / W;
-    constexpr uint32_t kPart = kThreads * KE;
+    constexpr int W = Wide<DT>::W, KE = kPart / kThreads, NV = KE / W;
     __shared__ uint32_t count[kPart], entry[kPart];
     const uint32_t n = blockIdx.x / a.parts, lo = blockIdx.x % a.parts * kPart;
     const uint32_t tid = threadIdx.x, hi = min(a.V, lo + kPart);
@@ -192,24 +192,16 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
     if (bad) latch(a.status, K3X_ERR_INVALID_STATE);
 }
 
-// Tokens a workgroup: few where there are few sequences, so that the parts fill the
-// chip, else more, since each part reads the whole history.
-uint32_t part_of(const k3x_hip_logits_params* p) {
-    return p->sequences * ((p->vocab + 4095) / 4096) < 512 ? 2048 : 4096;
-}
 template <uint32_t DT>
-int launch_logits(k3x_hip_ctx* ctx, const LogitsArgs& a, uint32_t part) {
-    const dim3 grid(a.N * a.parts), block(kThreads);
-    if (part == 2048)
-        hipLaunchKernelGGL((adjust_logits_kernel<DT, 8>), grid, block, 0, ctx->stream, a);
-    else
-        hipLaunchKernelGGL((adjust_logits_kernel<DT, 16>), grid, block, 0, ctx->stream, a);
+int launch_logits(k3x_hip_ctx* ctx, const LogitsArgs& a) {
+    hipLaunchKernelGGL((adjust_logits_kernel<DT>), dim3(a.N * a.parts), dim3(kThreads), 0,
+                       ctx->stream, a);
     return launched(ctx, 1);
 }
 
 bool logits_ok(const k3x_hip_logits_params* p) {
     const uint32_t words = (p->vocab + 31) / 32;
-    const uint64_t parts = (p->vocab + part_of(p) - 1) / part_of(p);
+    const uint64_t parts = (p->vocab + kPart - 1) / kPart;
     return p->sequences && p->sequences <= 65535 && p->drafts <= 64 && p->vocab &&
            p->vocab <= (1u << 20) && p->dtype <= K3X_DTYPE_BF16 &&
            (!p->row_stride || p->row_stride >= p->vocab) &&
@@ -269,11 +261,10 @@ int k3x_hip_adjust_logits(k3x_hip_ctx* ctx, const k3x_hip_logits_params* p, cons
     a.biases = p->biases;
     a.mask_rows = p->masks;
     a.mask_stride = p->mask_stride ? p->mask_stride : (p->vocab + 31) / 32;
-    const uint32_t part = part_of(p);
-    a.parts = (p->vocab + part - 1) / part;
+    a.parts = (p->vocab + kPart - 1) / kPart;
     a.status = ctx->status;
-    return p->dtype == K3X_DTYPE_F32 ? launch_logits<K3X_DTYPE_F32>(ctx, a, part)
-                                     : launch_logits<K3X_DTYPE_BF16>(ctx, a, part);
+    return p->dtype == K3X_DTYPE_F32 ? launch_logits<K3X_DTYPE_F32>(ctx, a)
+                                     : launch_logits<K3X_DTYPE_BF16>(ctx, a);
 }
 
 }  // extern "C"

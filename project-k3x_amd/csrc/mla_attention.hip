@@ -135,7 +135,13 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         return;
     }
     const uint32_t total = (uint32_t)all;
-    const uint32_t chunk = max(kLeast / kTile, (total + a.G - 1) / a.G);
+    // More than its share where the join of so many pieces would take longer: c tiles a
+    // range and t / c pieces of a sequence of t tiles cost least together at about
+    // sqrt(t / (kTile / 2)).  One sequence on 16 heads: of 16000 tokens 25.3 us without this
+    // and 19.7 with it, of 131072 54.4 and 43.2; two of 32000 the same, of four with N in
+    // place of N^2 28.2 and 30.8.
+    const uint32_t chunk = max(max(kLeast / kTile, (total + a.G - 1) / a.G),
+                               (uint32_t)(__builtin_sqrtf((float)total / (kTile / 2)) / a.pages.N));
     const uint32_t ranges = (total + chunk - 1) / chunk;  // in use, G at most
     // Consecutive ranges, and a range's row blocks, lie on one die: they share cached
     // tokens and queries.
@@ -751,7 +757,12 @@ Plan plan_of(const k3x_hip_mla_params* p) {
     Plan x;
     const uint64_t most = (uint64_t)(p->longest ? p->longest : p->tokens) * p->heads;
     x.LP = p->latent <= 256 ? 256 : 512;
-    x.rows = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : 128;
+    // As few rows as hold a sequence's.  More than 64 in blocks of 64, or of 128 once those
+    // of all sequences pass 64: half as many reads of the cache and of LDS, but twice the
+    // outputs of a range for the join.  128 heads, 16 bits, in blocks of 128 and of 64: 8
+    // sequences of 16384 69.6 and 58.4 us, 32 of 2048 57.3 and 43.1, of 8192 113 and 107; 64
+    // of 1000 54.5 and 45.5, of 4096 108 and 110, of 8192 184 and 198, in 8 bits 184 and 220.
+    x.rows = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : (most + 127) / 128 * p->sequences < 64 ? 64 : 128;
     x.full = p->latent == x.LP && (p->cache_format != K3X_CACHE_16BIT || p->page_size % 8 == 0);
     if (!x.full && x.rows > 16) x.rows = 64;  // the others: two shapes
     x.RB = (uint32_t)std::max<uint64_t>(1, (most + x.rows - 1) / x.rows);

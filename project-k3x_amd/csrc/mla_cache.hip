@@ -274,12 +274,15 @@ int cache_args(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const void* latent
     return K3X_OK;
 }
 
-// Eight tokens a wave once there are more than the waves that are held at once.
-// SPLIT
+// One token a wave, or eight past twice the waves that are held at once: with fewer, waves
+// that wait hide each other's time better.  In 4 bits one and eight, stored 8192 tokens 12.9
+// and 15.9 us, 16384 22.5 and 21.3, 32768 38.8 and 33.8; read 5.4 and 7.2, 8.2 and 8.7, 15.3
+// and 12.5.
+constexpr uint32_t kByEights = 16384;
 template <uint32_t DT, uint32_t F>
 int launch_store(k3x_hip_ctx* ctx, const CacheArgs& a) {
     const uint32_t T = a.pages.T;
-    if (T > 8192)
+    if (T > kByEights)
         hipLaunchKernelGGL((mla_store_kernel<DT, F, 8>), dim3((T + 31) / 32), dim3(kThreads), 0, ctx->stream, a);
     else
         hipLaunchKernelGGL((mla_store_kernel<DT, F, 1>), dim3((T + 3) / 4 + !T), dim3(kThreads), 0, ctx->stream, a);
@@ -288,7 +291,7 @@ int launch_store(k3x_hip_ctx* ctx, const CacheArgs& a) {
 template <uint32_t F>
 int launch_load(k3x_hip_ctx* ctx, const CacheArgs& a) {
     const uint32_t T = a.pages.T;
-    if (T > 8192)
+    if (T > kByEights)
         hipLaunchKernelGGL((mla_load_kernel<F, 8>), dim3((T + 31) / 32), dim3(kThreads), 0, ctx->stream, a);
     else
         hipLaunchKernelGGL((mla_load_kernel<F, 1>), dim3((T + 3) / 4 + !T), dim3(kThreads), 0, ctx->stream, a);

@@ -240,6 +240,17 @@ def test_many_sequences(hip, N):
     attend_case(hip, counts, [max(a, b) for a, b in zip(lens, counts)], 4, 64, 16, 16, extra=3)
 
 
+@pytest.mark.parametrize("fmt,dtype", FORMATS, ids=IDS)
+@pytest.mark.parametrize("L,R", [(512, 64), (256, 0), (160, 8)])
+def test_many_sequences_of_many_rows(hip, fmt, dtype, L, R):
+    """Enough rows for the largest blocks, part of them empty, one sequence in many ranges."""
+    lens = [900, 0, 1, 33] + [1 + 11 * n % 70 for n in range(61)]
+    attend_case(hip, [1] * 65, lens, 68, L, R, 16, fmt, dtype)
+    counts = [n % 3 for n in range(33)]
+    lens = [max(a, b) for a, b in zip(lens, counts)]
+    attend_case(hip, counts, lens, 100, L, R, 64, fmt, dtype, extra=2, spread=4.0)
+
+
 def test_without_offsets(hip):
     attend_case(hip, [2, 2, 2], [30, 2, 64], 16, offsets=False, longest=False)
     attend_case(hip, [3], [64], 16, offsets=True, longest=False, extra=2)

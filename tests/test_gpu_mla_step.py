@@ -410,14 +410,14 @@ def test_rising_and_falling_scores(hip, fmt, H):
 @pytest.mark.parametrize("fmt", ["16bit", "mxfp8", "mxfp4"])
 @pytest.mark.parametrize("norm", [True, False], ids=["norm", "plain"])
 def test_many_tokens(hip, fmt, norm):
-    """More tokens than one a wave, with empty sequences, ones padded to the left, first rows that
+    """More tokens than waves take one by one, with empty sequences, ones padded to the left, first rows that
     are no sequence's and rows past the last."""
     k3x, ctx = hip
-    counts = [0, 0, 3, 4100, 0, 1] + [1] * 75 + [0] * 70 + [4200, 0, 9, 17]
-    lens = [5, 0, 2, 4100, 9, 1] + [3] * 75 + [0] * 70 + [4300, 1, 9, 10]
+    counts = [0, 0, 3, 8200, 0, 1] + [1] * 75 + [0] * 70 + [8200, 0, 9, 17]
+    lens = [5, 0, 2, 8200, 9, 1] + [3] * 75 + [0] * 70 + [8300, 1, 9, 10]
     first, spare, page = 5, 30, 64
     T = first + sum(counts) + spare
-    assert T > 8192
+    assert T > 16384
     print(f"[gpu-test] {T} tokens {fmt}", flush=True)
     g = ref.gen(8)
     c = ref.make_cache(lens, L, R, page, fmt, seed=4)
