@@ -43,8 +43,11 @@ struct LogitsArgs {
 
 // KE tokens a thread, by 16 bytes.  A row's loads are on their way while the one
 // before it is adjusted; counts and biases of the thread's tokens stay in registers.
-// 64 sequences of 4 drafts and 100003 fp32 logits with histories of 8000 (259 MB):
-// TIME.
+// Bound: memory, and in small calls the part's history.  64 sequences of 4 drafts and
+// 100003 fp32 logits with histories of 8000 (259 MB): 70 us, 3.7 TB/s, from memory, 54
+// where half of it lies in the last cache; one sequence of 163840 bf16 logits 10.6 us.
+// Parts of 4096 read each history half as often, but fill the chip worse: 18.6 for 12.0 us
+// with one sequence (fp32), 26.8 for 22.2 with 16, 55.5 for 51.0 with 64.
 template <uint32_t DT>
 __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
     typedef typename Wide<DT>::E E;

@@ -14,6 +14,14 @@
 // The cached tokens of all sequences, in tiles of 32, are one line that is cut
 // into equal ranges for the workgroups: a sequence that falls into several
 // ranges is joined by a second launch.
+//
+// Bound: with many rows the reads of LDS, which each wave makes for both products, beside
+// the matrix cores (busy for 33 to 39% of the cycles) and the weights between them; with
+// few rows memory.  At a latent of 512 and a rotary part of 64: 64 sequences of 208000
+// tokens, 128 heads, 16 bits 107 us (88 and the join's 18, whose pieces are 82 MB written
+// and read); 8 windows of 5 tokens on 32 heads over 77000 tokens in E4M3 72 us; 4 sequences
+// of 417000 tokens, 64 heads, in E2M1 99 us, 581 TFLOP/s; 64 sequences of 8192 tokens, 32
+// heads, 16 bits 127 us, 4.8 TB/s; one of 1000 tokens on 16 heads 12.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -29,7 +37,9 @@ using namespace k3x_mla;
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kLeast = 64;  // cached tokens of a range at least
+// Cached tokens of a range at least.  One sequence of 500 tokens on 16 heads: 11.7 us, with
+// 128 13.5; on 128 heads 18.9 and 21.5.
+constexpr uint32_t kLeast = 64;
 
 // A sequence that begins in range w and ends in another.
 struct Split {
@@ -57,6 +67,9 @@ struct AttentionArgs {
 // latent; RT blocks of HT rows a wave.  Of 32 tokens each wave forms the scores of its own
 // rows.  Of 64 (JOINT) it forms those of one block of rows and half of the tokens, and
 // all waves take the weights from LDS: each part of a tile is read from there fewer times.
+// 64 sequences of 8192 tokens, 64 heads in E2M1: 139 us with 32 tokens, 109 with 64; 32
+// heads 132 and 98, in 16 bits 150 and 127.  (Of 128 rows a wave's outputs and queries fill
+// the registers with its own 32; of 16 two workgroups share a compute unit, and its LDS.)
 template <int HT_, int WM_, int WD_, int RT_, int TILE_>
 struct Shape {
     static constexpr int HT = HT_, WM = WM_, WD = WD_, RT = RT_, TILE = TILE_;
@@ -88,7 +101,8 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                        kFlags = kTops + RT * 256;
     constexpr int KS = HT == 32 ? 4 : 2;        // products over 64 columns
     constexpr int OT = LP / HT / WD;            // tiles of the latent, a wave
-    constexpr int AHEAD = F != K3X_CACHE_16BIT && S::rows == 128 ? 4 : 8;  // operands on their way
+    // Operands on their way; eight where the registers hold them.
+    constexpr int AHEAD = F != K3X_CACHE_16BIT && S::rows == 128 ? 4 : 8;
     typedef Mma<DT, HT> M;
     typedef typename M::Acc Acc;
     // One array: with several the compiler tells them apart, and waits for all direct
@@ -135,11 +149,11 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         return;
     }
     const uint32_t total = (uint32_t)all;
-    // More than its share where the join of so many pieces would take longer: c tiles a
-    // range and t / c pieces of a sequence of t tiles cost least together at about
-    // sqrt(t / (kTile / 2)).  One sequence on 16 heads: of 16000 tokens 25.3 us without this
-    // and 19.7 with it, of 131072 54.4 and 43.2; two of 32000 the same, of four with N in
-    // place of N^2 28.2 and 30.8.
+    // More than its share where the join of so many pieces takes longer: of a sequence of t
+    // tiles, c a range, both cost least together at about c = sqrt(t / (kTile / 2)); of N
+    // sequences the pieces are joined side by side, and c is less by another sqrt(N).  One
+    // sequence on 16 heads, of 16000 tokens: 25.3 us with its share alone and 19.7 so, of
+    // 131072 54.4 and 43.2; two of 32000 32.9 and 31.6, four of 16384 28.2 and 28.8.
     const uint32_t chunk = max(max(kLeast / kTile, (total + a.G - 1) / a.G),
                                (uint32_t)(__builtin_sqrtf((float)total / (kTile / 2)) / a.pages.N));
     const uint32_t ranges = (total + chunk - 1) / chunk;  // in use, G at most
@@ -762,7 +776,8 @@ Plan plan_of(const k3x_hip_mla_params* p) {
     // outputs of a range for the join.  128 heads, 16 bits, in blocks of 128 and of 64: 8
     // sequences of 16384 69.6 and 58.4 us, 32 of 2048 57.3 and 43.1, of 8192 113 and 107; 64
     // of 1000 54.5 and 45.5, of 4096 108 and 110, of 8192 184 and 198, in 8 bits 184 and 220.
-    x.rows = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : (most + 127) / 128 * p->sequences < 64 ? 64 : 128;
+    x.rows = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : 128;
+    if (x.rows == 128 && (most + 127) / 128 * p->sequences < 64) x.rows = 64;
     x.full = p->latent == x.LP && (p->cache_format != K3X_CACHE_16BIT || p->page_size % 8 == 0);
     if (!x.full && x.rows > 16) x.rows = 64;  // the others: two shapes
     x.RB = (uint32_t)std::max<uint64_t>(1, (most + x.rows - 1) / x.rows);
@@ -776,10 +791,13 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <uint32_t DT, uint32_t F, int LP, typename S, bool FULL>
 int launch(k3x_hip_ctx* ctx, const AttentionArgs& a) {
+    // Tiles in LDS: what it holds, for two workgroups of 16 rows.
     constexpr int BUFS = F == K3X_CACHE_16BIT && FULL && S::rows == 128 ? 3 : 2;
     hipLaunchKernelGGL((mla_attention_kernel<DT, F, LP, S, BUFS, FULL>), dim3(a.G * a.RB),
                        dim3(kThreads), 0, ctx->stream, a);
     const uint32_t splits = std::min(a.G, a.pages.N) * a.RB;
+    // Eight ranges a sequence and more: pieces by four waves.  One sequence in 250 ranges, 16
+    // heads: 26 us, with one wave 59; 64 in 4 each, 128 heads: 195, with one wave 181.
     if (a.G / a.pages.N >= 8)
         hipLaunchKernelGGL((mla_join_kernel<DT, LP, S, true>), dim3(splits * (S::rows * LP / 256)),
                            dim3(kThreads), 0, ctx->stream, a);

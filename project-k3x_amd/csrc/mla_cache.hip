@@ -5,6 +5,12 @@
 // of 32 is four lanes, its largest two exchanges within them, and a row one load and
 // one store a lane.  Of many tokens a wave takes eight, looked up together, with
 // their loads on their way together.
+//
+// Bound: memory, and with few tokens the chain of a token's sequence, page and row.
+// Kernels at a latent of 512 and a rotary part of 64: 64 decode tokens in E4M3 4.4 us
+// written and 3.8 read; 8192 tokens with their norm in E2M1 8.6 (13 MB) and 6.2; six
+// prefixes of 131072 tokens together read in 57 us, 237 MB at 4.1 TB/s, where a large
+// copy reaches 5.1.
 #include <hip/hip_runtime.h>
 
 #include "k3x_mla.hpp"
