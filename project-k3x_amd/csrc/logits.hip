@@ -37,7 +37,7 @@ struct LogitsArgs {
     const uint32_t *bias_offsets, *bias_tokens;
     const float* bias_values;
     const uint32_t *masks, *mask_index;
-    uint32_t N, D, V, stride, out_stride, width, biases, mask_rows, mask_stride, parts;
+    uint32_t N, D, V, stride, out_stride, width, biases, mask_rows, mask_stride;
     uint32_t* status;
 };
 
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
     typedef typename Wide<DT>::Vec Vec;
     constexpr int W = Wide<DT>::W, KE = kPart / kThreads, NV = KE / W;
     __shared__ uint32_t count[kPart], entry[kPart];
-    const uint32_t n = blockIdx.x / a.parts, lo = blockIdx.x % a.parts * kPart;
+    const uint32_t n = blockIdx.y, lo = blockIdx.x * kPart;
     const uint32_t tid = threadIdx.x, hi = min(a.V, lo + kPart);
     const uint32_t status = *(volatile uint32_t*)a.status;
     const uint32_t drafts = a.draft_counts ? a.draft_counts[n] : a.D;
@@ -197,20 +197,18 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
 
 template <uint32_t DT>
 int launch_logits(k3x_hip_ctx* ctx, const LogitsArgs& a) {
-    hipLaunchKernelGGL((adjust_logits_kernel<DT>), dim3(a.N * a.parts), dim3(kThreads), 0,
-                       ctx->stream, a);
+    hipLaunchKernelGGL((adjust_logits_kernel<DT>), dim3((a.V + kPart - 1) / kPart, a.N), dim3(kThreads),
+                       0, ctx->stream, a);
     return launched(ctx, 1);
 }
 
 bool logits_ok(const k3x_hip_logits_params* p) {
     const uint32_t words = (p->vocab + 31) / 32;
-    const uint64_t parts = (p->vocab + kPart - 1) / kPart;
     return p->sequences && p->sequences <= 65535 && p->drafts <= 64 && p->vocab &&
            p->vocab <= (1u << 20) && p->dtype <= K3X_DTYPE_BF16 &&
            (!p->row_stride || p->row_stride >= p->vocab) &&
            (!p->out_stride || p->out_stride >= p->vocab) &&
-           (!p->mask_stride || p->mask_stride >= words) &&
-           p->sequences * parts * kThreads < (1ull << 32);  // threads of a launch
+           (!p->mask_stride || p->mask_stride >= words);
 }
 
 }  // namespace
@@ -264,7 +262,6 @@ int k3x_hip_adjust_logits(k3x_hip_ctx* ctx, const k3x_hip_logits_params* p, cons
     a.biases = p->biases;
     a.mask_rows = p->masks;
     a.mask_stride = p->mask_stride ? p->mask_stride : (p->vocab + 31) / 32;
-    a.parts = (p->vocab + kPart - 1) / kPart;
     a.status = ctx->status;
     return p->dtype == K3X_DTYPE_F32 ? launch_logits<K3X_DTYPE_F32>(ctx, a)
                                      : launch_logits<K3X_DTYPE_BF16>(ctx, a);

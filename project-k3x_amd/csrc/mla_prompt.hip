@@ -125,9 +125,10 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
             count += blocks_of(r, lane * unit);
         }
         const uint32_t blocks = __builtin_amdgcn_readfirstlane(count);
-        // One sequence's blocks, up to two a compute unit, all begin at once: then the second
-        // half goes the other way, so that a long and a short one share a unit.  2048 tokens,
-        // 32 heads: 60.5 us, 62.4 without; 4096 tokens, in two rounds: 201, 184 without.
+        // Blocks mostly of one sequence, up to two a compute unit, all begin at once: then the
+        // second half goes the other way, so that a long and a short one share a unit.  2048
+        // tokens, 32 heads: 60.5 us, 62.4 without; 4096 tokens, in two rounds: 201, 184
+        // without; 1000, 700 and 300 tokens: 38.5, 34.2 without.
         if (a.flip && at < blocks && at >= blocks - blocks / 2)
             at = 2 * blocks - 1 - blocks / 2 - at;
         const uint64_t above = __ballot(count > at);
@@ -452,7 +453,8 @@ int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* p, con
     // Blocks of all sequences at most, each with one that is not full; the threads of a
     // launch, and eight rows apart within 32 bits.
     a.blocks = a.T / kRows + std::min(a.N, a.T);
-    a.flip = a.N == 1 && a.T / kRows * a.H <= 512;
+    const uint32_t longest = p->longest ? p->longest : a.T / a.N;
+    a.flip = longest > a.T / 2 && a.T / kRows * a.H <= 512;
     if ((uint64_t)a.blocks * a.H * kThreads >= (1ull << 32) ||
         a.ks > (1u << 27) || a.vs > (1u << 27) || a.rs > (1u << 27))
         return K3X_ERR_INVALID_EXTENT;

@@ -103,7 +103,7 @@ def test_long(hip):
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("Dn,R", [(128, 64), (128, 0), (64, 64)])
 def test_many_rows(hip, dtype, Dn, R):
-    """Enough rows of all heads for two tiles of queries a wave."""
+    """More workgroups than begin at once."""
     case(hip, [300, 1, 0, 257, 40, 140], [300, 77, 5, 400, 39, 140], 256, Dn, R, 128, dtype)
     case(hip, [1100], [1300], 128, Dn, R, 128, dtype, causal=False)
 
@@ -111,6 +111,20 @@ def test_many_rows(hip, dtype, Dn, R):
 def test_many_sequences(hip):
     counts = [n % 5 for n in range(150)]
     case(hip, counts, [c + n % 7 for n, c in enumerate(counts)], 2, 64, 32, 64)
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+@pytest.mark.parametrize("N", [2, 63, 64, 65])
+@pytest.mark.parametrize("hint", [None, 5000])
+def test_order_of_blocks(hip, N, causal, hint):
+    """Each block of queries is taken once, however lengths order them: one long sequence, many
+    equal ones, more queries than keys and none."""
+    g = ref.gen(N)
+    counts = torch.randint(0, 300, (N,), generator=g).tolist()
+    keys = [c + int(k) for c, k in zip(counts, torch.randint(-40, 200, (N,), generator=g))]
+    counts[0], keys[0], keys[1] = 1400, 1500, 0
+    case(hip, counts, [max(0, k) for k in keys], 1, 64, 0, 64, causal=causal, longest=hint)
+    case(hip, [130] * N, [200] * N, 1, 64, 0, 64, causal=causal, longest=hint)
 
 
 def test_without_offsets(hip):
