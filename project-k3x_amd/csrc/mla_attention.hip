@@ -210,9 +210,11 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                           (i16 & 1) * 8;
     // What the lane brings of each tile: one of eight columns of 16 bytes (codes: 16
     // bytes) of a token.  Direct loads fill LDS lane by lane, eight tokens a wave;
-    // through registers sixteen lanes write sixteen tokens, which do not meet in a bank.
+    // through registers eight lanes write every other one of sixteen tokens, which do not
+    // meet in a bank.
     constexpr bool DIRECT = F == K3X_CACHE_16BIT && FULL;
-    const uint32_t btok = DIRECT ? 8 * wave + lane / 8 : 16 * (wave / 2) + lane % 16;
+    const uint32_t btok = DIRECT ? 8 * wave + lane / 8
+                                 : 16 * (wave / 2) + lane % 8 * 2 + lane / 8 % 2;
     const uint32_t bcol = DIRECT ? lane % 8 : lane / 16 + 4 * (wave % 2);
     const uint32_t bput = bcol ^ swizzle(btok);
 
