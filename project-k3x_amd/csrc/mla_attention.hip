@@ -16,10 +16,10 @@
 // ranges is joined by a second launch.
 //
 // Bound: with many rows the reads of LDS, which each wave makes for both products, beside
-// the matrix cores (busy for 33 to 39% of the cycles) and the weights between them; with
+// the matrix cores (busy for 29 to 39% of the cycles) and the weights between them; with
 // few rows memory.  At a latent of 512 and a rotary part of 64: 64 sequences of 208000
 // tokens, 128 heads, 16 bits 107 us (88 and the join's 18, whose pieces are 82 MB written
-// and read); 8 windows of 5 tokens on 32 heads over 77000 tokens in E4M3 72 us; 4 sequences
+// and read); 8 windows of 5 tokens on 32 heads over 77000 tokens in E4M3 71 us; 4 sequences
 // of 417000 tokens, 64 heads, in E2M1 99 us, 581 TFLOP/s; 64 sequences of 8192 tokens, 32
 // heads, 16 bits 127 us, 4.8 TB/s; one of 1000 tokens on 16 heads 12.
 #include <hip/hip_runtime.h>
