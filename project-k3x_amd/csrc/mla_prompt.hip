@@ -6,12 +6,13 @@
 // wave holds 32 queries of one head and their outputs; the tiles of K and V of a
 // workgroup's head lie in LDS, brought straight from memory a tile ahead.
 //
-// Bound: the matrix cores, busy for 53% of the cycles: two waves a SIMD, and while both
-// form weights (some 500 of 2000 cycles a tile of 64 keys) nothing multiplies.  One prompt
-// of 2048 tokens, 32 heads of 128 + 64 and 128: 57 us, 757 TFLOP/s of products that count
-// (a large matrix product reaches 1218); seven ragged ones of 8192 tokens together 305 to
-// 312 us, 797 to 813 TFLOP/s.  Two tiles of 32 queries a wave, one wave a SIMD, take 547: then every cycle
-// of weights is one without products.
+// Bound: the matrix cores (busy for 53% of the cycles) and LDS: the two workgroups of a
+// compute unit take 3900 cycles for a tile of 64 keys each, 2560 of them products; reads of
+// LDS take about as long, and weights, 420 a wave, stand between.  One prompt of 2048
+// tokens, 32 heads of 128 + 64 and 128: 57 us, 757 TFLOP/s of products that count (a large
+// matrix product reaches 1218); seven ragged ones of 8192 tokens together 305 to 312 us,
+// 797 to 813 TFLOP/s.  Two tiles of 32 queries a wave, one wave a SIMD, read LDS half as
+// often, but take 547: then every cycle of weights is one without products.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
