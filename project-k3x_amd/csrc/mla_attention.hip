@@ -773,7 +773,8 @@ Plan plan_of(const k3x_hip_mla_params* p) {
     Plan x;
     const uint64_t most = (uint64_t)(p->longest ? p->longest : p->tokens) * p->heads;
     x.LP = p->latent <= 256 ? 256 : 512;
-    // As few rows as hold a sequence's.  More than 64 in blocks of 64, or of 128 once those
+    // As few rows as hold a sequence's: 16 heads, 64 sequences of 8192 tokens in 16 and 4 bits
+    // 120 and 81 us, with 32 rows 126 and 92.  More than 64 in blocks of 64, or of 128 once those
     // of all sequences pass 64: half as many reads of the cache and of LDS, but twice the
     // outputs of a range for the join.  128 heads, 16 bits, in blocks of 128 and of 64: 8
     // sequences of 16384 69.6 and 58.4 us, 32 of 2048 57.3 and 43.1, of 8192 113 and 107; 64
@@ -797,6 +798,7 @@ int launch(k3x_hip_ctx* ctx, const AttentionArgs& a) {
     constexpr int BUFS = F == K3X_CACHE_16BIT && FULL && S::rows == 128 ? 3 : 2;
     hipLaunchKernelGGL((mla_attention_kernel<DT, F, LP, S, BUFS, FULL>), dim3(a.G * a.RB),
                        dim3(kThreads), 0, ctx->stream, a);
+    if (a.G == 1) return launched(ctx, 1);  // nothing is cut
     const uint32_t splits = std::min(a.G, a.pages.N) * a.RB;
     // Eight ranges a sequence and more: pieces by four waves.  One sequence in 250 ranges, 16
     // heads: 26 us, with one wave 59; 64 in 4 each, 128 heads: 195, with one wave 181.
@@ -829,7 +831,8 @@ int launch_width(k3x_hip_ctx* ctx, const AttentionArgs& a, const Plan& x) {
 bool attention_ok(const k3x_hip_mla_params* p) {
     if (!mla_ok(p)) return false;
     const Plan x = plan_of(p);
-    return (uint64_t)x.G * x.RB * (x.rows * x.LP / 256) * kThreads < (1ull << 32);
+    // Threads of a launch; of one range there is no join.
+    return (uint64_t)x.G * x.RB * (x.G == 1 ? 1 : x.rows * x.LP / 256) * kThreads < (1ull << 32);
 }
 
 }  // namespace
@@ -839,7 +842,7 @@ extern "C" {
 size_t k3x_hip_mla_attention_workspace(const k3x_hip_mla_params* p) {
     if (!p || !attention_ok(p)) return 0;
     const Plan x = plan_of(p);
-    const size_t pieces = (size_t)x.G * x.RB * 2;
+    const size_t pieces = x.G == 1 ? 0 : (size_t)x.G * x.RB * 2;
     return up256(x.G * sizeof(Split)) + up256(pieces * x.rows * sizeof(float2)) +
            pieces * x.rows * x.LP * sizeof(float);
 }

@@ -251,6 +251,17 @@ def test_many_sequences_of_many_rows(hip, fmt, dtype, L, R):
     attend_case(hip, counts, lens, 100, L, R, 64, fmt, dtype, extra=2, spread=4.0)
 
 
+@pytest.mark.parametrize("fmt,dtype", FORMATS, ids=IDS)
+@pytest.mark.parametrize("L,R", [(512, 64), (96, 8)])
+def test_more_rows_than_workgroups(hip, fmt, dtype, L, R):
+    """Windows so long that no sequence is cut: no pieces, so next to no workspace."""
+    counts, lens = [270, 0, 31], [300, 50, 20]
+    attend_case(hip, counts, lens, 128, L, R, 16, fmt, dtype, extra=3)
+    k3x, _ = hip
+    p = params(k3x, to_device(ref.make_cache(lens, L, R, 16, fmt, dtype)), 304, 128, longest=270)
+    assert k3x.mla_attention_workspace_bytes(p) <= 256
+
+
 def test_without_offsets(hip):
     attend_case(hip, [2, 2, 2], [30, 2, 64], 16, offsets=False, longest=False)
     attend_case(hip, [3], [64], 16, offsets=True, longest=False, extra=2)
