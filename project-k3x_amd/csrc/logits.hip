@@ -53,10 +53,10 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
     typedef typename Wide<DT>::E E;
     typedef typename Wide<DT>::Vec Vec;
     constexpr int W = Wide<DT>::W, KE = kPart / kThreads, NV = KE / W;
-    __shared__ uint32_t count[kPart], entry[kPart];
+    __shared__ uint32_t count[kPart], entry[kPart], stop;
     const uint32_t n = blockIdx.y, lo = blockIdx.x * kPart;
     const uint32_t tid = threadIdx.x, hi = min(a.V, lo + kPart);
-    const uint32_t status = *(volatile uint32_t*)a.status;
+    if (tid == 0) stop = *(volatile uint32_t*)a.status;
     const uint32_t drafts = a.draft_counts ? a.draft_counts[n] : a.D;
     const uint32_t length = a.history ? a.history_lens[n] : 0;
     const uint32_t prompt = a.history && a.prompt_lens ? a.prompt_lens[n] : 0;
@@ -65,7 +65,9 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
     const float rep = a.repetition ? a.repetition[n] : 1.0f;
     const float freq = a.frequency ? a.frequency[n] : 0.0f;
     const float pres = a.presence ? a.presence[n] : 0.0f;
-    if (status || drafts == K3X_VERIFY_SKIP) return;
+    // All waves or none: another workgroup may latch between their looks.
+    __syncthreads();
+    if (stop || drafts == K3X_VERIFY_SKIP) return;
     if (drafts > a.D || length > a.width || prompt > length || b1 < b0 || b1 > a.biases ||
         !(rep > 0.0f && rep < __builtin_inff()) || !(fabsf(freq) < __builtin_inff()) ||
         !(fabsf(pres) < __builtin_inff())) {

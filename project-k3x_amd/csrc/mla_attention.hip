@@ -41,10 +41,10 @@ constexpr uint32_t kThreads = 256;
 // 128 13.5; on 128 heads 18.9 and 21.5.
 constexpr uint32_t kLeast = 64;
 
-// A sequence that begins in range w and ends in another.
+// A group of row blocks of a sequence that begins in range w and ends in another.
 struct Split {
     uint32_t pieces;  // ranges that it lies in; 0: none to join
-    uint32_t w, begin, count;
+    uint32_t w, begin, count, group;
 };
 
 struct AttentionArgs {
@@ -56,8 +56,9 @@ struct AttentionArgs {
     uint32_t H, L, R;
     uint64_t qs, os;
     float rate;  // scale * log2(e)
-    uint32_t G, RB;  // ranges, row blocks of a sequence at most
-    Split* splits;   // [N], or where there are more sequences than ranges [G], by range
+    uint32_t G, RB;  // ranges, row blocks of a group
+    uint32_t one;    // no sequence has more than one group
+    Split* splits;   // [N], or where there are more sequences or groups than ranges [G], by range
     float2* sums;    // [G][RB][2][rows]: maximum (log2) and sum of a piece
     float4* parts;   // [G][RB][2][rows * LP / 4]: its outputs, as the lanes hold them
     uint32_t* status;
@@ -77,13 +78,19 @@ struct Shape {
     static constexpr bool JOINT = TILE == 64;
 };
 
-// Tiles of a sequence in the line; an empty one takes one, in which its rows are
-// written as empty.
+// Tiles of a sequence; an empty one takes one, in which its rows are written as empty.
 template <uint32_t TILE>
 __device__ inline uint32_t tiles_in(const Tokens& s) { return max(1u, (s.len + TILE - 1) / TILE); }
+// Groups of row blocks that it has.
+__device__ inline uint32_t groups_in(const AttentionArgs& a, const Tokens& s, uint32_t rows) {
+    return a.one ? 1 : (s.count * a.H + a.RB * rows - 1) / (a.RB * rows);
+}
+// What it takes in the line, each group its tiles; kLong: more than is run.
+constexpr uint32_t kLong = 1u << 25;
 template <uint32_t TILE>
-__device__ inline uint32_t tiles_of(const Pages& a, uint32_t n, Tokens* s) {
-    return tokens_of(a, n, s) && s->count ? tiles_in<TILE>(*s) : 0;
+__device__ inline uint32_t tiles_of(const AttentionArgs& a, uint32_t n, uint32_t rows, Tokens* s) {
+    if (!tokens_of(a.pages, n, s) || !s->count) return 0;
+    return (uint32_t)min((uint64_t)kLong, (uint64_t)tiles_in<TILE>(*s) * groups_in(a, *s, rows));
 }
 
 // FULL: L is LP (else the columns past L are zeros, and not brought or written) and
@@ -110,6 +117,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     __shared__ __attribute__((aligned(256))) uint8_t smem[JOINT ? kFlags + 16 : kWeights];
     uint32_t* const scan = reinterpret_cast<uint32_t*>(smem);  // before the first tile
     uint32_t* const at_s = scan + 4;
+    uint32_t* const stop_s = scan + 12;
     lds_byte* const lds = (lds_byte*)smem;
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -121,7 +129,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     Tokens mine;
     auto scan_tiles = [&](uint32_t base, uint32_t* own) {
         const uint32_t n = base + tid;
-        uint32_t c = *own = n < a.pages.N ? tiles_of<kTile>(a.pages, n, &mine) : 0;
+        uint32_t c = *own = n < a.pages.N ? tiles_of<kTile>(a, n, S::rows, &mine) : 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t o = __shfl_up(c, d);
@@ -134,20 +142,25 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         for (uint32_t i = 0; i < wave; ++i) before += scan[i];
         return before + c;  // with the thread's own
     };
-    const bool by_sequence = a.pages.N <= a.G;
+    const bool by_sequence = a.one && a.pages.N <= a.G;
     uint64_t all = 0;
+    bool over_long = false;
     uint32_t own, upto = 0;
     for (uint32_t base = 0; base < a.pages.N; base += kThreads) {
         upto = scan_tiles(base, &own);
+        over_long |= own >= kLong;
         all += (uint64_t)scan[0] + scan[1] + scan[2] + scan[3];
         if (by_sequence && blockIdx.x == 0 && !own && base + tid < a.pages.N)
             a.splits[base + tid].pieces = 0;  // in no range
     }
-    if (status) return;
-    if (all >> 32) {
-        if (tid == 0) latch(a.status, K3X_ERR_INVALID_STATE);
-        return;
-    }
+    // All waves or none: another workgroup may latch between their looks.  (Not by the
+    // barrier that counts, which has an array of LDS of its own.)
+    over_long |= all >> 32;
+    if (over_long) latch(a.status, K3X_ERR_INVALID_STATE);
+    const bool stop = __any(status || over_long);
+    if (lane == 0) stop_s[wave] = stop;
+    __syncthreads();
+    if (stop_s[0] | stop_s[1] | stop_s[2] | stop_s[3]) return;
     const uint32_t total = (uint32_t)all;
     // More than its share where the join of so many pieces takes longer: of a sequence of t
     // tiles, c a range, both cost least together at about c = sqrt(t / (kTile / 2)); of N
@@ -186,9 +199,13 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     }
     __syncthreads();
     auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane(x); };
-    uint32_t n = uniform(at_s[0]), first = uniform(at_s[1]);
+    uint32_t n = uniform(at_s[0]), first = uniform(at_s[1]), group = 0;
     Tokens s{uniform(at_s[2]), uniform(at_s[3]), uniform(at_s[4])};
     __syncthreads();
+    if (!a.one) {
+        group = (from - first) / tiles_in<kTile>(s);
+        first += group * tiles_in<kTile>(s);
+    }
 
     // What is not brought to LDS stays zero there.
     if (!FULL) {
@@ -226,8 +243,8 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         const bool whole = t0 == 0 && t1 == tiles;
         if (rb == 0 && tid == 0 && t0 == 0 && (by_sequence || t1 < tiles))
             a.splits[by_sequence ? n : w] =
-                Split{t1 < tiles ? (first + tiles - 1) / chunk - w + 1 : 0, w, s.begin, s.count};
-        const uint32_t r0 = rb * S::rows;
+                Split{t1 < tiles ? (first + tiles - 1) / chunk - w + 1 : 0, w, s.begin, s.count, group};
+        const uint32_t r0 = (group * a.RB + rb) * S::rows;
         if (r0 < rows) {
             // The row of this lane, and how many tokens it sees.
             const uint32_t r = min(r0 + srow * HT + opaque(col), rows - 1), ri = r / a.H;
@@ -672,8 +689,10 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         }
         first += tiles;
         if (first >= to) break;
+        if (++group < groups_in(a, s, S::rows)) continue;
+        group = 0;
         do ++n;
-        while (n < a.pages.N && !tiles_of<kTile>(a.pages, n, &s));
+        while (n < a.pages.N && !tiles_of<kTile>(a, n, S::rows, &s));
         if (n == a.pages.N) break;
     }
     if (bad_page) latch(a.status, K3X_ERR_INVALID_STATE);
@@ -695,10 +714,11 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
     const uint32_t status = *(volatile uint32_t*)a.status;
     const Split s = a.splits[x / a.RB];
     const uint32_t rows = s.count * a.H;
-    if (status || !s.pieces || rb * S::rows >= rows) return;
+    const uint32_t r0 = (s.group * a.RB + rb) * S::rows;
+    if (status || !s.pieces || r0 >= rows) return;
     const uint32_t f = FOUR ? slice : slice * 4 + quarter, wave = f / NF, i = f % NF;
     const uint32_t wd = wave / RT % WD;  // (wave: with its block of rows)
-    const uint32_t at = (wave / RT / WD * RT + wave % RT) * HT + lane % HT, r = rb * S::rows + at;
+    const uint32_t at = (wave / RT / WD * RT + wave % RT) * HT + lane % HT, r = r0 + at;
     const uint32_t d = HT == 32 ? wd * (LP / WD) + i / 4 * 32 + i % 4 * 8 + lane / 32 * 4
                                 : wd * (LP / WD) + i * 16 + lane / 16 * 4;
     const bool live = r < rows && d < a.L;
@@ -767,7 +787,7 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
 // How a call is laid out: rows of a workgroup, ranges, row blocks.
 struct Plan {
     uint32_t rows, G, RB, LP;
-    bool full;
+    bool full, one;
 };
 Plan plan_of(const k3x_hip_mla_params* p) {
     Plan x;
@@ -783,7 +803,15 @@ Plan plan_of(const k3x_hip_mla_params* p) {
     if (x.rows == 128 && (most + 127) / 128 * p->sequences < 64) x.rows = 64;
     x.full = p->latent == x.LP && (p->cache_format != K3X_CACHE_16BIT || p->page_size % 8 == 0);
     if (!x.full && x.rows > 16) x.rows = 64;  // the others: two shapes
-    x.RB = (uint32_t)std::max<uint64_t>(1, (most + x.rows - 1) / x.rows);
+    // The row blocks of a sequence run side by side and share its cached tokens; of more than
+    // eight a group of as many as sequences have on average, so that a long window does not
+    // leave single tokens beside it to one workgroup: a window of 512 tokens and 63 tokens over
+    // 4096 each, 128 heads in 16 bits, 358 us, with all blocks of a sequence in one group 13274;
+    // the window alone 179, and 492.
+    const uint64_t blocks = std::max<uint64_t>(1, (most + x.rows - 1) / x.rows);
+    const uint64_t average = (uint64_t)p->tokens * p->heads / p->sequences / x.rows + 1;
+    x.one = blocks <= 8;
+    x.RB = (uint32_t)(x.one ? blocks : std::min<uint64_t>(8, average));
     // Two workgroups a compute unit where registers and LDS allow.
     const uint32_t places = x.rows == 16 ? 512 : 256;
     x.G = std::max(1u, places / x.RB);
@@ -798,8 +826,7 @@ int launch(k3x_hip_ctx* ctx, const AttentionArgs& a) {
     constexpr int BUFS = F == K3X_CACHE_16BIT && FULL && S::rows == 128 ? 3 : 2;
     hipLaunchKernelGGL((mla_attention_kernel<DT, F, LP, S, BUFS, FULL>), dim3(a.G * a.RB),
                        dim3(kThreads), 0, ctx->stream, a);
-    if (a.G == 1) return launched(ctx, 1);  // nothing is cut
-    const uint32_t splits = std::min(a.G, a.pages.N) * a.RB;
+    const uint32_t splits = (a.one ? std::min(a.G, a.pages.N) : a.G) * a.RB;
     // Eight ranges a sequence and more: pieces by four waves.  One sequence in 250 ranges, 16
     // heads: 26 us, with one wave 59; 64 in 4 each, 128 heads: 195, with one wave 181.
     if (a.G / a.pages.N >= 8)
@@ -831,8 +858,7 @@ int launch_width(k3x_hip_ctx* ctx, const AttentionArgs& a, const Plan& x) {
 bool attention_ok(const k3x_hip_mla_params* p) {
     if (!mla_ok(p)) return false;
     const Plan x = plan_of(p);
-    // Threads of a launch; of one range there is no join.
-    return (uint64_t)x.G * x.RB * (x.G == 1 ? 1 : x.rows * x.LP / 256) * kThreads < (1ull << 32);
+    return (uint64_t)(p->longest ? p->longest : p->tokens) * p->heads < (1ull << 31) && x.G;
 }
 
 }  // namespace
@@ -842,7 +868,7 @@ extern "C" {
 size_t k3x_hip_mla_attention_workspace(const k3x_hip_mla_params* p) {
     if (!p || !attention_ok(p)) return 0;
     const Plan x = plan_of(p);
-    const size_t pieces = x.G == 1 ? 0 : (size_t)x.G * x.RB * 2;
+    const size_t pieces = (size_t)x.G * x.RB * 2;
     return up256(x.G * sizeof(Split)) + up256(pieces * x.rows * sizeof(float2)) +
            pieces * x.rows * x.LP * sizeof(float);
 }
@@ -876,6 +902,7 @@ int k3x_hip_mla_attention(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const v
     a.rate = p->scale * 1.4426950408889634f;
     a.G = x.G;
     a.RB = x.RB;
+    a.one = x.one;
     uint8_t* w = static_cast<uint8_t*>(workspace);
     const size_t pieces = (size_t)x.G * x.RB * 2;
     a.splits = reinterpret_cast<Split*>(w);

@@ -83,7 +83,12 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t h = blockIdx.x % a.H;
-    if (*(volatile uint32_t*)a.status) return;
+    // All waves or none: another workgroup may latch between their looks.
+    if (tid == 0) scan[0] = *(volatile uint32_t*)a.status;
+    __syncthreads();
+    const uint32_t status = scan[0];
+    __syncthreads();
+    if (status) return;
 
     // The workgroup's block of queries.  Blocks of up to 64 sequences are taken from those
     // with the most keys to those with the fewest, in 64 classes, so that no long one begins

@@ -253,13 +253,15 @@ def test_many_sequences_of_many_rows(hip, fmt, dtype, L, R):
 
 @pytest.mark.parametrize("fmt,dtype", FORMATS, ids=IDS)
 @pytest.mark.parametrize("L,R", [(512, 64), (96, 8)])
-def test_more_rows_than_workgroups(hip, fmt, dtype, L, R):
-    """Windows so long that no sequence is cut: no pieces, so next to no workspace."""
-    counts, lens = [270, 0, 31], [300, 50, 20]
-    attend_case(hip, counts, lens, 128, L, R, 16, fmt, dtype, extra=3)
+def test_more_row_blocks_than_a_group(hip, fmt, dtype, L, R):
+    """Long windows beside single tokens: groups of row blocks, several a range and cut between
+    ranges, with and without `longest`."""
+    attend_case(hip, [270, 0, 31], [300, 50, 20], 128, L, R, 16, fmt, dtype, extra=3)
+    attend_case(hip, [1, 70] + [1, 2] * 3, [900, 400, 5, 2, 300, 3, 1, 64], 24, L, R, 16, fmt, dtype,
+                longest=False)
     k3x, _ = hip
-    p = params(k3x, to_device(ref.make_cache(lens, L, R, 16, fmt, dtype)), 304, 128, longest=270)
-    assert k3x.mla_attention_workspace_bytes(p) <= 256
+    p = params(k3x, to_device(ref.make_cache([9], L, R, 16, fmt, dtype)), 1 << 14, 128)
+    assert k3x.mla_attention_workspace_bytes(p) <= 1 << 28
 
 
 def test_without_offsets(hip):
