@@ -627,9 +627,10 @@ enum k3x_cache_format { K3X_CACHE_16BIT = 0, K3X_CACHE_MXFP8 = 1, K3X_CACHE_MXFP
  * Latched as K3X_ERR_INVALID_STATE by every call, which then reads and writes
  * nothing outside its tensors and the pool, and leaves outputs undefined: offsets
  * that fall or pass T, a length past table_width * page_size or 2^29, a page in use
- * that is not below `pages`, more tokens in a sequence than `longest`, and by
- * k3x_hip_mla_attention a sequence whose rows (tokens x heads) times positions pass
- * 2^36. */
+ * that is not below `pages`, more tokens in a sequence than `longest`.  Attention
+ * may also latch more work than one call takes: a sequence whose rows (tokens x
+ * heads) times positions pass 2^36, or sequences for which these products together
+ * pass 2^40 or whose positions together pass 2^34. */
 typedef struct k3x_hip_mla_params {
     uint32_t sequences;    /* N, 1 .. 65535 */
     uint32_t tokens;       /* T, 0 .. 2^22 */

@@ -85,8 +85,11 @@ __device__ inline uint32_t tiles_in(const Tokens& s) { return max(1u, (s.len + T
 __device__ inline uint32_t groups_in(const AttentionArgs& a, const Tokens& s, uint32_t rows) {
     return a.one ? 1 : (s.count * a.H + a.RB * rows - 1) / (a.RB * rows);
 }
-// What it takes in the line, each group its tiles; kLong: more than is run.
-constexpr uint32_t kLong = 1u << 25;
+// What it takes in the line, each group its tiles; kLong: more than is run.  Up to 2^36 rows
+// times positions stay below it: (rows + 63) (positions + 31) / 2048, of fewer than 2^31 rows
+// and at most 2^29 positions.  64 sequences below it are counted in 32 bits, and all together
+// have to stay below 2^31, so that ranges and their ends do too.
+constexpr uint32_t kLong = 1u << 26;
 template <uint32_t TILE>
 __device__ inline uint32_t tiles_of(const AttentionArgs& a, uint32_t n, uint32_t rows, Tokens* s) {
     if (!tokens_of(a.pages, n, s) || !s->count) return 0;
@@ -155,7 +158,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     }
     // All waves or none: another workgroup may latch between their looks.  (Not by the
     // barrier that counts, which has an array of LDS of its own.)
-    over_long |= all >> 32;
+    over_long |= all >> 31 != 0;
     if (over_long) latch(a.status, K3X_ERR_INVALID_STATE);
     const bool stop = __any(status || over_long);
     if (lane == 0) stop_s[wave] = stop;

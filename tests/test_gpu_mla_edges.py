@@ -1,0 +1,103 @@
+"""Latent attention where it can go wrong silently: scores that are no numbers, small weights
+beside a large one, values at the end of their type, calls of no tokens, the most that a call
+takes, distances past 32 bits, and largest scores that rise within a range in every layout."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+import mla_reference as ref
+import test_gpu_mla as mla
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+DEV = "cuda:0"
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def hip():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import k3x_amd
+    ctx = k3x_amd.Context(0)
+    yield k3x_amd, ctx
+    ctx.close()
+
+
+def plain_cache(lens, L, R, page, latent, rotary, dtype=BF16):
+    """A 16-bit cache of one row for every position: latent [n][L] and rotary [n][R] of the longest
+    sequence, of which the others have the first rows."""
+    counts = [-(-n // page) for n in lens]
+    width = max(counts)
+    n = max(lens)
+    data = ref.encode(latent.to(dtype), rotary.to(dtype), "16bit")[0]
+    pool = torch.zeros((width * page, data.shape[1]), dtype=torch.uint8)
+    pool[:n] = data
+    table = torch.arange(width, dtype=torch.int32).repeat(len(lens), 1)
+    return dict(pool=pool.view(width, page, -1).to(DEV), table=table.to(DEV), L=L, R=R,
+                fmt="16bit", dtype=dtype)
+
+
+def attend(hip, c, q, lens, scale=1.0, longest=1, offsets=None):
+    """(status that was latched, out, lse); workspace and outputs full of other bytes."""
+    k3x, ctx = hip
+    T, H = q.shape[:2]
+    p = mla.params(k3x, c, T, H, scale, longest=longest)
+    out = torch.full((T, H, c["L"]), 7.0, dtype=c["dtype"], device=DEV)
+    lse = torch.full((T, H), 7.0, device=DEV)
+    ws = torch.full((k3x.mla_attention_workspace_bytes(p),), 255, dtype=torch.uint8, device=DEV)
+    assert k3x.mla_attention(ctx, p, q.to(DEV), c["pool"], c["table"], mla.ints(lens), out,
+                             offsets=offsets, lse=lse, workspace=ws) == 0
+    return ctx.synchronize(), out.double().cpu(), lse.double().cpu()
+
+
+def prompt(hip, q, k, v, rotary, scale=1.0, causal=True, **kw):
+    k3x, ctx = hip
+    q, k, v = q.to(DEV), k.to(DEV), v.to(DEV)
+    rotary = None if rotary is None else rotary.to(DEV)
+    out = torch.full((q.shape[0], q.shape[1], v.shape[2]), 7.0, dtype=q.dtype, device=DEV)
+    lse = torch.full(q.shape[:2], 7.0, device=DEV)
+    p = k3x.make_mla_prompt_params(q, k, v, 1, rotary=rotary, causal=causal, scale=scale)
+    assert k3x.mla_prompt(ctx, p, q, k, v, out, rotary=rotary, lse=lse, **kw) == 0
+    return ctx.synchronize(), out.double().cpu(), lse.double().cpu()
+
+
+def long_calls(hip, counts, lens, H, longest, L=32):
+    """Attention over one page of equal rows that every position of every sequence is in."""
+    page, width = 65536, 8192
+    N = len(lens)
+    data = ref.encode(torch.ones((1, L), dtype=BF16), torch.zeros((1, 0), dtype=BF16), "16bit")[0]
+    c = dict(pool=data.repeat(page, 1).view(1, page, -1).to(DEV),
+             table=torch.zeros((N, width), dtype=torch.int32, device=DEV), L=L, R=0, fmt="16bit",
+             dtype=BF16)
+    q = torch.ones((sum(counts), H, L), dtype=BF16)
+    mla.say(f"{N} sequences, longest {max(lens)}, {H} heads")
+    return attend(hip, c, q, lens, 1.0, longest, mla.offsets_of(counts))
+
+
+def test_most_rows_of_the_longest_sequence(hip):
+    """128 rows over 2^29 positions, in blocks of 64 beside single tokens."""
+    n = 1 << 29
+    st, out, lse = long_calls(hip, [2] + [1] * 31 + [0] * 32, [n] + [1] * 31 + [0] * 32, 64, 16)
+    assert st == 0
+    assert (out == 1).all()
+    sees = torch.tensor([n - 1, n] + [1] * 31, dtype=torch.float64)
+    # Equal weights: sums of ones up to 2^21 a range, exact, and their 256 pieces.
+    assert float((lse - 32 - sees.log()[:, None]).abs().max()) <= 2.0 ** -17
+
+
+@pytest.mark.parametrize("total", [1 << 31, (1 << 31) + 5, (1 << 32) - 600, (1 << 32) - 100,
+                                   (1 << 32) - 1, 1 << 32, (1 << 32) + 70], ids=hex)
+def test_more_than_a_call_takes_is_latched(hip, total):
+    """Sequences that make 2^31 tiles of 32 positions together and more, around what 32 bits hold:
+    latched before a page is looked at."""
+    k3x, ctx = hip
+    each, lens = 1 << 24, []
+    while total:
+        lens.append(min(each, total) * 32)
+        total -= min(each, total)
+    st, _, _ = long_calls(hip, [1] * len(lens), lens, 1, 1)
+    assert st == k3x.ERR_INVALID_STATE
+    assert ctx.synchronize() == 0
