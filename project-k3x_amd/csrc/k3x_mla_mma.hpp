@@ -71,6 +71,10 @@ __device__ inline float across(float x, Op op) {
     return x;
 }
 
+// A row that sees tokens has a sum: its largest weight is 1.  None (or NaN) is that of scores
+// that are all minus infinity, or no numbers.
+__device__ inline bool no_softmax(int32_t sees, float sum) { return sees > 0 && !(sum > 0.0f); }
+
 // x, as a value that is not computed ahead of the place and held until then.
 __device__ inline uint32_t opaque(uint32_t x) {
     asm volatile("" : "+v"(x));

@@ -45,6 +45,7 @@ constexpr uint32_t kLeast = 64;
 struct Split {
     uint32_t pieces;  // ranges that it lies in; 0: none to join
     uint32_t w, begin, count, group;
+    int32_t before;   // positions before the first of its tokens
 };
 
 struct AttentionArgs {
@@ -246,7 +247,8 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
         const bool whole = t0 == 0 && t1 == tiles;
         if (rb == 0 && tid == 0 && t0 == 0 && (by_sequence || t1 < tiles))
             a.splits[by_sequence ? n : w] =
-                Split{t1 < tiles ? (first + tiles - 1) / chunk - w + 1 : 0, w, s.begin, s.count, group};
+                Split{t1 < tiles ? (first + tiles - 1) / chunk - w + 1 : 0, w, s.begin, s.count, group,
+                      (int32_t)s.len - (int32_t)s.count};
         const uint32_t r0 = (group * a.RB + rb) * S::rows;
         if (r0 < rows) {
             // The row of this lane, and how many tokens it sees.
@@ -678,6 +680,9 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                             uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
                     });
                 bad_value |= live && !(check == 0.0f);
+                if (whole)
+                    bad_value |= live && no_softmax((int32_t)s.len - (int32_t)s.count +
+                                                        (int32_t)(re / a.H) + 1, l1);
                 if (g == 0 && wd == 0) {
                     if (!whole)
                         a.sums[piece * S::rows + at + col] = float2{m1, l1};
@@ -778,6 +783,7 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
     }
     if (!live) return;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (no_softmax(s.before + (int32_t)(r / a.H) + 1, l)) latch(a.status, K3X_ERR_INVALID_MXFP4);
     const uint64_t t = s.begin + r / a.H;
     uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.os + (uint64_t)(r % a.H) * a.L + d;
     *reinterpret_cast<uint2*>(out) = uint2{pack2<DT>(o.x * inv, o.y * inv),

@@ -101,3 +101,50 @@ def test_more_than_a_call_takes_is_latched(hip, total):
     st, _, _ = long_calls(hip, [1] * len(lens), lens, 1, 1)
     assert st == k3x.ERR_INVALID_STATE
     assert ctx.synchronize() == 0
+
+
+# Rows a block and layouts: heads, latent, rotary part.
+LAYOUTS = [(4, 512, 64), (24, 512, 64), (48, 512, 64), (96, 512, 64), (4, 96, 16), (48, 96, 16)]
+
+
+@pytest.mark.parametrize("H,L,R", LAYOUTS)
+@pytest.mark.parametrize("n", [1, 20, 4000])
+@pytest.mark.parametrize("finite", [False, True], ids=["infinity", "overflow"])
+def test_scores_of_minus_infinity_are_latched(hip, H, L, R, n, finite):
+    """A row whose scores are all minus infinity has no softmax: it is not one that sees nothing."""
+    k3x, ctx = hip
+    mla.say(f"scores of minus infinity H={H} L={L} n={n} finite={finite}")
+    rotary = torch.zeros((n, R))
+    rotary[:, 3] = 3e38 if finite else 1.0
+    c = plain_cache([n, n], L, R, 16, torch.ones((n, L)), rotary)
+    q = torch.ones((2, H, L + R), dtype=BF16)
+    q[:, :, L + 3] = 0
+    q[1, H - 1, L + 3] = -3e38 if finite else -math.inf
+    st, out, lse = attend(hip, c, q, [n, n], 2.0 ** -20)
+    assert st == k3x.ERR_INVALID_MXFP4
+    assert ctx.synchronize() == 0
+    # Without that row nothing is latched, and a token that sees nothing has zeros.
+    q[1, H - 1, L + 3] = 0
+    st, out, lse = attend(hip, c, q, [n, 0], 2.0 ** -20)
+    assert st == 0
+    assert (out[0] == 1).all() and (out[1] == 0).all() and (lse[1] == -math.inf).all()
+
+
+@pytest.mark.parametrize("Dn,R", [(128, 64), (128, 0), (64, 16)])
+@pytest.mark.parametrize("m,n", [(1, 1), (70, 300), (40, 3)])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+def test_prompt_scores_of_minus_infinity_are_latched(hip, Dn, R, m, n, causal):
+    k3x, ctx = hip
+    mla.say(f"prompt scores of minus infinity {Dn}+{R} {m} over {n}")
+    q = torch.ones((m, 2, Dn + R), dtype=BF16)
+    k, v = torch.ones((n, 2, Dn), dtype=BF16), torch.ones((n, 2, 64), dtype=BF16)
+    rotary = torch.ones((n, R), dtype=BF16) if R else None
+    st, out, lse = prompt(hip, q, k, v, rotary, 0.1, causal)
+    assert st == 0
+    none = max(0, m - n) if causal else 0  # queries that see nothing
+    assert (out[none:] == 1).all() and (out[:none] == 0).all()
+    assert (lse[:none] == -math.inf).all()
+    q[m - 1, 1, 5] = -math.inf
+    st, out, lse = prompt(hip, q, k, v, rotary, 0.1, causal)
+    assert st == k3x.ERR_INVALID_MXFP4
+    assert ctx.synchronize() == 0
