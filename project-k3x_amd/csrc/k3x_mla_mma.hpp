@@ -71,7 +71,22 @@ __device__ inline float across(float x, Op op) {
     return x;
 }
 
-// A row that sees tokens has a sum: its largest weight is 1.  None (or NaN) is that of scores
+// Weights are powers of two of the scores past a row's reference, which is its largest score so
+// far less kLift, and may lag behind it: by kLag in all, so that sums and outputs are seldom
+// multiplied again.  They are rounded to the call's type for the second product (the matrix
+// cores take 16 bits a value; sums are of the unrounded ones).  bf16 has fp32's exponents.
+// Of fp16 the range is spent above: with the largest at 2^0 weights below 2^-25 would vanish,
+// 0.3% of the output where 10^5 are of about that size; at 2^7 (2^15 at most of its 2^16) they
+// are rounded by 2^-32 of the largest.
+template <uint32_t DT>
+struct Weights {
+    static constexpr float kLift = DT == K3X_DTYPE_F16 ? 7.0f : 0.0f;
+    static constexpr float kLag = DT == K3X_DTYPE_F16 ? 15.0f : 8.0f;
+    static __device__ inline bool over(float top, float m) { return top > m + kLag; }
+    static __device__ inline float reference(float top, float m) { return fmaxf(m, top - kLift); }
+};
+
+// A row that sees tokens has a sum: its largest weight is 1 or more.  None (or NaN) is that of scores
 // that are all minus infinity, or no numbers.
 __device__ inline bool no_softmax(int32_t sees, float sum) { return sees > 0 && !(sum > 0.0f); }
 

@@ -60,7 +60,7 @@ struct AttentionArgs {
     uint32_t G, RB;  // ranges, row blocks of a group
     uint32_t one;    // no sequence has more than one group
     Split* splits;   // [N], or where there are more sequences or groups than ranges [G], by range
-    float2* sums;    // [G][RB][2][rows]: maximum (log2) and sum of a piece
+    float2* sums;    // [G][RB][2][rows]: reference (log2) and sum of a piece
     float4* parts;   // [G][RB][2][rows * LP / 4]: its outputs, as the lanes hold them
     uint32_t* status;
 };
@@ -487,11 +487,9 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
 #pragma unroll
                 for (int i = 1; i < NV; ++i) top = fmaxf(top, x[i]);
                 top = across<HT>(top, [](float p, float r) { return fmaxf(p, r); }) * a.rate;
-                // The maximum that weights are taken from may lag by 2^8: sums and
-                // outputs keep their bits, and are seldom multiplied again.
                 constexpr bool HELD = RT * OT * sizeof(Acc) >= 512;
                 float now = RT > 1 && srow ? m[RT - 1] : m[0];
-                const bool over = __any(top > now + 8.0f);
+                const bool over = __any(Weights<DT>::over(top, now));
                 uint32_t p[NV / 2];
                 float sum;
                 auto weights = [&] {
@@ -538,8 +536,8 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
 #pragma unroll
                         for (int i = 0; i < RT; ++i) {
                             const float* tops = reinterpret_cast<const float*>(smem + kTops);
-                            const float up = fmaxf(m[i], fmaxf(tops[i * 64 + col],
-                                                               tops[i * 64 + 32 + col]));
+                            const float up = Weights<DT>::reference(
+                                fmaxf(tops[i * 64 + col], tops[i * 64 + 32 + col]), m[i]);
                             const float keep = __builtin_amdgcn_exp2f(m[i] - up);
                             m[i] = up;
                             if ((uint32_t)i == srow) l *= keep;
@@ -556,7 +554,8 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     l += sum;
                 } else {
                     if (over) {
-                        const float up = fmaxf(m[0], top), keep = __builtin_amdgcn_exp2f(m[0] - up);
+                        const float up = Weights<DT>::reference(top, m[0]);
+                        const float keep = __builtin_amdgcn_exp2f(m[0] - up);
                         m[0] = now = up;
                         l *= keep;
                         if (t != t0) scale_tiles<HELD, 0, OT>(o, keep);

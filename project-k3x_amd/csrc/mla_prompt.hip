@@ -315,9 +315,9 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
 #pragma unroll
             for (int y = 0; y < 16; ++y) top = fmaxf(top, sc[x][y]);
         top = across<32>(top, [](float u, float v) { return fmaxf(u, v); }) * a.rate;
-        // The maximum may lag by 2^8: see mla_attention.hip.
-        if (__any(top > m + 8.0f)) {
-            const float up = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - up);
+        if (__any(Weights<DT>::over(top, m))) {
+            const float up = Weights<DT>::reference(top, m);
+            const float keep = __builtin_amdgcn_exp2f(m - up);
             m = up;
             l *= keep;
             scale_tiles<false, 0, OT>(o, keep);

@@ -148,3 +148,53 @@ def test_prompt_scores_of_minus_infinity_are_latched(hip, Dn, R, m, n, causal):
     st, out, lse = prompt(hip, q, k, v, rotary, 0.1, causal)
     assert st == k3x.ERR_INVALID_MXFP4
     assert ctx.synchronize() == 0
+
+
+# What many equal weights beside a large one are off by, all values 1.  A weight is rounded by
+# half a step of fp16, 2^-11 of it or (below 2^-14) 2^-25; the row's largest is 2^7 at least, so
+# that n weights miss n 2^-32 of the sum.  The sums of weights and of outputs are `adds` fp32
+# additions in a row (the matrix cores may cut where they do not round: 2^-23 each), the
+# exponentials 2^-20, and the output is rounded by 2^-11.
+def small_weights_tolerance(n, adds):
+    return 2 * 2.0 ** -11 + n * 2.0 ** -32 + adds * 2.0 ** -23 + 2.0 ** -20
+
+
+@pytest.mark.parametrize("N,H,L,R", [(512, 1, 512, 64), (256, 24, 512, 64), (256, 48, 512, 64),
+                                     (256, 96, 512, 64), (512, 1, 96, 16), (256, 48, 96, 16)])
+def test_small_weights_in_fp16(hip, N, H, L, R):
+    """Weights just below 2^-25 of the largest one: alone they are nothing, together 0.3%.  So many
+    sequences (of the same pages) that each lies in one range or two."""
+    n = 100001
+    mla.say(f"small weights N={N} H={H} L={L}")
+    rotary = torch.zeros((n, R))
+    rotary[0, 0] = 1
+    c = plain_cache([n] * N, L, R, 64, torch.ones((n, L)), rotary, F16)
+    q = torch.zeros((N, H, L + R), dtype=F16)
+    q[:, :, L] = 1
+    scale = 25.05 * math.log(2)
+    st, out, lse = attend(hip, c, q, [n] * N, scale)
+    assert st == 0
+    rest = (n - 1) * 2.0 ** -25.05
+    # 16 tokens a product at least: 6251 additions to an output, fewer to a sum.
+    assert rest > small_weights_tolerance(n, 6400)
+    assert float((out - 1).abs().max()) <= small_weights_tolerance(n, 6400)
+    assert float((lse - scale - math.log1p(rest)).abs().max()) <= 2.0 ** -9
+
+
+@pytest.mark.parametrize("Dn,R", [(128, 64), (64, 16)])
+def test_small_weights_in_fp16_prompts(hip, Dn, R):
+    n, m = 80000, 3
+    mla.say(f"small weights of a prompt {Dn}+{R}")
+    rotary = torch.zeros((n, R), dtype=F16)
+    rotary[0, 0] = 1
+    q = torch.zeros((m, 1, Dn + R), dtype=F16)
+    q[:, :, Dn] = 1
+    k, v = torch.zeros((n, 1, Dn), dtype=F16), torch.ones((n, 1, 64), dtype=F16)
+    scale = 25.05 * math.log(2)
+    st, out, lse = prompt(hip, q, k, v, rotary, scale)
+    assert st == 0
+    rest = (n - m) * 2.0 ** -25.05
+    # 16 keys a product: 5000 additions to an output, fewer to a sum.
+    assert rest > small_weights_tolerance(n, 5100)
+    assert float((out - 1).abs().max()) <= small_weights_tolerance(n, 5100)
+    assert float((lse - scale - math.log1p(rest)).abs().max()) <= 2.0 ** -9
