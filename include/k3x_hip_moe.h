@@ -684,9 +684,9 @@ int k3x_hip_mla_load(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const v
  * q, out and pool 16-byte aligned, strides of q and out multiples of 8 elements.
  * workspace as k3x_hip_delta_rule's, k3x_hip_mla_attention_workspace(params)
  * bytes.  Also latched, as K3X_ERR_INVALID_MXFP4: an output that is not finite
- * (for a query or a cached row that is not), and scores of a token that are all minus
- * infinity, past fp32 or for such a query.  Replaces the attention of
- * reference/k3x_ref/mla.py, batched.  Asynchronous. */
+ * (for a query or a cached row that is not, or sums of weighted latents past fp32),
+ * and scores of a token that are all minus infinity, past fp32 or for such a query.
+ * Replaces the attention of reference/k3x_ref/mla.py, batched.  Asynchronous. */
 int k3x_hip_mla_attention(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const void* q,
                           const void* pool, const uint32_t* table, const uint32_t* offsets,
                           const uint32_t* lens, void* out, float* lse, void* workspace,

@@ -56,6 +56,17 @@ __device__ inline uint32_t pack2(float a, float b) {
         return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
 }
 
+// Four outputs as the type's bits.  An output lies between the values that it is a mean of, but
+// rounded weights and their unrounded sum may put it past them by 2^-11 of itself: not past
+// fp16's largest number.  (Values of bf16 so large have sums past fp32 first.)
+template <uint32_t DT>
+__device__ inline uint2 outputs4(float4 v) {
+    auto within = [](float x) {
+        return DT == K3X_DTYPE_F16 ? __builtin_amdgcn_fmed3f(x, -65504.0f, 65504.0f) : x;
+    };
+    return uint2{pack2<DT>(within(v.x), within(v.y)), pack2<DT>(within(v.z), within(v.w))};
+}
+
 // Over the lanes that hold one row's scores: the halves, and for 16 rows the
 // 16-lane rows too.
 template <int HT, typename Op>

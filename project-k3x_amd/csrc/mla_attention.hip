@@ -675,8 +675,7 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     each([&](int f, uint32_t, float4 v) { part[f * 64] = v; });
                 else if (live)
                     each([&](int, uint32_t d, float4 v) {
-                        *reinterpret_cast<uint2*>(out + d) =
-                            uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+                        *reinterpret_cast<uint2*>(out + d) = outputs4<DT>(v);
                     });
                 bad_value |= live && !(check == 0.0f);
                 if (whole)
@@ -782,11 +781,14 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
     }
     if (!live) return;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    if (no_softmax(s.before + (int32_t)(r / a.H) + 1, l)) latch(a.status, K3X_ERR_INVALID_MXFP4);
     const uint64_t t = s.begin + r / a.H;
     uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.os + (uint64_t)(r % a.H) * a.L + d;
-    *reinterpret_cast<uint2*>(out) = uint2{pack2<DT>(o.x * inv, o.y * inv),
-                                           pack2<DT>(o.z * inv, o.w * inv)};
+    o = float4{o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    // Pieces that are numbers may have a sum that is none.
+    const float check = o.x * 0.0f + o.y * 0.0f + o.z * 0.0f + o.w * 0.0f;
+    if (!(check == 0.0f) || no_softmax(s.before + (int32_t)(r / a.H) + 1, l))
+        latch(a.status, K3X_ERR_INVALID_MXFP4);
+    *reinterpret_cast<uint2*>(out) = outputs4<DT>(o);
     if (a.lse && d == 0)
         a.lse[t * a.H + r % a.H] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
                                             : -__builtin_inff();

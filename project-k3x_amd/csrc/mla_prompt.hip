@@ -378,9 +378,7 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
                 check = __builtin_fmaf(v.y, 0.0f, check);
                 check = __builtin_fmaf(v.z, 0.0f, check);
                 check = __builtin_fmaf(v.w, 0.0f, check);
-                if (live)
-                    *reinterpret_cast<uint2*>(out + d) =
-                        uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+                if (live) *reinterpret_cast<uint2*>(out + d) = outputs4<DT>(v);
             }
         }
     if (live && (!(check == 0.0f) || no_softmax(sees, l))) latch(a.status, K3X_ERR_INVALID_MXFP4);

@@ -198,3 +198,46 @@ def test_small_weights_in_fp16_prompts(hip, Dn, R):
     assert rest > small_weights_tolerance(n, 5100)
     assert float((out - 1).abs().max()) <= small_weights_tolerance(n, 5100)
     assert float((lse - scale - math.log1p(rest)).abs().max()) <= 2.0 ** -9
+
+
+@pytest.mark.parametrize("H,L,R", [(1, 512, 64), (24, 512, 64), (48, 512, 64), (96, 512, 64),
+                                   (1, 96, 16), (48, 96, 16)])
+@pytest.mark.parametrize("n", [40, 2001])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_largest_values_of_fp16(hip, H, L, R, n, sign):
+    """Outputs are between the values, also where all weights but the largest round up and their
+    sum does not: 65504 times that passes what fp16 holds."""
+    mla.say(f"largest values H={H} L={L} n={n}")
+    rotary = torch.full((n, R), -1.0)
+    rotary[0] = 0
+    c = plain_cache([n], L, R, 16, torch.full((n, L), sign * 65504.0), rotary, F16)
+    q = torch.zeros((1, H, L + R), dtype=F16)
+    q[:, :, L] = 1
+    st, out, _ = attend(hip, c, q, [n], -math.log((1 + 2.0 ** -11 + 2.0 ** -13) / 2))
+    assert st == 0 and (out == sign * 65504).all()
+
+
+@pytest.mark.parametrize("Dn,R", [(128, 64), (64, 16)])
+def test_largest_values_of_fp16_in_prompts(hip, Dn, R):
+    n = 200
+    rotary = torch.full((n, R), -1.0, dtype=F16)
+    rotary[0] = 0
+    q = torch.zeros((n, 1, Dn + R), dtype=F16)
+    q[:, :, Dn] = 1
+    k, v = torch.zeros((n, 1, Dn), dtype=F16), torch.full((n, 1, 64), 65504.0, dtype=F16)
+    mla.say(f"largest values of a prompt {Dn}+{R}")
+    st, out, _ = prompt(hip, q, k, v, rotary, -math.log((1 + 2.0 ** -11 + 2.0 ** -13) / 2))
+    assert st == 0 and (out == 65504).all()
+
+
+@pytest.mark.parametrize("H", [1, 24, 48, 96])
+def test_sums_past_fp32_are_latched(hip, H):
+    """Pieces of a sequence that are numbers each, and whose sum is not."""
+    k3x, ctx = hip
+    n = 60000
+    mla.say(f"sums past fp32 H={H}")
+    c = plain_cache([n], 512, 64, 64, torch.full((n, 512), 1e35), torch.zeros((n, 64)))
+    q = torch.zeros((1, H, 576), dtype=BF16)
+    st, out, _ = attend(hip, c, q, [n])
+    assert st == k3x.ERR_INVALID_MXFP4
+    assert ctx.synchronize() == 0
