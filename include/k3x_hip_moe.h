@@ -685,7 +685,8 @@ int k3x_hip_mla_load(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const v
  * workspace as k3x_hip_delta_rule's, k3x_hip_mla_attention_workspace(params)
  * bytes.  Also latched, as K3X_ERR_INVALID_MXFP4: an output that is not finite
  * (for a query or a cached row that is not, or sums of weighted latents past fp32),
- * and scores of a token that are all minus infinity, past fp32 or for such a query.
+ * and scores of a token that are all minus infinity, past fp32 or for such a query;
+ * with fp16 also scores (times scale) of 2^24 and more, which may be past its weights.
  * Replaces the attention of reference/k3x_ref/mla.py, batched.  Asynchronous. */
 int k3x_hip_mla_attention(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const void* q,
                           const void* pool, const uint32_t* table, const uint32_t* offsets,
@@ -724,8 +725,8 @@ typedef struct k3x_hip_mla_prompt_params {
  * k3x_hip_mla_attention.  q, k, v, rotary and out 16-byte aligned, those without rows
  * may be NULL.
  * Latched: offsets that fall, pass T or S (K3X_ERR_INVALID_STATE; nothing of such
- * a sequence is read), an output that is not finite or scores that are all minus
- * infinity (K3X_ERR_INVALID_MXFP4).
+ * a sequence is read), and as for k3x_hip_mla_attention outputs that are not finite
+ * and scores (K3X_ERR_INVALID_MXFP4).
  * Asynchronous. */
 int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* params, const void* q,
                        const void* k, const void* v, const void* rotary, const uint32_t* offsets,

@@ -98,8 +98,13 @@ struct Weights {
 };
 
 // A row that sees tokens has a sum: its largest weight is 1 or more.  None (or NaN) is that of scores
-// that are all minus infinity, or no numbers.
-__device__ inline bool no_softmax(int32_t sees, float sum) { return sees > 0 && !(sum > 0.0f); }
+// that are all minus infinity, or no numbers.  And of scores of 2^28 and more a weight's power
+// of two is off by the rounding of its reference m, more than 2^4 either way: in fp16 even the
+// largest weight may vanish while the sum, in fp32, is there.
+template <uint32_t DT>
+__device__ inline bool no_softmax(int32_t sees, float sum, float m) {
+    return sees > 0 && (!(sum > 0.0f) || (DT == K3X_DTYPE_F16 && fabsf(m) > 0x1p28f));
+}
 
 // x, as a value that is not computed ahead of the place and held until then.
 __device__ inline uint32_t opaque(uint32_t x) {

@@ -679,8 +679,8 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
                     });
                 bad_value |= live && !(check == 0.0f);
                 if (whole)
-                    bad_value |= live && no_softmax((int32_t)s.len - (int32_t)s.count +
-                                                        (int32_t)(re / a.H) + 1, l1);
+                    bad_value |= live && no_softmax<DT>((int32_t)s.len - (int32_t)s.count +
+                                                            (int32_t)(re / a.H) + 1, l1, m1);
                 if (g == 0 && wd == 0) {
                     if (!whole)
                         a.sums[piece * S::rows + at + col] = float2{m1, l1};
@@ -786,7 +786,7 @@ __global__ __launch_bounds__(kThreads) void mla_join_kernel(AttentionArgs a) {
     o = float4{o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     // Pieces that are numbers may have a sum that is none.
     const float check = o.x * 0.0f + o.y * 0.0f + o.z * 0.0f + o.w * 0.0f;
-    if (!(check == 0.0f) || no_softmax(s.before + (int32_t)(r / a.H) + 1, l))
+    if (!(check == 0.0f) || no_softmax<DT>(s.before + (int32_t)(r / a.H) + 1, l, m))
         latch(a.status, K3X_ERR_INVALID_MXFP4);
     *reinterpret_cast<uint2*>(out) = outputs4<DT>(o);
     if (a.lse && d == 0)

@@ -381,7 +381,7 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
                 if (live) *reinterpret_cast<uint2*>(out + d) = outputs4<DT>(v);
             }
         }
-    if (live && (!(check == 0.0f) || no_softmax(sees, l))) latch(a.status, K3X_ERR_INVALID_MXFP4);
+    if (live && (!(check == 0.0f) || no_softmax<DT>(sees, l, m))) latch(a.status, K3X_ERR_INVALID_MXFP4);
     if (a.lse && live && g == 0)
         a.lse[row * a.H + h] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
                                         : -__builtin_inff();

@@ -241,3 +241,39 @@ def test_sums_past_fp32_are_latched(hip, H):
     st, out, _ = attend(hip, c, q, [n])
     assert st == k3x.ERR_INVALID_MXFP4
     assert ctx.synchronize() == 0
+
+
+# Scores of 3.6e9 times this: their rounded product with log2(e) is 82 off, so that in fp32 the
+# largest weight is 2^-82, and its sum a number; in fp16 it is nothing.
+FAR = 1.01
+
+
+@pytest.mark.parametrize("H,L,R", [(1, 512, 64), (24, 512, 64), (48, 512, 64), (96, 512, 64),
+                                   (1, 96, 16), (48, 96, 16)])
+@pytest.mark.parametrize("n", [1, 2001])
+def test_scores_past_fp16_weights_are_latched(hip, H, L, R, n):
+    k3x, ctx = hip
+    mla.say(f"scores of 3.6e9 H={H} L={L} n={n}")
+    for dtype, want in ((F16, k3x.ERR_INVALID_MXFP4), (BF16, 0)):
+        # 60000 in fp16, in bf16 59904.
+        c = plain_cache([n], L, R, 16, torch.ones((n, L)), torch.full((n, R), 60000.0), dtype)
+        q = torch.zeros((1, H, L + R), dtype=dtype)
+        q[:, :, L] = 60000
+        st, out, _ = attend(hip, c, q, [n], FAR)
+        assert st == want
+        assert ctx.synchronize() == 0
+        if not want:
+            assert (out == 1).all()
+
+
+@pytest.mark.parametrize("Dn,R", [(128, 64), (64, 16)])
+def test_prompt_scores_past_fp16_weights_are_latched(hip, Dn, R):
+    k3x, ctx = hip
+    mla.say(f"prompt scores of 3.6e9 {Dn}+{R}")
+    rotary = torch.full((40, R), 60000.0, dtype=F16)
+    q = torch.zeros((5, 1, Dn + R), dtype=F16)
+    q[:, :, Dn] = 60000
+    k, v = torch.zeros((40, 1, Dn), dtype=F16), torch.ones((40, 1, 64), dtype=F16)
+    st, _, _ = prompt(hip, q, k, v, rotary, FAR)
+    assert st == k3x.ERR_INVALID_MXFP4
+    assert ctx.synchronize() == 0
