@@ -571,7 +571,8 @@ typedef struct k3x_hip_logits_params {
  *   l - frequency c, then l - presence        where c > 0
  *   l + its bias
  *   minus infinity                            where the row's mask bit is 0
- * and is rounded to its type once.  out (device [N][D + 1][V]) may be logits.
+ * and is rounded to its type once.  out (device [N][D + 1][V]) is logits or apart
+ * from it.
  * history: device u32 [N][history_width], of which sequence n has
  * history_lens[n] tokens and of those prompt_lens[n] (NULL: 0) in its prompt;
  * drafts as k3x_hip_verify_draft's tokens, u32 [N][D], and draft_counts: rows of
@@ -588,7 +589,9 @@ typedef struct k3x_hip_logits_params {
  * than its history, a token of the history, a draft or a bias past V, bias offsets
  * that fall or pass `biases`, a mask past `masks`, a draft count past D, a
  * repetition that is not a number above 0, a frequency or presence that is not
- * finite; rows of that sequence may then be missing or hold some of the steps.
+ * finite; rows of that sequence may then be missing or hold some of the steps.  With
+ * out = logits all rows of the other sequences are adjusted (such a call cannot be
+ * repeated); of any other call they may be missing.
  * Logits and biases may hold anything and go through the arithmetic as they are.
  * Asynchronous. */
 int k3x_hip_adjust_logits(k3x_hip_ctx* ctx, const k3x_hip_logits_params* params,

@@ -9,6 +9,18 @@ namespace k3x_ops {
 
 __device__ inline void latch(uint32_t* status, uint32_t code) { atomicCAS(status, 0u, code); }
 
+// A call of several sequences in place is not to stop half way at an error of one
+// of them: the others' workgroups that start later would leave their part behind,
+// and the call could not be repeated.  So its errors are latched apart, in the
+// word behind the status, where its workgroups do not look, and become the
+// context's here, behind them.
+static __global__ void report_kernel(uint32_t* errors, uint32_t* status) {
+    const uint32_t code = *errors;
+    if (!code) return;
+    *errors = 0;
+    latch(status, code);
+}
+
 // One element type of a caller's tensor: its storage, and fp32 in and out
 // (out rounds to nearest even).
 template <uint32_t DT>

@@ -38,7 +38,8 @@ struct LogitsArgs {
     const float* bias_values;
     const uint32_t *masks, *mask_index;
     uint32_t N, D, V, stride, out_stride, width, biases, mask_rows, mask_stride;
-    uint32_t* status;
+    const uint32_t* status;  // set: nothing is done
+    uint32_t* errors;        // the call's own: status, or apart from it (report_kernel)
 };
 
 // KE tokens a thread, by 16 bytes.  A row's loads are on their way while the one
@@ -56,7 +57,7 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
     __shared__ uint32_t count[kPart], entry[kPart], stop;
     const uint32_t n = blockIdx.y, lo = blockIdx.x * kPart;
     const uint32_t tid = threadIdx.x, hi = min(a.V, lo + kPart);
-    if (tid == 0) stop = *(volatile uint32_t*)a.status;
+    if (tid == 0) stop = *(volatile const uint32_t*)a.status;
     const uint32_t drafts = a.draft_counts ? a.draft_counts[n] : a.D;
     const uint32_t length = a.history ? a.history_lens[n] : 0;
     const uint32_t prompt = a.history && a.prompt_lens ? a.prompt_lens[n] : 0;
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
     if (drafts > a.D || length > a.width || prompt > length || b1 < b0 || b1 > a.biases ||
         !(rep > 0.0f && rep < __builtin_inff()) || !(fabsf(freq) < __builtin_inff()) ||
         !(fabsf(pres) < __builtin_inff())) {
-        if (tid == 0) latch(a.status, K3X_ERR_INVALID_STATE);
+        if (tid == 0) latch(a.errors, K3X_ERR_INVALID_STATE);
         return;
     }
     bool bad = false;
@@ -194,14 +195,16 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
                 for (int y = 0; y < W; ++y) c[v * W + y] += t == first(v) + y;
         }
     }
-    if (bad) latch(a.status, K3X_ERR_INVALID_STATE);
+    if (bad) latch(a.errors, K3X_ERR_INVALID_STATE);
 }
 
 template <uint32_t DT>
 int launch_logits(k3x_hip_ctx* ctx, const LogitsArgs& a) {
     hipLaunchKernelGGL((adjust_logits_kernel<DT>), dim3((a.V + kPart - 1) / kPart, a.N), dim3(kThreads),
                        0, ctx->stream, a);
-    return launched(ctx, 1);
+    if (a.errors == a.status) return launched(ctx, 1);
+    hipLaunchKernelGGL(report_kernel, dim3(1), dim3(1), 0, ctx->stream, a.errors, ctx->status);
+    return launched(ctx, 2);
 }
 
 bool logits_ok(const k3x_hip_logits_params* p) {
@@ -265,6 +268,7 @@ int k3x_hip_adjust_logits(k3x_hip_ctx* ctx, const k3x_hip_logits_params* p, cons
     a.mask_rows = p->masks;
     a.mask_stride = p->mask_stride ? p->mask_stride : (p->vocab + 31) / 32;
     a.status = ctx->status;
+    a.errors = out == logits && a.N > 1 ? ctx->status + 1 : ctx->status;
     return p->dtype == K3X_DTYPE_F32 ? launch_logits<K3X_DTYPE_F32>(ctx, a)
                                      : launch_logits<K3X_DTYPE_BF16>(ctx, a);
 }
