@@ -705,6 +705,11 @@ __global__ __launch_bounds__(kThreads, S::rows == 16 ? 2 : 1) void mla_attention
     if (bad_value) latch(a.status, K3X_ERR_INVALID_MXFP4);
 }
 
+// A call of no tokens: its offsets and lengths are looked at all the same.
+__global__ __launch_bounds__(kThreads) void mla_check_kernel(Pages pages, uint32_t* status) {
+    check_sequences(pages, status);
+}
+
 // Joins the pieces of a sequence that lies in several ranges, 64 float4 as a
 // wave of the first launch held them: a wave each, or (FOUR, for many pieces) four
 // waves, each every fourth piece.
@@ -921,7 +926,11 @@ int k3x_hip_mla_attention(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const v
     w += up256(pieces * x.rows * sizeof(float2));
     a.parts = reinterpret_cast<float4*>(w);
     a.status = ctx->status;
-    if (!p->tokens) return K3X_OK;
+    if (!p->tokens) {
+        hipLaunchKernelGGL(mla_check_kernel, dim3(1), dim3(kThreads), 0, ctx->stream, a.pages,
+                           a.status);
+        return launched(ctx, 1);
+    }
     if (p->dtype == K3X_DTYPE_F16) return launch_width<K3X_DTYPE_F16, K3X_CACHE_16BIT>(ctx, a, x);
     switch (p->cache_format) {
         case K3X_CACHE_16BIT: return launch_width<K3X_DTYPE_BF16, K3X_CACHE_16BIT>(ctx, a, x);

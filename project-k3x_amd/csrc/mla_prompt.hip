@@ -387,6 +387,16 @@ __global__ __launch_bounds__(kThreads, 2) void mla_prompt_kernel(PromptArgs a) {
                                         : -__builtin_inff();
 }
 
+// A call of no queries: its offsets are looked at all the same.
+__global__ __launch_bounds__(kThreads) void prompt_check_kernel(PromptArgs a) {
+    bool bad = false;
+    for (uint32_t n = threadIdx.x; n < a.N; n += kThreads) {
+        Ranges r;
+        bad |= !ranges_of(a, n, &r);
+    }
+    if (bad) latch(a.status, K3X_ERR_INVALID_STATE);
+}
+
 bool prompt_ok(const k3x_hip_mla_prompt_params* p) {
     const uint64_t most = 1ull << 32, H = p->heads, kh = p->k_head_stride, vh = p->v_head_stride;
     auto fits = [&](uint64_t stride, uint64_t least) {
@@ -463,7 +473,10 @@ int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* p, con
         a.ks > (1u << 27) || a.vs > (1u << 27) || a.rs > (1u << 27))
         return K3X_ERR_INVALID_EXTENT;
     if (hipSetDevice(ctx->device) != hipSuccess) return K3X_ERR_BACKEND_UNAVAILABLE;
-    if (!a.T) return K3X_OK;
+    if (!a.T) {
+        hipLaunchKernelGGL(prompt_check_kernel, dim3(1), dim3(kThreads), 0, ctx->stream, a);
+        return launched(ctx, 1);
+    }
     return p->dtype == K3X_DTYPE_F16 ? launch<K3X_DTYPE_F16>(ctx, a)
                                      : launch<K3X_DTYPE_BF16>(ctx, a);
 }

@@ -277,3 +277,35 @@ def test_prompt_scores_past_fp16_weights_are_latched(hip, Dn, R):
     st, _, _ = prompt(hip, q, k, v, rotary, FAR)
     assert st == k3x.ERR_INVALID_MXFP4
     assert ctx.synchronize() == 0
+
+
+@pytest.mark.parametrize("what", ["offsets", "length", "keys"])
+def test_calls_of_no_tokens_are_checked(hip, what):
+    """Offsets and lengths are looked at in calls of no tokens too, by every call."""
+    k3x, ctx = hip
+    c = mla.to_device(ref.make_cache([4, 9], 64, 16, 16))
+    p = mla.params(k3x, c, 0, 4)
+    lens = mla.ints([4, 17 if what == "length" else 9])
+    offsets = mla.ints([0, 1, 1] if what == "offsets" else [0, 0, 0])
+    q, out = (torch.empty((0, 4, d), dtype=BF16, device=DEV) for d in (80, 64))
+    latent = torch.empty((0, 64), dtype=BF16, device=DEV)
+    ws = torch.empty((k3x.mla_attention_workspace_bytes(p),), dtype=torch.uint8, device=DEV)
+    k = torch.zeros((6, 4, 64), dtype=BF16, device=DEV)
+    pp = k3x.make_mla_prompt_params(q[..., :64].contiguous(), k, k, 2)
+    calls = [lambda: k3x.mla_prompt(ctx, pp, q[..., :64].contiguous(), k, k, out, offsets=offsets,
+                                    key_offsets=mla.ints([0, 7, 7] if what == "keys" else
+                                                         [0, 3, 6]))]
+    if what != "keys":
+        calls += [lambda: k3x.mla_attention(ctx, p, q, c["pool"], c["table"], lens, out,
+                                            offsets=offsets, workspace=ws),
+                  lambda: k3x.mla_store(ctx, p, latent, c["pool"], c["table"], lens,
+                                        rotary=latent[:, :16], offsets=offsets),
+                  lambda: k3x.mla_load(ctx, p, c["pool"], c["table"], lens, latent,
+                                       offsets=offsets)]
+    if what == "length":
+        calls = calls[1:]
+    for i, call in enumerate(calls):
+        mla.say(f"no tokens, unfit {what}, call {i}")
+        assert call() == 0
+        assert ctx.synchronize() == k3x.ERR_INVALID_STATE
+        assert ctx.synchronize() == 0
