@@ -710,9 +710,9 @@ typedef struct k3x_hip_mla_prompt_params {
     uint32_t longest;   /* queries of the longest sequence if known, 0: not (then T).  Only
                            how the work is laid out: results hold whatever it says. */
     float scale;        /* of the scores, > 0 */
-    /* Elements from row to row (of k, v and rotary 2^27 at most), and of k and v from
-     * head to head (k and v may be parts of one projection's rows); multiples of 8;
-     * 0: packed. */
+    /* Elements from row to row (of k, v and rotary 2^27 at most; with one key not
+     * used), and of k and v from head to head (k and v may be parts of one
+     * projection's rows); multiples of 8; 0: packed. */
     uint64_t q_stride, k_stride, v_stride, rotary_stride, out_stride;
     uint64_t k_head_stride, v_head_stride;
 } k3x_hip_mla_prompt_params;

@@ -461,6 +461,7 @@ int k3x_hip_mla_prompt(k3x_hip_ctx* ctx, const k3x_hip_mla_prompt_params* p, con
     a.ks = p->k_stride ? p->k_stride : a.H * a.kh;
     a.vs = p->v_stride ? p->v_stride : a.H * a.vh;
     a.rs = p->rotary_stride ? p->rotary_stride : a.R;
+    if (a.S <= 1) a.ks = a.vs = a.rs = 0;  // no row lies behind another
     a.os = p->out_stride ? p->out_stride : (uint64_t)a.H * a.Dv;
     a.rate = p->scale * 1.4426950408889634f;
     a.status = ctx->status;

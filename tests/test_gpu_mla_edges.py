@@ -309,3 +309,21 @@ def test_calls_of_no_tokens_are_checked(hip, what):
         assert call() == 0
         assert ctx.synchronize() == k3x.ERR_INVALID_STATE
         assert ctx.synchronize() == 0
+
+
+@pytest.mark.parametrize("m", [1, 5])
+def test_prompt_over_one_key_of_a_cache(hip, m):
+    """One key of a cache whose heads lie far apart: rows of it have no distance."""
+    k3x, ctx = hip
+    H, D, most = 9, 64, (1 << 18) + 8
+    g = ref.gen(m)
+    store = torch.zeros((H, most, D), dtype=BF16, device=DEV)
+    kv = torch.randn((1, H, D), generator=g).to(BF16)
+    store[:, 0] = kv[0].to(DEV)
+    k = store[:, :1].transpose(0, 1)
+    q = torch.randn((m, H, D), generator=g).to(BF16)
+    mla.say(f"prompt of {m} over one key")
+    st, out, lse = prompt(hip, q, k, k, None, 0.125)
+    assert st == 0
+    want, wl, tol, ltol = ref.prompt(q, kv, kv, None, [m], [1], True, 0.125)
+    assert ref.close(out, want, tol) <= 1 and ref.close(lse, wl, ltol) <= 1
