@@ -327,3 +327,44 @@ def test_prompt_over_one_key_of_a_cache(hip, m):
     assert st == 0
     want, wl, tol, ltol = ref.prompt(q, kv, kv, None, [m], [1], True, 0.125)
     assert ref.close(out, want, tol) <= 1 and ref.close(lse, wl, ltol) <= 1
+
+
+@pytest.mark.parametrize("fmt", ["16bit", "mxfp8", "mxfp4"])
+@pytest.mark.parametrize("H,N,L,R", [
+    (5, 1, 512, 64), (12, 1, 512, 64), (29, 1, 512, 64), (128, 64, 512, 64),
+    (5, 1, 256, 0), (12, 1, 256, 0), (29, 1, 256, 0), (128, 64, 256, 0),
+    (5, 1, 480, 56), (12, 1, 480, 56), (29, 1, 288, 8)])
+def test_largest_scores_that_rise_within_a_range(hip, fmt, H, N, L, R):
+    """16, 32, 64 and 128 rows a block: a sequence of 40000 positions, several tiles a range, whose
+    1024 different rows come again and again, with scores that rise or fall by hundreds over
+    them, each row's with a slope and a sign of its own."""
+    k3x, ctx = hip
+    m, n = 1024, 40000
+    two = N == 1  # a window of two tokens, else single ones beside the long sequence
+    mla.say(f"rising scores H={H} N={N} {L}+{R} {fmt}")
+    lens = [m] + [1 + 5 * i % 33 for i in range(1, N)]
+    c = ref.make_cache(lens, L, R, 16, fmt, seed=H)
+    g = ref.gen(H + L)
+    latent = torch.randn((m, L), generator=g)
+    pos = torch.arange(m)
+    latent[:, 0] = torch.linspace(-30, 30, m)
+    latent[:, 1] = -torch.linspace(-20, 20, m).abs()
+    latent[:, 2] = torch.where(pos // 32 % 2 == 1, 16.0, -16.0)
+    rotary = torch.randn((m, R), generator=g).to(BF16)
+    data, values = ref.encode(latent.to(BF16), rotary, fmt)
+    c["pool"][c["table"][0][pos // 16].long(), pos % 16] = data
+    again = torch.arange(n) % m
+    c["rows"][0] = (values[again], rotary.double()[again])
+    table = torch.full((N, n // 16), -1, dtype=torch.int32)
+    table[:, :m // 16] = c["table"]
+    table[0] = c["table"][0].repeat(-(-n // m))[:n // 16]
+    c["table"], c["lens"] = table, [n] + lens[1:]
+    counts = [2] if two else [1] * N
+    q = torch.randn((sum(counts), H, L + R), generator=g) * 0.1
+    q[..., :3] = torch.randn((sum(counts), H, 3), generator=g) * 8
+    q = q.to(BF16)
+    st, out, lse = attend(hip, mla.to_device(c), q, c["lens"], 1.0, counts[0],
+                          mla.offsets_of(counts))
+    assert st == 0
+    want, wl, tol, ltol = ref.attention(c, q, counts, 1.0)
+    assert ref.close(out, want, tol) <= 1 and ref.close(lse, wl, ltol) <= 1
