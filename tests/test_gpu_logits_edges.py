@@ -98,3 +98,20 @@ def test_captured_calls_beside_an_unfit_sequence(hip):
         left = [n for n in range(N) if n != 5 or not i % 2]
         assert torch.equal(y[left], want[left])
     ctx.close()
+
+
+@pytest.mark.parametrize("in_place", [False, True], ids=["out", "in_place"])
+def test_rows_past_32_bit_offsets(hip, in_place):
+    """Rows 2^31 elements apart."""
+    k3x, ctx = hip
+    s = base.make(2, 1, 5001, torch.bfloat16)
+    wide = torch.empty((4, (1 << 31) + 8), dtype=torch.bfloat16, device=DEV)
+    x = wide[:, :5001].unflatten(0, (2, 2))
+    x.copy_(s["logits"].to(DEV))
+    out = x if in_place else wide[:, 8192:8192 + 5001].unflatten(0, (2, 2))
+    d = {k: tuple(t.to(DEV) for t in v) if isinstance(v, tuple) else v.to(DEV)
+         for k, v in s.items() if k != "logits"}
+    print("[gpu-test] logits 2^31 elements apart", flush=True)
+    assert k3x.adjust_logits(ctx, k3x.make_logits_params(x), x, out, **d) == 0
+    assert ctx.synchronize() == 0
+    assert torch.equal(out.double().cpu(), base.definition(s))

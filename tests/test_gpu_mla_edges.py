@@ -368,3 +368,53 @@ def test_largest_scores_that_rise_within_a_range(hip, fmt, H, N, L, R):
     assert st == 0
     want, wl, tol, ltol = ref.attention(c, q, counts, 1.0)
     assert ref.close(out, want, tol) <= 1 and ref.close(lse, wl, ltol) <= 1
+
+
+def test_store_past_32_bit_offsets(hip):
+    """Rows 2^31 elements apart, to pages on both sides of 4 GiB."""
+    k3x, ctx = hip
+    L, R, page = 512, 64, 64
+    pages = (5 << 30) // (page * 1152)
+    pool = torch.zeros((pages, page, 1152), dtype=torch.uint8, device=DEV)
+    table = mla.ints([[3, pages - 1], [pages - 2, 0]])
+    wide = torch.empty((3, (1 << 31) + 64), dtype=BF16, device=DEV)
+    rows = torch.randn((3, L + R), generator=ref.gen(2)).to(BF16)
+    wide[:, :L + R] = rows.to(DEV)
+    c = dict(pool=pool, table=table, L=L, R=R, fmt="16bit", dtype=BF16)
+    mla.say("store to a pool of 5 GiB")
+    assert k3x.mla_store(ctx, mla.params(k3x, c, 3), wide[:, :L], pool, table, mla.ints([65, 2]),
+                         rotary=wide[:, L:L + R], offsets=mla.ints([0, 2, 3])) == 0
+    assert ctx.synchronize() == 0
+    data = ref.encode(rows[:, :L], rows[:, L:], "16bit")[0]
+    for i, (pg, at) in enumerate([(3, 63), (pages - 1, 0), (pages - 2, 1)]):
+        assert torch.equal(pool[pg, at].cpu(), data[i])
+        pool[pg, at] = 0
+    assert not pool.any()
+
+
+def test_prompt_past_32_bit_offsets(hip):
+    """Rows of queries, outputs, keys, values and rotary parts far apart: 10 GiB between the first
+    key and the last."""
+    k3x, ctx = hip
+    m, n, H, Dn, R, Dv = 3, 40, 2, 128, 64, 128
+    g = ref.gen(6)
+    q = torch.randn((m, H, Dn + R), generator=g).to(BF16)
+    kv = torch.randn((n, H, Dn + Dv), generator=g).to(BF16)
+    rotary = torch.randn((n, R), generator=g).to(BF16)
+    keys = torch.empty((n, 1 << 27), dtype=BF16, device=DEV)
+    kd = keys[:, :H * (Dn + Dv)].view(n, H, Dn + Dv)
+    kd.copy_(kv.to(DEV))
+    rd = keys[:, 1 << 20:(1 << 20) + R]
+    rd.copy_(rotary.to(DEV))
+    rows = torch.empty((m, (1 << 31) + 64), dtype=BF16, device=DEV)
+    qd = rows[:, :H * (Dn + R)].view(m, H, Dn + R)
+    qd.copy_(q.to(DEV))
+    out = rows[:, 1 << 16:(1 << 16) + H * Dv].view(m, H, Dv)
+    p = k3x.make_mla_prompt_params(qd, kd[..., :Dn], kd[..., Dn:], 1, rotary=rd, scale=0.0722)
+    lse = torch.zeros((m, H), device=DEV)
+    mla.say("prompt over keys 2^27 elements apart")
+    assert k3x.mla_prompt(ctx, p, qd, kd[..., :Dn], kd[..., Dn:], out, rotary=rd, lse=lse) == 0
+    assert ctx.synchronize() == 0
+    want, wl, tol, ltol = ref.prompt(q, kv[..., :Dn], kv[..., Dn:], rotary, [m], [n], True,
+                                     float(torch.tensor(0.0722)))
+    assert ref.close(out, want, tol) <= 1 and ref.close(lse, wl, ltol) <= 1
