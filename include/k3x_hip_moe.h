@@ -645,7 +645,8 @@ typedef struct k3x_hip_mla_params {
     uint32_t page_size;    /* 1 .. 65536 */
     uint32_t pages;        /* of the pool, pages * page_size at most 2^31 */
     uint32_t table_width;  /* 1 .. 2^20 */
-    uint32_t longest;      /* tokens of the call in a sequence at most; 0: T */
+    uint32_t longest;      /* tokens of the call in a sequence at most; 0: T.  Times heads
+                              below 2^31 (k3x_hip_mla_attention). */
     float scale;           /* of the scores, > 0 (k3x_hip_mla_attention) */
     float norm_epsilon;    /* >= 0, with gamma (k3x_hip_mla_store) */
     /* Elements from token to token of latent, rotary, q and out; 0: packed. */
@@ -658,12 +659,14 @@ size_t k3x_hip_mla_row_bytes(const k3x_hip_mla_params* params);
 /* Writes the call's tokens to their pages: latent device [T][L], rotary [T][R]
  * (NULL with R = 0), both of the call's type.  gamma (device fp32 [L], or NULL):
  * the latent is normalised first, x / sqrt(mean(x^2) + norm_epsilon) * gamma,
- * formed in double and rounded to the call's type.  Codes are rounded to nearest,
- * ties to even, with the least scale (2^-110 at least) by which the largest of its
- * 32 is at most 448 (E4M3) or 6 (E2M1), so that nothing saturates.  Tokens of
- * sequences that share the page of their last positions overwrite one another.
+ * formed in double, rounded to fp32 and then to the call's type.  Codes are rounded
+ * to nearest, ties to even, with the least scale (2^-110 at least) by which the
+ * largest of its 32 is at most 448 (E4M3) or 6 (E2M1), so that nothing saturates.
+ * Tokens of sequences that share the page of their last positions overwrite one
+ * another.
  * Also latched, as K3X_ERR_INVALID_MXFP4, the token's row left as it was: a latent
- * or rotary part that is not finite as it is written.  Asynchronous. */
+ * or rotary part that is not finite as it is written; other tokens' rows may then
+ * be missing (repeated, such a call writes what it wrote again).  Asynchronous. */
 int k3x_hip_mla_store(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const void* latent,
                       const void* rotary, const float* gamma, const uint32_t* table,
                       const uint32_t* offsets, const uint32_t* lens, void* pool);
@@ -686,11 +689,12 @@ int k3x_hip_mla_load(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const v
  * a key's weight is rounded to the call's type before it multiplies the latent.
  * q, out and pool 16-byte aligned, strides of q and out multiples of 8 elements.
  * workspace as k3x_hip_delta_rule's, k3x_hip_mla_attention_workspace(params)
- * bytes.  Also latched, as K3X_ERR_INVALID_MXFP4: an output that is not finite
- * (for a query or a cached row that is not, or sums of weighted latents past fp32),
- * and scores of a token that are all minus infinity, past fp32 or for such a query;
- * with fp16 also scores (times scale) of 2^24 and more, which may be past its weights.
- * Replaces the attention of reference/k3x_ref/mla.py, batched.  Asynchronous. */
+ * bytes, also for a call without tokens (0: parameters that it refuses).
+ * Also latched, as K3X_ERR_INVALID_MXFP4: an output that is not finite (for a query
+ * or a cached row that is not, or sums of weighted latents past fp32), scores of a
+ * token that are all minus infinity (past fp32, or for such a query), and with fp16
+ * scores (times scale) of 2^24 and more, which its weights may not hold.  Replaces
+ * the attention of reference/k3x_ref/mla.py, batched.  Asynchronous. */
 int k3x_hip_mla_attention(k3x_hip_ctx* ctx, const k3x_hip_mla_params* params, const void* q,
                           const void* pool, const uint32_t* table, const uint32_t* offsets,
                           const uint32_t* lens, void* out, float* lse, void* workspace,
@@ -726,7 +730,7 @@ typedef struct k3x_hip_mla_prompt_params {
  * S / N rows each), a cached prefix's first.  causal: query i of m sees the first
  * n - m + i + 1 of n keys.  lse, empty rows, sums and weights as for
  * k3x_hip_mla_attention.  q, k, v, rotary and out 16-byte aligned, those without rows
- * may be NULL.
+ * may be NULL.  Heads times (T / 128 + min(N, T)) are below 2^24.
  * Latched: offsets that fall, pass T or S (K3X_ERR_INVALID_STATE; nothing of such
  * a sequence is read), and as for k3x_hip_mla_attention outputs that are not finite
  * and scores (K3X_ERR_INVALID_MXFP4).
