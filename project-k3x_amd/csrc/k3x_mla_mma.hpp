@@ -84,8 +84,10 @@ __device__ inline float across(float x, Op op) {
 
 // Weights are powers of two of the scores past a row's reference, which is its largest score so
 // far less kLift, and may lag behind it: by kLag in all, so that sums and outputs are seldom
-// multiplied again.  They are rounded to the call's type for the second product (the matrix
-// cores take 16 bits a value; sums are of the unrounded ones).  bf16 has fp32's exponents.
+// multiplied again.  They are rounded to the call's type for the second product, as the matrix
+// cores take operands of 16 bits; sums are of the unrounded ones.  Outputs of bf16 are off by
+// 0.0017 to 0.0021 of themselves so, with fp32 weights by the 0.0016 to 0.0017 of their own
+// rounding.  bf16 has fp32's exponents.
 // Of fp16 the range is spent above: with the largest at 2^0 weights below 2^-25 would vanish,
 // 0.3% of the output where 10^5 are of about that size; at 2^7 (2^15 at most of its 2^16) they
 // are rounded by 2^-32 of the largest.

@@ -16,12 +16,12 @@
 // ranges is joined by a second launch.
 //
 // Bound: with many rows the reads of LDS, which each wave makes for both products, beside
-// the matrix cores (busy for 29 to 39% of the cycles) and the weights between them; with
+// the matrix cores (busy for 28 to 38% of the cycles) and the weights between them; with
 // few rows memory.  At a latent of 512 and a rotary part of 64: 64 sequences of 208000
-// tokens, 128 heads, 16 bits 107 us (88 and the join's 18, whose pieces are 82 MB written
+// tokens, 128 heads, 16 bits 106 us (90 and the join's 18, whose pieces are 82 MB written
 // and read); 8 windows of 5 tokens on 32 heads over 77000 tokens in E4M3 71 us; 4 sequences
 // of 417000 tokens, 64 heads, in E2M1 99 us, 581 TFLOP/s; 64 sequences of 8192 tokens, 32
-// heads, 16 bits 127 us, 4.8 TB/s; one of 1000 tokens on 16 heads 12.
+// heads, 16 bits 127 us, 4.8 TB/s; one of 1000 tokens on 16 heads 14, in two launches.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -810,7 +810,7 @@ Plan plan_of(const k3x_hip_mla_params* p) {
     x.LP = p->latent <= 256 ? 256 : 512;
     // As few rows as hold a sequence's: 16 heads, 64 sequences of 8192 tokens in 16 and 4 bits
     // 120 and 81 us, with 32 rows 126 and 92.  More than 64 in blocks of 64, or of 128 once those
-    // of all sequences pass 64: half as many reads of the cache and of LDS, but twice the
+    // of all sequences are 64: half as many reads of the cache and of LDS, but twice the
     // outputs of a range for the join.  128 heads, 16 bits, in blocks of 128 and of 64: 8
     // sequences of 16384 69.6 and 58.4 us, 32 of 2048 57.3 and 43.1, of 8192 113 and 107; 64
     // of 1000 54.5 and 45.5, of 4096 108 and 110, of 8192 184 and 198, in 8 bits 184 and 220.

@@ -8,9 +8,9 @@
 //
 // Bound: memory, and with few tokens the chain of a token's sequence, page and row.
 // Kernels at a latent of 512 and a rotary part of 64: 64 decode tokens in E4M3 4.4 us
-// written and 3.8 read; 8192 tokens with their norm in E2M1 8.6 (13 MB) and 6.2; six
+// written and 3.8 read; 8192 tokens with their norm in E2M1 8.7 (13 MB) and 6.3; six
 // prefixes of 131072 tokens together read in 57 us, 237 MB at 4.1 TB/s, where a large
-// copy reaches 5.1.
+// copy reaches 5.1 (38 us where the last cache holds the rows).
 #include <hip/hip_runtime.h>
 
 #include "k3x_mla.hpp"
@@ -281,9 +281,9 @@ int cache_args(k3x_hip_ctx* ctx, const k3x_hip_mla_params* p, const void* latent
 }
 
 // One token a wave, or eight past twice the waves that are held at once: with fewer, waves
-// that wait hide each other's time better.  In 4 bits one and eight, stored 8192 tokens 12.9
-// and 15.9 us, 16384 22.5 and 21.3, 32768 38.8 and 33.8; read 5.4 and 7.2, 8.2 and 8.7, 15.3
-// and 12.5.
+// that wait hide each other's time better.  Kernels over eight inputs in turn, E2M1 with the
+// norm, one and eight: 8192 tokens stored 9.2 and 10.5 us, 16384 16.8 and 16.6, 32768 28.0 and
+// 26.4; read 6.4 and 7.8, 9.0 and 8.6, 14.7 and 11.1.
 constexpr uint32_t kByEights = 16384;
 template <uint32_t DT, uint32_t F>
 int launch_store(k3x_hip_ctx* ctx, const CacheArgs& a) {

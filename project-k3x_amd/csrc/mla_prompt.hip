@@ -9,9 +9,9 @@
 // Bound: the matrix cores (busy for 53% of the cycles) and LDS: the two workgroups of a
 // compute unit take 3900 cycles for a tile of 64 keys each, 2560 of them products; reads of
 // LDS take about as long, and weights, 420 a wave, stand between.  One prompt of 2048
-// tokens, 32 heads of 128 + 64 and 128: 57 us, 757 TFLOP/s of products that count (a large
-// matrix product reaches 1218); seven ragged ones of 8192 tokens together 305 to 312 us,
-// 797 to 813 TFLOP/s.  Two tiles of 32 queries a wave, one wave a SIMD, read LDS half as
+// tokens, 32 heads of 128 + 64 and 128: 56 us, 765 TFLOP/s of products that count (a large
+// matrix product reaches 1218); seven ragged ones of 8192 tokens together 305 to 315 us,
+// 788 to 813 TFLOP/s.  Two tiles of 32 queries a wave, one wave a SIMD, read LDS half as
 // often, but take 547: then every cycle of weights is one without products.
 #include <hip/hip_runtime.h>
 
