@@ -591,7 +591,8 @@ typedef struct k3x_hip_logits_params {
  * repetition that is not a number above 0, a frequency or presence that is not
  * finite; rows of that sequence may then be missing or hold some of the steps.  With
  * out = logits all rows of the other sequences are adjusted (such a call cannot be
- * repeated); of any other call they may be missing.
+ * repeated); of any other call they may be missing.  Calls that overlap on one
+ * context: as for k3x_hip_delta_rule.
  * Logits and biases may hold anything and go through the arithmetic as they are.
  * Asynchronous. */
 int k3x_hip_adjust_logits(k3x_hip_ctx* ctx, const k3x_hip_logits_params* params,
